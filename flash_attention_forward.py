@@ -27,6 +27,7 @@ import torch
 from flash_attn_npu_b200 import host_stream as _host_stream
 from flash_attn_npu_b200.ops import check_device_status  # noqa: F401  (device failure check)
 from flash_attn_npu_b200 import ops as _ops
+from flash_attn_npu_b200 import paged as _paged
 from flash_attn_npu_b200 import tiling as _tiling
 
 DEVICE = "cuda"
@@ -204,6 +205,25 @@ def attention_host(q, k, v, causal, sm_scale, BM=None, BN=None, return_lse=False
     if return_lse:
         return o, l
     return o
+
+
+# ------------------------------------------------------------------------- paged key/value cache
+# Sequences of unequal lengths whose keys and values stay in a cache of pages from call to call
+# (layouts and rules: flash_attn_npu_b200/paged.py).
+paged_cache_empty = _paged.empty_cache
+paged_cache_write = _paged.write
+paged_cache_read = _paged.read
+
+
+def paged_attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scale,
+                    k_scale=None, v_scale=None, max_q_len=None, return_lse=False, out=None,
+                    lse=None):
+    """`attention` of packed new tokens q [total, heads_q, head_dim] over a paged cache."""
+    out, lse = _paged.attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scale,
+                                k_scale, v_scale, max_q_len, out, lse)
+    if return_lse:
+        return out, lse
+    return out
 
 
 # ----------------------------------------------------------------------------- profiling
@@ -422,6 +442,10 @@ __all__ = [
     "get_tiling",
     "get_tile_config",
     "attention",
+    "paged_attention",
+    "paged_cache_empty",
+    "paged_cache_read",
+    "paged_cache_write",
     "profile_once",
     "profiling",
 ]

@@ -17,6 +17,7 @@ LIB_PATH = Path(os.environ.get("FA_SM100_LIB", PKG_DIR / "libfa_sm100.so"))
 FA_DTYPE_FP16 = 0
 FA_DTYPE_BF16 = 1
 FA_DTYPE_FP32 = 2
+FA_DTYPE_FP8_E4M3 = 3  # paged caches only
 
 FA_FLAG_FP32_TF32 = 1
 FA_FLAG_V_FP8_E5M2 = 2
@@ -32,8 +33,9 @@ FA_ERR_TENSOR_MAP = -6
 FA_ERR_LAUNCH = -7
 FA_ERR_DEVICE = -8
 FA_ERR_DEVICE_TIMEOUT = -9
+FA_ERR_PAGE_TABLE = -10
 
-# Every symbol include/fa_fwd_sm100.h declares (checked by the tests).
+# Every symbol the headers of include/ declare (checked by the tests).
 EXPORTED_SYMBOLS = (
     "fa_fwd_sm100",
     "fa_fwd_sm100_default_tile",
@@ -42,6 +44,10 @@ EXPORTED_SYMBOLS = (
     "fa_fwd_sm100_grid_size",
     "fa_fwd_sm100_status_string",
     "fa_fwd_sm100_version",
+    "fa_paged_write_sm100",
+    "fa_paged_read_sm100",
+    "fa_paged_attn_sm100",
+    "fa_paged_workspace_bytes",
 )
 
 
@@ -76,6 +82,65 @@ class FaFwdArgs(ctypes.Structure):
         ("tile", FaTileConfig),
         ("dev_status", ctypes.c_void_p),
         ("flags", ctypes.c_int32),
+    ]
+
+
+class FaPagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("kv_lens", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("k_scale_stride", ctypes.c_int64 * 2),
+        ("v_scale_stride", ctypes.c_int64 * 2),
+        ("num_pages", ctypes.c_int64),
+        ("heads_kv", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("table_stride", ctypes.c_int64),
+        ("table_cols", ctypes.c_int64),
+        ("seqs", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class FaPagedCopyArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_int32),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("dev_status", ctypes.c_void_p),
+        ("cache", FaPagedCache),
+        ("k_stride", ctypes.c_int64 * 2),
+        ("v_stride", ctypes.c_int64 * 2),
+        ("total", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class FaPagedAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("dev_status", ctypes.c_void_p),
+        ("cache", FaPagedCache),
+        ("q_stride", ctypes.c_int64 * 2),
+        ("o_stride", ctypes.c_int64 * 2),
+        ("total", ctypes.c_int64),
+        ("heads_q", ctypes.c_int64),
+        ("max_q_len", ctypes.c_int64),
+        ("workspace_bytes", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
     ]
 
 
@@ -122,6 +187,13 @@ def load() -> ctypes.CDLL:
         lib.fa_fwd_sm100_max_stages.restype = ctypes.c_int
         lib.fa_fwd_sm100_grid_size.argtypes = [ctypes.POINTER(FaFwdArgs)]
         lib.fa_fwd_sm100_grid_size.restype = ctypes.c_int64
+        # the paged calls take a block of bytes laid out as their structure (see paged.py)
+        for name in ("fa_paged_write_sm100", "fa_paged_read_sm100", "fa_paged_attn_sm100"):
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+            fn.restype = ctypes.c_int
+        lib.fa_paged_workspace_bytes.argtypes = [ctypes.c_void_p]
+        lib.fa_paged_workspace_bytes.restype = ctypes.c_int64
         lib.fa_fwd_sm100_status_string.argtypes = [ctypes.c_int]
         lib.fa_fwd_sm100_status_string.restype = ctypes.c_char_p
         lib.fa_fwd_sm100_version.argtypes = []

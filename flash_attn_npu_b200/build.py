@@ -46,6 +46,13 @@ SOURCES = [
     "fa_fwd_d64.cu",
     "fa_fwd_d128.cu",
     "fa_fwd_d256.cu",
+    "fa_paged_api.cu",
+    "fa_paged_cache.cu",
+    "fa_paged_rows_d16.cu",
+    "fa_paged_rows_d32.cu",
+    "fa_paged_rows_d64.cu",
+    "fa_paged_rows_d128.cu",
+    "fa_paged_rows_d256.cu",
 ]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

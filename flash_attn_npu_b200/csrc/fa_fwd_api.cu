@@ -19,6 +19,7 @@
 #include <mutex>
 
 #include "../../include/fa_fwd_sm100.h"
+#include "../../include/fa_paged_sm100.h"
 #include "fa_fp32.h"
 #include "fa_launch.h"
 
@@ -150,7 +151,8 @@ int encode_map(CUtensorMap* map, const void* ptr, int dtype, int64_t B, int64_t 
   CUtensorMapSwizzle sw = atom32             ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
                           : swz_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
                           : swz_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                            : CU_TENSOR_MAP_SWIZZLE_32B;
+                          : swz_bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
+                                            : CU_TENSOR_MAP_SWIZZLE_NONE;
   CUresult r = enc(map, dt, 4, const_cast<void*>(ptr), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -217,6 +219,31 @@ int resolve_tile(const FaFwdArgs* a, FaTileConfig* t) {
 }  // namespace
 
 namespace fa {
+int check_device() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return FA_ERR_DEVICE;
+  }
+  return device_ok(dev) ? FA_OK : FA_ERR_DEVICE;
+}
+
+int sm_count_of_current() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    (void)cudaGetLastError();
+    dev = -1;
+  }
+  return sm_count(dev);
+}
+
+int encode_cache_map(CUtensorMap* map, const void* ptr, int dtype, int64_t pages, int64_t heads,
+                     int64_t rows, int64_t head_dim, const int64_t st[3], int box_cols,
+                     int box_rows, int swz_bytes) {
+  return encode_map(map, ptr, dtype == FA_DTYPE_FP8_E4M3 ? kDtypeByte : dtype, pages, heads, rows,
+                    head_dim, st, box_cols, box_rows, swz_bytes);
+}
+
 KernelInfo kernel_info(int head_dim, int dtype, int block_n, int qt, bool vf8) {
   return info_for(head_dim, dtype, block_n, qt, vf8);
 }
@@ -396,6 +423,8 @@ const char* fa_fwd_sm100_status_string(int code) {
     case FA_ERR_LAUNCH: return "kernel launch failed";
     case FA_ERR_DEVICE: return "current CUDA device is not an sm_100 (B200) part";
     case FA_ERR_DEVICE_TIMEOUT: return "a pipeline wait in the kernel timed out";
+    case FA_ERR_PAGE_TABLE:
+      return "a page index, length or offset of a paged call lies outside its page table or cache";
     default: return "unknown status";
   }
 }

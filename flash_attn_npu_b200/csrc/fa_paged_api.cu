@@ -1,0 +1,151 @@
+// C-ABI front end of the paged attention (declared in include/fa_paged_sm100.h): checks, kernel
+// choice, tensor maps, workspace layout, launch.
+#include <algorithm>
+#include <cmath>
+
+#include "fa_paged_host.h"
+#include "fa_paged_launch.h"
+#include "fa_paged_rows.cuh"
+
+namespace fa {
+
+// fa_fwd_api.cu: 4-D tiled map over [pages, heads, rows, head_dim].
+int encode_cache_map(CUtensorMap* map, const void* ptr, int dtype, int64_t pages, int64_t heads,
+                     int64_t rows, int64_t head_dim, const int64_t st[3], int box_cols,
+                     int box_rows, int swz_bytes);
+
+namespace {
+
+template <int D, bool FP8>
+PagedInfo info_of(int mt) {
+  using G = RowsGeo<D, FP8, 1>;
+  return PagedInfo{16 * mt, G::KEYS, G::SPAN, FP8 ? G::SPAN : G::SPAN / 2};
+}
+
+int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+
+// What a call runs with, from its arguments alone.
+struct Choice {
+  int mt;
+  int grid;
+  int64_t parts, lse, o, bytes;  // workspace offsets
+};
+
+int check_attn(const FaPagedAttnArgs* a) {
+  if (!a || a->struct_size != static_cast<int32_t>(sizeof(FaPagedAttnArgs)))
+    return FA_ERR_INVALID_ARG;
+  const int rc = check_layout(a->cache, a->dtype, a->total);
+  if (rc != FA_OK) return rc;
+  if (a->heads_q <= 0 || a->heads_q % a->cache.heads_kv || a->max_q_len < 0)
+    return FA_ERR_INVALID_ARG;
+  // rows of a sequence (tokens x query heads) are counted in 32 bits
+  if (a->total * a->heads_q > INT32_MAX / 2) return FA_ERR_INVALID_ARG;
+  if (!std::isfinite(a->sm_scale)) return FA_ERR_INVALID_ARG;
+  return FA_OK;
+}
+
+Choice choose(const FaPagedAttnArgs* a) {
+  Choice c{};
+  const int64_t group = a->heads_q / a->cache.heads_kv;
+  const int64_t longest = a->max_q_len ? std::min(a->max_q_len, a->total) : a->total;
+  c.mt = longest * group > 16 && a->cache.head_dim <= 128 ? 2 : 1;
+  c.grid = sm_count_of_current();
+  const int64_t rows = 2 * 16 * c.mt * static_cast<int64_t>(c.grid);
+  c.parts = 0;
+  c.lse = up256(c.parts + static_cast<int64_t>(sizeof(PagedPart)) * c.grid);
+  c.o = up256(c.lse + 4 * rows);
+  c.bytes = up256(c.o + 4 * rows * a->cache.head_dim);
+  return c;
+}
+
+}  // namespace
+
+PagedInfo rows_info(int head_dim, bool fp8, int mt) {
+  switch (head_dim) {
+    case 16: return fp8 ? info_of<16, true>(mt) : info_of<16, false>(mt);
+    case 32: return fp8 ? info_of<32, true>(mt) : info_of<32, false>(mt);
+    case 64: return fp8 ? info_of<64, true>(mt) : info_of<64, false>(mt);
+    case 128: return fp8 ? info_of<128, true>(mt) : info_of<128, false>(mt);
+    default: return fp8 ? info_of<256, true>(mt) : info_of<256, false>(mt);
+  }
+}
+
+}  // namespace fa
+
+extern "C" {
+
+int64_t fa_paged_workspace_bytes(const FaPagedAttnArgs* a) {
+  const int rc = fa::check_attn(a);
+  return rc != FA_OK ? rc : fa::choose(a).bytes;
+}
+
+int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
+  int rc = fa::check_attn(a);
+  if (rc == FA_OK) rc = fa::check_cache(a->cache, a->dtype, a->total);
+  if (rc != FA_OK) return rc;
+  if (a->total == 0 || a->cache.seqs == 0) return FA_OK;
+  if (!a->q || !a->o || !a->lse || !a->workspace) return FA_ERR_INVALID_ARG;
+  for (const void* x : {a->q, static_cast<const void*>(a->o)})
+    if (reinterpret_cast<uintptr_t>(x) % 16) return FA_ERR_MISALIGNED;
+  for (const int64_t* st : {a->q_stride, a->o_stride})
+    if ((a->total > 1 && st[0] % 8) || (a->heads_q > 1 && st[1] % 8)) return FA_ERR_MISALIGNED;
+  if (reinterpret_cast<uintptr_t>(a->lse) % 4 ||
+      reinterpret_cast<uintptr_t>(a->workspace) % 256)
+    return FA_ERR_MISALIGNED;
+  rc = fa::check_device();
+  if (rc != FA_OK) return rc;
+  const fa::Choice c = fa::choose(a);
+  if (a->workspace_bytes < c.bytes) return FA_ERR_INVALID_ARG;
+
+  const FaPagedCache& kv = a->cache;
+  fa::PagedPlan plan{};
+  plan.half = a->dtype == FA_DTYPE_FP16;
+  plan.fp8 = kv.dtype == FA_DTYPE_FP8_E4M3;
+  plan.mt = c.mt;
+  plan.grid = c.grid;
+  plan.stream = static_cast<cudaStream_t>(stream);
+  const fa::PagedInfo info = fa::rows_info(static_cast<int>(kv.head_dim), plan.fp8, c.mt);
+  const int box = static_cast<int>(std::min<int64_t>(kv.page_size, info.keys));
+  rc = fa::encode_cache_map(&plan.tmK, kv.k, kv.dtype, kv.num_pages, kv.heads_kv, kv.page_size,
+                            kv.head_dim, kv.k_stride, info.cols, box, info.span);
+  if (rc == FA_OK)
+    rc = fa::encode_cache_map(&plan.tmV, kv.v, kv.dtype, kv.num_pages, kv.heads_kv, kv.page_size,
+                              kv.head_dim, kv.v_stride, info.cols, box, info.span);
+  if (rc != FA_OK) return rc;
+
+  fa::PagedAttnParams& p = plan.params;
+  p.seqs = fa::seqs_of(kv, a->total, a->dev_status);
+  p.q = a->q;
+  p.o = a->o;
+  p.lse = a->lse;
+  for (int d = 0; d < 2; ++d) {
+    p.q_stride[d] = a->q_stride[d];
+    p.o_stride[d] = a->o_stride[d];
+    p.k_scale_stride[d] = kv.k_scale_stride[d];
+    p.v_scale_stride[d] = kv.v_scale_stride[d];
+  }
+  p.k_scale = kv.k_scale;
+  p.v_scale = kv.v_scale;
+  p.heads_kv = static_cast<int>(kv.heads_kv);
+  p.group = static_cast<int>(a->heads_q / kv.heads_kv);
+  p.head_dim = static_cast<int>(kv.head_dim);
+  p.causal = a->causal ? 1 : 0;
+  p.scale_log2 = a->sm_scale * fa::kLog2e;
+  p.min_steps = 2;
+  p.rows_from = 1;
+  p.rows_to = INT32_MAX;
+  char* ws = static_cast<char*>(a->workspace);
+  p.parts = reinterpret_cast<fa::PagedPart*>(ws + c.parts);
+  p.part_lse = reinterpret_cast<float*>(ws + c.lse);
+  p.part_o = reinterpret_cast<float*>(ws + c.o);
+
+  switch (kv.head_dim) {
+    case 16: return fa::launch_rows_d16(plan);
+    case 32: return fa::launch_rows_d32(plan);
+    case 64: return fa::launch_rows_d64(plan);
+    case 128: return fa::launch_rows_d128(plan);
+    default: return fa::launch_rows_d256(plan);
+  }
+}
+
+}  // extern "C"

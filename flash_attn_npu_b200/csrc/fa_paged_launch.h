@@ -1,0 +1,51 @@
+// Launch plan of a paged attention call, shared by the C-ABI front end (fa_paged_api.cu) and the
+// translation units that hold the kernel instantiations (fa_paged_rows_d*.cu).
+#pragma once
+
+#include "fa_paged_attn.cuh"
+
+namespace fa {
+
+// Facts of a kernel that the host needs: rows of a block, keys of a tile, and the boxes of its
+// TMA copies.
+struct PagedInfo {
+  int rows, keys;
+  int span;  // bytes of a copied row: the swizzle width
+  int cols;  // elements of a copied row
+};
+
+struct PagedPlan {
+  CUtensorMap tmK, tmV;
+  PagedAttnParams params;
+  bool half;  // q and the output are fp16 (else bf16)
+  bool fp8;
+  int mt;     // 16-row tiles of a block (1 or 2)
+  int grid;
+  cudaStream_t stream;
+};
+
+PagedInfo rows_info(int head_dim, bool fp8, int mt);
+int launch_rows_d16(const PagedPlan& plan);
+int launch_rows_d32(const PagedPlan& plan);
+int launch_rows_d64(const PagedPlan& plan);
+int launch_rows_d128(const PagedPlan& plan);
+int launch_rows_d256(const PagedPlan& plan);
+
+// Brings the combine kernel up beside the kernel before it in the stream (programmatic dependent
+// launch): it waits for that kernel's end itself, so only the launch latency overlaps.
+template <typename Kernel>
+int launch_dependent(Kernel kernel, dim3 grid, int threads, cudaStream_t stream,
+                     const PagedAttnParams& params) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, params) == cudaSuccess ? 0 : -7;
+}
+
+}  // namespace fa

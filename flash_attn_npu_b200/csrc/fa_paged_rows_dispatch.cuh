@@ -1,0 +1,63 @@
+// Instantiations of the paged row kernel for one head dimension: included with FA_HEAD_DIM defined
+// by fa_paged_rows_d*.cu, so that the head dimensions compile as separate translation units.
+//   q fp16 / bf16, cache of the same type or float8, blocks of 16 rows, or 32 for head_dim <= 128
+//   (two tiles' fragments of 256 columns do not fit a thread's registers)
+#pragma once
+
+#include "fa_paged_launch.h"
+#include "fa_paged_rows.cuh"
+
+#ifndef FA_HEAD_DIM
+#error "define FA_HEAD_DIM"
+#endif
+
+namespace fa {
+namespace {
+
+template <typename T, bool FP8, int MT>
+int launch_rows(const PagedPlan& plan) {
+  using G = RowsGeo<FA_HEAD_DIM, FP8, MT>;
+  auto kernel = paged_rows_kernel<T, FA_HEAD_DIM, FP8, MT>;
+  if constexpr (G::SPLIT) {
+    // the split redistributes exactly the launch allocation: refuse a build that differs
+    static int regs_ok = 0;  // 0 unknown, 1 ok, -1 mismatch
+    if (regs_ok == 0) {
+      cudaFuncAttributes attr{};
+      regs_ok = cudaFuncGetAttributes(&attr, kernel) == cudaSuccess && attr.numRegs == G::REG_LAUNCH
+                    ? 1
+                    : -1;
+      (void)cudaGetLastError();
+    }
+    if (regs_ok != 1) return -7;
+  }
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) !=
+      cudaSuccess) {
+    (void)cudaGetLastError();
+    return -7;
+  }
+  kernel<<<plan.grid, G::THREADS, G::SMEM, plan.stream>>>(plan.tmK, plan.tmV, plan.params);
+  if (cudaGetLastError() != cudaSuccess) return -7;
+  if (plan.grid == 1) return 0;  // no shared item
+  const int64_t most = static_cast<int64_t>(plan.params.seqs.total) * plan.params.group;
+  const unsigned rows = static_cast<unsigned>(most < G::ROWS ? most : G::ROWS);
+  constexpr int kWarps = 4;
+  return launch_dependent(paged_combine_kernel<T, G::ROWS, kWarps>, dim3(plan.grid - 1, rows),
+                          kWarps * 32, plan.stream, plan.params);
+}
+
+template <typename T, bool FP8>
+int launch_mt(const PagedPlan& plan) {
+  if constexpr (FA_HEAD_DIM <= 128) {
+    if (plan.mt == 2) return launch_rows<T, FP8, 2>(plan);
+  }
+  return launch_rows<T, FP8, 1>(plan);
+}
+
+int launch_any(const PagedPlan& plan) {
+  if (plan.fp8)
+    return plan.half ? launch_mt<__half, true>(plan) : launch_mt<__nv_bfloat16, true>(plan);
+  return plan.half ? launch_mt<__half, false>(plan) : launch_mt<__nv_bfloat16, false>(plan);
+}
+
+}  // namespace
+}  // namespace fa

@@ -62,7 +62,9 @@ enum FaStatus {
   FA_ERR_TENSOR_MAP = -6,           /* cuTensorMapEncodeTiled rejected a descriptor */
   FA_ERR_LAUNCH = -7,               /* the CUDA launch itself failed */
   FA_ERR_DEVICE = -8,               /* current device is not an sm_100 part */
-  FA_ERR_DEVICE_TIMEOUT = -9        /* written to *dev_status: a pipeline wait gave up */
+  FA_ERR_DEVICE_TIMEOUT = -9,       /* written to *dev_status: a pipeline wait gave up */
+  FA_ERR_PAGE_TABLE = -10           /* written to *dev_status: a page, length or offset of a paged
+                                       cache call lies outside its table or cache */
 };
 
 typedef struct FaTileConfig {
