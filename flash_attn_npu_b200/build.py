@@ -53,6 +53,11 @@ SOURCES = [
     "fa_paged_rows_d64.cu",
     "fa_paged_rows_d128.cu",
     "fa_paged_rows_d256.cu",
+    "fa_paged_tile_d16.cu",
+    "fa_paged_tile_d32.cu",
+    "fa_paged_tile_d64.cu",
+    "fa_paged_tile_d128.cu",
+    "fa_paged_tile_d256.cu",
 ]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

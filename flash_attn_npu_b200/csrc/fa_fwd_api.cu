@@ -244,6 +244,31 @@ int encode_cache_map(CUtensorMap* map, const void* ptr, int dtype, int64_t pages
                     head_dim, st, box_cols, box_rows, swz_bytes);
 }
 
+int encode_query_map(CUtensorMap* map, const void* ptr, int dtype, int64_t total, int64_t heads,
+                     int64_t head_dim, const int64_t st[2], int box_cols, int box_heads,
+                     int box_tokens, int swz_bytes) {
+  const int64_t s_head = st[1] * 2, s_tok = st[0] * 2;
+  if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0) return FA_ERR_MISALIGNED;
+  for (int64_t s : {s_head, s_tok})
+    if (s <= 0 || s % 16 != 0 || s >= (int64_t{1} << 40)) return FA_ERR_MISALIGNED;
+  auto enc = encode_fn();
+  if (!enc) return FA_ERR_TENSOR_MAP;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(total)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(s_head), static_cast<cuuint64_t>(s_tok)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_heads),
+                             static_cast<cuuint32_t>(box_tokens)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r =
+      enc(map, dtype == FA_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+          3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+          swz_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+          : swz_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                            : CU_TENSOR_MAP_SWIZZLE_32B,
+          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FA_OK : FA_ERR_TENSOR_MAP;
+}
+
 KernelInfo kernel_info(int head_dim, int dtype, int block_n, int qt, bool vf8) {
   return info_for(head_dim, dtype, block_n, qt, vf8);
 }

@@ -6,6 +6,7 @@
 #include "fa_paged_host.h"
 #include "fa_paged_launch.h"
 #include "fa_paged_rows.cuh"
+#include "fa_paged_tile.cuh"
 
 namespace fa {
 
@@ -13,20 +14,43 @@ namespace fa {
 int encode_cache_map(CUtensorMap* map, const void* ptr, int dtype, int64_t pages, int64_t heads,
                      int64_t rows, int64_t head_dim, const int64_t st[3], int box_cols,
                      int box_rows, int swz_bytes);
+// fa_fwd_api.cu: 3-D tiled map over packed queries [total, heads, head_dim].
+int encode_query_map(CUtensorMap* map, const void* ptr, int dtype, int64_t total, int64_t heads,
+                     int64_t head_dim, const int64_t st[2], int box_cols, int box_heads,
+                     int box_tokens, int swz_bytes);
 
 namespace {
 
-template <int D, bool FP8>
-PagedInfo info_of(int mt) {
-  using G = RowsGeo<D, FP8, 1>;
-  return PagedInfo{16 * mt, G::KEYS, G::SPAN, FP8 ? G::SPAN : G::SPAN / 2};
+template <int D>
+PagedInfo info_of(bool tile, bool fp8, int mt) {
+  if (tile) {
+    using G = TileGeo<D, false>;  // float8 tiles land as they are, without a swizzle
+    return fp8 ? PagedInfo{128 * G::TILES, G::KEYS, 16, D}
+               : PagedInfo{128 * G::TILES, G::KEYS, G::SWZ, G::SWZ / 2};
+  }
+  using R = RowsGeo<D, false, 1>;
+  using F = RowsGeo<D, true, 1>;
+  return fp8 ? PagedInfo{16 * mt, F::KEYS, F::SPAN, F::SPAN}
+             : PagedInfo{16 * mt, R::KEYS, R::SPAN, R::SPAN / 2};
+}
+
+PagedInfo info_for(int64_t head_dim, bool tile, bool fp8, int mt) {
+  switch (head_dim) {
+    case 16: return info_of<16>(tile, fp8, mt);
+    case 32: return info_of<32>(tile, fp8, mt);
+    case 64: return info_of<64>(tile, fp8, mt);
+    case 128: return info_of<128>(tile, fp8, mt);
+    default: return info_of<256>(tile, fp8, mt);
+  }
 }
 
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // What a call runs with, from its arguments alone.
 struct Choice {
+  bool tile;  // tile kernel, else row kernel
   int mt;
+  PagedInfo info;
   int grid;
   int64_t parts, lse, o, bytes;  // workspace offsets
 };
@@ -48,9 +72,14 @@ Choice choose(const FaPagedAttnArgs* a) {
   Choice c{};
   const int64_t group = a->heads_q / a->cache.heads_kv;
   const int64_t longest = a->max_q_len ? std::min(a->max_q_len, a->total) : a->total;
-  c.mt = longest * group > 16 && a->cache.head_dim <= 128 ? 2 : 1;
+  // Up to 32 rows a kv head every sequence is one block of the row kernel, which reads the cache
+  // once; above that the tile kernel does so for 128 or 256 rows.  It needs a positive scale, and
+  // a group that fits a tile.
+  c.tile = longest * group > 32 && group <= 128 && a->sm_scale > 0.f;
+  c.mt = !c.tile && longest * group > 16 && a->cache.head_dim <= 128 ? 2 : 1;
+  c.info = info_for(a->cache.head_dim, c.tile, a->cache.dtype == FA_DTYPE_FP8_E4M3, c.mt);
   c.grid = sm_count_of_current();
-  const int64_t rows = 2 * 16 * c.mt * static_cast<int64_t>(c.grid);
+  const int64_t rows = 2 * static_cast<int64_t>(c.info.rows) * c.grid;
   c.parts = 0;
   c.lse = up256(c.parts + static_cast<int64_t>(sizeof(PagedPart)) * c.grid);
   c.o = up256(c.lse + 4 * rows);
@@ -59,16 +88,6 @@ Choice choose(const FaPagedAttnArgs* a) {
 }
 
 }  // namespace
-
-PagedInfo rows_info(int head_dim, bool fp8, int mt) {
-  switch (head_dim) {
-    case 16: return fp8 ? info_of<16, true>(mt) : info_of<16, false>(mt);
-    case 32: return fp8 ? info_of<32, true>(mt) : info_of<32, false>(mt);
-    case 64: return fp8 ? info_of<64, true>(mt) : info_of<64, false>(mt);
-    case 128: return fp8 ? info_of<128, true>(mt) : info_of<128, false>(mt);
-    default: return fp8 ? info_of<256, true>(mt) : info_of<256, false>(mt);
-  }
-}
 
 }  // namespace fa
 
@@ -88,7 +107,7 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   for (const void* x : {a->q, static_cast<const void*>(a->o)})
     if (reinterpret_cast<uintptr_t>(x) % 16) return FA_ERR_MISALIGNED;
   for (const int64_t* st : {a->q_stride, a->o_stride})
-    if ((a->total > 1 && st[0] % 8) || (a->heads_q > 1 && st[1] % 8)) return FA_ERR_MISALIGNED;
+    if (st[0] <= 0 || st[1] <= 0 || st[0] % 8 || st[1] % 8) return FA_ERR_MISALIGNED;
   if (reinterpret_cast<uintptr_t>(a->lse) % 4 ||
       reinterpret_cast<uintptr_t>(a->workspace) % 256)
     return FA_ERR_MISALIGNED;
@@ -104,7 +123,7 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   plan.mt = c.mt;
   plan.grid = c.grid;
   plan.stream = static_cast<cudaStream_t>(stream);
-  const fa::PagedInfo info = fa::rows_info(static_cast<int>(kv.head_dim), plan.fp8, c.mt);
+  const fa::PagedInfo& info = c.info;
   const int box = static_cast<int>(std::min<int64_t>(kv.page_size, info.keys));
   rc = fa::encode_cache_map(&plan.tmK, kv.k, kv.dtype, kv.num_pages, kv.heads_kv, kv.page_size,
                             kv.head_dim, kv.k_stride, info.cols, box, info.span);
@@ -131,14 +150,27 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   p.head_dim = static_cast<int>(kv.head_dim);
   p.causal = a->causal ? 1 : 0;
   p.scale_log2 = a->sm_scale * fa::kLog2e;
-  p.min_steps = 2;
-  p.rows_from = 1;
-  p.rows_to = INT32_MAX;
+  p.min_steps = c.tile ? 4 : 2;
+  p.tile_toks = c.tile ? 128 / p.group : 0;
+  p.tile_live = c.tile ? p.tile_toks * p.group : info.rows;
   char* ws = static_cast<char*>(a->workspace);
   p.parts = reinterpret_cast<fa::PagedPart*>(ws + c.parts);
   p.part_lse = reinterpret_cast<float*>(ws + c.lse);
   p.part_o = reinterpret_cast<float*>(ws + c.o);
 
+  if (c.tile) {
+    rc = fa::encode_query_map(&plan.tmQ, a->q, a->dtype, a->total, a->heads_q, kv.head_dim,
+                              a->q_stride, static_cast<int>(std::min<int64_t>(kv.head_dim, 64)),
+                              p.group, p.tile_toks, static_cast<int>(std::min<int64_t>(2 * kv.head_dim, 128)));
+    if (rc != FA_OK) return rc;
+    switch (kv.head_dim) {
+      case 16: return fa::launch_tile_d16(plan);
+      case 32: return fa::launch_tile_d32(plan);
+      case 64: return fa::launch_tile_d64(plan);
+      case 128: return fa::launch_tile_d128(plan);
+      default: return fa::launch_tile_d256(plan);
+    }
+  }
   switch (kv.head_dim) {
     case 16: return fa::launch_rows_d16(plan);
     case 32: return fa::launch_rows_d32(plan);

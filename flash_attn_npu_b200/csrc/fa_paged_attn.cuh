@@ -48,8 +48,8 @@ struct PagedAttnParams {
   int causal;
   float scale_log2;  // sm_scale * log2(e)
   int min_steps;     // steps of a CTA's range, at least
-  int rows_from;     // this launch takes the sequences with rows_from <= count * group <= rows_to
-  int rows_to;
+  int tile_live;     // rows of a tile that are used: a multiple of `group` in the tile kernel
+  int tile_toks;     // tokens of a tile (tile kernel)
   PagedPart* parts;  // [gridDim.x]
   float* part_o;     // [gridDim.x][2][block rows][head_dim]
   float* part_lse;   // [gridDim.x][2][block rows]
@@ -63,6 +63,7 @@ struct PagedSeq {
   int64_t steps;
 };
 
+// Work of the row kernel: blocks of ROWS rows, each over all key tiles of its sequence.
 template <int ROWS, int KEYS>
 __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
   PagedSeq s;
@@ -71,7 +72,6 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
   const int rows = s.count * p.group;  // at most total * heads_q, which the host bounds
   s.blocks = (rows + ROWS - 1) / ROWS;
   s.tiles = max(1, (s.len + KEYS - 1) / KEYS);
-  if (rows < p.rows_from || rows > p.rows_to) s.blocks = 0;
   s.steps = static_cast<int64_t>(p.heads_kv) * s.blocks * s.tiles;
   return s;
 }
@@ -85,16 +85,17 @@ struct PagedRange {
   int seq;
 };
 
-// By all threads of the CTA; `scratch`: 40 words of shared memory.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ PagedRange paged_range(const PagedAttnParams& p, int64_t* scratch) {
+// By all threads of the CTA; `scratch`: 40 words of shared memory; steps_of(b): steps of sequence b.
+template <typename Steps>
+__device__ __forceinline__ PagedRange paged_range(const PagedAttnParams& p, int64_t* scratch,
+                                                  Steps steps_of) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int threads = blockDim.x, warps = threads >> 5;
   const int mine = threadIdx.x;
-  const int64_t first = mine < p.seqs.seqs ? paged_seq<ROWS, KEYS>(p, mine).steps : 0;
+  const int64_t first = mine < p.seqs.seqs ? steps_of(mine) : 0;
   int64_t sum = first;
   for (int b = mine + threads; b < p.seqs.seqs; b += threads)
-    sum += paged_seq<ROWS, KEYS>(p, b).steps;
+    sum += steps_of(b);
 #pragma unroll
   for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (lane == 0) scratch[warp] = sum;
@@ -115,7 +116,7 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttnParams& p, int6
   for (int at = 0; at < p.seqs.seqs; at += threads) {
     const int b = at + mine;
     const int64_t own =
-        at == 0 ? first : (b < p.seqs.seqs ? paged_seq<ROWS, KEYS>(p, b).steps : 0);
+        at == 0 ? first : (b < p.seqs.seqs ? steps_of(b) : 0);
     int64_t upto = own;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -141,6 +142,11 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttnParams& p, int6
   r.seq = static_cast<int>(scratch[33]);
   r.base = scratch[34];
   return r;
+}
+
+// CTA whose range holds a step
+__device__ __forceinline__ int cta_of(int64_t step, int ctas, int64_t all) {
+  return static_cast<int>(((step + 1) * ctas - 1) / all);
 }
 
 // Walks the items of a CTA's range; every role of the kernel walks the same ones.
@@ -179,76 +185,181 @@ struct PagedWalk {
   }
   __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == s.tiles; }
   __device__ __forceinline__ int slot() const { return tile0 == 0 ? 1 : 0; }
-  // CTA whose range holds a step
-  __device__ __forceinline__ int cta_of(int64_t step) const {
-    return static_cast<int>(((step + 1) * ctas - 1) / all);
-  }
   // What the combine kernel has to know of the current part (slot 0).
   __device__ __forceinline__ PagedPart note() const {
-    return PagedPart{cta_of(item), cta_of(item + s.tiles - 1), s.first, s.count, head, block};
+    return PagedPart{cta_of(item, ctas, all), cta_of(item + s.tiles - 1, ctas, all), s.first,
+                     s.count, head, block};
   }
 };
 
-// Joins the parts of shared items.  Block (c, r): row r of the item that CTA c continues, if it
-// is the item's second part.  WARPS warps take every WARPS-th part each.
-template <typename T, int ROWS, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32)
+// Work of the tile kernel: blocks of TILES tiles of `tile_toks` tokens with all their heads, each
+// over the key tiles up to its last token's position (causal) or the sequence's end.
+template <int TILES, int KEYS>
+struct PagedTiles {
+  int first, count, len;
+  int blocks;
+  int64_t per_head;  // steps of one kv head
+
+  // Key tiles that the tokens before `tok_end` attend to; 1 if there is none.
+  __device__ __forceinline__ int tiles(const PagedAttnParams& p, int tok_end) const {
+    const int end = p.causal ? min(len, len - count + min(tok_end, count)) : len;
+    return max(1, (end + KEYS - 1) / KEYS);
+  }
+  __device__ __forceinline__ int block_tiles(const PagedAttnParams& p, int block) const {
+    return tiles(p, (block + 1) * TILES * p.tile_toks);
+  }
+  __device__ __forceinline__ PagedTiles() {}
+  __device__ __forceinline__ PagedTiles(const PagedAttnParams& p, int b) {
+    seq_rows(p.seqs, b, first, count);
+    len = seq_len(p.seqs, b);
+    blocks = (count + TILES * p.tile_toks - 1) / (TILES * p.tile_toks);
+    per_head = 0;
+    if (!p.causal) {
+      per_head = static_cast<int64_t>(blocks) * block_tiles(p, 0);
+    } else {
+      for (int m = 0; m < blocks; ++m) per_head += block_tiles(p, m);
+    }
+  }
+  __device__ __forceinline__ int64_t steps(const PagedAttnParams& p) const {
+    return per_head * p.heads_kv;
+  }
+};
+
+template <int TILES, int KEYS>
+struct PagedTileWalk {
+  const PagedAttnParams& p;
+  int64_t pos, hi, all;
+  int ctas;
+  int b;
+  PagedTiles<TILES, KEYS> s;
+  // the current part
+  int head, block;
+  int n;             // key tiles of the item
+  int tile0, tile1;  // those of the part
+  int64_t item;      // the item's first step
+
+  __device__ __forceinline__ PagedTileWalk(const PagedAttnParams& params, const PagedRange& r)
+      : p(params), pos(r.lo), hi(r.hi), all(r.all), ctas(r.ctas), b(r.seq) {
+    if (pos >= hi) return;
+    s = PagedTiles<TILES, KEYS>(p, b);
+    int64_t at = pos - r.base;
+    head = static_cast<int>(at / s.per_head);
+    at -= head * s.per_head;
+    block = 0;
+    for (n = s.block_tiles(p, 0); at >= n; n = s.block_tiles(p, ++block)) at -= n;
+    tile1 = static_cast<int>(at);
+  }
+  // (the walk stands before tile `tile1` of the current item)
+  __device__ __forceinline__ bool next() {
+    if (pos >= hi) return false;
+    if (tile1 == n) {
+      tile1 = 0;
+      if (++block == s.blocks) {
+        block = 0;
+        if (++head == p.heads_kv) {
+          head = 0;
+          do s = PagedTiles<TILES, KEYS>(p, ++b);
+          while (s.blocks == 0);
+        }
+      }
+      n = s.block_tiles(p, block);
+    }
+    tile0 = tile1;
+    const int64_t left = hi - pos;
+    tile1 = static_cast<int>(left < n - tile0 ? tile0 + left : n);
+    item = pos - tile0;
+    pos += tile1 - tile0;
+    return true;
+  }
+  // First token of tile i of the block, and the steps of this part that the tile takes part in.
+  __device__ __forceinline__ int tok0(int i) const { return (block * TILES + i) * p.tile_toks; }
+  __device__ __forceinline__ int steps(int i) const {
+    if (tok0(i) >= s.count) return 0;
+    return min(max(s.tiles(p, tok0(i) + p.tile_toks) - tile0, 0), tile1 - tile0);
+  }
+  // The part's last tile goes past the sequence's end.
+  __device__ __forceinline__ bool tail() const { return tile1 * KEYS > s.len; }
+  __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == n; }
+  __device__ __forceinline__ int slot() const { return tile0 == 0 ? 1 : 0; }
+  __device__ __forceinline__ PagedPart note() const {
+    return PagedPart{cta_of(item, ctas, all), cta_of(item + n - 1, ctas, all), s.first, s.count,
+                     head, block};
+  }
+};
+
+// Joins the parts of shared items.  An item has TILES tiles of TILE rows.  Block (c, y) takes rows
+// y * ROWS .. + ROWS - 1 of the item that CTA c + 1 continues, if that is the item's second part;
+// WARPS warps to a row, which take every WARPS-th part each.
+template <typename T, int TILE, int TILES, int WARPS, int ROWS>
+__global__ void __launch_bounds__(WARPS * ROWS * 32)
     paged_combine_kernel(const PagedAttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ float s_o[WARPS][256];
+  __shared__ float s_o[ROWS][WARPS][256];
   const int c = blockIdx.x + 1;
-  const int row = blockIdx.y;
   const PagedPart part = p.parts[c];
   if (part.first_cta != c - 1) return;
-  const int at = part.block * ROWS + row;
-  if (at >= part.count * p.group) return;
   const int n = part.last_cta - c + 2;  // slot 1 of CTA c - 1, then slots 0 of c .. last_cta
+  const int lane = threadIdx.x & 31;
+  const int mine = threadIdx.x / (WARPS * 32);  // row of the block
+  const int warp = (threadIdx.x >> 5) % WARPS;
+  const int row = blockIdx.y * ROWS + mine;
+  const int in_tile = row % TILE;
+  const int at = (part.block * TILES + row / TILE) * p.tile_live + in_tile;
+  const bool live = in_tile < p.tile_live && at < part.count * p.group;
   auto slot_row = [&](int i) -> int64_t {
     const int64_t slot = i == 0 ? static_cast<int64_t>(c - 1) * 2 + 1
                                 : static_cast<int64_t>(c - 1 + i) * 2;
-    return slot * ROWS + row;
+    return slot * (TILE * TILES) + row;
   };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_lse[slot_row(i)]);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  const float base = top == -INFINITY ? 0.f : top;  // no part has a key: all weights are 0
-  float sum = 0.f;
-  for (int i = lane; i < n; i += 32) sum += exp2f(p.part_lse[slot_row(i)] - base);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-
-  // each lane owns up to 8 values of the row
   const int D = p.head_dim;
-  float acc[8];
+  float acc[8];  // columns 32 k + lane
 #pragma unroll
   for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-#pragma unroll 4
-  for (int i = warp; i < n; i += WARPS) {
-    const int64_t r = slot_row(i);
-    const float w = exp2f(p.part_lse[r] - base) * inv;
+  float top = -INFINITY, sum = 0.f;
+  if (live) {
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_lse[slot_row(i)]);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int d = k * 32 + lane;
-      if (k * 32 < D && d < D) acc[k] += w * p.part_o[r * D + d];
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float base = top == -INFINITY ? 0.f : top;  // no part has a key: all weights are 0
+    for (int i = lane; i < n; i += 32) sum += exp2f(p.part_lse[slot_row(i)] - base);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 4
+    for (int i = warp; i < n; i += WARPS) {
+      const int64_t r = slot_row(i);
+      const float w = exp2f(p.part_lse[r] - base) * inv;
+      if (w == 0.f) continue;  // a part without keys for the row may have left no values
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int d = k * 32 + lane;
+        if (k * 32 < D && d < D) acc[k] += w * p.part_o[r * D + d];
+      }
     }
   }
+  if (WARPS > 1) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (k * 32 + lane < D) s_o[warp][k * 32 + lane] = acc[k];
-  __syncthreads();
+    for (int k = 0; k < 8; ++k)
+      if (k * 32 + lane < D) s_o[mine][warp][k * 32 + lane] = acc[k];
+    __syncthreads();
+  }
+  if (!live) return;
   const int64_t tok = part.first_row + at / p.group;
   const int64_t head = part.head_kv * p.group + at % p.group;
   T* out = static_cast<T*>(p.o) + tok * p.o_stride[0] + head * p.o_stride[1];
-  for (int d = threadIdx.x; d < D; d += WARPS * 32) {
-    float v = 0.f;
+  if (WARPS > 1) {
+    for (int d = warp * 32 + lane; d < D; d += WARPS * 32) {
+      float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) v += s_o[w][d];
-    out[d] = static_cast<T>(v);
+      for (int w = 0; w < WARPS; ++w) v += s_o[mine][w][d];
+      out[d] = static_cast<T>(v);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k * 32 + lane < D) out[k * 32 + lane] = static_cast<T>(acc[k]);
   }
-  if (threadIdx.x == 0)
+  if (warp == 0 && lane == 0)
     p.lse[tok * p.heads_kv * p.group + head] = (top + log2f(sum)) * kLn2;
 }
 

@@ -15,16 +15,20 @@ struct PagedInfo {
 };
 
 struct PagedPlan {
-  CUtensorMap tmK, tmV;
+  CUtensorMap tmQ, tmK, tmV;  // tmQ: tile kernel
   PagedAttnParams params;
   bool half;  // q and the output are fp16 (else bf16)
   bool fp8;
-  int mt;     // 16-row tiles of a block (1 or 2)
+  int mt;     // row kernel: 16-row tiles of a block (1 or 2)
   int grid;
   cudaStream_t stream;
 };
 
-PagedInfo rows_info(int head_dim, bool fp8, int mt);
+int launch_tile_d16(const PagedPlan& plan);
+int launch_tile_d32(const PagedPlan& plan);
+int launch_tile_d64(const PagedPlan& plan);
+int launch_tile_d128(const PagedPlan& plan);
+int launch_tile_d256(const PagedPlan& plan);
 int launch_rows_d16(const PagedPlan& plan);
 int launch_rows_d32(const PagedPlan& plan);
 int launch_rows_d64(const PagedPlan& plan);

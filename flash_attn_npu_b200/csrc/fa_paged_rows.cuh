@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, MT>::THREADS, 1)
     fence_mbar_init();
     p.parts[blockIdx.x].first_cta = -2;
   }
-  const PagedRange range = paged_range<G::ROWS, KEYS>(p, s_scratch);
+  const PagedRange range = paged_range(
+      p, s_scratch, [&](int b) { return paged_seq<G::ROWS, KEYS>(p, b).steps; });
   __syncthreads();
   PagedWalk<G::ROWS, KEYS> w(p, range);
   int* const status = p.seqs.status;

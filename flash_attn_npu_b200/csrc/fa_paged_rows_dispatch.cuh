@@ -41,7 +41,7 @@ int launch_rows(const PagedPlan& plan) {
   const int64_t most = static_cast<int64_t>(plan.params.seqs.total) * plan.params.group;
   const unsigned rows = static_cast<unsigned>(most < G::ROWS ? most : G::ROWS);
   constexpr int kWarps = 4;
-  return launch_dependent(paged_combine_kernel<T, G::ROWS, kWarps>, dim3(plan.grid - 1, rows),
+  return launch_dependent(paged_combine_kernel<T, G::ROWS, 1, kWarps, 1>, dim3(plan.grid - 1, rows),
                           kWarps * 32, plan.stream, plan.params);
 }
 

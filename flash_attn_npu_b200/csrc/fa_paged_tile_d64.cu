@@ -1,0 +1,7 @@
+// Paged tile kernel for head_dim = 64 (see fa_paged_tile_dispatch.cuh).
+#define FA_HEAD_DIM 64
+#include "fa_paged_tile_dispatch.cuh"
+
+namespace fa {
+int launch_tile_d64(const PagedPlan& plan) { return launch_any(plan); }
+}  // namespace fa

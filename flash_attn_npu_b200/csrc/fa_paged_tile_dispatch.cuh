@@ -1,0 +1,50 @@
+// Instantiations of the paged tile kernel for one head dimension: included with FA_HEAD_DIM defined
+// by fa_paged_tile_d*.cu.  q fp16 / bf16, cache of the same type or float8.
+#pragma once
+
+#include "fa_paged_launch.h"
+#include "fa_paged_tile.cuh"
+
+#ifndef FA_HEAD_DIM
+#error "define FA_HEAD_DIM"
+#endif
+
+namespace fa {
+namespace {
+
+template <typename T, bool FP8>
+int launch_tile(const PagedPlan& plan) {
+  using G = TileGeo<FA_HEAD_DIM, FP8>;
+  auto kernel = paged_tile_kernel<T, FA_HEAD_DIM, FP8>;
+  // setmaxnreg redistributes exactly the launch allocation: refuse a build that differs
+  static int regs_ok = 0;  // 0 unknown, 1 ok, -1 mismatch
+  if (regs_ok == 0) {
+    cudaFuncAttributes attr{};
+    regs_ok = cudaFuncGetAttributes(&attr, kernel) == cudaSuccess && attr.numRegs == G::REG_LAUNCH
+                  ? 1
+                  : -1;
+    (void)cudaGetLastError();
+  }
+  if (regs_ok != 1) return -7;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) !=
+      cudaSuccess) {
+    (void)cudaGetLastError();
+    return -7;
+  }
+  kernel<<<plan.grid, G::THREADS, G::SMEM, plan.stream>>>(plan.tmQ, plan.tmK, plan.tmV, plan.params);
+  if (cudaGetLastError() != cudaSuccess) return -7;
+  if (plan.grid == 1) return 0;  // no shared item
+  constexpr int kRows = 8;  // a warp each: shared items mostly have two or three parts
+  return launch_dependent(paged_combine_kernel<T, 128, G::TILES, 1, kRows>,
+                          dim3(plan.grid - 1, 128 * G::TILES / kRows), kRows * 32, plan.stream,
+                          plan.params);
+}
+
+int launch_any(const PagedPlan& plan) {
+  if (plan.fp8)
+    return plan.half ? launch_tile<__half, true>(plan) : launch_tile<__nv_bfloat16, true>(plan);
+  return plan.half ? launch_tile<__half, false>(plan) : launch_tile<__nv_bfloat16, false>(plan);
+}
+
+}  // namespace
+}  // namespace fa

@@ -1,14 +1,17 @@
 """Plain 64-bit forms of the paged cache operators, and inputs for their tests.
 
 Tolerances count roundings.  u = eps / 2 of the output's type is the largest relative error of one
-rounding to it.  The kernels round each probability to 16 bits (fp16 for fp16 and float8 caches,
-else bf16: u_p) and the output once:
+rounding to it.  The kernels round each probability to 16 bits and the output once.  A probability is
+rounded to the type of the products (u_p): that is q's, but fp16 where at most 32 query rows a kv
+head meet a float8 cache, whose codes that kernel takes as fp16.  So
+
     |out - ref| <= (u_p + e) A + u |ref| + tiny,    A = sum_j p_j |v_j|
 where e bounds the relative error of a probability from fp32 arithmetic: a logit is a sum of D
 products accumulated in fp32, off by at most (D + 8) 2^-23 sum_d |q_d k_d| (truncating adders
 counted as a whole step), the exponential and the scalings by a few 2^-22; the same bound, taken
-twice, covers the sum l as well.  fp16 probabilities carry a factor of at least 2^10, so what falls
-below fp16's subnormal step loses at most 2^-35 of the row's largest: tiny = keys 2^-35 max |v|.
+twice, covers the sum l as well.  fp16 probabilities carry a factor of at least 2^7, so what falls
+below fp16's subnormal step of 2^-24 loses at most 2^-32 of the row's largest: tiny = keys 2^-32
+max |v|.
 Without the factor u_p the same e bounds the logsumexp's absolute error, next to its own rounding.
 """
 from __future__ import annotations
@@ -48,7 +51,7 @@ def gather(x, table, b, n):
     return x[pages].transpose(1, 2).flatten(0, 1)[:n]
 
 
-def attention(q, k_cache, v_cache, table, offsets, lens, causal, scale, k_scale=None, v_scale=None):
+def attention(q, k_cache, v_cache, table, offsets, lens, causal, scale, k_scale=None, v_scale=None, max_q_len=None):
     """(out, lse, tolerance of out, tolerance of lse) in 64 bits; NaN where no sequence has a row."""
     dev = q.device
     total, hq, d = q.shape
@@ -58,7 +61,8 @@ def attention(q, k_cache, v_cache, table, offsets, lens, causal, scale, k_scale=
     lse = torch.full((total, hq), float("nan"), dtype=torch.float64, device=dev)
     tol, tol_lse = torch.zeros_like(out), torch.zeros_like(lse)
     u = torch.finfo(q.dtype).eps / 2
-    half = q.dtype == torch.float16 or k_cache.dtype == FP8
+    few = min(max_q_len or total, total) * group <= 32 or scale <= 0 or group > 128
+    half = q.dtype == torch.float16 or (k_cache.dtype == FP8 and few)
     u_p = torch.finfo(torch.float16 if half else torch.bfloat16).eps / 2
     offsets, lens = offsets.tolist(), lens.tolist()
     for b in range(len(lens)):
@@ -84,7 +88,7 @@ def attention(q, k_cache, v_cache, table, offsets, lens, causal, scale, k_scale=
             o = torch.einsum("hgij,jhd->hgid", p, v)
             e = (d + 8) * 2.0 ** -23 * size.amax(-1) + 2.0 ** -20
             big = torch.einsum("hgij,jhd->hgid", p, v.abs())
-            t = (u_p + 2 * e)[..., None] * big + u * o.abs() + n * 2.0 ** -35 * v.abs().amax()
+            t = (u_p + 2 * e)[..., None] * big + u * o.abs() + n * 2.0 ** -32 * v.abs().amax()
             tl = e + 2.0 ** -22 * torch.where(torch.isfinite(m), m.abs(), torch.zeros_like(m))
         out[a:z] = o.permute(2, 0, 1, 3).reshape(count, hq, d)
         lse[a:z] = m.permute(2, 0, 1).reshape(count, hq)

@@ -24,7 +24,8 @@ def _check(b, causal=True, scale=None, max_q_len=None):
     out, lse = fam.paged_attention(b.q, b.k_cache, b.v_cache, *b.where, causal, scale, **b.scales,
                                    max_q_len=max_q_len, return_lse=True)
     ops.check_device_status(b.q.device)
-    want, want_lse, tol, tol_lse = ref.attention(b.q, b.k_cache, b.v_cache, *b.where, causal, scale, **b.scales)
+    want, want_lse, tol, tol_lse = ref.attention(b.q, b.k_cache, b.v_cache, *b.where, causal, scale, **b.scales,
+                                                 max_q_len=max_q_len)
     n = int(b.offsets[-1])
     assert torch.equal(torch.isfinite(lse[:n]), torch.isfinite(want_lse[:n]))
     over = (out.double() - want).abs()[:n] - tol[:n]
