@@ -187,7 +187,6 @@ def load() -> ctypes.CDLL:
         lib.fa_fwd_sm100_max_stages.restype = ctypes.c_int
         lib.fa_fwd_sm100_grid_size.argtypes = [ctypes.POINTER(FaFwdArgs)]
         lib.fa_fwd_sm100_grid_size.restype = ctypes.c_int64
-        # the paged calls take a block of bytes laid out as their structure (see paged.py)
         for name in ("fa_paged_write_sm100", "fa_paged_read_sm100", "fa_paged_attn_sm100"):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]

@@ -1,8 +1,9 @@
 """Build the sm_100a shared library `libfa_sm100.so` in-tree with nvcc.
 
-The library is a plain C-ABI shared object (see include/fa_fwd_sm100.h); it has no PyTorch
-dependency, so it is compiled directly with nvcc rather than through torch's extension
-machinery.  The five head-dimension translation units compile in parallel.
+The library is a plain C-ABI shared object (see include/fa_fwd_sm100.h and fa_paged_sm100.h); it
+has no PyTorch dependency, so it is compiled directly with nvcc rather than through torch's
+extension machinery.  The translation units compile in parallel.  `_paged_binding.so`, a small
+Python module that reads tensors for the paged calls, is compiled with the host compiler.
 
 Usage:  python -m flash_attn_npu_b200.build [--force] [--verbose]
 """
@@ -115,6 +116,45 @@ def _compile_one(nvcc: str, src: str, extra: list[str], verbose: bool,
     return obj
 
 
+# The Python binding of the paged calls: host code only, against torch's headers.
+BINDING_SOURCE = "paged_binding.cpp"
+BINDING_PATH = PKG_DIR / "_paged_binding.so"
+
+
+def _binding_command() -> list[str]:
+    import sysconfig
+
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    nvcc = Path(nvcc_path()).resolve()
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-I", str(root / "include"), "-isystem", str(nvcc.parent.parent / "include"),
+            "-I", sysconfig.get_paths()["include"], str(CSRC / BINDING_SOURCE),
+            "-L", str(root / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+            "-lc10_cuda"]
+
+
+def build_binding(force: bool = False) -> Path:
+    """Compile `_paged_binding.so` next to this file."""
+    import torch
+    h = hashlib.sha256((torch.__version__ + sys.version).encode())
+    for p in [CSRC / BINDING_SOURCE, *sorted(INCLUDE.glob("*.h"))]:
+        h.update(p.read_bytes())
+    digest = h.hexdigest()
+    stamp = _stamp_path(BINDING_PATH)
+    if (not force and BINDING_PATH.exists() and stamp.exists()
+            and stamp.read_text().strip() == digest):
+        return BINDING_PATH
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    res = subprocess.run([*_binding_command(), "-o", str(tmp)], capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compiling {BINDING_SOURCE} failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING_PATH)
+    stamp.write_text(digest + "\n")
+    return BINDING_PATH
+
+
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None,
           variant: str | None = None) -> Path:
     """Compile every CUDA source for sm_100a and link `libfa_sm100.so` next to this file
@@ -150,6 +190,8 @@ def main(argv: list[str] | None = None) -> int:
                     help="build a test variant of the library instead of the product")
     args = ap.parse_args(argv)
     path = build(force=args.force, verbose=args.verbose, variant=args.variant)
+    if args.variant is None:
+        build_binding(force=args.force)
     print(path)
     return 0
 

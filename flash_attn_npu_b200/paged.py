@@ -27,7 +27,6 @@ the cache or the table are never followed: the call reports them through the dev
 from __future__ import annotations
 
 import ctypes
-import struct
 
 import torch
 
@@ -141,81 +140,67 @@ def _aligned(t) -> bool:
     return t.device.type == "meta" or t.data_ptr() % 16 == 0
 
 
-def _strides(t) -> tuple:
-    """Strides of the outer dimensions, a contiguous one where a dimension of size 1 has any."""
-    out, inner = [], t.shape[-1]
-    for d in range(t.ndim - 2, -1, -1):
-        st = t.stride(d) if t.shape[d] > 1 else inner
-        out.append(st)
-        inner = max(inner, st * t.shape[d])
-    return tuple(reversed(out))
-
-
 def _require_cuda(t) -> None:
     if t.device.type != "cuda":
         raise ValueError(f"paged calls take CUDA tensors on an sm_100 device (got {t.device})")
 
 
 # ------------------------------------------------------------------------------------ launching
-# A call's argument block has its addresses first (PREFIX) and its layout behind them.  The layout
-# part of a call that was validated and launched once is kept under the call's shapes, strides,
-# types and options, so a call of the same layout only fills in its addresses: the full checks cost
-# several times what a decoding step's kernel takes.  Nothing is kept by address.
-_FAST: dict = {}
-_FAST_LIMIT = 256
-_ATTN_PTRS = struct.Struct("@12Q")  # q, o, lse, workspace, status, k, v, scales, table, offsets, lens
-_COPY_PTRS = struct.Struct("@10Q")  # k, v, status, k, v, scales, table, offsets, lens
-_PTRS_AT = 8                        # behind struct_size
+# A call goes to the native binding first, which does the checks above on the tensors themselves.
+# What it hands back (None) is looked at here: refused with a reason, or prepared and called again.
+_binding = None
+_PREPARED: set[int] = set()  # devices whose status word the binding knows
 
 
-def _remember(key, value) -> None:
-    if len(_FAST) >= _FAST_LIMIT:
-        _FAST.pop(next(iter(_FAST)))
-    _FAST[key] = value
+def _native_binding():
+    global _binding
+    if _binding is None:
+        try:
+            from . import _paged_binding
+        except ImportError as exc:
+            raise RuntimeError(f"the paged calls need {exc.name or '_paged_binding'}; build it with "
+                               "`python -m flash_attn_npu_b200.build`") from None
+        lib = _native.load()
+        _paged_binding.setup(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+            lib.fa_paged_attn_sm100, lib.fa_paged_workspace_bytes, lib.fa_paged_write_sm100,
+            lib.fa_paged_read_sm100)))
+        _binding = _paged_binding
+    return _binding
 
 
-def _fill_cache(c, k_cache, v_cache, page_table, k_scale, v_scale) -> None:
-    for name, t in (("k_stride", k_cache), ("v_stride", v_cache)):
-        getattr(c, name)[:] = _strides(t)
-    if k_scale is not None:
-        for name, t in (("k_scale_stride", k_scale), ("v_scale_stride", v_scale)):
-            getattr(c, name)[:] = _strides(t)
-    c.num_pages, c.heads_kv, c.page_size, c.head_dim = k_cache.shape
-    c.seqs, c.table_cols = page_table.shape
-    c.table_stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
-    c.dtype = _CACHE_CODES[k_cache.dtype]
-
-
-def _status_of(device):
-    """The device's status word, or None in a capture that comes before its first launch (an
-    allocation there would belong to the graph's private pool)."""
-    if (ops._device_index(device) in ops._STATUS_WORDS
-            or not torch.cuda.is_current_stream_capturing()):
-        return ops.device_status_word(device)
-    return None
-
-
-def _launch(fn, block, index) -> None:
-    """Launch on the current stream of device `index`, whatever device is current."""
-    buf = (ctypes.c_char * len(block)).from_buffer(block)
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(buf, torch._C._cuda_getCurrentRawStream(index))
+def _call(name, device, *args):
+    """Call the binding once its device is prepared."""
+    binding = _native_binding()
+    index = ops._device_index(device)
+    if index in _PREPARED:
+        res = getattr(binding, name)(*args)
+    elif index in ops._STATUS_WORDS or not torch.cuda.is_current_stream_capturing():
+        binding.set_status(index, ops.device_status_word(device).data_ptr(), True)
+        _PREPARED.add(index)
+        res = getattr(binding, name)(*args)
     else:
-        with torch.cuda.device(index):
-            rc = fn(buf, torch._C._cuda_getCurrentRawStream(index))
-    if rc != _native.FA_OK:
-        exc = _native.NativeError(rc, _native.status_string(rc))
-        if rc in (_native.FA_ERR_UNSUPPORTED_HEAD_DIM, _native.FA_ERR_UNSUPPORTED_DTYPE,
-                  _native.FA_ERR_INVALID_ARG, _native.FA_ERR_MISALIGNED):
-            raise ValueError(str(exc)) from None
+        # a capture before the device's first launch gets no word: an allocation here would belong
+        # to the graph's private pool
+        binding.set_status(index, 0, True)
+        try:
+            res = getattr(binding, name)(*args)
+        finally:
+            binding.set_status(index, 0, False)
+    if res is None:
+        raise ValueError("paged calls take plain CUDA tensors")
+    return res
+
+
+def _check(res, device) -> None:
+    """Raise for a status code of the library; look at the device's word if that is asked for."""
+    if type(res) is int and res != _native.FA_OK:
+        exc = _native.NativeError(res, _native.status_string(res))
+        if res in (_native.FA_ERR_UNSUPPORTED_HEAD_DIM, _native.FA_ERR_UNSUPPORTED_DTYPE,
+                   _native.FA_ERR_INVALID_ARG, _native.FA_ERR_MISALIGNED):
+            raise ValueError(str(exc))
         raise exc
     if ops._CHECK_EVERY_CALL:
-        ops.check_device_status(torch.device("cuda", index))
-
-
-def _layout(*tensors):
-    return tuple((t.shape, t.stride(), t.dtype, t.device) if t is not None else None
-                 for t in tensors)
+        ops.check_device_status(device)
 
 
 def _rows_like(t):
@@ -233,97 +218,42 @@ def attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scal
     bound of a sequence's new tokens that the kernel choice goes by (default: total).  `out` and
     `lse` may be given; rows that belong to no sequence are not written.
     """
-    key = ("attention", _layout(q, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale),
-           bool(causal), float(sm_scale), max_q_len)
-    ent = _FAST.get(key)
-    if ent is None:
+    res = None
+    if _binding is not None:
+        res = _binding.attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scale,
+                                 k_scale, v_scale, max_q_len, out, lse)
+    if res is None:
         validate_attention(q, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale,
                            max_q_len)
         _require_cuda(q)
-    q = _rows_like(q)
-    if out is None:
-        out = torch.empty_like(q)
-        if not _aligned(out):
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not _aligned(out):
-        raise ValueError("out must match q in shape, dtype and device, with a unit inner stride and "
-                         "16-byte aligned strides")
-    if lse is None:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    elif (lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != q.device
-          or not lse.is_contiguous()):
-        raise ValueError("lse must be a contiguous float32 tensor [total, heads_q]")
-    if q.shape[0] == 0 or page_table.shape[0] == 0:
-        return out, lse
-    if ent is None:
-        args = _native.FaPagedAttnArgs(struct_size=ctypes.sizeof(_native.FaPagedAttnArgs))
-        _fill_cache(args.cache, k_cache, v_cache, page_table, k_scale, v_scale)
-        args.total, args.heads_q = q.shape[:2]
-        args.max_q_len = 0 if max_q_len is None else int(max_q_len)
-        args.dtype, args.causal = _ROW_CODES[q.dtype], int(bool(causal))
-        args.sm_scale = float(sm_scale)
-        ent = (args, ops._device_index(q.device))
-    args, index = ent
-    block = bytearray(args)
-    _STRIDES.pack_into(block, _Q_STRIDE_AT, *_strides(q), *_strides(out))
-    return _attention_launch(key, args, index, block, q, k_cache, v_cache, page_table, offsets,
-                             kv_lens, k_scale, v_scale, out, lse)
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype
+                                or out.device != q.device or not _aligned(out)):
+            raise ValueError("out must match q in shape, dtype and device, with a unit inner stride "
+                             "and 16-byte aligned strides")
+        if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32
+                                or lse.device != q.device or not lse.is_contiguous()):
+            raise ValueError("lse must be a contiguous float32 tensor [total, heads_q]")
+        res = _call("attention", q.device, _rows_like(q), k_cache, v_cache, page_table, offsets,
+                    kv_lens, bool(causal), float(sm_scale), k_scale, v_scale, max_q_len, out, lse)
+    if type(res) is int or ops._CHECK_EVERY_CALL:
+        _check(res, q.device)
+    return res
 
 
-_STRIDES = struct.Struct("@4q")
-_Q_STRIDE_AT = _native.FaPagedAttnArgs.q_stride.offset
-_COPY_STRIDE_AT = _native.FaPagedCopyArgs.k_stride.offset
-
-
-def _attention_launch(key, args, index, block, q, k_cache, v_cache, page_table, offsets, kv_lens,
-                      k_scale, v_scale, out, lse):
-    lib = _native.load()
-    if args.workspace_bytes == 0:
-        with torch.cuda.device(index):
-            need = lib.fa_paged_workspace_bytes(ctypes.byref(args))
-        if need < 0:
-            raise ValueError(_native.status_string(need))
-        args.workspace_bytes = need
-        block[_WS_AT:_WS_AT + 8] = struct.pack("@q", need)
-    workspace = torch.empty(args.workspace_bytes, dtype=torch.uint8, device=q.device)
-    status = _status_of(q.device)
-    _ATTN_PTRS.pack_into(
-        block, _PTRS_AT, q.data_ptr(), out.data_ptr(), lse.data_ptr(), workspace.data_ptr(),
-        status.data_ptr() if status is not None else 0, k_cache.data_ptr(), v_cache.data_ptr(),
-        k_scale.data_ptr() if k_scale is not None else 0,
-        v_scale.data_ptr() if v_scale is not None else 0, page_table.data_ptr(),
-        offsets.data_ptr(), kv_lens.data_ptr())
-    _launch(lib.fa_paged_attn_sm100, block, index)
-    if key not in _FAST:
-        _remember(key, (args, index))
-    return out, lse
-
-
-_WS_AT = _native.FaPagedAttnArgs.workspace_bytes.offset
-
-
-def _copy(fn_name, k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale, key):
-    if k.shape[0] == 0 or page_table.shape[0] == 0:
-        return
-    ent = _FAST.get(key)
-    if ent is None:
-        args = _native.FaPagedCopyArgs(struct_size=ctypes.sizeof(_native.FaPagedCopyArgs))
-        _fill_cache(args.cache, k_cache, v_cache, page_table, k_scale, v_scale)
-        args.total, args.dtype = k.shape[0], _ROW_CODES[k.dtype]
-        ent = (args, ops._device_index(k.device))
-    args, index = ent
-    block = bytearray(args)
-    _STRIDES.pack_into(block, _COPY_STRIDE_AT, *_strides(k), *_strides(v))
-    status = _status_of(k.device)
-    _COPY_PTRS.pack_into(
-        block, _PTRS_AT, k.data_ptr(), v.data_ptr(),
-        status.data_ptr() if status is not None else 0, k_cache.data_ptr(), v_cache.data_ptr(),
-        k_scale.data_ptr() if k_scale is not None else 0,
-        v_scale.data_ptr() if v_scale is not None else 0, page_table.data_ptr(),
-        offsets.data_ptr(), kv_lens.data_ptr())
-    _launch(getattr(_native.load(), fn_name), block, index)
-    if key not in _FAST:
-        _remember(key, ent)
+def _copy(write, k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale) -> None:
+    res = None
+    if _binding is not None:
+        res = _binding.copy(write, k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale,
+                            v_scale)
+    if res is None:
+        validate_copy(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale)
+        _require_cuda(k)
+        if write:
+            k, v = _rows_like(k), _rows_like(v)
+        res = _call("copy", k.device, write, k, v, k_cache, v_cache, page_table, offsets, kv_lens,
+                    k_scale, v_scale)
+    if res != _native.FA_OK or ops._CHECK_EVERY_CALL:
+        _check(res, k.device)
 
 
 def write(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale=None, v_scale=None) -> None:
@@ -333,12 +263,7 @@ def write(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale=None, v_
     row's largest finite magnitude is at most 448 * 2^e (1 for a row of zeros), code =
     round_e4m3(x / scale); infinities and NaN become NaN.
     """
-    key = ("write", _layout(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale))
-    if key not in _FAST:
-        validate_copy(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale)
-        _require_cuda(k)
-    _copy("fa_paged_write_sm100", _rows_like(k), _rows_like(v), k_cache, v_cache, page_table,
-          offsets, kv_lens, k_scale, v_scale, key)
+    _copy(True, k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale)
 
 
 def read(k_cache, v_cache, page_table, offsets, kv_lens, total, k_scale=None, v_scale=None,
@@ -347,24 +272,20 @@ def read(k_cache, v_cache, page_table, offsets, kv_lens, total, k_scale=None, v_
     position kv_lens[b] - (offsets[b + 1] - offsets[b]) + i.
 
     `total` is offsets[-1], or more (rows behind it are not written).  Rows of a float8 cache are
-    dequantised and rounded to `dtype` (float16 or bfloat16, default bfloat16); others keep the cache's
-    type.  `out`: a pair of tensors to fill.
+    dequantised and rounded to `dtype` (float16 or bfloat16, default bfloat16); others keep the
+    cache's type.  `out`: a pair of tensors to fill.
     """
     if out is None:
         if dtype is None:
             dtype = torch.bfloat16 if k_cache.dtype == FP8 else k_cache.dtype
         shape = (int(total), k_cache.shape[1], k_cache.shape[-1])
-        k, v = (torch.empty(shape, dtype=dtype, device=k_cache.device) for _ in range(2))
+        k = torch.empty(shape, dtype=dtype, device=k_cache.device)
+        v = torch.empty_like(k)
     else:
         k, v = out
         if k.shape[0] != total or (dtype is not None and k.dtype != dtype):
             raise ValueError("out must have `total` rows of the given dtype")
         if not (_aligned(k) and _aligned(v)):
             raise ValueError("out needs a unit inner stride and 16-byte aligned strides")
-    key = ("read", _layout(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale))
-    if key not in _FAST:
-        validate_copy(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale)
-        _require_cuda(k)
-    _copy("fa_paged_read_sm100", k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale,
-          v_scale, key)
+    _copy(False, k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale)
     return k, v

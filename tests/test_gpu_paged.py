@@ -6,10 +6,15 @@ import torch
 
 import flash_attention_forward as fam
 import paged_ref as ref
-from flash_attn_npu_b200 import ops
+from flash_attn_npu_b200 import build, ops
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def binding(native_lib):
+    build.build_binding()
 
 
 def _same(a, b):

@@ -8,9 +8,14 @@ import torch
 
 import flash_attention_forward as fam
 import paged_ref as ref
-from flash_attn_npu_b200 import _native, paged
+from flash_attn_npu_b200 import _native, build
 
 BF16, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def binding(native_lib):
+    build.build_binding()
 
 
 def _batch(**kw):
@@ -178,15 +183,3 @@ def test_native_checks(native_lib):
     assert lib.fa_paged_workspace_bytes(ctypes.byref(a)) > 0
     a.heads_q = 3
     assert lib.fa_paged_workspace_bytes(ctypes.byref(a)) == inv
-
-
-def test_argument_blocks_match_the_header():
-    """The addresses of a call lie together behind the size, in the order in which paged.py packs them."""
-    a, c, k = _native.FaPagedAttnArgs, _native.FaPagedCache, _native.FaPagedCopyArgs
-    tail = [c.k, c.v, c.k_scale, c.v_scale, c.page_table, c.offsets, c.kv_lens]
-    order = [a.q.offset, a.o.offset, a.lse.offset, a.workspace.offset, a.dev_status.offset]
-    order += [a.cache.offset + x.offset for x in tail]
-    assert order == [paged._PTRS_AT + 8 * i for i in range(12)]
-    order = [k.k.offset, k.v.offset, k.dev_status.offset] + [k.cache.offset + x.offset for x in tail]
-    assert order == [paged._PTRS_AT + 8 * i for i in range(10)]
-    assert a.o_stride.offset == a.q_stride.offset + 16 and k.v_stride.offset == k.k_stride.offset + 16
