@@ -287,6 +287,26 @@ struct PagedTileWalk {
   }
 };
 
+// Several warps issue the copies of one stage.  When a wait of theirs gives up, they stop at the
+// same stage, so that every phase that one of them has begun completes and can be drained: each
+// comes here once, giving up or done, and those behind catch up with the farthest (which has seen
+// the stages in between free).
+template <int WARPS>
+struct ProducersMeet {
+  int* issued;   // shared, one word per warp
+  uint32_t bar;  // named barrier
+  int limit = INT_MAX;
+  bool met = false;
+  __device__ __forceinline__ void operator()(int warp, int count) {
+    if (met) return;
+    met = true;
+    if ((threadIdx.x & 31) == 0) issued[warp] = count;
+    named_barrier_sync(bar, WARPS * 32);
+    limit = 0;
+    for (int w = 0; w < WARPS; ++w) limit = max(limit, issued[w]);
+  }
+};
+
 // Joins the parts of shared items.  An item has TILES tiles of TILE rows.  Block (c, y) takes rows
 // y * ROWS .. + ROWS - 1 of the item that CTA c + 1 continues, if that is the item's second part;
 // WARPS warps to a row, which take every WARPS-th part each.

@@ -44,13 +44,14 @@ struct RowsGeo {
   static constexpr int GROUP_COLS = D < 32 ? D : 32;   // columns joined at a time
   static constexpr int JOIN_PITCH = GROUP_COLS + 4;
   static constexpr int JOIN = NW * 16 * JOIN_PITCH * 4;
-  // With 8 consumer warps of 128 columns or more, a fourth of the registers is taken from the
-  // producer's warpgroup (three of its warps only give theirs away): launched at 168 a thread,
-  // 256 * 224 + 128 * 40 <= 384 * 168.
+  // With 8 consumer warps of 128 columns or more the producers give most of their registers away:
+  // launched at 168 a thread, 256 * 224 + 128 * 40 <= 384 * 168.
   static constexpr bool SPLIT = NW == 8 && D >= 128;
   static constexpr int REG_LAUNCH = 168, REG_CONSUMER = 224, REG_PRODUCER = 40;
   static_assert(256 * REG_CONSUMER + 128 * REG_PRODUCER <= 384 * REG_LAUNCH, "register split");
-  static constexpr int THREADS = SPLIT ? 384 : NW * 32 + 32;
+  static constexpr int NP = 4;  // producer warps
+  static constexpr int THREADS = (NW + NP) * 32;
+  static constexpr int COPIES = 2 * NSPAN + (FP8 ? 2 : 0);  // of one page
   static constexpr int kMostStages = 8;
   static constexpr int FIXED = 1024 + JOIN;
   static constexpr int STAGES = (222 * 1024 - FIXED) / STAGE < kMostStages
@@ -136,6 +137,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, MT>::THREADS, 1)
   __shared__ int64_t s_scratch[40];
   __shared__ float s_m[MT][NW][16], s_l[MT][NW][16];
   __shared__ volatile uint32_t s_abort;
+  __shared__ int s_issued[G::NP];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   float* s_join = reinterpret_cast<float*>(smem + G::STAGES * G::STAGE);
@@ -160,57 +162,70 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, MT>::THREADS, 1)
 
   if (warp >= NW) {
     if constexpr (G::SPLIT) setmaxnreg_dec<G::REG_PRODUCER>();
-    if (warp > NW) return;
-    // ------------------------------------------------------------------------ producer
+    // ------------------------------------------------------------------------ producers
+    // Every copy of a tile has a lane of its own, spread over the warps: a warp issues the copies
+    // of its lanes one after the other, one in 65 cycles (measured), and pages of 8 or 16 tokens
+    // make up to 64 copies a tile.
+    const int pw = warp - NW;
+    const int op = lane * G::NP + pw;
     const int box = min(1 << p.seqs.page_log2, KEYS);  // rows of one copy
     const int boxes = KEYS / box;
+    const int my_box = op / G::COPIES, kind = op % G::COPIES;
+    const bool is_scale = kind >= 2 * G::NSPAN;
+    const bool is_v = is_scale ? kind == 2 * G::NSPAN + 1 : kind >= G::NSPAN;
+    const int span = is_v ? kind - G::NSPAN : kind;
+    const CUtensorMap* const map = is_v ? &tmV : &tmK;
+    const float* const scales = is_v ? p.v_scale : p.k_scale;
+    const int64_t* const scale_stride = is_v ? p.v_scale_stride : p.k_scale_stride;
+    const uint32_t to = is_scale ? 2 * G::TILE + (is_v ? G::SCALES : 0) + my_box * box * 4
+                                 : (is_v ? G::TILE : 0) + span * KEYS * G::SPAN + my_box * box * G::SPAN;
     int slot = 0, issued = 0;
     uint32_t ph = 0;
     bool ok = true;
-    while (ok && w.next()) {
-      if (lane == 0) {
-        const int n = __ldg(p.seqs.kv_lens + w.b);
-        if (n != w.s.len || w.s.count != __ldg(p.seqs.offsets + w.b + 1) - __ldg(p.seqs.offsets + w.b))
+    ProducersMeet<G::NP> meet{s_issued, 2};
+    while (issued < meet.limit && w.next()) {
+      if (pw == 0 && lane == 0) {
+        if (__ldg(p.seqs.kv_lens + w.b) != w.s.len ||
+            __ldg(p.seqs.offsets + w.b + 1) - __ldg(p.seqs.offsets + w.b) != w.s.count)
           report(status, kStatusPageTable);
       }
+      // the page of this lane's copy for a tile; looked up one tile ahead
+      auto look_up = [&](int t) -> int {
+        const int key = t * KEYS + my_box * box;
+        if (my_box >= boxes || t >= w.tile1 || key >= w.s.len) return -1;
+        const int page = page_of(p.seqs, w.b, key);
+        if (page < 0) report(status, kStatusPageTable);
+        return max(page, 0);
+      };
+      int next_page = look_up(w.tile0);
       for (int t = w.tile0; t < w.tile1; ++t) {
         const int key0 = t * KEYS;
-        const int live = min(boxes, (w.s.len - key0 + box - 1) / box);  // boxes with a key
-        // the pages are looked up while the slot is still being read
-        int page = 0;
-        if (lane < live) {
-          page = page_of(p.seqs, w.b, key0 + lane * box);
-          if (page < 0) {
-            report(status, kStatusPageTable);
-            page = 0;
-          }
+        const int page = next_page;
+        next_page = look_up(t + 1);
+        if (ok) {
+          ok = wait_bar_flag(&s_abort, smem_u32(&s_empty[slot]), ph ^ 1u, status);
+          ok = __all_sync(0xffffffffu, ok);
         }
-        ok = wait_bar_flag(&s_abort, smem_u32(&s_empty[slot]), ph ^ 1u, status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        if (!ok) {
+          meet(pw, issued);
+          if (issued >= meet.limit) break;
+        }
         const uint32_t bar = smem_u32(&s_full[slot]);
-        const uint32_t dst = smem_u32(smem + slot * G::STAGE);
-        if (lane == 0)
-          mbar_arrive_expect_tx(bar, live > 0 ? live * box * (2 * G::ROW_BYTES + (FP8 ? 8 : 0)) : 0);
-        __syncwarp();
-        if (lane < live) {
-          const int row = (key0 + lane * box) & ((1 << p.seqs.page_log2) - 1);
-#pragma unroll
-          for (int c = 0; c < G::NSPAN; ++c) {
-            const uint32_t at = dst + c * KEYS * G::SPAN + lane * box * G::SPAN;
-            const int col = c * (FP8 ? G::SPAN : G::SPAN / 2);
-            tma_load_4d(at, &tmK, bar, col, row, w.head, page);
-            tma_load_4d(at + G::TILE, &tmV, bar, col, row, w.head, page);
-          }
-          if (FP8) {
-            const uint32_t at = dst + 2 * G::TILE + lane * box * 4;
-            bulk_load(at, p.k_scale + page * p.k_scale_stride[0] + w.head * p.k_scale_stride[1] + row,
-                      box * 4, bar);
-            bulk_load(at + G::SCALES,
-                      p.v_scale + page * p.v_scale_stride[0] + w.head * p.v_scale_stride[1] + row,
-                      box * 4, bar);
-          }
+        // (the other warps' copies may land before this arrival: the phase waits for it)
+        if (pw == 0 && lane == 0) {
+          const int live = min(boxes, max(0, (w.s.len - key0 + box - 1) / box));  // with a key
+          mbar_arrive_expect_tx(bar, live * box * (2 * G::ROW_BYTES + (FP8 ? 8 : 0)));
         }
+        __syncwarp();
+        if (page >= 0) {
+          const uint32_t dst = smem_u32(smem + slot * G::STAGE) + to;
+          const int row = (key0 + my_box * box) & ((1 << p.seqs.page_log2) - 1);
+          if (FP8 && is_scale)
+            bulk_load(dst, scales + page * scale_stride[0] + w.head * scale_stride[1] + row, box * 4, bar);
+          else
+            tma_load_4d(dst, map, bar, span * (FP8 ? G::SPAN : G::SPAN / 2), row, w.head, page);
+        }
+        __syncwarp();
         ++issued;
         if (++slot == G::STAGES) {
           slot = 0;
@@ -218,6 +233,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, MT>::THREADS, 1)
         }
       }
     }
+    meet(pw, issued);
     // the copies issued last land before shared memory goes away
     for (int u = 0; u < min(issued, G::STAGES); ++u) {
       const int i = issued - 1 - u;

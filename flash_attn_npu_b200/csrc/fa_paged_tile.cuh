@@ -11,7 +11,7 @@
 // Warps (16):  0-3, 4-7  softmax of tile 0, 1 (thread r owns row r), rescaling and output
 //              8-11      16-bit cache: clean the sequence's end; float8: dequantise the tiles
 //              12, 14    MMA issuers of tile 0, 1 (they take turns); 12 also owns TMEM
-//              13        TMA producer; 15 idle
+//              13, 15    TMA producers
 //
 // Pages: the producer's lanes look a tile's pages up and each copies one (rows of at most 128
 // bytes per copy).  What lies behind a sequence's last key may be any bits.  Its logits are
@@ -75,6 +75,7 @@ struct TileShared {
   uint64_t s_full[2], p_ready[2], o_full[2], o_empty[2];
   uint64_t mma_done;
   int64_t scratch[40];
+  int issued[2];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
@@ -174,11 +175,19 @@ __global__ void __launch_bounds__(512, 1)
   if (warp >= 8) {
     setmaxnreg_dec<G::REG_OTHER>();
     Walk w(p, range);
-    if (warp == 13) {
-      // ---------------------------------------------------------------- TMA producer
+    if (warp == 13 || warp == 15) {
+      // ---------------------------------------------------------------- TMA producers
+      // The copies of a tile, a lane each, spread over both warps (see the row kernel).
+      const int pw = warp == 15;
+      const int op = lane * 2 + pw;
+      constexpr int COPIES = FP8 ? 2 : G::NBLK;  // of one page of K or V
       const int size = 1 << p.seqs.page_log2;
       const int box = min(size, KEYS);
       const int boxes = KEYS / box;
+      const int my_box = op / COPIES, part = op % COPIES;
+      const uint32_t to = !FP8        ? part * G::KV_BLK + my_box * box * G::SWZ
+                          : part == 0 ? my_box * box * D
+                                      : KEYS * D + my_box * box * 4;
       uint32_t qe_ph[2] = {0u, 0u};    // q_empty
       uint32_t q_par[2] = {1u, 1u};    // parity of the last Q load's q_full phase
       bool q_loaded[2] = {false, false};
@@ -188,66 +197,78 @@ __global__ void __launch_bounds__(512, 1)
       int slot = 0, issued = 0;
       uint32_t ph = 0;
       bool ok = true;
-      while (ok && w.next()) {
-        if (lane == 0) {
-          if (__ldg(p.seqs.kv_lens + w.b) != w.s.len ||
-              __ldg(p.seqs.offsets + w.b + 1) - __ldg(p.seqs.offsets + w.b) != w.s.count)
+      ProducersMeet<2> meet{sh->issued, 3};
+      while (issued < meet.limit && w.next()) {
+        if (pw == 0) {
+          if (lane == 0 && (__ldg(p.seqs.kv_lens + w.b) != w.s.len ||
+                            __ldg(p.seqs.offsets + w.b + 1) - __ldg(p.seqs.offsets + w.b) != w.s.count))
             report(status, kStatusPageTable);
-        }
 #pragma unroll
-        for (int i = 0; i < TILES; ++i) {
-          if (!ok || w.steps(i) == 0) continue;
-          ok = wait(sh->q_empty[i], qe_ph[i] ^ 1u);
-          if (!ok) continue;
-          qe_ph[i] ^= 1u;
-          q_par[i] ^= 1u;
-          q_loaded[i] = true;
-          if (lane == 0) {
-            const uint32_t bar = smem_u32(&sh->q_full[i]);
-            mbar_arrive_expect_tx(bar, p.tile_live * G::ROW_BYTES);
+          for (int i = 0; i < TILES; ++i) {
+            if (!ok || w.steps(i) == 0) continue;
+            ok = wait(sh->q_empty[i], qe_ph[i] ^ 1u);
+            if (!ok) continue;
+            qe_ph[i] ^= 1u;
+            q_par[i] ^= 1u;
+            q_loaded[i] = true;
+            if (lane == 0) {
+              const uint32_t bar = smem_u32(&sh->q_full[i]);
+              mbar_arrive_expect_tx(bar, p.tile_live * G::ROW_BYTES);
 #pragma unroll
-            for (int c = 0; c < G::NBLK; ++c)
-              tma_load_3d(smem_u32(q_smem + i * G::Q_TILE + c * G::Q_BLK), &tmQ, bar,
-                          c * (G::SWZ / 2), w.head * p.group, w.s.first + w.tok0(i));
-          }
-        }
-        for (int t = w.tile0; t < w.tile1 && ok; ++t) {
-          const int key0 = t * KEYS;
-          const int live = min(boxes, max(0, (w.s.len - key0 + box - 1) / box));
-          int page = 0;
-          if (lane < live) {
-            page = page_of(p.seqs, w.b, key0 + lane * box);
-            if (page < 0) {
-              report(status, kStatusPageTable);
-              page = 0;
+              for (int c = 0; c < G::NBLK; ++c)
+                tma_load_3d(smem_u32(q_smem + i * G::Q_TILE + c * G::Q_BLK), &tmQ, bar,
+                            c * (G::SWZ / 2), w.head * p.group, w.s.first + w.tok0(i));
             }
           }
-          const int row = (key0 + lane * box) & (size - 1);
+        }
+        // the page of this lane's copies for a tile; looked up one tile ahead
+        auto look_up = [&](int t) -> int {
+          const int key = t * KEYS + my_box * box;
+          if (my_box >= boxes || t >= w.tile1 || key >= w.s.len) return -1;
+          const int page = page_of(p.seqs, w.b, key);
+          if (page < 0) report(status, kStatusPageTable);
+          return max(page, 0);
+        };
+        int next_page = look_up(w.tile0);
+        bool stop = false;
+        for (int t = w.tile0; t < w.tile1 && !stop; ++t) {
+          const int key0 = t * KEYS;
+          const int page = next_page;
+          next_page = look_up(t + 1);
+          const int row = (key0 + my_box * box) & (size - 1);
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             if (ok) ok = wait(empty[slot], ph ^ 1u);
-            if (!ok) break;
+            if (!ok) {
+              meet(pw, issued);
+              stop = issued >= meet.limit;
+              if (stop) break;
+            }
             const uint32_t bar = smem_u32(&full[slot]);
-            if (lane == 0)
+            // (the other warp's copies may land before this arrival: the phase waits for it)
+            if (pw == 0 && lane == 0) {
+              const int live = min(boxes, max(0, (w.s.len - key0 + box - 1) / box));  // with a key
               mbar_arrive_expect_tx(bar, live * box * (FP8 ? D + 4 : G::ROW_BYTES));
+            }
             __syncwarp();
-            if (lane < live) {
+            if (page >= 0) {
               const CUtensorMap* map = kv ? &tmV : &tmK;
               if constexpr (FP8) {
-                const uint32_t dst = smem_u32(raw_smem + slot * G::RAW);
-                tma_load_4d(dst + lane * box * D, map, bar, 0, row, w.head, page);
-                const float* src = kv ? p.v_scale + page * p.v_scale_stride[0] + w.head * p.v_scale_stride[1]
-                                      : p.k_scale + page * p.k_scale_stride[0] + w.head * p.k_scale_stride[1];
-                bulk_load_tile(dst + KEYS * D + lane * box * 4, src + row, box * 4, bar);
+                const uint32_t dst = smem_u32(raw_smem + slot * G::RAW) + to;
+                if (part == 0) {
+                  tma_load_4d(dst, map, bar, 0, row, w.head, page);
+                } else {
+                  const float* src = kv ? p.v_scale + page * p.v_scale_stride[0] + w.head * p.v_scale_stride[1]
+                                        : p.k_scale + page * p.k_scale_stride[0] + w.head * p.k_scale_stride[1];
+                  bulk_load_tile(dst, src + row, box * 4, bar);
+                }
               } else {
-                const uint32_t dst = smem_u32(kv_smem + slot * G::KV_TILE);
-#pragma unroll
-                for (int c = 0; c < G::NBLK; ++c)
-                  tma_load_4d(dst + c * G::KV_BLK + lane * box * G::SWZ, map, bar,
-                              c * (G::SWZ / 2), row, w.head, page);
+                tma_load_4d(smem_u32(kv_smem + slot * G::KV_TILE) + to, map, bar,
+                            part * (G::SWZ / 2), row, w.head, page);
               }
             }
-            if (!FP8 && kv == 1 && t + 1 == w.tile1 && w.tail() && lane == 0)
+            __syncwarp();
+            if (!FP8 && kv == 1 && t + 1 == w.tile1 && w.tail() && pw == 0 && lane == 0)
               mbar_arrive(smem_u32(&sh->v_go[slot]));
             ++issued;
             if (++slot == RING) {
@@ -257,6 +278,7 @@ __global__ void __launch_bounds__(512, 1)
           }
         }
       }
+      meet(pw, issued);
       // the copies issued last land before shared memory goes away
 #pragma unroll
       for (int i = 0; i < TILES; ++i)
