@@ -22,25 +22,28 @@ int encode_query_map(CUtensorMap* map, const void* ptr, int dtype, int64_t total
 namespace {
 
 template <int D>
-PagedInfo info_of(bool tile, bool fp8, int mt) {
+PagedInfo info_of(bool tile, bool fp8, int wm) {
   if (tile) {
     using G = TileGeo<D, false>;  // float8 tiles land as they are, without a swizzle
     return fp8 ? PagedInfo{128 * G::TILES, G::KEYS, 16, D}
                : PagedInfo{128 * G::TILES, G::KEYS, G::SWZ, G::SWZ / 2};
   }
+  constexpr int W2 = D <= 128 ? 2 : 1;
   using R = RowsGeo<D, false, 1>;
   using F = RowsGeo<D, true, 1>;
-  return fp8 ? PagedInfo{16 * mt, F::KEYS, F::SPAN, F::SPAN}
-             : PagedInfo{16 * mt, R::KEYS, R::SPAN, R::SPAN / 2};
+  const int keys = wm == 2 ? (fp8 ? RowsGeo<D, true, W2>::KEYS : RowsGeo<D, false, W2>::KEYS)
+                           : (fp8 ? F::KEYS : R::KEYS);
+  return fp8 ? PagedInfo{16 * wm, keys, F::SPAN, F::SPAN}
+             : PagedInfo{16 * wm, keys, R::SPAN, R::SPAN / 2};
 }
 
-PagedInfo info_for(int64_t head_dim, bool tile, bool fp8, int mt) {
+PagedInfo info_for(int64_t head_dim, bool tile, bool fp8, int wm) {
   switch (head_dim) {
-    case 16: return info_of<16>(tile, fp8, mt);
-    case 32: return info_of<32>(tile, fp8, mt);
-    case 64: return info_of<64>(tile, fp8, mt);
-    case 128: return info_of<128>(tile, fp8, mt);
-    default: return info_of<256>(tile, fp8, mt);
+    case 16: return info_of<16>(tile, fp8, wm);
+    case 32: return info_of<32>(tile, fp8, wm);
+    case 64: return info_of<64>(tile, fp8, wm);
+    case 128: return info_of<128>(tile, fp8, wm);
+    default: return info_of<256>(tile, fp8, wm);
   }
 }
 
@@ -49,7 +52,7 @@ int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 // What a call runs with, from its arguments alone.
 struct Choice {
   bool tile;  // tile kernel, else row kernel
-  int mt;
+  int wm;
   PagedInfo info;
   int grid;
   int64_t parts, lse, o, bytes;  // workspace offsets
@@ -76,8 +79,8 @@ Choice choose(const FaPagedAttnArgs* a) {
   // once; above that the tile kernel does so for 128 or 256 rows.  It needs a positive scale, and
   // a group that fits a tile.
   c.tile = longest * group > 32 && group <= 128 && a->sm_scale > 0.f;
-  c.mt = !c.tile && longest * group > 16 && a->cache.head_dim <= 128 ? 2 : 1;
-  c.info = info_for(a->cache.head_dim, c.tile, a->cache.dtype == FA_DTYPE_FP8_E4M3, c.mt);
+  c.wm = !c.tile && longest * group > 16 && a->cache.head_dim <= 128 ? 2 : 1;
+  c.info = info_for(a->cache.head_dim, c.tile, a->cache.dtype == FA_DTYPE_FP8_E4M3, c.wm);
   c.grid = sm_count_of_current();
   const int64_t rows = 2 * static_cast<int64_t>(c.info.rows) * c.grid;
   c.parts = 0;
@@ -120,7 +123,7 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   fa::PagedPlan plan{};
   plan.half = a->dtype == FA_DTYPE_FP16;
   plan.fp8 = kv.dtype == FA_DTYPE_FP8_E4M3;
-  plan.mt = c.mt;
+  plan.wm = c.wm;
   plan.grid = c.grid;
   plan.stream = static_cast<cudaStream_t>(stream);
   const fa::PagedInfo& info = c.info;

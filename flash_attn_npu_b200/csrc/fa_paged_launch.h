@@ -19,7 +19,7 @@ struct PagedPlan {
   PagedAttnParams params;
   bool half;  // q and the output are fp16 (else bf16)
   bool fp8;
-  int mt;     // row kernel: 16-row tiles of a block (1 or 2)
+  int wm;     // row kernel: 16-row groups of a block (1 or 2)
   int grid;
   cudaStream_t stream;
 };

@@ -1,7 +1,7 @@
 // Instantiations of the paged row kernel for one head dimension: included with FA_HEAD_DIM defined
 // by fa_paged_rows_d*.cu, so that the head dimensions compile as separate translation units.
 //   q fp16 / bf16, cache of the same type or float8, blocks of 16 rows, or 32 for head_dim <= 128
-//   (two tiles' fragments of 256 columns do not fit a thread's registers)
+//   (with 256 columns there are four warps, which share 16 rows)
 #pragma once
 
 #include "fa_paged_launch.h"
@@ -14,10 +14,10 @@
 namespace fa {
 namespace {
 
-template <typename T, bool FP8, int MT>
+template <typename T, bool FP8, int WM>
 int launch_rows(const PagedPlan& plan) {
-  using G = RowsGeo<FA_HEAD_DIM, FP8, MT>;
-  auto kernel = paged_rows_kernel<T, FA_HEAD_DIM, FP8, MT>;
+  using G = RowsGeo<FA_HEAD_DIM, FP8, WM>;
+  auto kernel = paged_rows_kernel<T, FA_HEAD_DIM, FP8, WM>;
   if constexpr (G::SPLIT) {
     // the split redistributes exactly the launch allocation: refuse a build that differs
     static int regs_ok = 0;  // 0 unknown, 1 ok, -1 mismatch
@@ -46,17 +46,17 @@ int launch_rows(const PagedPlan& plan) {
 }
 
 template <typename T, bool FP8>
-int launch_mt(const PagedPlan& plan) {
+int launch_wm(const PagedPlan& plan) {
   if constexpr (FA_HEAD_DIM <= 128) {
-    if (plan.mt == 2) return launch_rows<T, FP8, 2>(plan);
+    if (plan.wm == 2) return launch_rows<T, FP8, 2>(plan);
   }
   return launch_rows<T, FP8, 1>(plan);
 }
 
 int launch_any(const PagedPlan& plan) {
   if (plan.fp8)
-    return plan.half ? launch_mt<__half, true>(plan) : launch_mt<__nv_bfloat16, true>(plan);
-  return plan.half ? launch_mt<__half, false>(plan) : launch_mt<__nv_bfloat16, false>(plan);
+    return plan.half ? launch_wm<__half, true>(plan) : launch_wm<__nv_bfloat16, true>(plan);
+  return plan.half ? launch_wm<__half, false>(plan) : launch_wm<__nv_bfloat16, false>(plan);
 }
 
 }  // namespace
