@@ -48,6 +48,7 @@ struct PagedAttnParams {
   int causal;
   float scale_log2;  // sm_scale * log2(e)
   int min_steps;     // steps of a CTA's range, at least
+  int whole_items;   // a CTA takes the items that begin in its range, whole: nothing is shared
   int tile_live;     // rows of a tile that are used: a multiple of `group` in the tile kernel
   int tile_toks;     // tokens of a tile (tile kernel)
   PagedPart* parts;  // [gridDim.x]
@@ -164,7 +165,9 @@ struct PagedWalk {
 
   __device__ __forceinline__ PagedWalk(const PagedAttnParams& params, const PagedRange& r)
       : p(params), pos(r.lo), hi(r.hi), base(r.base), all(r.all), ctas(r.ctas), b(r.seq) {
-    if (pos < hi) s = paged_seq<ROWS, KEYS>(p, b);
+    if (pos >= hi) return;
+    s = paged_seq<ROWS, KEYS>(p, b);
+    if (p.whole_items) pos = base + (pos - base + s.tiles - 1) / s.tiles * s.tiles;
   }
   __device__ __forceinline__ bool next() {
     if (pos >= hi) return false;
@@ -176,7 +179,7 @@ struct PagedWalk {
     const int64_t n = at / s.tiles;
     tile0 = static_cast<int>(at - n * s.tiles);
     const int64_t left = hi - pos;
-    tile1 = static_cast<int>(left < s.tiles - tile0 ? tile0 + left : s.tiles);
+    tile1 = static_cast<int>(!p.whole_items && left < s.tiles - tile0 ? tile0 + left : s.tiles);
     head = static_cast<int>(n / s.blocks);
     block = static_cast<int>(n - static_cast<int64_t>(head) * s.blocks);
     item = pos - tile0;
@@ -248,6 +251,10 @@ struct PagedTileWalk {
     block = 0;
     for (n = s.block_tiles(p, 0); at >= n; n = s.block_tiles(p, ++block)) at -= n;
     tile1 = static_cast<int>(at);
+    if (p.whole_items && at > 0) {
+      pos += n - at;
+      tile1 = n;
+    }
   }
   // (the walk stands before tile `tile1` of the current item)
   __device__ __forceinline__ bool next() {
@@ -266,7 +273,7 @@ struct PagedTileWalk {
     }
     tile0 = tile1;
     const int64_t left = hi - pos;
-    tile1 = static_cast<int>(left < n - tile0 ? tile0 + left : n);
+    tile1 = static_cast<int>(!p.whole_items && left < n - tile0 ? tile0 + left : n);
     item = pos - tile0;
     pos += tile1 - tile0;
     return true;
@@ -307,8 +314,9 @@ struct ProducersMeet {
   }
 };
 
-// Joins the parts of shared items.  An item has TILES tiles of TILE rows.  Block (c, y) takes rows
-// y * ROWS .. + ROWS - 1 of the item that CTA c + 1 continues, if that is the item's second part;
+// Joins the parts of shared items.  An item has TILES tiles of TILE rows.  An item of n parts has
+// n - 1 CTAs that continue it; blocks (c, y) belong to CTA c + 1 and take every (n - 1)-th row of
+// its item, so that each CTA's blocks have about the same to read however often items are cut.
 // WARPS warps to a row, which take every WARPS-th part each.
 template <typename T, int TILE, int TILES, int WARPS, int ROWS>
 __global__ void __launch_bounds__(WARPS * ROWS * 32)
@@ -317,70 +325,72 @@ __global__ void __launch_bounds__(WARPS * ROWS * 32)
   __shared__ float s_o[ROWS][WARPS][256];
   const int c = blockIdx.x + 1;
   const PagedPart part = p.parts[c];
-  if (part.first_cta != c - 1) return;
-  const int n = part.last_cta - c + 2;  // slot 1 of CTA c - 1, then slots 0 of c .. last_cta
+  if (part.first_cta < 0) return;
+  const int step = part.last_cta - part.first_cta;  // CTAs that share the rows
+  const int n = step + 1;  // parts: slot 1 of first_cta, then slots 0 up to last_cta
   const int lane = threadIdx.x & 31;
   const int mine = threadIdx.x / (WARPS * 32);  // row of the block
   const int warp = (threadIdx.x >> 5) % WARPS;
-  const int row = blockIdx.y * ROWS + mine;
-  const int in_tile = row % TILE;
-  const int at = (part.block * TILES + row / TILE) * p.tile_live + in_tile;
-  const bool live = in_tile < p.tile_live && at < part.count * p.group;
-  auto slot_row = [&](int i) -> int64_t {
-    const int64_t slot = i == 0 ? static_cast<int64_t>(c - 1) * 2 + 1
-                                : static_cast<int64_t>(c - 1 + i) * 2;
-    return slot * (TILE * TILES) + row;
-  };
   const int D = p.head_dim;
-  float acc[8];  // columns 32 k + lane
+  for (int turn = blockIdx.y * ROWS; turn * step < TILE * TILES; turn += gridDim.y * ROWS) {
+    const int row = (turn + mine) * step + (c - part.first_cta - 1);
+    const int in_tile = row % TILE;
+    const int at = (part.block * TILES + row / TILE) * p.tile_live + in_tile;
+    const bool live = row < TILE * TILES && in_tile < p.tile_live && at < part.count * p.group;
+    auto slot_row = [&](int i) -> int64_t {
+      const int64_t slot = i == 0 ? static_cast<int64_t>(part.first_cta) * 2 + 1
+                                  : static_cast<int64_t>(part.first_cta + i) * 2;
+      return slot * (TILE * TILES) + row;
+    };
+    float acc[8];  // columns 32 k + lane
 #pragma unroll
-  for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-  float top = -INFINITY, sum = 0.f;
-  if (live) {
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_lse[slot_row(i)]);
+    for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+    float top = -INFINITY, sum = 0.f;
+    if (live) {
+      for (int i = lane; i < n; i += 32) top = fmaxf(top, p.part_lse[slot_row(i)]);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const float base = top == -INFINITY ? 0.f : top;  // no part has a key: all weights are 0
-    for (int i = lane; i < n; i += 32) sum += exp2f(p.part_lse[slot_row(i)] - base);
+      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float base = top == -INFINITY ? 0.f : top;  // no part has a key: all weights are 0
+      for (int i = lane; i < n; i += 32) sum += exp2f(p.part_lse[slot_row(i)] - base);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll 4
-    for (int i = warp; i < n; i += WARPS) {
-      const int64_t r = slot_row(i);
-      const float w = exp2f(p.part_lse[r] - base) * inv;
-      if (w == 0.f) continue;  // a part without keys for the row may have left no values
+      for (int i = warp; i < n; i += WARPS) {
+        const int64_t r = slot_row(i);
+        const float w = exp2f(p.part_lse[r] - base) * inv;
+        if (w == 0.f) continue;  // a part without keys for the row may have left no values
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int d = k * 32 + lane;
-        if (k * 32 < D && d < D) acc[k] += w * p.part_o[r * D + d];
+        for (int k = 0; k < 8; ++k) {
+          const int d = k * 32 + lane;
+          if (k * 32 < D && d < D) acc[k] += w * p.part_o[r * D + d];
+        }
       }
     }
-  }
-  if (WARPS > 1) {
+    const int64_t tok = part.first_row + at / p.group;
+    const int64_t head = part.head_kv * p.group + at % p.group;
+    T* out = static_cast<T*>(p.o) + tok * p.o_stride[0] + head * p.o_stride[1];
+    if constexpr (WARPS > 1) {
+      __syncthreads();  // the last row's sums have been read
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k * 32 + lane < D) s_o[mine][warp][k * 32 + lane] = acc[k];
-    __syncthreads();
-  }
-  if (!live) return;
-  const int64_t tok = part.first_row + at / p.group;
-  const int64_t head = part.head_kv * p.group + at % p.group;
-  T* out = static_cast<T*>(p.o) + tok * p.o_stride[0] + head * p.o_stride[1];
-  if (WARPS > 1) {
-    for (int d = warp * 32 + lane; d < D; d += WARPS * 32) {
-      float v = 0.f;
+      for (int k = 0; k < 8; ++k)
+        if (k * 32 + lane < D) s_o[mine][warp][k * 32 + lane] = acc[k];
+      __syncthreads();
+      if (live)
+        for (int d = warp * 32 + lane; d < D; d += WARPS * 32) {
+          float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) v += s_o[mine][w][d];
-      out[d] = static_cast<T>(v);
+          for (int w = 0; w < WARPS; ++w) v += s_o[mine][w][d];
+          out[d] = static_cast<T>(v);
+        }
+    } else if (live) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k * 32 + lane < D) out[k * 32 + lane] = static_cast<T>(acc[k]);
     }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k * 32 + lane < D) out[k * 32 + lane] = static_cast<T>(acc[k]);
+    if (live && warp == 0 && lane == 0)
+      p.lse[tok * p.heads_kv * p.group + head] = (top + log2f(sum)) * kLn2;
   }
-  if (warp == 0 && lane == 0)
-    p.lse[tok * p.heads_kv * p.group + head] = (top + log2f(sum)) * kLn2;
 }
 
 }  // namespace fa

@@ -35,6 +35,24 @@ int launch_rows_d64(const PagedPlan& plan);
 int launch_rows_d128(const PagedPlan& plan);
 int launch_rows_d256(const PagedPlan& plan);
 
+// A kernel's opt-in to more than 48 KB of shared memory, made once per device: the call costs as
+// much as a small part of a launch.
+struct SmemOptIn {
+  bool done[16] = {};
+  bool operator()(const void* kernel, int bytes) {
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
+    if (dev >= 0 && dev < 16 && done[dev]) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+        cudaSuccess) {
+      (void)cudaGetLastError();
+      return false;
+    }
+    if (dev >= 0 && dev < 16) done[dev] = true;
+    return true;
+  }
+};
+
 // Brings the combine kernel up beside the kernel before it in the stream (programmatic dependent
 // launch): it waits for that kernel's end itself, so only the launch latency overlaps.
 template <typename Kernel>

@@ -30,14 +30,11 @@ int launch_rows(const PagedPlan& plan) {
     }
     if (regs_ok != 1) return -7;
   }
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) !=
-      cudaSuccess) {
-    (void)cudaGetLastError();
-    return -7;
-  }
+  static SmemOptIn opt_in;
+  if (!opt_in(reinterpret_cast<const void*>(kernel), G::SMEM)) return -7;
   kernel<<<plan.grid, G::THREADS, G::SMEM, plan.stream>>>(plan.tmK, plan.tmV, plan.params);
   if (cudaGetLastError() != cudaSuccess) return -7;
-  if (plan.grid == 1) return 0;  // no shared item
+  if (plan.grid == 1 || plan.params.whole_items) return 0;  // no shared item
   const int64_t most = static_cast<int64_t>(plan.params.seqs.total) * plan.params.group;
   const unsigned rows = static_cast<unsigned>(most < G::ROWS ? most : G::ROWS);
   constexpr int kWarps = 4;

@@ -12,6 +12,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -199,8 +200,10 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (x.total > 0 && x.cache.seqs > 0) {
     x.workspace_bytes = g_workspace(&x);
     if (x.workspace_bytes < 0) return none();
-    const Tensor workspace = at::empty({x.workspace_bytes}, q->options().dtype(at::kByte));
-    x.workspace = workspace.mutable_data_ptr();
+    // freed when this returns, in the order of the current stream
+    const c10::DataPtr workspace =
+        c10::cuda::CUDACachingAllocator::get()->allocate(x.workspace_bytes);
+    x.workspace = workspace.get();
     const int rc = g_attn(&x, c10::cuda::getCurrentCUDAStream(index).stream());
     if (rc != FA_OK) return PyLong_FromLong(rc);
   }
@@ -208,6 +211,45 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!r) return nullptr;
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(out)));
   PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(lse)));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// read_new(total, dtype code, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale)
+//   -> (k, v), a status code, or None
+PyObject* read_new(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !PyLong_Check(a[0]) || !PyLong_Check(a[1])) return none();
+  FaPagedCopyArgs x{};
+  x.struct_size = sizeof(x);
+  int index = -1;
+  if (!fill_cache({a[2], a[3], a[4], a[5], a[6], a[7], a[8]}, x.cache, index)) return none();
+  x.total = PyLong_AsLongLong(a[0]);
+  x.dtype = static_cast<int32_t>(PyLong_AsLong(a[1]));
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  if (x.total < 0 || (x.dtype != FA_DTYPE_FP16 && x.dtype != FA_DTYPE_BF16) ||
+      (x.dtype != x.cache.dtype && x.cache.dtype != FA_DTYPE_FP8_E4M3))
+    return none();
+  const Tensor& cache = *tensor_of(a[2]);
+  const c10::cuda::OptionalCUDAGuard guard(cache.device());
+  const auto options =
+      cache.options().dtype(x.dtype == FA_DTYPE_FP16 ? at::kHalf : at::kBFloat16);
+  Tensor k = at::empty({x.total, x.cache.heads_kv, x.cache.head_dim}, options);
+  Tensor v = at::empty({x.total, x.cache.heads_kv, x.cache.head_dim}, options);
+  strides(k, x.k_stride);
+  strides(v, x.v_stride);
+  x.k = k.mutable_data_ptr();
+  x.v = v.mutable_data_ptr();
+  x.dev_status = g_status[index];
+  const int rc = g_read(&x, c10::cuda::getCurrentCUDAStream(index).stream());
+  if (rc != FA_OK) return PyLong_FromLong(rc);
+  PyObject* r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(k)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(v)));
   return r;
   END_HANDLE_TH_ERRORS
 }
@@ -268,6 +310,7 @@ PyObject* set_status(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attention)), METH_FASTCALL, nullptr},
+    {"read_new", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(read_new)), METH_FASTCALL, nullptr},
     {"copy", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(copy)), METH_FASTCALL, nullptr},
     {"setup", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(setup)), METH_FASTCALL, nullptr},
     {"set_status", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(set_status)), METH_FASTCALL, nullptr},

@@ -278,6 +278,13 @@ def read(k_cache, v_cache, page_table, offsets, kv_lens, total, k_scale=None, v_
     if out is None:
         if dtype is None:
             dtype = torch.bfloat16 if k_cache.dtype == FP8 else k_cache.dtype
+        if _binding is not None and dtype in _ROW_CODES:
+            res = _binding.read_new(total, _ROW_CODES[dtype], k_cache, v_cache, page_table, offsets,
+                                    kv_lens, k_scale, v_scale)
+            if res is not None:
+                if type(res) is int or ops._CHECK_EVERY_CALL:
+                    _check(res, k_cache.device)
+                return res
         shape = (int(total), k_cache.shape[1], k_cache.shape[-1])
         k = torch.empty(shape, dtype=dtype, device=k_cache.device)
         v = torch.empty_like(k)
