@@ -21,29 +21,34 @@ int encode_query_map(CUtensorMap* map, const void* ptr, int dtype, int64_t total
 
 namespace {
 
+template <int D, bool FP8, int ROWS>
+constexpr PagedInfo rows_info() {
+  using G = RowsGeo<D, FP8, ROWS>;
+  return PagedInfo{ROWS, G::KEYS, G::SPAN, FP8 ? G::SPAN : G::SPAN / 2};
+}
+
+// rows: of a block of the row kernel; 0: the tile kernel.
 template <int D>
-PagedInfo info_of(bool tile, bool fp8, int wm) {
-  if (tile) {
+PagedInfo info_of(bool fp8, int rows) {
+  if (rows == 0) {
     using G = TileGeo<D, false>;  // float8 tiles land as they are, without a swizzle
     return fp8 ? PagedInfo{128 * G::TILES, G::KEYS, 16, D}
                : PagedInfo{128 * G::TILES, G::KEYS, G::SWZ, G::SWZ / 2};
   }
-  constexpr int W2 = D <= 128 ? 2 : 1;
-  using R = RowsGeo<D, false, 1>;
-  using F = RowsGeo<D, true, 1>;
-  const int keys = wm == 2 ? (fp8 ? RowsGeo<D, true, W2>::KEYS : RowsGeo<D, false, W2>::KEYS)
-                           : (fp8 ? F::KEYS : R::KEYS);
-  return fp8 ? PagedInfo{16 * wm, keys, F::SPAN, F::SPAN}
-             : PagedInfo{16 * wm, keys, R::SPAN, R::SPAN / 2};
+  if (rows == 8) return fp8 ? rows_info<D, true, 8>() : rows_info<D, false, 8>();
+  if constexpr (D <= 128) {
+    if (rows == 32) return fp8 ? rows_info<D, true, 32>() : rows_info<D, false, 32>();
+  }
+  return fp8 ? rows_info<D, true, 16>() : rows_info<D, false, 16>();
 }
 
-PagedInfo info_for(int64_t head_dim, bool tile, bool fp8, int wm) {
+PagedInfo info_for(int64_t head_dim, bool fp8, int rows) {
   switch (head_dim) {
-    case 16: return info_of<16>(tile, fp8, wm);
-    case 32: return info_of<32>(tile, fp8, wm);
-    case 64: return info_of<64>(tile, fp8, wm);
-    case 128: return info_of<128>(tile, fp8, wm);
-    default: return info_of<256>(tile, fp8, wm);
+    case 16: return info_of<16>(fp8, rows);
+    case 32: return info_of<32>(fp8, rows);
+    case 64: return info_of<64>(fp8, rows);
+    case 128: return info_of<128>(fp8, rows);
+    default: return info_of<256>(fp8, rows);
   }
 }
 
@@ -51,8 +56,7 @@ int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // What a call runs with, from its arguments alone.
 struct Choice {
-  bool tile;  // tile kernel, else row kernel
-  int wm;
+  int rows;  // of a block of the row kernel; 0: the tile kernel
   PagedInfo info;
   int grid;
   int64_t parts, lse, o, bytes;  // workspace offsets
@@ -65,6 +69,7 @@ int check_attn(const FaPagedAttnArgs* a) {
   if (rc != FA_OK) return rc;
   if (a->heads_q <= 0 || a->heads_q % a->cache.heads_kv || a->max_q_len < 0)
     return FA_ERR_INVALID_ARG;
+  if (a->heads_q > 32768) return FA_ERR_INVALID_ARG;
   // rows of a sequence (tokens x query heads) are counted in 32 bits
   if (a->total * a->heads_q > INT32_MAX / 2) return FA_ERR_INVALID_ARG;
   if (!std::isfinite(a->sm_scale)) return FA_ERR_INVALID_ARG;
@@ -78,9 +83,11 @@ Choice choose(const FaPagedAttnArgs* a) {
   // Up to 32 rows a kv head every sequence is one block of the row kernel, which reads the cache
   // once; above that the tile kernel does so for 128 or 256 rows.  It needs a positive scale, and
   // a group that fits a tile.
-  c.tile = longest * group > 32 && group <= 128 && a->sm_scale > 0.f;
-  c.wm = !c.tile && longest * group > 16 && a->cache.head_dim <= 128 ? 2 : 1;
-  c.info = info_for(a->cache.head_dim, c.tile, a->cache.dtype == FA_DTYPE_FP8_E4M3, c.wm);
+  const int64_t most = longest * group;
+  if (most > 32 && group <= 128 && a->sm_scale > 0.f) c.rows = 0;
+  else if (most <= 8) c.rows = 8;
+  else c.rows = most <= 16 || a->cache.head_dim > 128 ? 16 : 32;
+  c.info = info_for(a->cache.head_dim, a->cache.dtype == FA_DTYPE_FP8_E4M3, c.rows);
   c.grid = sm_count_of_current();
   const int64_t rows = 2 * static_cast<int64_t>(c.info.rows) * c.grid;
   c.parts = 0;
@@ -123,7 +130,7 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   fa::PagedPlan plan{};
   plan.half = a->dtype == FA_DTYPE_FP16;
   plan.fp8 = kv.dtype == FA_DTYPE_FP8_E4M3;
-  plan.wm = c.wm;
+  plan.rows = c.rows;
   plan.grid = c.grid;
   plan.stream = static_cast<cudaStream_t>(stream);
   const fa::PagedInfo& info = c.info;
@@ -150,23 +157,25 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   p.v_scale = kv.v_scale;
   p.heads_kv = static_cast<int>(kv.heads_kv);
   p.group = static_cast<int>(a->heads_q / kv.heads_kv);
+  p.group_inv = static_cast<uint32_t>((int64_t{1} << 32) / p.group + 1);
   p.head_dim = static_cast<int>(kv.head_dim);
   p.causal = a->causal ? 1 : 0;
   p.scale_log2 = a->sm_scale * fa::kLog2e;
-  p.min_steps = c.tile ? 4 : 2;
+  const bool tile = c.rows == 0;
+  p.min_steps_log2 = tile ? 2 : 1;
   // Sequences of at most kWholeTiles tiles are not cut: the joining launch costs more (3 .. 10 us)
   // than the tiles that a CTA then takes one after the other (~0.5 us each in the row kernel,
   // ~1.3 us in the tile kernel).
   constexpr int64_t kWholeTiles = 8;
   p.whole_items = kv.table_cols * kv.page_size <= kWholeTiles * info.keys;
-  p.tile_toks = c.tile ? 128 / p.group : 0;
-  p.tile_live = c.tile ? p.tile_toks * p.group : info.rows;
+  p.tile_toks = tile ? 128 / p.group : 0;
+  p.tile_live = tile ? p.tile_toks * p.group : info.rows;
   char* ws = static_cast<char*>(a->workspace);
   p.parts = reinterpret_cast<fa::PagedPart*>(ws + c.parts);
   p.part_lse = reinterpret_cast<float*>(ws + c.lse);
   p.part_o = reinterpret_cast<float*>(ws + c.o);
 
-  if (c.tile) {
+  if (tile) {
     rc = fa::encode_query_map(&plan.tmQ, a->q, a->dtype, a->total, a->heads_q, kv.head_dim,
                               a->q_stride, static_cast<int>(std::min<int64_t>(kv.head_dim, 64)),
                               p.group, p.tile_toks, static_cast<int>(std::min<int64_t>(2 * kv.head_dim, 128)));

@@ -21,6 +21,16 @@
 
 namespace fa {
 
+// Programmatic dependent launch: a kernel of the paged calls is brought up while the one before it
+// in the stream still runs, and waits here for its end (and its memory) before it reads anything.
+__device__ __forceinline__ void wait_for_launch_before() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// From here on the next kernel may be brought up.
+__device__ __forceinline__ void let_next_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // What a CTA notes about its slot 0 for the combine kernel.
 struct PagedPart {
   int first_cta; // CTA that holds the item's first part, in its slot 1; -1: slot 0 is empty
@@ -44,10 +54,12 @@ struct PagedAttnParams {
   int64_t v_scale_stride[2];
   int heads_kv;
   int group;         // query heads per kv head
+  uint32_t group_inv;  // floor(2^32 / group) + 1: n / group = umulhi(n, .) for n * group < 2^32,
+                       // group > 1
   int head_dim;
   int causal;
   float scale_log2;  // sm_scale * log2(e)
-  int min_steps;     // steps of a CTA's range, at least
+  int min_steps_log2;  // steps of a CTA's range, at least
   int whole_items;   // a CTA takes the items that begin in its range, whole: nothing is shared
   int tile_live;     // rows of a tile that are used: a multiple of `group` in the tile kernel
   int tile_toks;     // tokens of a tile (tile kernel)
@@ -77,85 +89,79 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
   return s;
 }
 
+// Quotient of non-negative numbers, by the short division where they allow it (the long one takes
+// ~150 cycles, which a call of a few microseconds would see several times).
+__device__ __forceinline__ int64_t quot(int64_t a, int b) {
+  return (a >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b))
+                        : a / b;
+}
+
 // A CTA's range of the line, and where it begins.
 struct PagedRange {
   int64_t lo, hi;  // steps
   int64_t base;    // first step of sequence `seq`
   int64_t all;     // steps of the call
+  int64_t share;   // steps of a CTA, one more for the first `rest`
+  int rest;
   int ctas;        // CTAs with a range
   int seq;
+
+  // CTA whose range holds a step
+  __device__ __forceinline__ int cta_of(int64_t step) const {
+    const int64_t more = rest * (share + 1);  // steps of the CTAs that take one more
+    const int64_t at = step < more ? step : step - more;
+    const int64_t each = step < more ? share + 1 : share;
+    const int64_t n = (at | each) >> 31 ? at / each : quot(at, static_cast<int>(each));
+    return static_cast<int>(step < more ? n : rest + n);
+  }
 };
 
-// By all threads of the CTA; `scratch`: 40 words of shared memory; steps_of(b): steps of sequence b.
+// steps_of(b): steps of sequence b.  Every warp of the CTA finds the range by itself, a lane for
+// each 32nd of the sequences: two sums with a block barrier between them took longer than reading
+// the same few lines in every warp.
 template <typename Steps>
-__device__ __forceinline__ PagedRange paged_range(const PagedAttnParams& p, int64_t* scratch,
-                                                  Steps steps_of) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int threads = blockDim.x, warps = threads >> 5;
-  const int mine = threadIdx.x;
-  const int64_t first = mine < p.seqs.seqs ? steps_of(mine) : 0;
-  int64_t sum = first;
-  for (int b = mine + threads; b < p.seqs.seqs; b += threads)
-    sum += steps_of(b);
+__device__ __forceinline__ PagedRange paged_range(const PagedAttnParams& p, Steps steps_of) {
+  const int lane = threadIdx.x & 31;
+  const int seqs = p.seqs.seqs;
+  const int each = (seqs + 31) / 32;
+  const int b0 = min(lane * each, seqs), b1 = min(b0 + each, seqs);
+  int64_t own = 0;
+  for (int b = b0; b < b1; ++b) own += steps_of(b);
+  int64_t upto = own;
 #pragma unroll
-  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (lane == 0) scratch[warp] = sum;
-  __syncthreads();
-  int64_t all = 0;
-  for (int w = 0; w < warps; ++w) all += scratch[w];
-  __syncthreads();
-
-  PagedRange r{0, 0, 0, all, 0, 0};
-  int64_t ctas = (all + p.min_steps - 1) / p.min_steps;
-  if (ctas > gridDim.x) ctas = gridDim.x;
-  r.ctas = static_cast<int>(ctas);
-  const int64_t c = blockIdx.x;
-  if (c >= ctas) return r;
-  r.lo = all * c / ctas;
-  r.hi = all * (c + 1) / ctas;
-  int64_t before = 0;
-  for (int at = 0; at < p.seqs.seqs; at += threads) {
-    const int b = at + mine;
-    const int64_t own =
-        at == 0 ? first : (b < p.seqs.seqs ? steps_of(b) : 0);
-    int64_t upto = own;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += v;
-    }
-    if (lane == 31) scratch[warp] = upto;
-    __syncthreads();
-    int64_t chunk = 0, skip = 0;
-    for (int w = 0; w < warps; ++w) {
-      if (w < warp) skip += scratch[w];
-      chunk += scratch[w];
-    }
-    const int64_t from = before + skip + upto - own;
-    if (from <= r.lo && r.lo < from + own) {
-      scratch[33] = b;
-      scratch[34] = from;
-    }
-    __syncthreads();
-    before += chunk;
-    if (before > r.lo) break;
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += v;
   }
-  r.seq = static_cast<int>(scratch[33]);
-  r.base = scratch[34];
+  PagedRange r{0, 0, 0, __shfl_sync(0xffffffffu, upto, 31), 1, 0, 0, 0};
+  const int64_t most = (r.all + (1 << p.min_steps_log2) - 1) >> p.min_steps_log2;
+  r.ctas = static_cast<int>(most < gridDim.x ? most : gridDim.x);
+  const int c = static_cast<int>(blockIdx.x);
+  if (c >= r.ctas) return r;
+  // the first `rest` CTAs take a step more than the others
+  r.share = quot(r.all, r.ctas);
+  r.rest = static_cast<int>(r.all - r.share * r.ctas);
+  r.lo = r.share * c + min(c, r.rest);
+  r.hi = r.lo + r.share + (c < r.rest);
+  // the one lane whose sequences hold step `lo`
+  int64_t from = upto - own;
+  const bool mine = from <= r.lo && r.lo < upto;
+  int b = b0;
+  if (mine && each > 1) {
+    for (int64_t n; from + (n = steps_of(b)) <= r.lo; ++b) from += n;
+  }
+  const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+  r.seq = __shfl_sync(0xffffffffu, b, src);
+  r.base = __shfl_sync(0xffffffffu, from, src);
   return r;
-}
-
-// CTA whose range holds a step
-__device__ __forceinline__ int cta_of(int64_t step, int ctas, int64_t all) {
-  return static_cast<int>(((step + 1) * ctas - 1) / all);
 }
 
 // Walks the items of a CTA's range; every role of the kernel walks the same ones.
 template <int ROWS, int KEYS>
 struct PagedWalk {
   const PagedAttnParams& p;
-  int64_t pos, hi, base, all;
-  int ctas;
+  const PagedRange& range;
+  int64_t pos;
   int b;
   PagedSeq s;
   // the current part
@@ -163,25 +169,37 @@ struct PagedWalk {
   int tile0, tile1;  // key tiles [tile0, tile1) of the item
   int64_t item;      // its first step
 
+  // (the walk stands before tile `tile1` of the current item)
   __device__ __forceinline__ PagedWalk(const PagedAttnParams& params, const PagedRange& r)
-      : p(params), pos(r.lo), hi(r.hi), base(r.base), all(r.all), ctas(r.ctas), b(r.seq) {
-    if (pos >= hi) return;
+      : p(params), range(r), pos(r.lo), b(r.seq) {
+    if (pos >= range.hi) return;
     s = paged_seq<ROWS, KEYS>(p, b);
-    if (p.whole_items) pos = base + (pos - base + s.tiles - 1) / s.tiles * s.tiles;
+    const int64_t at = pos - r.base;
+    const int64_t n = quot(at, s.tiles);
+    tile1 = static_cast<int>(at - n * s.tiles);
+    head = static_cast<int>(s.blocks == 1 ? n : quot(n, s.blocks));
+    block = static_cast<int>(n - static_cast<int64_t>(head) * s.blocks);
+    if (p.whole_items && tile1 > 0) {
+      pos += s.tiles - tile1;
+      tile1 = s.tiles;
+    }
   }
   __device__ __forceinline__ bool next() {
-    if (pos >= hi) return false;
-    while (pos >= base + s.steps) {
-      base += s.steps;
-      s = paged_seq<ROWS, KEYS>(p, ++b);
+    if (pos >= range.hi) return false;
+    if (tile1 == s.tiles) {
+      tile1 = 0;
+      if (++block == s.blocks) {
+        block = 0;
+        if (++head == p.heads_kv) {
+          head = 0;
+          do s = paged_seq<ROWS, KEYS>(p, ++b);
+          while (s.blocks == 0);
+        }
+      }
     }
-    const int64_t at = pos - base;
-    const int64_t n = at / s.tiles;
-    tile0 = static_cast<int>(at - n * s.tiles);
-    const int64_t left = hi - pos;
+    tile0 = tile1;
+    const int64_t left = range.hi - pos;
     tile1 = static_cast<int>(!p.whole_items && left < s.tiles - tile0 ? tile0 + left : s.tiles);
-    head = static_cast<int>(n / s.blocks);
-    block = static_cast<int>(n - static_cast<int64_t>(head) * s.blocks);
     item = pos - tile0;
     pos += tile1 - tile0;
     return true;
@@ -190,8 +208,8 @@ struct PagedWalk {
   __device__ __forceinline__ int slot() const { return tile0 == 0 ? 1 : 0; }
   // What the combine kernel has to know of the current part (slot 0).
   __device__ __forceinline__ PagedPart note() const {
-    return PagedPart{cta_of(item, ctas, all), cta_of(item + s.tiles - 1, ctas, all), s.first,
-                     s.count, head, block};
+    return PagedPart{range.cta_of(item), range.cta_of(item + s.tiles - 1), s.first, s.count,
+                     head, block};
   }
 };
 
@@ -231,8 +249,8 @@ struct PagedTiles {
 template <int TILES, int KEYS>
 struct PagedTileWalk {
   const PagedAttnParams& p;
-  int64_t pos, hi, all;
-  int ctas;
+  const PagedRange& range;
+  int64_t pos;
   int b;
   PagedTiles<TILES, KEYS> s;
   // the current part
@@ -242,11 +260,12 @@ struct PagedTileWalk {
   int64_t item;      // the item's first step
 
   __device__ __forceinline__ PagedTileWalk(const PagedAttnParams& params, const PagedRange& r)
-      : p(params), pos(r.lo), hi(r.hi), all(r.all), ctas(r.ctas), b(r.seq) {
-    if (pos >= hi) return;
+      : p(params), range(r), pos(r.lo), b(r.seq) {
+    if (pos >= range.hi) return;
     s = PagedTiles<TILES, KEYS>(p, b);
     int64_t at = pos - r.base;
-    head = static_cast<int>(at / s.per_head);
+    head = static_cast<int>(s.per_head >> 31 ? at / s.per_head
+                                             : quot(at, static_cast<int>(s.per_head)));
     at -= head * s.per_head;
     block = 0;
     for (n = s.block_tiles(p, 0); at >= n; n = s.block_tiles(p, ++block)) at -= n;
@@ -258,7 +277,7 @@ struct PagedTileWalk {
   }
   // (the walk stands before tile `tile1` of the current item)
   __device__ __forceinline__ bool next() {
-    if (pos >= hi) return false;
+    if (pos >= range.hi) return false;
     if (tile1 == n) {
       tile1 = 0;
       if (++block == s.blocks) {
@@ -272,7 +291,7 @@ struct PagedTileWalk {
       n = s.block_tiles(p, block);
     }
     tile0 = tile1;
-    const int64_t left = hi - pos;
+    const int64_t left = range.hi - pos;
     tile1 = static_cast<int>(!p.whole_items && left < n - tile0 ? tile0 + left : n);
     item = pos - tile0;
     pos += tile1 - tile0;
@@ -289,8 +308,7 @@ struct PagedTileWalk {
   __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == n; }
   __device__ __forceinline__ int slot() const { return tile0 == 0 ? 1 : 0; }
   __device__ __forceinline__ PagedPart note() const {
-    return PagedPart{cta_of(item, ctas, all), cta_of(item + n - 1, ctas, all), s.first, s.count,
-                     head, block};
+    return PagedPart{range.cta_of(item), range.cta_of(item + n - 1), s.first, s.count, head, block};
   }
 };
 
@@ -321,7 +339,7 @@ struct ProducersMeet {
 template <typename T, int TILE, int TILES, int WARPS, int ROWS>
 __global__ void __launch_bounds__(WARPS * ROWS * 32)
     paged_combine_kernel(const PagedAttnParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_launch_before();
   __shared__ float s_o[ROWS][WARPS][256];
   const int c = blockIdx.x + 1;
   const PagedPart part = p.parts[c];

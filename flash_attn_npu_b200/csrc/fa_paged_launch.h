@@ -19,7 +19,7 @@ struct PagedPlan {
   PagedAttnParams params;
   bool half;  // q and the output are fp16 (else bf16)
   bool fp8;
-  int wm;     // row kernel: 16-row groups of a block (1 or 2)
+  int rows;   // row kernel: rows of a block (8, 16 or 32)
   int grid;
   cudaStream_t stream;
 };
@@ -53,21 +53,24 @@ struct SmemOptIn {
   }
 };
 
-// Brings the combine kernel up beside the kernel before it in the stream (programmatic dependent
-// launch): it waits for that kernel's end itself, so only the launch latency overlaps.
-template <typename Kernel>
-int launch_dependent(Kernel kernel, dim3 grid, int threads, cudaStream_t stream,
-                     const PagedAttnParams& params) {
+// Launch with programmatic dependence on the kernel before it in the stream (see
+// wait_for_launch_before): only launch latency and set-up overlap.
+template <typename... Params, typename... Args>
+int launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, int smem,
+                     cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, params) == cudaSuccess ? 0 : -7;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return 0;
+  (void)cudaGetLastError();
+  return -7;
 }
 
 }  // namespace fa

@@ -1,17 +1,19 @@
 // Paged attention of few query rows per kv head (decode, drafts): bound by reading the cache.
 //
-// Rows of a block are (token, query head of the group) pairs, 16 or 32 of them (WM groups), so
-// that every key and value is read once for all query heads that share it.  A CTA walks its range
-// of key tiles (fa_paged_attn.cuh).  A producer warp looks the tile's pages up and brings them
-// with one TMA copy per page (rows of at most 128 bytes per copy, swizzled) and, for float8, the
-// rows' scales with bulk copies, into a ring of stages that is as deep as shared memory allows: what
-// it has to hide is one memory latency at full bandwidth, ~45 KB per SM.  NW consumer warps take 16
-// keys of the tile each, with an online softmax of their own:
-//   S = Q K^T (m16n8k16), p = 2^(S * scale * log2 e - m), O += P V (m16n8k16),
-// and join their (m, l, O) through shared memory at the item's end.  The tensor work is far from
-// its limit here, so mma.sync on register fragments is enough: at head_dim 128 a warp spends ~500
-// cycles on 16 keys (8 KB of 16-bit cache), 8 warps take in ~130 bytes a cycle, and an SM's share
-// of the measured memory bandwidth is 23 bytes a cycle.
+// Rows of a block are (token, query head of the group) pairs, 8, 16 or 32 of them, so that every
+// key and value is read once for all query heads that share it.  A CTA walks its range of key tiles
+// (fa_paged_attn.cuh).  Producer warps look the tile's pages up and bring them with TMA copies (rows
+// of at most 128 bytes per copy, swizzled) and, for float8, the rows' scales with bulk copies, into
+// a ring of stages that is as deep as shared memory allows: what it has to hide is one memory
+// latency at full bandwidth, ~45 KB per SM.  Consumer warps take 16 KN keys of the tile each, with
+// an online softmax of their own, and join their (m, l, O) through shared memory at the item's end.
+//
+// The products are formed transposed, with mma m16n8k16 on register fragments:
+//   S^T [16 keys x 8 rows] = K Q^T,   p = 2^(S * scale * log2 e - m),   O^T [16 dims x 8 rows] += V^T P^T
+// so that K and V are the 16-row operands and decoding's few query rows fill the 8 columns (keys
+// as columns would leave half of a 16-row operand empty).  mma.sync takes ~9 cycles a sub-partition
+// here (measured), a warp ~1000 cycles for 16 keys at head_dim 128: 8 warps take in ~65 bytes a
+// cycle, and an SM's share of the measured memory bandwidth is 23.
 //
 // Float8 caches: codes convert exactly to fp16, so the products run in fp16.  Queries in bf16 are
 // scaled per row by a power of two into fp16's range first (exact but for values 2^-24 below the
@@ -20,8 +22,8 @@
 //
 // p in fp16 (fp16 caches, float8 caches) carries the factor 2^kPOffset, which l carries too: fp16
 // keeps full precision down to 2^-14, and so p does down to 2^-(14 + kPOffset) of the row's
-// largest.  Rounding p to 16 bits costs a relative 2^-9 (bf16) or 2^-12 (fp16) per term, as much
-// as rounding the output once; l sums the unrounded p.
+// largest.  Rounding p to 16 bits costs a relative 2^-8 (bf16) or 2^-11 (fp16) per term at most, as
+// much as rounding the output once; l sums the unrounded p.
 #pragma once
 
 #include <type_traits>
@@ -30,25 +32,31 @@
 
 namespace fa {
 
-// WM: 16-row groups of a block.
-template <int D, bool FP8, int WM>
+// ROWS rows of a block: 8 (one column group), 16 (two, in every warp) or 32 (two for each half of the
+// warps).
+template <int D, bool FP8, int ROWS_>
 struct RowsGeo {
+  static constexpr int ROWS = ROWS_;
+  static constexpr int WN = ROWS >= 16 ? 2 : 1;   // column groups of a warp
+  static constexpr int WM = ROWS / (8 * WN);      // row groups
   static constexpr int ROW_BYTES = FP8 ? D : 2 * D;
   static constexpr int SPAN = ROW_BYTES >= 128 ? 128 : ROW_BYTES;  // bytes of a copied row
   static constexpr int NSPAN = ROW_BYTES / SPAN;
-  // Consumer warps: 8, or 4 where 256 columns of O and Q take a thread's 255 registers.  WK of
-  // them share a row group and split the keys of a tile, 16 KN each.
+  // Consumer warps: 8, or 4 where 256 columns of O and Q take a thread's registers.  WK of them
+  // share a row group and split the keys of a tile, 16 KN each.
   static constexpr int NW = D == 256 ? 4 : 8;
   static constexpr int WK = NW / WM;
-  static constexpr int KN = WM == 1 && 32 * NW * ROW_BYTES >= 65536 ? 1 : 2;  // stages of ~64 KB
+  static constexpr int KN = WM == 1 && 32 * NW * ROW_BYTES >= 65536 ? 1  // stages of ~64 KB
+                            : WM == 2 && FP8 && D <= 32             ? 4  // (see DR)
+                                                                    : 2;
   static constexpr int KEYS = 16 * WK * KN;            // of a tile
-  static constexpr int ROWS = 16 * WM;
   static constexpr int TILE = KEYS * ROW_BYTES;        // K or V of a stage
   static constexpr int SCALES = FP8 ? KEYS * 4 : 0;    // K or V scales of a stage
   static constexpr int STAGE = 2 * TILE + 2 * SCALES;  // a multiple of 1024
-  static constexpr int GROUP_COLS = D < 32 ? D : 32;   // columns joined at a time
-  static constexpr int JOIN_PITCH = GROUP_COLS + 4;
-  static constexpr int JOIN = NW * 16 * JOIN_PITCH * 4;
+  // The warps' O are joined in the memory of the item's last stage, DR columns at a time.
+  static constexpr int DR = NW * 8 * WN * D * 4 <= STAGE ? D : D / 2;
+  static_assert(NW * 8 * WN * DR * 4 <= STAGE && DR >= 16, "joining");
+  static constexpr int Q_PITCH = 2 * D + 16;  // bytes; rows of the query block in shared memory
   // With 8 consumer warps of 128 columns the producers give most of their registers away:
   // launched at 168 a thread, 256 * 224 + 128 * 40 <= 384 * 168.
   static constexpr bool SPLIT = NW == 8 && D >= 128;
@@ -59,7 +67,7 @@ struct RowsGeo {
   static constexpr int COPIES = 2 * NSPAN + (FP8 ? 2 : 0);  // of one page
   static_assert(KEYS / 8 * COPIES <= NP * 32, "a lane for every copy of a tile of smallest pages");
   static constexpr int kMostStages = 8;
-  static constexpr int FIXED = 1024 + JOIN;
+  static constexpr int FIXED = 1024 + ROWS * Q_PITCH;
   static constexpr int STAGES = (222 * 1024 - FIXED) / STAGE < kMostStages
                                     ? (222 * 1024 - FIXED) / STAGE
                                     : kMostStages;
@@ -108,6 +116,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Transposes an 8 x 8 matrix of 16-bit values held as a fragment.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
+
 // Untiled bulk copy global -> shared (16-byte addresses and size), counted on `bar`.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
                                           uint32_t bar) {
@@ -129,28 +144,26 @@ __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
 constexpr float kRescale = 4.f;  // a row's base moves once its max passes it by 2^4
 
 // T: type of q and the output (and of a 16-bit cache).
-template <typename T, int D, bool FP8, int WM>
-__global__ void __launch_bounds__(RowsGeo<D, FP8, WM>::THREADS, 1)
+template <typename T, int D, bool FP8, int ROWS>
+__global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
     paged_rows_kernel(const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const PagedAttnParams p) {
-  using G = RowsGeo<D, FP8, WM>;
+  using G = RowsGeo<D, FP8, ROWS>;
   using C = std::conditional_t<FP8, __half, T>;  // type of the products
   constexpr bool kHalf = std::is_same_v<C, __half>;
   constexpr float kPOffset = kHalf ? 10.f : 0.f;  // p <= 2^(kPOffset + kRescale) < 65504
   constexpr int NW = G::NW, KEYS = G::KEYS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t s_full[G::STAGES], s_empty[G::STAGES];
-  __shared__ int64_t s_scratch[40];
-  __shared__ float s_m[NW][16], s_l[NW][16];
+  __shared__ alignas(16) float s_m[ROWS][G::WK], s_l[ROWS][G::WK];
   __shared__ volatile uint32_t s_abort;
   __shared__ int s_issued[G::NP];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  float* s_join = reinterpret_cast<float*>(smem + G::STAGES * G::STAGE);
+  uint8_t* s_q = smem + G::STAGES * G::STAGE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // The combine kernel may be brought up while this one runs; it waits for its end.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_launch();
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::STAGES; ++s) {
       mbar_init(smem_u32(&s_full[s]), 1);
@@ -158,12 +171,13 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, WM>::THREADS, 1)
     }
     s_abort = 0u;
     fence_mbar_init();
-    p.parts[blockIdx.x].first_cta = -2;
   }
-  const PagedRange range = paged_range(
-      p, s_scratch, [&](int b) { return paged_seq<G::ROWS, KEYS>(p, b).steps; });
   __syncthreads();
-  PagedWalk<G::ROWS, KEYS> w(p, range);
+  wait_for_launch_before();
+  if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
+  const PagedRange range =
+      paged_range(p, [&](int b) { return paged_seq<ROWS, KEYS>(p, b).steps; });
+  PagedWalk<ROWS, KEYS> w(p, range);
   int* const status = p.seqs.status;
 
   if (warp >= NW) {
@@ -250,17 +264,20 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, WM>::THREADS, 1)
 
   // -------------------------------------------------------------------------- consumers
   if constexpr (G::SPLIT) setmaxnreg_inc<G::REG_CONSUMER>();
-  constexpr int KN = G::KN, WK = G::WK;
-  const int g = lane >> 2, t4 = lane & 3;
-  const int wm = warp / WK;                 // row group
-  const int key_w = (warp % WK) * 16 * KN;  // this warp's keys of a tile
+  constexpr int KN = G::KN, WK = G::WK, WN = G::WN;
   constexpr int KSTEPS = D / 16;
-  constexpr int NT = D / 8;
-  // fragment addresses: matrices of 8 rows x 16 bytes, one row per lane
-  const int k_row = key_w + (lane & 7) + ((lane >> 4) << 3);  // K: matrices (n, c), (n, c+1), (n+8, c), ..
-  const int k_piece = (lane >> 3) & 1;
-  const int v_row = key_w + (lane & 15);                      // V: matrices (k, c), (k+8, c), (k, c+1), ..
-  const int v_piece = lane >> 4;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int wk = warp % WK;
+  const int first = warp / WK * 8 * WN;  // the warp's first row of the block
+  const int key_w = wk * 16 * KN;        // its first key of a tile
+  // fragment addresses: 8 x 8 matrices of 16-byte rows, one row per lane; a: (0, c), (8, c),
+  // (0, c+1), (8, c+1) and b: (0, c), (0, c+1), (8, c), (8, c+1)
+  const int a_row = key_w + (lane & 15), a_piece = lane >> 4;
+  const int b_row = key_w + (lane & 7) + ((lane >> 4) << 3), b_piece = (lane >> 3) & 1;
+  auto at = [&](uint32_t tile, int row, int piece) -> uint32_t {
+    return tile + (piece * 16 / G::SPAN) * KEYS * G::SPAN +
+           swizzled<G::SPAN>(row, piece % (G::SPAN / 16));
+  };
   int slot = 0;
   uint32_t ph = 0;
   bool ok = true;
@@ -271,41 +288,68 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, WM>::THREADS, 1)
 
   while (w.next()) {
     const int rows = w.s.count * p.group;
-    const int row0 = w.block * G::ROWS;
+    const int row0 = w.block * ROWS;
     const int past = w.s.len - w.s.count;  // position of the sequence's first query
-    // this thread's rows: g and g + 8 of its group
-    int lim[2];       // keys that the row may attend to
-    float qs[2];      // factor of the row's logits
-    uint32_t qf[KSTEPS][4];
+    // token and head of a row of the block
+    const int tok0 = w.block == 0 ? 0 : row0 / p.group;
+    const int head0 = row0 - tok0 * p.group;
+    auto tok_of = [&](int r) -> int {  // (exact: the sum is far below 2^16)
+      return tok0 + (p.group == 1 ? r : static_cast<int>(__umulhi(static_cast<uint32_t>(head0 + r), p.group_inv)));
+    };
+    // The query block comes through shared memory: as fragments straight from global memory it
+    // would cost each warp many scattered requests.
+    for (int i = threadIdx.x; i < ROWS * D / 8; i += NW * 32) {
+      const int r = i / (D / 8), piece = i % (D / 8);
+      const int tok = tok_of(r), h = row0 + r - tok * p.group;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (row0 + r < rows && p.scale_log2 != 0.f)
+        x = __ldg(reinterpret_cast<const uint4*>(
+            static_cast<const T*>(p.q) + static_cast<int64_t>(w.s.first + tok) * p.q_stride[0] +
+            static_cast<int64_t>(w.head * p.group + h) * p.q_stride[1] + piece * 8));
+      *reinterpret_cast<uint4*>(s_q + r * G::Q_PITCH + piece * 16) = x;
+    }
+    // the row that this thread will write
+    constexpr int TPR = NW * 32 / ROWS;  // threads of a row
+    const int my_r = threadIdx.x / TPR;
+    const bool my_live = row0 + my_r < rows;
+    const int my_tok = tok_of(my_r);
+    const int64_t my_head = w.head * p.group + row0 + my_r - my_tok * p.group;
+    // this thread's logits belong to rows first + 8 n + 2 t4 + {0, 1}
+    int lim[WN][2];       // keys that the row may attend to
+    float qs[WN][2];      // factor of the row's logits
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = row0 + wm * 16 + e * 8 + g;
-      const int tok = r / p.group;
-      const int h = r - tok * p.group;
-      const bool live = r < rows;
-      lim[e] = p.causal && live ? min(w.s.len, past + tok + 1) : w.s.len;
-      qs[e] = scale;
-      const T* src = static_cast<const T*>(p.q) + static_cast<int64_t>(w.s.first + tok) * p.q_stride[0] +
-                     static_cast<int64_t>(w.head * p.group + h) * p.q_stride[1];
-      const bool load = live && p.scale_log2 != 0.f;
-      uint32_t lo[KSTEPS], hi[KSTEPS];
+    for (int n = 0; n < WN; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = first + 8 * n + 2 * t4 + e;
+        lim[n][e] = p.causal && row0 + r < rows ? min(w.s.len, past + tok_of(r) + 1) : w.s.len;
+        qs[n][e] = scale;
+      }
+    // keys that every row of the warp may attend to, and that any row may
+    const int last = min(rows - row0, first + 8 * WN) - 1;
+    const int lim_all = p.causal ? min(w.s.len, past + tok_of(first) + 1) : w.s.len;
+    const int lim_any = last < first ? 0 : p.causal ? min(w.s.len, past + tok_of(last) + 1) : w.s.len;
+    named_barrier_sync(1, NW * 32);
+    uint32_t qf[WN][KSTEPS][2];
+#pragma unroll
+    for (int n = 0; n < WN; ++n) {
+      const uint8_t* src = s_q + (first + 8 * n + g) * G::Q_PITCH;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
-        if (FP8) {  // columns 16 k + 4 t4 .. + 3: the order in which codes come (below)
-          const uint2 x = load ? __ldg(reinterpret_cast<const uint2*>(src + 16 * k + 4 * t4))
-                               : make_uint2(0, 0);
-          lo[k] = x.x;
-          hi[k] = x.y;
+        if constexpr (FP8) {  // columns 16 k + 4 t4 .. + 3: the order in which codes come (below)
+          const uint2 x = *reinterpret_cast<const uint2*>(src + (16 * k + 4 * t4) * 2);
+          qf[n][k][0] = x.x;
+          qf[n][k][1] = x.y;
         } else {
-          lo[k] = load ? __ldg(reinterpret_cast<const unsigned*>(src + 16 * k + 2 * t4)) : 0u;
-          hi[k] = load ? __ldg(reinterpret_cast<const unsigned*>(src + 16 * k + 8 + 2 * t4)) : 0u;
+          qf[n][k][0] = *reinterpret_cast<const uint32_t*>(src + (16 * k + 2 * t4) * 2);
+          qf[n][k][1] = *reinterpret_cast<const uint32_t*>(src + (16 * k + 8 + 2 * t4) * 2);
         }
       }
       if constexpr (FP8 && std::is_same_v<T, __nv_bfloat16>) {
         float top = 0.f;
 #pragma unroll
         for (int k = 0; k < KSTEPS; ++k) {
-          const float2 a = Cvt16<T>::unpack(lo[k]), z = Cvt16<T>::unpack(hi[k]);
+          const float2 a = Cvt16<T>::unpack(qf[n][k][0]), z = Cvt16<T>::unpack(qf[n][k][1]);
           top = fmaxf(fmaxf(top, fmaxf(fabsf(a.x), fabsf(a.y))), fmaxf(fabsf(z.x), fabsf(z.y)));
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -313,34 +357,39 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, WM>::THREADS, 1)
         // 2^-x brings the row's largest into [1, 2)
         const int x = min(max(static_cast<int>(__float_as_uint(top) >> 23), 2), 252);
         const float inv = __uint_as_float(static_cast<uint32_t>(254 - x) << 23);
-        qs[e] = scale * __uint_as_float(static_cast<uint32_t>(x) << 23);
+        const float back = __uint_as_float(static_cast<uint32_t>(x) << 23);
 #pragma unroll
-        for (int k = 0; k < KSTEPS; ++k) {
-          const float2 a = Cvt16<T>::unpack(lo[k]), z = Cvt16<T>::unpack(hi[k]);
-          lo[k] = pack2(a.x * inv, a.y * inv, static_cast<__half*>(nullptr));
-          hi[k] = pack2(z.x * inv, z.y * inv, static_cast<__half*>(nullptr));
-        }
+        for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float2 a = Cvt16<T>::unpack(qf[n][k][c]);
+            qf[n][k][c] = pack2(a.x * inv, a.y * inv, static_cast<__half*>(nullptr));
+          }
+        // this lane's fragment is of row g, its logits are of rows 2 t4 and 2 t4 + 1
+        qs[n][0] = scale * __shfl_sync(0xffffffffu, back, 8 * t4);
+        qs[n][1] = scale * __shfl_sync(0xffffffffu, back, 8 * t4 + 4);
       }
 #pragma unroll
-      for (int k = 0; k < KSTEPS; ++k) {
-        qf[k][e] = lo[k] ^ q_flip;
-        qf[k][2 + e] = hi[k] ^ q_flip;
-      }
+      for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) qf[n][k][c] ^= q_flip;
     }
-    // keys that every row of the group may attend to, and that any row may
-    const int first_row = row0 + wm * 16, last_row = min(rows, first_row + 16) - 1;
-    const int lim_all = p.causal ? min(w.s.len, past + first_row / p.group + 1) : w.s.len;
-    const int lim_any = first_row >= rows ? 0
-                        : p.causal        ? min(w.s.len, past + last_row / p.group + 1)
-                                          : w.s.len;
 
-    float o[NT][4];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[KSTEPS][WN][4];
+    float m[WN][2], l[WN][2];
     float mv = 0.f, inv_mv = 0.f;  // float8: largest value scale so far, and its inverse
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < WN; ++n) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o[n][c] = 0.f;
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.f;
+      }
+#pragma unroll
+      for (int d = 0; d < KSTEPS; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[d][n][c] = 0.f;
+    }
 
     for (int t = w.tile0; t < w.tile1; ++t) {
       if (ok) {
@@ -351,148 +400,174 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, WM>::THREADS, 1)
       if (ok && key0 < lim_any) {
         const uint32_t kb = smem_u32(smem + slot * G::STAGE);
         const uint32_t vb = kb + G::TILE;
-        // ---- S = Q K^T: 2 KN tiles of 8 keys
-        float s[2 * KN][4];
+        // ---- S^T = K Q^T, KN tiles of 16 keys: entries (key g, row 2 t4), (g, 2 t4 + 1),
+        // (g + 8, ..); two sums each where there is one chain only, as an mma waits ~35 cycles for
+        // the last one of its sum
+        constexpr int SUMS = KN * WN == 1 && KSTEPS > 1 ? 2 : 1;
+        float s[KN][WN][4], s2[4];
 #pragma unroll
-        for (int n = 0; n < 2 * KN; ++n)
+        for (int kn = 0; kn < KN; ++kn)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[n][c] = 0.f;
+          for (int n = 0; n < WN; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[kn][n][c] = s2[c] = 0.f;
         if constexpr (FP8) {
-          // a lane's 4 codes of a 16-byte piece are columns 4 t4 .. + 3: they serve as the
-          // fragment's k = 2 t4, + 1 and 2 t4 + 8, + 9, and the query fragments are laid out alike
-          if constexpr (KSTEPS == 1) {
+          // A lane's 4 codes of a 16-byte piece are columns 4 t4 .. + 3: they serve as the
+          // fragment's k = 2 t4, + 1 and 2 t4 + 8, + 9, and the query fragments are laid out alike.
 #pragma unroll
-            for (int kn = 0; kn < KN; ++kn) {
-              uint32_t a, z;
-              ldsm_x2(kb + swizzled<G::SPAN>(key_w + 16 * kn + (lane & 15), 0), a, z);
-              mma16816(s[2 * kn], qf[0], e4m3x2_to_h2(a), e4m3x2_to_h2(a >> 16), (C*)nullptr);
-              mma16816(s[2 * kn + 1], qf[0], e4m3x2_to_h2(z), e4m3x2_to_h2(z >> 16), (C*)nullptr);
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < KSTEPS; k += 2) {
-              const int piece = k + k_piece;
-#pragma unroll
-              for (int kn = 0; kn < KN; ++kn) {
-                uint32_t r[4];
-                ldsm_x4(kb + (piece * 16 / G::SPAN) * KEYS * G::SPAN +
-                            swizzled<G::SPAN>(k_row + 16 * kn, piece % (G::SPAN / 16)),
-                        r);
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                  mma16816(s[2 * kn + (u >> 1)], qf[k + (u & 1)], e4m3x2_to_h2(r[u]),
-                           e4m3x2_to_h2(r[u] >> 16), (C*)nullptr);
-              }
-            }
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < KSTEPS; ++k) {
-            const int piece = 2 * k + k_piece;
+          for (int k = 0; k < KSTEPS; k += 2)
 #pragma unroll
             for (int kn = 0; kn < KN; ++kn) {
               uint32_t r[4];
-              ldsm_x4(kb + (piece * 16 / G::SPAN) * KEYS * G::SPAN +
-                          swizzled<G::SPAN>(k_row + 16 * kn, piece % (G::SPAN / 16)),
-                      r);
-              mma16816(s[2 * kn], qf[k], r[0], r[1], (C*)nullptr);
-              mma16816(s[2 * kn + 1], qf[k], r[2], r[3], (C*)nullptr);
+              if constexpr (KSTEPS == 1) ldsm_x2(at(kb, a_row + 16 * kn, 0), r[0], r[1]);
+              else ldsm_x4(at(kb, a_row + 16 * kn, k + a_piece), r);
+#pragma unroll
+              for (int u = 0; u < (KSTEPS == 1 ? 1 : 2); ++u) {
+                const uint32_t a[4] = {e4m3x2_to_h2(r[2 * u]), e4m3x2_to_h2(r[2 * u + 1]),
+                                       e4m3x2_to_h2(r[2 * u] >> 16), e4m3x2_to_h2(r[2 * u + 1] >> 16)};
+#pragma unroll
+                for (int n = 0; n < WN; ++n)
+                  mma16816(SUMS == 2 && u ? s2 : s[kn][n], a, qf[n][k + u][0], qf[n][k + u][1], (C*)nullptr);
+              }
+            }
+        } else {
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+            for (int kn = 0; kn < KN; ++kn) {
+              uint32_t r[4];
+              ldsm_x4(at(kb, a_row + 16 * kn, 2 * k + a_piece), r);
+#pragma unroll
+              for (int n = 0; n < WN; ++n)
+                mma16816(SUMS == 2 && k % 2 ? s2 : s[kn][n], r, qf[n][k][0], qf[n][k][1], (C*)nullptr);
+            }
+        }
+        // ---- the V fragments are on their way during the softmax.  Float8: after the
+        // transposition a register holds keys 2 t4, + 1 at columns 2 g, + 1 of a piece.
+        uint32_t vr[KN][KSTEPS][FP8 ? 2 : 4];
+#pragma unroll
+        for (int kn = 0; kn < KN; ++kn)
+#pragma unroll
+          for (int d = 0; d < KSTEPS; d += FP8 ? 2 : 1) {
+            if constexpr (!FP8) {
+              ldsm_x4_t(at(vb, b_row + 16 * kn, 2 * d + b_piece), vr[kn][d]);
+            } else if constexpr (KSTEPS == 1) {
+              ldsm_x2_t(at(vb, a_row + 16 * kn, 0), vr[kn][0][0], vr[kn][0][1]);
+            } else {
+              uint32_t r[4];
+              ldsm_x4_t(at(vb, a_row + 16 * kn, d + a_piece), r);
+              vr[kn][d][0] = r[0];
+              vr[kn][d][1] = r[1];
+              vr[kn][d + 1][0] = r[2];
+              vr[kn][d + 1][1] = r[3];
             }
           }
+        if constexpr (SUMS == 2) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[0][0][c] += s2[c];
         }
-        // ---- scales and mask; this thread's keys are key0 + 8 n + 2 t4 + {0, 1}
-        float2 vs[2 * KN];
+        const bool tail = key0 + 16 * KN > w.s.len;
+        // ---- scales and mask; this thread's keys are key0 + 16 kn + g + {0, 8}
+        float vs[KN][2];
         if constexpr (FP8) {
-          const float* sk = reinterpret_cast<const float*>(smem + slot * G::STAGE + 2 * G::TILE) +
-                            key_w + 2 * t4;
+          const float* sk = reinterpret_cast<const float*>(smem + slot * G::STAGE + 2 * G::TILE) + key_w + g;
           float top = 0.f;
 #pragma unroll
-          for (int n = 0; n < 2 * KN; ++n) {
-            const float2 ks = *reinterpret_cast<const float2*>(sk + 8 * n);
-            vs[n] = *reinterpret_cast<const float2*>(sk + KEYS + 8 * n);
-            s[n][0] *= ks.x;
-            s[n][1] *= ks.y;
-            s[n][2] *= ks.x;
-            s[n][3] *= ks.y;
-          }
-          if (key0 + 16 * KN > w.s.len) {  // a scale behind the last key may be any bits
+          for (int kn = 0; kn < KN; ++kn)
 #pragma unroll
-            for (int n = 0; n < 2 * KN; ++n) {
-              const int k = key0 + 8 * n + 2 * t4;
-              vs[n].x = k < w.s.len ? vs[n].x : 0.f;
-              vs[n].y = k + 1 < w.s.len ? vs[n].y : 0.f;
+            for (int h = 0; h < 2; ++h) {
+              const float ks = sk[16 * kn + 8 * h];
+              vs[kn][h] = sk[KEYS + 16 * kn + 8 * h];
+              // a scale behind the last key may be any bits
+              if (tail && key0 + 16 * kn + 8 * h + g >= w.s.len) vs[kn][h] = 0.f;
+              top = fmaxf(top, vs[kn][h]);
+#pragma unroll
+              for (int n = 0; n < WN; ++n) {
+                s[kn][n][2 * h] *= ks;
+                s[kn][n][2 * h + 1] *= ks;
+              }
             }
-          }
-#pragma unroll
-          for (int n = 0; n < 2 * KN; ++n) top = fmax3(top, vs[n].x, vs[n].y);
           if (__any_sync(0xffffffffu, top > mv)) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const float f = mv / top;  // the same in every lane
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int d = 0; d < KSTEPS; ++d)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) o[n][c] *= f;
+              for (int n = 0; n < WN; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[d][n][c] *= f;
             mv = top;
             inv_mv = 1.f / top;
           }
 #pragma unroll
-          for (int n = 0; n < 2 * KN; ++n) {
-            vs[n].x *= inv_mv;
-            vs[n].y *= inv_mv;
-          }
+          for (int kn = 0; kn < KN; ++kn)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) vs[kn][h] *= inv_mv;
         }
         if (key0 + 16 * KN > lim_all) {
 #pragma unroll
-          for (int n = 0; n < 2 * KN; ++n)
+          for (int kn = 0; kn < KN; ++kn)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (key0 + 8 * n + 2 * t4 + (c & 1) >= lim[c >> 1]) s[n][c] = -INFINITY;
+            for (int n = 0; n < WN; ++n)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                if (key0 + 16 * kn + g + 8 * (c >> 1) >= lim[n][c & 1]) s[kn][n][c] = -INFINITY;
         }
         // ---- online softmax of each row; the base moves by steps
-        float top[2];
+        bool move = false;
+        float top[WN][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(s[0][2 * e], s[0][2 * e + 1]);
-#pragma unroll
-          for (int n = 1; n < 2 * KN; ++n) x = fmax3(x, s[n][2 * e], s[n][2 * e + 1]);
-          top[e] = x * qs[e];
-        }
-        if (__any_sync(0xffffffffu, top[0] > m[0] + kRescale || top[1] > m[1] + kRescale)) {
+        for (int n = 0; n < WN; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = top[e];
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-            const float to = x > m[e] + kRescale ? x : m[e];
-            const float f = m[e] == to ? 1.f : ex2_approx(m[e] - to);
-            m[e] = to;
-            l[e] *= f;
+            float x = fmaxf(s[0][n][e], s[0][n][2 + e]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              o[n][2 * e] *= f;
-              o[n][2 * e + 1] *= f;
-            }
+            for (int kn = 1; kn < KN; ++kn) x = fmax3(x, s[kn][n][e], s[kn][n][2 + e]);
+            top[n][e] = x * qs[n][e];
+            move |= top[n][e] > m[n][e] + kRescale;
           }
-        }
-        uint32_t pf[KN][4];
+        if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float shift = (m[e] == -INFINITY ? 0.f : -m[e]) + kPOffset;
+          for (int n = 0; n < WN; ++n)
 #pragma unroll
-          for (int n = 0; n < 2 * KN; ++n) {
-            float a = ex2_approx(fmaf(s[n][2 * e], qs[e], shift));
-            float z = ex2_approx(fmaf(s[n][2 * e + 1], qs[e], shift));
-            l[e] += a + z;
-            if constexpr (FP8) {
-              a *= vs[n].x;
-              z *= vs[n].y;
+            for (int e = 0; e < 2; ++e) {
+              float x = top[n][e];
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+              const float to = x > m[n][e] + kRescale ? x : m[n][e];
+              const float f = m[n][e] == to ? 1.f : ex2_approx(m[n][e] - to);
+              m[n][e] = to;
+              l[n][e] *= f;
+#pragma unroll
+              for (int d = 0; d < KSTEPS; ++d) {
+                o[d][n][e] *= f;
+                o[d][n][2 + e] *= f;
+              }
             }
-            pf[n >> 1][2 * (n & 1) + e] = pack2(a, z, static_cast<C*>(nullptr));
-          }
         }
-        // ---- O += P V; what lies behind the sequence's last key may be any bits: it counts as 0
-        const bool tail = key0 + 16 * KN > w.s.len;
+        uint32_t pf[KN][WN][2];  // P^T: keys 2 t4, + 1 (and + 8) of row g
+#pragma unroll
+        for (int n = 0; n < WN; ++n) {
+          const float shift0 = (m[n][0] == -INFINITY ? 0.f : -m[n][0]) + kPOffset;
+          const float shift1 = (m[n][1] == -INFINITY ? 0.f : -m[n][1]) + kPOffset;
+#pragma unroll
+          for (int kn = 0; kn < KN; ++kn)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float a = ex2_approx(fmaf(s[kn][n][2 * h], qs[n][0], shift0));
+              float z = ex2_approx(fmaf(s[kn][n][2 * h + 1], qs[n][1], shift1));
+              l[n][0] += a;
+              l[n][1] += z;
+              if constexpr (FP8) {
+                a *= vs[kn][h];
+                z *= vs[kn][h];
+              }
+              pf[kn][n][h] = transposed(pack2(a, z, static_cast<C*>(nullptr)));
+            }
+        }
+        // ---- O^T += V^T P^T; what lies behind the sequence's last key may be any bits: it counts
+        // as 0
 #pragma unroll
         for (int kn = 0; kn < KN; ++kn) {
           uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
@@ -501,57 +576,33 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, WM>::THREADS, 1)
             keep0 = a >= 2 ? 0xffffffffu : a == 1 ? 0xffffu : 0u;
             keep1 = z >= 2 ? 0xffffffffu : z == 1 ? 0xffffu : 0u;
           }
-          if constexpr (FP8) {
-            // after the transposition a register holds keys 2 t4, + 1 at columns 2 g, + 1 of the
-            // piece; its bytes regrouped give the fragments of the even and the odd columns
 #pragma unroll
-            for (int c = 0; c < KSTEPS; c += 2) {
-              uint32_t r[4];
-              if constexpr (KSTEPS == 1) {
-                ldsm_x2_t(vb + swizzled<G::SPAN>(v_row + 16 * kn, 0), r[0], r[1]);
-                r[2] = r[3] = 0;
-              } else {
-                const int piece = c + v_piece;
-                ldsm_x4_t(vb + (piece * 16 / G::SPAN) * KEYS * G::SPAN +
-                              swizzled<G::SPAN>(v_row + 16 * kn, piece % (G::SPAN / 16)),
-                          r);
-              }
+          for (int d = 0; d < KSTEPS; ++d) {
+            uint32_t a[4];
+            if constexpr (FP8) {  // bytes regrouped by column: 2 g in rows g, 2 g + 1 in rows g + 8
+              const uint32_t x = __byte_perm(vr[kn][d][0], 0, 0x3120);
+              const uint32_t z = __byte_perm(vr[kn][d][1], 0, 0x3120);
+              a[0] = e4m3x2_to_h2(x);
+              a[1] = e4m3x2_to_h2(x >> 16);
+              a[2] = e4m3x2_to_h2(z);
+              a[3] = e4m3x2_to_h2(z >> 16);
+            } else {
 #pragma unroll
-              for (int u = 0; u < (KSTEPS == 1 ? 1 : 2); ++u) {
-                const uint32_t a = __byte_perm(r[2 * u], 0, 0x3120);
-                const uint32_t z = __byte_perm(r[2 * u + 1], 0, 0x3120);
-                uint32_t e0 = e4m3x2_to_h2(a), e1 = e4m3x2_to_h2(z);
-                uint32_t d0 = e4m3x2_to_h2(a >> 16), d1 = e4m3x2_to_h2(z >> 16);
-                if (tail) {
-                  e0 &= keep0;
-                  d0 &= keep0;
-                  e1 &= keep1;
-                  d1 &= keep1;
-                }
-                mma16816(o[2 * (c + u)], pf[kn], e0, e1, (C*)nullptr);
-                mma16816(o[2 * (c + u) + 1], pf[kn], d0, d1, (C*)nullptr);
-              }
+              for (int c = 0; c < 4; ++c) a[c] = vr[kn][d][c];
             }
-          } else {
-#pragma unroll
-            for (int c = 0; c < KSTEPS; ++c) {
-              uint32_t r[4];
-              const int piece = 2 * c + v_piece;
-              ldsm_x4_t(vb + (piece * 16 / G::SPAN) * KEYS * G::SPAN +
-                            swizzled<G::SPAN>(v_row + 16 * kn, piece % (G::SPAN / 16)),
-                        r);
-              if (tail) {
-                r[0] &= keep0;
-                r[1] &= keep1;
-                r[2] &= keep0;
-                r[3] &= keep1;
-              }
-              mma16816(o[2 * c], pf[kn], r[0], r[1], (C*)nullptr);
-              mma16816(o[2 * c + 1], pf[kn], r[2], r[3], (C*)nullptr);
+            if (tail) {
+              a[0] &= keep0;
+              a[1] &= keep0;
+              a[2] &= keep1;
+              a[3] &= keep1;
             }
+#pragma unroll
+            for (int n = 0; n < WN; ++n)
+              mma16816(o[d][n], a, pf[kn][n][0], pf[kn][n][1], (C*)nullptr);
           }
         }
       }
+      if (t + 1 == w.tile1) break;  // the last stage is kept for joining
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&s_empty[slot]));
       if (++slot == G::STAGES) {
@@ -562,91 +613,115 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, WM>::THREADS, 1)
 
     // ---- join the warps' parts and write the rows (the barriers are passed on every path)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-      if (t4 == 0) {
-        s_m[warp][e * 8 + g] = m[e];
-        s_l[warp][e * 8 + g] = l[e];
+    for (int n = 0; n < WN; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+        if (g == 0) {
+          s_m[first + 8 * n + 2 * t4 + e][wk] = m[n][e];
+          s_l[first + 8 * n + 2 * t4 + e][wk] = l[n][e];
+        }
       }
-    }
     named_barrier_sync(1, NW * 32);
     const bool whole = w.whole();
-    const int64_t part_row = (static_cast<int64_t>(blockIdx.x) * 2 + w.slot()) * G::ROWS;
+    const int64_t part_row = (static_cast<int64_t>(blockIdx.x) * 2 + w.slot()) * ROWS + my_r;
     if (!whole && w.slot() == 0 && threadIdx.x == 0) p.parts[blockIdx.x] = w.note();
-    float f[2];  // this warp's weight in its rows
+    // the largest base of a row's warps
+    auto top_of = [&](int r) -> float {
+      float x = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < WK; ++u) top = fmaxf(top, s_m[wm * WK + u][e * 8 + g]);
-      f[e] = m[e] == -INFINITY ? 0.f : ex2_approx(m[e] - top);
-      if (FP8) f[e] *= mv;
-    }
-    // the row that this thread writes, and 1 / l of it
-    constexpr int TPR = NW * 32 / G::ROWS;  // threads of a row
-    const int r = threadIdx.x / TPR;
-    const int w0 = r / 16 * WK;             // the first warp of its group
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int u = 0; u < WK; ++u) top = fmaxf(top, s_m[w0 + u][r % 16]);
-#pragma unroll
-    for (int u = 0; u < WK; ++u) {
-      const float x = s_m[w0 + u][r % 16];
-      sum += s_l[w0 + u][r % 16] * (x == -INFINITY ? 1.f : ex2_approx(x - top));  // 1: l is 0, or NaN
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int row = row0 + r;
-    const bool live = row < rows;
-    const int64_t tok = w.s.first + row / p.group;
-    const int64_t h = w.head * p.group + row % p.group;
-    if (live && threadIdx.x % TPR == 0) {
-      const float lse2 = sum == 0.f ? -INFINITY : top + (log2f(sum) - kPOffset);
-      if (whole) p.lse[tok * p.heads_kv * p.group + h] = lse2 * kLn2;
-      else p.part_lse[part_row + r] = lse2;
-    }
-    T* out = static_cast<T*>(p.o) + tok * p.o_stride[0] + h * p.o_stride[1];
-    float* part = p.part_o + (part_row + r) * D;
-#pragma unroll
-    for (int c0 = 0; c0 < D; c0 += G::GROUP_COLS) {
-      float* mine = s_join + warp * 16 * G::JOIN_PITCH;
-      if constexpr (FP8) {
-#pragma unroll
-        for (int c = 0; c < G::GROUP_COLS / 16; ++c) {
-          const int n = 2 * (c0 / 16 + c);
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<float4*>(mine + (e * 8 + g) * G::JOIN_PITCH + 16 * c + 4 * t4) =
-                make_float4(o[n][2 * e] * f[e], o[n + 1][2 * e] * f[e],
-                            o[n][2 * e + 1] * f[e], o[n + 1][2 * e + 1] * f[e]);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < G::GROUP_COLS / 8; ++c) {
-          const int n = c0 / 8 + c;
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            *reinterpret_cast<float2*>(mine + (e * 8 + g) * G::JOIN_PITCH + 8 * c + 2 * t4) =
-                make_float2(o[n][2 * e] * f[e], o[n][2 * e + 1] * f[e]);
-        }
+      for (int u = 0; u < WK; u += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(&s_m[r][u]);
+        x = fmax3(fmax3(x, v.x, v.y), v.z, v.w);
       }
-      named_barrier_sync(1, NW * 32);
-      for (int c = (threadIdx.x % TPR) * 2; c < G::GROUP_COLS; c += TPR * 2) {
-        float a = 0.f, z = 0.f;
+      return x;
+    };
+    float f[WN][2];  // this warp's weight in its rows
+#pragma unroll
+    for (int n = 0; n < WN; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        f[n][e] = m[n][e] == -INFINITY ? 0.f : ex2_approx(m[n][e] - top_of(first + 8 * n + 2 * t4 + e));
+        if (FP8) f[n][e] *= mv;
+      }
+    float* const join = reinterpret_cast<float*>(smem + slot * G::STAGE);
+    // column c of row x lies at c ^ turn(x): the rows that are written at once differ in banks
+    auto turn = [](int x) { return ((x >> 1) & 3) * 8 & (G::DR - 1); };
+    float inv = 0.f;
+#pragma unroll
+    for (int c0 = 0; c0 < D; c0 += G::DR) {
+      if (c0 > 0) named_barrier_sync(1, NW * 32);
+#pragma unroll
+      for (int n = 0; n < WN; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int x = 8 * n + 2 * t4 + e;
+          if (row0 + first + x >= rows) continue;  // decoding uses few of the rows
+          float* mine = join + (warp * 8 * WN + x) * G::DR;
+#pragma unroll
+          for (int d = 0; d < G::DR / 16; ++d) {
+            const float(&v)[4] = o[c0 / 16 + d][n];
+            if constexpr (FP8) {
+              *reinterpret_cast<float2*>(mine + ((16 * d + 2 * g) ^ turn(x))) =
+                  make_float2(v[e] * f[n][e], v[2 + e] * f[n][e]);
+            } else {
+              mine[(16 * d + g) ^ turn(x)] = v[e] * f[n][e];
+              mine[(16 * d + 8 + g) ^ turn(x)] = v[2 + e] * f[n][e];
+            }
+          }
+        }
+      if (c0 == 0 && my_live) {
+        // 1 / l of the thread's row, and its logsumexp
+        const float top = top_of(my_r);
+        float sum = 0.f;
 #pragma unroll
         for (int u = 0; u < WK; ++u) {
-          const float2 x = *reinterpret_cast<const float2*>(s_join + ((w0 + u) * 16 + r % 16) * G::JOIN_PITCH + c);
-          a += x.x;
-          z += x.y;
+          const float x = s_m[my_r][u];
+          sum += s_l[my_r][u] * (x == -INFINITY ? 1.f : ex2_approx(x - top));  // 1: l is 0, or NaN
         }
-        if (live) {
-          if (whole)
-            *reinterpret_cast<uint32_t*>(out + c0 + c) = pack2(a * inv, z * inv, static_cast<T*>(nullptr));
-          else
-            *reinterpret_cast<float2*>(part + c0 + c) = make_float2(a * inv, z * inv);
+        inv = sum == 0.f ? 0.f : 1.f / sum;
+        if (threadIdx.x % TPR == 0) {
+          const float lse2 = sum == 0.f ? -INFINITY : top + (log2f(sum) - kPOffset);
+          if (whole) p.lse[static_cast<int64_t>(w.s.first + my_tok) * p.heads_kv * p.group + my_head] = lse2 * kLn2;
+          else p.part_lse[part_row] = lse2;
         }
       }
       named_barrier_sync(1, NW * 32);
+      const int w0 = my_r / (8 * WN) * WK;  // the first warp of the row's group
+#pragma unroll
+      for (int i = 0; i < (G::DR + TPR * 4 - 1) / (TPR * 4); ++i) {
+        const int c = (threadIdx.x % TPR + i * TPR) * 4;
+        if (c >= G::DR || !my_live) break;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < WK; ++u) {
+          const int x = my_r % (8 * WN);
+          const float4 v = *reinterpret_cast<const float4*>(
+              join + ((w0 + u) * 8 * WN + x) * G::DR + (c ^ turn(x)));
+          a.x += v.x;
+          a.y += v.y;
+          a.z += v.z;
+          a.w += v.w;
+        }
+        if (whole)
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.o) +
+                                    static_cast<int64_t>(w.s.first + my_tok) * p.o_stride[0] +
+                                    my_head * p.o_stride[1] + c0 + c) =
+              make_uint2(pack2(a.x * inv, a.y * inv, static_cast<T*>(nullptr)),
+                         pack2(a.z * inv, a.w * inv, static_cast<T*>(nullptr)));
+        else
+          *reinterpret_cast<float4*>(p.part_o + part_row * D + c0 + c) =
+              make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+      }
+    }
+    // the stage goes back to the producers, whose copies are ordered behind these accesses
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&s_empty[slot]));
+    if (++slot == G::STAGES) {
+      slot = 0;
+      ph ^= 1u;
     }
   }
 }

@@ -74,7 +74,6 @@ struct TileShared {
   uint64_t raw_full[4], raw_empty[4];
   uint64_t s_full[2], p_ready[2], o_full[2], o_empty[2];
   uint64_t mma_done;
-  int64_t scratch[40];
   int issued[2];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
@@ -122,7 +121,7 @@ __global__ void __launch_bounds__(512, 1)
   const int lane = threadIdx.x & 31;
   int* const status = p.seqs.status;
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_launch();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&sh->kv_full[s]), FP8 ? 4 : 1);  // converting warps, or the producer
@@ -145,7 +144,6 @@ __global__ void __launch_bounds__(512, 1)
     mbar_init(smem_u32(&sh->mma_done), TILES);
     sh->abort_flag = 0u;
     fence_mbar_init();
-    p.parts[blockIdx.x].first_cta = -2;
   }
   if (warp == 12) {
     tmem_alloc(smem_u32(&sh->tmem_base), 512);
@@ -158,12 +156,14 @@ __global__ void __launch_bounds__(512, 1)
         *reinterpret_cast<uint4*>(q_smem + x) = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
   }
-  const PagedRange range = paged_range(
-      p, sh->scratch, [&](int b) { return PagedTiles<TILES, KEYS>(p, b).steps(p); });
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
+  wait_for_launch_before();
+  if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
+  const PagedRange range =
+      paged_range(p, [&](int b) { return PagedTiles<TILES, KEYS>(p, b).steps(p); });
 
   auto wait1 = [&](uint64_t& bar, uint32_t parity) {
     return wait_bar_flag(&sh->abort_flag, smem_u32(&bar), parity, status);

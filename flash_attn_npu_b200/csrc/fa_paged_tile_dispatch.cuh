@@ -28,13 +28,14 @@ int launch_tile(const PagedPlan& plan) {
   if (regs_ok != 1) return -7;
   static SmemOptIn opt_in;
   if (!opt_in(reinterpret_cast<const void*>(kernel), G::SMEM)) return -7;
-  kernel<<<plan.grid, G::THREADS, G::SMEM, plan.stream>>>(plan.tmQ, plan.tmK, plan.tmV, plan.params);
-  if (cudaGetLastError() != cudaSuccess) return -7;
+  const int rc = launch_dependent(kernel, dim3(plan.grid), G::THREADS, G::SMEM, plan.stream,
+                                  plan.tmQ, plan.tmK, plan.tmV, plan.params);
+  if (rc != 0) return rc;
   if (plan.grid == 1 || plan.params.whole_items) return 0;  // no shared item
   // a warp to a row: shared items mostly have two or three parts
   constexpr int kRows = 8;
   return launch_dependent(paged_combine_kernel<T, 128, G::TILES, 1, kRows>, dim3(plan.grid - 1, 16),
-                          kRows * 32, plan.stream, plan.params);
+                          kRows * 32, 0, plan.stream, plan.params);
 }
 
 int launch_any(const PagedPlan& plan) {

@@ -113,6 +113,8 @@ def validate_attention(q, k_cache, v_cache, page_table, offsets, kv_lens, k_scal
     if q.ndim != 3 or q.shape[1] == 0 or q.shape[1] % heads_kv:
         raise ValueError("q must be [total, heads_q, head_dim], heads_q a multiple of heads_kv")
     _validate_rows("q", q, k_cache, q.shape[1])
+    if q.shape[1] > 32768:
+        raise ValueError("q has more than 32768 heads")
     if q.shape[0] * q.shape[1] > (1 << 30) - 1:
         raise ValueError("q has more than 2^30 - 1 (token, head) rows")
     if max_q_len is not None and max_q_len < 0:
