@@ -7,23 +7,23 @@
 // magnitude; only rows that spread over more than 2^14 reach its subnormals), makes x / s, c * s
 // and the scale itself exact, and leaves the one rounding to 4 bits.
 //
-// Both directions are bound by memory: each value is read and written once, in 16-byte pieces
-// (8 values, 8 bytes on the float8 side), head_dim / 8 threads to a row, so that a row's largest
-// magnitude is a few shuffles.  Each CTA takes a run of tokens: its warps first look up the
-// sequence and the page of one token each (a 32-way search of the offsets), then all threads move
-// the run's rows, kUnroll pieces in flight each.
+// Both directions are bound by memory: each value is read and written once, a thread's piece being 16
+// bytes of a 16-bit row or 16 codes of a float8 row (32 bytes of the packed one), head_dim / PIECE
+// threads to a row, so that a row's largest magnitude is a few shuffles.  Each CTA takes a run of
+// tokens, whose sequences and pages its warps look up (a 32-way search of the offsets).  A write has
+// its packed rows on their way before that; a read cannot, so its CTAs are small and many to an SM.
 #include <cmath>
 
 #include "../../include/fa_paged_sm100.h"
 #include "fa_paged_host.h"
-#include "sm100_ptx.cuh"
+#include "fa_paged_launch.h"
 
 namespace fa {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 64;  // tokens of one CTA's run
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 4;      // pieces of a thread in flight
 
 struct CopyParams {
   PagedSeqs seqs;
@@ -35,7 +35,9 @@ struct CopyParams {
   int64_t row_stride[2][2];
   int heads;
   int head_dim;
-  int tokens;  // per CTA
+  int tokens;           // per CTA
+  int lanes_log2;       // pieces of a row
+  uint32_t pieces_inv;  // floor(2^32 / pieces of a token) + 1; 0 for a run of one token
 };
 
 // Smallest b with offsets[b + 1] > t, by the whole warp (seqs - 1 if there is none).
@@ -54,93 +56,119 @@ __device__ __forceinline__ int find_seq(const PagedSeqs& s, int t, int lane) {
   return lo;
 }
 
+// Elements of a piece.
+template <bool FP8>
+constexpr int kPiece = FP8 ? 16 : 8;
+
 // T: type of the packed rows.  FP8: the cache holds e4m3 codes and scales, else T.  WRITE: rows
 // go to the cache, else from it.
 template <typename T, bool FP8, bool WRITE>
-__global__ void __launch_bounds__(kThreads) paged_copy_kernel(const CopyParams p) {
+__global__ void __launch_bounds__(kThreads, 4) paged_copy_kernel(const CopyParams p) {
+  constexpr int PIECE = kPiece<FP8>;
+  constexpr int WORDS = PIECE / 8;  // 16-byte words of a packed piece
   __shared__ int s_page[kMaxTokens];
   __shared__ int s_slot[kMaxTokens];
+  let_next_launch();
+  wait_for_launch_before();
   const int t0 = blockIdx.x * p.tokens;
   const int count = min(p.tokens, p.seqs.total - t0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = warp; i < count; i += kThreads / 32) {
-    const int t = t0 + i;
-    const int b = find_seq(p.seqs, t, lane);
-    if (lane == 0) {
-      const int end = __ldg(p.seqs.offsets + b + 1);
-      int page = -2, pos = 0;  // -2: behind the last sequence
-      if (t < end && t >= __ldg(p.seqs.offsets + b)) {
-        pos = __ldg(p.seqs.kv_lens + b) - (end - t);
-        page = page_of(p.seqs, b, pos);
-        if (page < 0) report(p.seqs.status, kStatusPageTable);
-      }
-      s_page[i] = page;
-      s_slot[i] = pos & ((1 << p.seqs.page_log2) - 1);
-    }
-  }
-  __syncthreads();
-
-  const int lanes = p.head_dim >> 3;            // threads of a row: 2 .. 32
-  const int pieces = lanes * p.heads * 2;       // of a token
+  const int lanes = 1 << p.lanes_log2;
+  const int pieces = lanes * p.heads * 2;  // of a token
   const int n = pieces * count;
+
+  // piece i of the run: its token, K or V, head, first element, and place in the packed rows
+  struct Place {
+    int tok, kv, head, elem;
+  };
+  auto place = [&](int i) -> Place {
+    Place x;
+    x.tok = static_cast<int>(__umulhi(static_cast<uint32_t>(i), p.pieces_inv));
+    const int rest = i - x.tok * pieces;
+    const int row = rest >> p.lanes_log2;
+    x.kv = row >= p.heads;
+    x.head = row - x.kv * p.heads;
+    x.elem = (rest & (lanes - 1)) * PIECE;
+    return x;
+  };
+  auto packed = [&](const Place& x) -> T* {
+    return static_cast<T*>(p.rows[x.kv]) + static_cast<int64_t>(t0 + x.tok) * p.row_stride[x.kv][0] +
+           x.head * p.row_stride[x.kv][1] + x.elem;
+  };
+  auto cached = [&](const Place& x) -> int64_t {
+    return s_page[x.tok] * p.cache_stride[x.kv][0] + x.head * p.cache_stride[x.kv][1] +
+           s_slot[x.tok] * p.cache_stride[x.kv][2] + x.elem;
+  };
+  auto scale_of = [&](const Place& x) -> float* {
+    return p.scale[x.kv] + s_page[x.tok] * p.scale_stride[x.kv][0] +
+           x.head * p.scale_stride[x.kv][1] + s_slot[x.tok];
+  };
+  auto look_up = [&]() {
+    for (int i = warp; i < count; i += kThreads / 32) {
+      const int t = t0 + i;
+      const int b = find_seq(p.seqs, t, lane);
+      if (lane == 0) {
+        const int end = __ldg(p.seqs.offsets + b + 1);
+        int page = -2, pos = 0;  // -2: of no sequence
+        if (t < end && t >= __ldg(p.seqs.offsets + b)) {
+          pos = __ldg(p.seqs.kv_lens + b) - (end - t);
+          page = page_of(p.seqs, b, pos);
+          if (page < 0) report(p.seqs.status, kStatusPageTable);
+        }
+        s_page[i] = page;
+        s_slot[i] = pos & ((1 << p.seqs.page_log2) - 1);
+      }
+    }
+    __syncthreads();
+  };
+
+  if (!WRITE) look_up();
   // every thread makes the same number of turns: the shuffles below take whole warps
   for (int at = 0; at < n; at += kThreads * kUnroll) {
-    uint4 x[kUnroll];
+    uint4 x[kUnroll][WORDS];
     float sc[kUnroll];
-    int64_t packed[kUnroll], held[kUnroll], held_scale[kUnroll];
-    int kv[kUnroll];
-    bool on[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int i = at + u * kThreads + threadIdx.x;
-      on[u] = i < n;
-      const int tok = on[u] ? i / pieces : 0;
-      const int rest = i - tok * pieces;
-      const int piece = rest & (lanes - 1);
-      const int hv = rest / lanes;
-      kv[u] = hv >= p.heads;
-      const int h = hv - kv[u] * p.heads;
-      const int page = s_page[tok];
-      on[u] = on[u] && page != -2 && (!WRITE || page >= 0);
-      packed[u] = (t0 + tok) * p.row_stride[kv[u]][0] + h * p.row_stride[kv[u]][1] + piece * 8;
-      const int64_t pg = page;
-      held[u] = pg < 0 ? -1
-                       : pg * p.cache_stride[kv[u]][0] + h * p.cache_stride[kv[u]][1] +
-                             s_slot[tok] * p.cache_stride[kv[u]][2] + piece * 8;
-      if (FP8)
-        held_scale[u] = pg * p.scale_stride[kv[u]][0] + h * p.scale_stride[kv[u]][1] + s_slot[tok];
-      x[u] = make_uint4(0, 0, 0, 0);
       sc[u] = 0.f;
-      if (WRITE) {
-        if (on[u])
-          x[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.rows[kv[u]]) +
-                                                      packed[u]));
-      } else if (on[u] && held[u] >= 0) {
-        if (FP8) {
-          const uint2 c = __ldg(reinterpret_cast<const uint2*>(
-              static_cast<const uint8_t*>(p.cache[kv[u]]) + held[u]));
-          x[u].x = c.x;
-          x[u].y = c.y;
-          sc[u] = __ldg(p.scale[kv[u]] + held_scale[u]);
-        } else {
-          x[u] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.cache[kv[u]]) +
-                                                      held[u]));
+#pragma unroll
+      for (int k = 0; k < WORDS; ++k) x[u][k] = make_uint4(0, 0, 0, 0);
+      if (i < n) {
+        const Place q = place(i);
+        if (WRITE) {
+#pragma unroll
+          for (int k = 0; k < WORDS; ++k) x[u][k] = __ldg(reinterpret_cast<const uint4*>(packed(q)) + k);
+        } else if (s_page[q.tok] >= 0) {
+          const int64_t c = cached(q);
+          if (FP8) {
+            x[u][0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.cache[q.kv]) + c));
+            sc[u] = __ldg(scale_of(q));
+          } else {
+            x[u][0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.cache[q.kv]) + c));
+          }
         }
       }
     }
+    if (WRITE && at == 0) look_up();
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (!FP8) {
-        T* dst = WRITE ? static_cast<T*>(p.cache[kv[u]]) + held[u]
-                       : static_cast<T*>(p.rows[kv[u]]) + packed[u];
-        if (on[u]) *reinterpret_cast<uint4*>(dst) = x[u];
-      } else if (WRITE) {
-        float2 f[4] = {Cvt16<T>::unpack(x[u].x), Cvt16<T>::unpack(x[u].y),
-                       Cvt16<T>::unpack(x[u].z), Cvt16<T>::unpack(x[u].w)};
-        float top = 0.f;
-        float* e = reinterpret_cast<float*>(f);
+      const int i = at + u * kThreads + threadIdx.x;
+      const bool in = i < n;
+      const Place q = place(in ? i : 0);
+      const bool on = in && (WRITE ? s_page[q.tok] >= 0 : s_page[q.tok] != -2);
+      if constexpr (!FP8) {
+        if (on) *reinterpret_cast<uint4*>(WRITE ? static_cast<T*>(p.cache[q.kv]) + cached(q) : packed(q)) = x[u][0];
+      } else if constexpr (WRITE) {
+        float e[16];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
+          const float2 f = Cvt16<T>::unpack(k < 4 ? (&x[u][0].x)[k] : (&x[u][WORDS - 1].x)[k - 4]);
+          e[2 * k] = f.x;
+          e[2 * k + 1] = f.y;
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
           const float a = fabsf(e[k]);
           if (a < INFINITY) top = fmaxf(top, a);
           else e[k] = NAN;
@@ -153,30 +181,30 @@ __global__ void __launch_bounds__(kThreads) paged_copy_kernel(const CopyParams p
         int ex = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u);
         ex = top == 0.f ? 0 : max(ex, -126);
         const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-        uint2 c;
-        c.x = pack2_e4m3(e[0] * inv, e[1] * inv) | (pack2_e4m3(e[2] * inv, e[3] * inv) << 16);
-        c.y = pack2_e4m3(e[4] * inv, e[5] * inv) | (pack2_e4m3(e[6] * inv, e[7] * inv) << 16);
-        if (on[u]) {
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.cache[kv[u]]) + held[u]) = c;
-          if ((threadIdx.x & (lanes - 1)) == 0)
-            p.scale[kv[u]][held_scale[u]] = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+        uint32_t c[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          c[k] = pack2_e4m3(e[4 * k] * inv, e[4 * k + 1] * inv) |
+                 (pack2_e4m3(e[4 * k + 2] * inv, e[4 * k + 3] * inv) << 16);
+        if (on) {
+          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.cache[q.kv]) + cached(q)) =
+              make_uint4(c[0], c[1], c[2], c[3]);
+          if (q.elem == 0) *scale_of(q) = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
         }
       } else {
-        uint32_t out[4];
+        uint32_t out[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t w = k < 2 ? x[u].x : x[u].y;
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t w = (&x[u][0].x)[k >> 1];
           const uint32_t h2 = e4m3x2_to_h2(static_cast<uint16_t>(w >> (16 * (k & 1))));
           const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-          if constexpr (sizeof(T) == 2) {
-            const T a = static_cast<T>(v.x * sc[u]), z = static_cast<T>(v.y * sc[u]);
-            out[k] = *reinterpret_cast<const uint16_t*>(&a) |
-                     (static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&z)) << 16);
-          }
+          out[k] = pack2(v.x * sc[u], v.y * sc[u], static_cast<T*>(nullptr));
         }
-        if (on[u])
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.rows[kv[u]]) + packed[u]) =
-              make_uint4(out[0], out[1], out[2], out[3]);
+        if (on) {
+          uint4* dst = reinterpret_cast<uint4*>(packed(q));
+          dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
+          dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+        }
       }
     }
   }
@@ -216,24 +244,26 @@ int copy_rows(const FaPagedCopyArgs* a, void* stream, bool write) {
   }
   p.heads = static_cast<int>(a->cache.heads_kv);
   p.head_dim = static_cast<int>(a->cache.head_dim);
-  // A CTA's run: enough tokens for two rounds of kUnroll pieces a thread, fewer where that would
+  // A CTA's run: enough tokens for one round of kUnroll pieces a thread, fewer where that would
   // leave SMs without a CTA.
-  const int64_t pieces = a->cache.head_dim / 8 * a->cache.heads_kv * 2;
-  int64_t tokens = 2 * kThreads * kUnroll / pieces;
-  const int64_t share = a->total / (4 * sm_count_of_current());
+  const bool f8 = a->cache.dtype == FA_DTYPE_FP8_E4M3, half = a->dtype == FA_DTYPE_FP16;
+  const int64_t lanes = a->cache.head_dim / (f8 ? kPiece<true> : kPiece<false>);
+  const int64_t pieces = lanes * a->cache.heads_kv * 2;
+  int64_t tokens = kThreads * kUnroll / pieces;
+  const int64_t share = a->total / (2 * sm_count_of_current());
   if (tokens > share) tokens = share;
   p.tokens = static_cast<int>(tokens < 1 ? 1 : tokens > kMaxTokens ? kMaxTokens : tokens);
+  p.lanes_log2 = log2_of(lanes);
+  p.pieces_inv = p.tokens == 1 ? 0u : static_cast<uint32_t>((int64_t{1} << 32) / pieces + 1);
   const int64_t grid = (a->total + p.tokens - 1) / p.tokens;
-  const dim3 g(static_cast<unsigned>(grid)), t(kThreads);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool f8 = a->cache.dtype == FA_DTYPE_FP8_E4M3, half = a->dtype == FA_DTYPE_FP16;
-  if (f8 && half && write) paged_copy_kernel<__half, true, true><<<g, t, 0, st>>>(p);
-  else if (f8 && half) paged_copy_kernel<__half, true, false><<<g, t, 0, st>>>(p);
-  else if (f8 && write) paged_copy_kernel<__nv_bfloat16, true, true><<<g, t, 0, st>>>(p);
-  else if (f8) paged_copy_kernel<__nv_bfloat16, true, false><<<g, t, 0, st>>>(p);
-  else if (write) paged_copy_kernel<__half, false, true><<<g, t, 0, st>>>(p);  // any 16-bit type
-  else paged_copy_kernel<__half, false, false><<<g, t, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+  const auto kernel = f8 && half ? (write ? paged_copy_kernel<__half, true, true>
+                                          : paged_copy_kernel<__half, true, false>)
+                      : f8       ? (write ? paged_copy_kernel<__nv_bfloat16, true, true>
+                                          : paged_copy_kernel<__nv_bfloat16, true, false>)
+                                 : (write ? paged_copy_kernel<__half, false, true>  // any 16 bits
+                                          : paged_copy_kernel<__half, false, false>);
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(grid)), kThreads, 0,
+                          static_cast<cudaStream_t>(stream), p);
 }
 
 }  // namespace
