@@ -229,7 +229,7 @@ struct PagedTiles {
   __device__ __forceinline__ int block_tiles(const PagedAttnParams& p, int block) const {
     return tiles(p, (block + 1) * TILES * p.tile_toks);
   }
-  __device__ __forceinline__ PagedTiles() {}
+  PagedTiles() = default;
   __device__ __forceinline__ PagedTiles(const PagedAttnParams& p, int b) {
     seq_rows(p.seqs, b, first, count);
     len = seq_len(p.seqs, b);
@@ -246,10 +246,9 @@ struct PagedTiles {
   }
 };
 
+// (plain data: it lives in shared memory)
 template <int TILES, int KEYS>
 struct PagedTileWalk {
-  const PagedAttnParams& p;
-  const PagedRange& range;
   int64_t pos;
   int b;
   PagedTiles<TILES, KEYS> s;
@@ -259,9 +258,10 @@ struct PagedTileWalk {
   int tile0, tile1;  // those of the part
   int64_t item;      // the item's first step
 
-  __device__ __forceinline__ PagedTileWalk(const PagedAttnParams& params, const PagedRange& r)
-      : p(params), range(r), pos(r.lo), b(r.seq) {
-    if (pos >= range.hi) return;
+  PagedTileWalk() = default;
+  __device__ __forceinline__ PagedTileWalk(const PagedAttnParams& p, const PagedRange& r)
+      : pos(r.lo), b(r.seq) {
+    if (pos >= r.hi) return;
     s = PagedTiles<TILES, KEYS>(p, b);
     int64_t at = pos - r.base;
     head = static_cast<int>(s.per_head >> 31 ? at / s.per_head
@@ -276,8 +276,8 @@ struct PagedTileWalk {
     }
   }
   // (the walk stands before tile `tile1` of the current item)
-  __device__ __forceinline__ bool next() {
-    if (pos >= range.hi) return false;
+  __device__ __forceinline__ bool next(const PagedAttnParams& p, int64_t hi) {
+    if (pos >= hi) return false;
     if (tile1 == n) {
       tile1 = 0;
       if (++block == s.blocks) {
@@ -291,24 +291,26 @@ struct PagedTileWalk {
       n = s.block_tiles(p, block);
     }
     tile0 = tile1;
-    const int64_t left = range.hi - pos;
+    const int64_t left = hi - pos;
     tile1 = static_cast<int>(!p.whole_items && left < n - tile0 ? tile0 + left : n);
     item = pos - tile0;
     pos += tile1 - tile0;
     return true;
   }
   // First token of tile i of the block, and the steps of this part that the tile takes part in.
-  __device__ __forceinline__ int tok0(int i) const { return (block * TILES + i) * p.tile_toks; }
-  __device__ __forceinline__ int steps(int i) const {
-    if (tok0(i) >= s.count) return 0;
-    return min(max(s.tiles(p, tok0(i) + p.tile_toks) - tile0, 0), tile1 - tile0);
+  __device__ __forceinline__ int tok0(const PagedAttnParams& p, int i) const {
+    return (block * TILES + i) * p.tile_toks;
+  }
+  __device__ __forceinline__ int steps(const PagedAttnParams& p, int i) const {
+    if (tok0(p, i) >= s.count) return 0;
+    return min(max(s.tiles(p, tok0(p, i) + p.tile_toks) - tile0, 0), tile1 - tile0);
   }
   // The part's last tile goes past the sequence's end.
   __device__ __forceinline__ bool tail() const { return tile1 * KEYS > s.len; }
   __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == n; }
   __device__ __forceinline__ int slot() const { return tile0 == 0 ? 1 : 0; }
-  __device__ __forceinline__ PagedPart note() const {
-    return PagedPart{range.cta_of(item), range.cta_of(item + n - 1), s.first, s.count, head, block};
+  __device__ __forceinline__ PagedPart note(const PagedRange& r) const {
+    return PagedPart{r.cta_of(item), r.cta_of(item + n - 1), s.first, s.count, head, block};
   }
 };
 

@@ -49,7 +49,7 @@ struct TileGeo {
   static constexpr int KV_TILE = KEYS * ROW_BYTES;
   static constexpr int RAW = FP8 ? KEYS * (D + 4) : 0;  // codes, scales
   static constexpr int RAW_STAGES = FP8 ? 3 : 0;
-  static constexpr int FIXED = 1024 + TILES * Q_TILE + RAW_STAGES * RAW + 1536;
+  static constexpr int FIXED = 1024 + TILES * Q_TILE + RAW_STAGES * RAW + 3072;
   static constexpr int FIT = (227 * 1024 - FIXED) / KV_TILE;
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   // More than half of an SM's shared memory in any case: one CTA per SM, which takes all its TMEM.
@@ -65,7 +65,7 @@ struct TileGeo {
   static_assert(TMEM_O + TILES * D <= 512, "TMEM");
 };
 
-template <int STAGES>
+template <int STAGES, typename Walk>
 struct TileShared {
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[STAGES], kv_empty[STAGES];
@@ -75,6 +75,8 @@ struct TileShared {
   uint64_t s_full[2], p_ready[2], o_full[2], o_empty[2];
   uint64_t mma_done;
   int issued[2];
+  Walk walks[16];  // one per warp: kept out of the registers of the roles' loops
+  int more[16];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
@@ -96,20 +98,26 @@ __device__ __forceinline__ void bulk_load_tile(uint32_t dst, const void* src, ui
       : "memory");
 }
 
+__device__ __forceinline__ void st_global_v8(void* to, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 template <typename T, int D, bool FP8>
 __global__ void __launch_bounds__(512, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ,
                       const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const PagedAttnParams p) {
   using G = TileGeo<D, FP8>;
-  using Sh = TileShared<G::STAGES>;
-  static_assert(sizeof(Sh) <= 1536, "barrier block");
+  using Walk = PagedTileWalk<G::TILES, G::KEYS>;
+  using Sh = TileShared<G::STAGES, Walk>;
+  static_assert(sizeof(Sh) <= 3072, "barrier block");
   constexpr int TILES = G::TILES, KEYS = G::KEYS, STAGES = G::STAGES;
   constexpr bool kHalf = std::is_same_v<T, __half>;
   constexpr float kPOffset = kHalf ? G::P_OFFSET : 0.f;
   constexpr uint32_t IDESC_S = make_idesc(Elt<T>::kFmt, false, 128, KEYS);
   constexpr uint32_t IDESC_O = make_idesc(Elt<T>::kFmt, true, 128, D);
-  using Walk = PagedTileWalk<TILES, KEYS>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -171,10 +179,17 @@ __global__ void __launch_bounds__(512, 1)
   auto wait = [&](uint64_t& bar, uint32_t parity) {
     return static_cast<bool>(__all_sync(0xffffffffu, wait1(bar, parity)));
   };
+  Walk& w = sh->walks[warp];
+  if (lane == 0) w = Walk(p, range);
+  auto next_part = [&]() -> bool {
+    __syncwarp();  // the warp is done with the last part
+    if (lane == 0) sh->more[warp] = w.next(p, range.hi);
+    __syncwarp();
+    return sh->more[warp] != 0;
+  };
 
   if (warp >= 8) {
     setmaxnreg_dec<G::REG_OTHER>();
-    Walk w(p, range);
     if (warp == 13 || warp == 15) {
       // ---------------------------------------------------------------- TMA producers
       // The copies of a tile, a lane each, spread over both warps (see the row kernel).
@@ -198,14 +213,14 @@ __global__ void __launch_bounds__(512, 1)
       uint32_t ph = 0;
       bool ok = true;
       ProducersMeet<2> meet{sh->issued, 3};
-      while (issued < meet.limit && w.next()) {
+      while (issued < meet.limit && next_part()) {
         if (pw == 0) {
           if (lane == 0 && (__ldg(p.seqs.kv_lens + w.b) != w.s.len ||
                             __ldg(p.seqs.offsets + w.b + 1) - __ldg(p.seqs.offsets + w.b) != w.s.count))
             report(status, kStatusPageTable);
 #pragma unroll
           for (int i = 0; i < TILES; ++i) {
-            if (!ok || w.steps(i) == 0) continue;
+            if (!ok || w.steps(p, i) == 0) continue;
             ok = wait(sh->q_empty[i], qe_ph[i] ^ 1u);
             if (!ok) continue;
             qe_ph[i] ^= 1u;
@@ -217,7 +232,7 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll
               for (int c = 0; c < G::NBLK; ++c)
                 tma_load_3d(smem_u32(q_smem + i * G::Q_TILE + c * G::Q_BLK), &tmQ, bar,
-                            c * (G::SWZ / 2), w.head * p.group, w.s.first + w.tok0(i));
+                            c * (G::SWZ / 2), w.head * p.group, w.s.first + w.tok0(p, i));
             }
           }
         }
@@ -332,9 +347,9 @@ __global__ void __launch_bounds__(512, 1)
       uint32_t ph = 0;
       bool ok = true;
       bool first_turn = true;  // tile 0's very first turn is the only one without a take
-      while (w.next()) {
+      while (next_part()) {
         const int n = w.tile1 - w.tile0;
-        const int mine = w.steps(ti);
+        const int mine = w.steps(p, ti);
         const bool tail = !FP8 && w.tail();
         const int k0 = slot;
         if (ok) ok = wait(sh->kv_full[slot], ph);
@@ -414,7 +429,7 @@ __global__ void __launch_bounds__(512, 1)
         // they do not see: v_go tells them that the one they clean is under way.  The issuers
         // need v_clean, so neither barrier of a slot can get a second phase ahead.
         uint32_t go_ph = 0;  // bit s: parity of v_go[s]
-        while (ok && w.next()) {
+        while (ok && next_part()) {
           const int n = 2 * (w.tile1 - w.tile0);  // slots of the part; V of the last step is last
           const int last = slot + n - 1;
           const int vslot = last % STAGES;
@@ -442,7 +457,7 @@ __global__ void __launch_bounds__(512, 1)
         int rslot = 0;
         uint32_t rph = 0;
         constexpr int PR = D / 16;  // 16-code pieces of a row
-        while (ok && w.next()) {
+        while (ok && next_part()) {
           for (int t = w.tile0; t < w.tile1 && ok; ++t) {
             const int keep = w.s.len - t * KEYS;
 #pragma unroll 1
@@ -492,7 +507,6 @@ __global__ void __launch_bounds__(512, 1)
     const int i = warp >> 2;  // query tile
     if (i < TILES) {
       // ---------------------------------------------------------------- softmax and output
-      Walk w(p, range);
       const int r = threadIdx.x & 127;
       const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t tS = tmem + lane_off + i * KEYS;
@@ -503,8 +517,9 @@ __global__ void __launch_bounds__(512, 1)
       uint32_t s_ph = 0, of_ph = 0;
       bool ok = true;
 
-      // p = 2^(s * scale + shift), P to TMEM in 32-key chunks; returns the sum of p
-      auto exp_pass = [&](const float* s, float m) -> float {
+      // p = 2^(s * scale + shift), P to TMEM in 32-key chunks; returns the sum of p.  With `upper`
+      // the upper half of s is still being loaded, and waited for behind the lower half.
+      auto exp_pass = [&](float* s, float m, bool upper) -> float {
         const float shift = (m == -INFINITY ? 0.f : -m) + kPOffset;
         const float2 nm = make_float2(shift, shift);
         float2 acc[4];
@@ -512,6 +527,11 @@ __global__ void __launch_bounds__(512, 1)
         for (int u = 0; u < 4; ++u) acc[u] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < KEYS / 32; ++c) {
+          if (c == KEYS / 64 && upper) {
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = KEYS / 2; k < KEYS; ++k) asm volatile("" : "+f"(s[k]));
+          }
           uint32_t pk[16];
 #pragma unroll
           for (int u = 0; u < 16; ++u) {
@@ -528,16 +548,16 @@ __global__ void __launch_bounds__(512, 1)
       };
       constexpr float kBound = kHalf ? P_SUM_BOUND * 128.f : P_SUM_BOUND;  // 2^P_OFFSET
 
-      while (ok && w.next()) {
-        const int n = w.steps(i);
-        const int tok = w.tok0(i) + r_tok;
+      while (ok && next_part()) {
+        const int n = w.steps(p, i);
+        const int tok = w.tok0(p, i) + r_tok;
         const bool live = r < p.tile_live && tok < w.s.count;
         const int64_t row = w.s.first + tok;
         const int head = w.head * p.group + r_head;
         const int64_t part_row = (static_cast<int64_t>(blockIdx.x) * 2 + w.slot()) * (128 * TILES) +
                                  i * 128 + r;
         const bool whole = w.whole();
-        if (threadIdx.x == 0 && !whole && w.slot() == 0) p.parts[blockIdx.x] = w.note();
+        if (threadIdx.x == 0 && !whole && w.slot() == 0) p.parts[blockIdx.x] = w.note(range);
         if (n == 0) {
           // nothing of this part concerns the tile (no token, or keys behind all of them)
           if (live && !whole) p.part_lse[part_row] = -INFINITY;
@@ -545,7 +565,8 @@ __global__ void __launch_bounds__(512, 1)
         }
         const int past = w.s.len - w.s.count;
         const int lim = p.causal ? min(w.s.len, past + tok + 1) : w.s.len;  // keys of this row
-        const int lim_all = p.causal ? min(w.s.len, past + w.tok0(i) + 1) : w.s.len;
+        const int lim_all = p.causal ? min(w.s.len, past + w.tok0(p, i) + 1) : w.s.len;
+        const int key_first = w.tile0 * KEYS;
         float m = -INFINITY;  // the row's base, log2 units
         float l = 0.f;
         float s[KEYS];
@@ -554,14 +575,27 @@ __global__ void __launch_bounds__(512, 1)
           if (!ok) break;
           s_ph ^= 1u;
           tc_fence_after();
+          const int key0 = key_first + j * KEYS;
+          const bool masked = key0 + KEYS > lim_all;
+          // the first step and masked ones take the whole row at once
+          const bool upper = j > 0 && !masked;
 #pragma unroll
-          for (int c = 0; c < KEYS / 32; ++c)
+          for (int c = 0; c < KEYS / 64; ++c)
             tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
-          tmem_wait_ld();
+          if (upper) {
+            tmem_wait_ld();
 #pragma unroll
-          for (int k = 0; k < KEYS; ++k) asm volatile("" : "+f"(s[k]));
-          const int key0 = (w.tile0 + j) * KEYS;
-          if (key0 + KEYS > lim_all) {
+            for (int k = 0; k < KEYS / 2; ++k) asm volatile("" : "+f"(s[k]));
+          }
+#pragma unroll
+          for (int c = KEYS / 64; c < KEYS / 32; ++c)
+            tmem_ld32(tS + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
+          if (!upper) {
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < KEYS; ++k) asm volatile("" : "+f"(s[k]));
+          }
+          if (masked) {
             const int keep = lim - key0;
 #pragma unroll
             for (int k = 0; k < KEYS; ++k)
@@ -569,9 +603,9 @@ __global__ void __launch_bounds__(512, 1)
           }
           if (j == 0) {
             m = row_max<KEYS>(s) * sl2;
-            l = exp_pass(s, m);
+            l = exp_pass(s, m, false);
           } else {
-            float sum = exp_pass(s, m);
+            float sum = exp_pass(s, m, upper);
             if (__any_sync(0xffffffffu, !(sum <= kBound) || m == -INFINITY)) {
               const float top = row_max<KEYS>(s) * sl2;
               const bool need = top > m + RESCALE_LOG2;
@@ -596,7 +630,7 @@ __global__ void __launch_bounds__(512, 1)
                   }
                   tmem_st16(tO + c * 16, o);
                 }
-                sum = exp_pass(s, m);
+                sum = exp_pass(s, m, false);
               }
             }
             l += sum;
@@ -632,18 +666,18 @@ __global__ void __launch_bounds__(512, 1)
             f[u] = __uint_as_float(o[u]) * inv;
           }
           if (live && whole) {
+            uint32_t pk[8];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-              *reinterpret_cast<uint4*>(out + c * 16 + u * 8) = make_uint4(
-                  pack2(f[8 * u], f[8 * u + 1], static_cast<T*>(nullptr)),
-                  pack2(f[8 * u + 2], f[8 * u + 3], static_cast<T*>(nullptr)),
-                  pack2(f[8 * u + 4], f[8 * u + 5], static_cast<T*>(nullptr)),
-                  pack2(f[8 * u + 6], f[8 * u + 7], static_cast<T*>(nullptr)));
+            for (int u = 0; u < 8; ++u) pk[u] = pack2(f[2 * u], f[2 * u + 1], static_cast<T*>(nullptr));
+            *reinterpret_cast<uint4*>(out + c * 16) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            *reinterpret_cast<uint4*>(out + c * 16 + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
           } else if (live) {
+            // whole 32-byte sectors: a thread owns a row, so lanes are a row apart
+            uint32_t b[16];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              *reinterpret_cast<float4*>(part + c * 16 + u * 4) =
-                  make_float4(f[4 * u], f[4 * u + 1], f[4 * u + 2], f[4 * u + 3]);
+            for (int u = 0; u < 16; ++u) b[u] = __float_as_uint(f[u]);
+            st_global_v8(part + c * 16, b);
+            st_global_v8(part + c * 16 + 8, b + 8);
           }
         }
         __syncwarp();
