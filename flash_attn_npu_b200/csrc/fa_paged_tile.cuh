@@ -8,19 +8,23 @@
 //   S = Q K^T -> p = 2^(S * scale * log2 e - m), row sums l -> O += P V
 // with S, P (16 bits, over S) and O in TMEM, tcgen05.mma throughout.
 //
-// Warps (16):  0-3, 4-7  softmax of tile 0, 1 (thread r owns row r), rescaling and output
-//              8-11      16-bit cache: clean the sequence's end; float8: dequantise the tiles
-//              12, 14    MMA issuers of tile 0, 1 (they take turns); 12 also owns TMEM
-//              13, 15    TMA producers
+// Warps (16, float8 20):
+//   0-3, 4-7  softmax of tile 0, 1 (thread r owns row r), rescaling and output
+//   next 4    16-bit cache: clean the sequence's end
+//   next 8    float8 cache: dequantise the tiles
+//   last 4    MMA issuer of tile 0 (owns TMEM), TMA producer, MMA issuer of tile 1, TMA producer;
+//             the issuers take turns
 //
 // Pages: the producer's lanes look a tile's pages up and each copies one (rows of at most 128
 // bytes per copy).  What lies behind a sequence's last key may be any bits.  Its logits are
 // masked, but 0 * NaN in P V is NaN, so those rows of V are zeroed in shared memory before the MMA
-// reads them, by warps 8-11 on the last tile.
+// reads them, by the helper warps on the last tile.
 //
-// Float8: tiles land in a ring of their own; warps 8-11 write code * scale, rounded to q's type
-// (exact for the powers of two that the cache's writer leaves), as operands in the layout that TMA
-// would have left.  That costs ~3 instructions a value once per key tile, for both query tiles.
+// Float8: tiles land in a ring of their own; the helper warps write code * scale, rounded to q's
+// type (exact for the powers of two that the cache's writer leaves), as operands in the layout that
+// TMA would have left.  That costs 1 (fp16) to 2.5 (bf16) instructions a value once per key tile, for
+// both query tiles; four warps took ~1600 cycles a tile (two tiles a step), longer than a step of
+// the rest, so there are eight.
 //
 // Softmax: exponentiate first, against the row's base, and look at the row sum; only a row whose
 // sum is large takes its maximum, and moves its base if that passed it by 2^8, rescaling O itself
@@ -56,9 +60,17 @@ struct TileGeo {
   static constexpr int SMEM =
       FIXED + STAGES * KV_TILE > 120 * 1024 ? FIXED + STAGES * KV_TILE : 120 * 1024;
   static constexpr int TMEM_O = TILES * KEYS;
-  static constexpr int THREADS = 512;
-  static constexpr int REG_LAUNCH = 128;
-  static constexpr int REG_SOFTMAX = 192, REG_OTHER = 64;  // 256 * 192 + 256 * 64 = 512 * 128
+  // Warps: 0-7 softmax, AUX helpers (see above), then MMA, TMA, MMA, TMA; and the split of the
+  // registers of the launch among the warpgroups.
+  static constexpr int AUX = FP8 ? 8 : 4;
+  static constexpr int MMA_WARP = 8 + AUX;
+  static constexpr int THREADS = (12 + AUX) * 32;
+  static constexpr int REG_LAUNCH = FP8 ? 96 : 128;
+  static constexpr int REG_SOFTMAX = FP8 ? 168 : 192;
+  static constexpr int REG_AUX = FP8 ? 48 : 64;
+  static constexpr int REG_MISC = FP8 ? 48 : 64;
+  static_assert(256 * REG_SOFTMAX + AUX * 32 * REG_AUX + 128 * REG_MISC <= THREADS * REG_LAUNCH,
+                "register split");
   static constexpr uint32_t LAYOUT = SWZ == 128 ? 2u : SWZ == 64 ? 4u : 6u;
   static constexpr float P_OFFSET = 7.f;  // of fp16 probabilities: at most 2^(7 + 8) < 65504
   static_assert(STAGES >= 3, "K and V of a step, and one to come");
@@ -75,8 +87,8 @@ struct TileShared {
   uint64_t s_full[2], p_ready[2], o_full[2], o_empty[2];
   uint64_t mma_done;
   int issued[2];
-  Walk walks[16];  // one per warp: kept out of the registers of the roles' loops
-  int more[16];
+  Walk walks[20];  // one per warp: kept out of the registers of the roles' loops
+  int more[20];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
@@ -105,7 +117,7 @@ __device__ __forceinline__ void st_global_v8(void* to, const uint32_t* r) {
 }
 
 template <typename T, int D, bool FP8>
-__global__ void __launch_bounds__(512, 1)
+__global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ,
                       const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const PagedAttnParams p) {
@@ -132,14 +144,14 @@ __global__ void __launch_bounds__(512, 1)
   let_next_launch();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&sh->kv_full[s]), FP8 ? 4 : 1);  // converting warps, or the producer
+      mbar_init(smem_u32(&sh->kv_full[s]), FP8 ? G::AUX : 1);  // converting warps, or the producer
       mbar_init(smem_u32(&sh->kv_empty[s]), TILES);       // one commit per issuer
       mbar_init(smem_u32(&sh->v_go[s]), 1);
       mbar_init(smem_u32(&sh->v_clean[s]), 4);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(smem_u32(&sh->raw_full[s]), 1);
-      mbar_init(smem_u32(&sh->raw_empty[s]), 4);
+      mbar_init(smem_u32(&sh->raw_empty[s]), G::AUX);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&sh->q_full[i]), 1);
@@ -153,13 +165,13 @@ __global__ void __launch_bounds__(512, 1)
     sh->abort_flag = 0u;
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == G::MMA_WARP) {
     tmem_alloc(smem_u32(&sh->tmem_base), 512);
     tmem_relinquish();
   }
   // Rows of the query tiles that no token fills are never written by a copy: they are zero.
   if (p.tile_live < 128) {
-    for (int x = threadIdx.x * 16; x < TILES * G::Q_TILE; x += 512 * 16)
+    for (int x = threadIdx.x * 16; x < TILES * G::Q_TILE; x += G::THREADS * 16)
       if ((x % G::Q_BLK) / G::SWZ >= p.tile_live)
         *reinterpret_cast<uint4*>(q_smem + x) = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
@@ -188,12 +200,12 @@ __global__ void __launch_bounds__(512, 1)
     return sh->more[warp] != 0;
   };
 
-  if (warp >= 8) {
-    setmaxnreg_dec<G::REG_OTHER>();
-    if (warp == 13 || warp == 15) {
+  if (warp >= G::MMA_WARP) {
+    setmaxnreg_dec<G::REG_MISC>();
+    if (warp == G::MMA_WARP + 1 || warp == G::MMA_WARP + 3) {
       // ---------------------------------------------------------------- TMA producers
       // The copies of a tile, a lane each, spread over both warps (see the row kernel).
-      const int pw = warp == 15;
+      const int pw = warp == G::MMA_WARP + 3;
       const int op = lane * 2 + pw;
       constexpr int COPIES = FP8 ? 2 : G::NBLK;  // of one page of K or V
       const int size = 1 << p.seqs.page_log2;
@@ -302,12 +314,12 @@ __global__ void __launch_bounds__(512, 1)
         const int x = issued - 1 - u;
         drain_bar(smem_u32(&full[x % RING]), static_cast<uint32_t>((x / RING) & 1));
       }
-    } else if (warp == 12 || (warp == 14 && TILES == 2)) {
+    } else if (warp == G::MMA_WARP || TILES == 2) {
       // ---------------------------------------------------------------- MMA issuers
       // Tile 0's issuer and tile 1's take turns through two named barriers, per part: S_0, S_1, then
       // per step tile 0's P V and next S, and tile 1's.  Both make every hand-off on every path.
       constexpr uint32_t kTok0 = 1, kTok1 = 2;
-      const int ti = warp == 12 ? 0 : 1;
+      const int ti = warp == G::MMA_WARP ? 0 : 1;
       constexpr uint32_t hi = ((8u * G::SWZ) >> 4) | (1u << 14) | (G::LAYOUT << 29);
       const uint32_t q_lo = (smem_u32(q_smem + ti * G::Q_TILE) >> 4) | (1u << 16);
       const uint32_t k_lo = (smem_u32(kv_smem) >> 4) | (1u << 16);
@@ -418,7 +430,10 @@ __global__ void __launch_bounds__(512, 1)
       if (lead) mma_commit(smem_u32(&sh->mma_done));
       __syncwarp();
       drain_bar(smem_u32(&sh->mma_done), 0);
-    } else if (warp < 12) {
+    }
+  } else if (warp >= 8) {
+    {
+      setmaxnreg_dec<G::REG_AUX>();
       // ------------------------------------------------ the sequence's end, or dequantising
       const int tid = threadIdx.x - 256;
       int slot = 0;
@@ -454,9 +469,22 @@ __global__ void __launch_bounds__(512, 1)
           if (lane == 0) mbar_arrive(smem_u32(&sh->v_clean[vslot]));
         }
       } else {
+        // A thread takes 16 codes of a row at a time.  The lanes of a warp are LP to a row, and
+        // neighbouring rows take different groups of pieces, so that neither the reads of codes
+        // nor the writes of operands (two 16-byte chunks, swizzled) meet in a bank.
         int rslot = 0;
         uint32_t rph = 0;
-        constexpr int PR = D / 16;  // 16-code pieces of a row
+        constexpr int PR = D / 16;                // pieces of a row
+        constexpr int LP = PR < 4 ? PR : 4;
+        constexpr int RW = 32 / LP;               // rows of a warp at a time
+        constexpr int NG = PR / LP;               // groups of pieces
+        // rows that the warps take at a time; with short rows not all of them have any
+        constexpr int AT_ONCE = G::AUX * RW < KEYS ? G::AUX * RW : KEYS;
+        constexpr int STEPS = KEYS / AT_ONCE;
+        static_assert(STEPS * AT_ONCE == KEYS, "rows");
+        const int row0 = (warp - 8) * RW + lane / LP;
+        const int group0 = row0 & (NG - 1);       // groups in an order that differs by row
+        static_assert(AT_ONCE % 8 == 0, "the swizzle repeats every 8 rows");
         while (ok && next_part()) {
           for (int t = w.tile0; t < w.tile1 && ok; ++t) {
             const int keep = w.s.len - t * KEYS;
@@ -467,27 +495,59 @@ __global__ void __launch_bounds__(512, 1)
               const uint8_t* raw = raw_smem + rslot * G::RAW;
               const float* scale = reinterpret_cast<const float*>(raw + KEYS * D);
               uint8_t* dst = kv_smem + slot * G::KV_TILE;
-#pragma unroll 4
-              for (int x = tid; x < KEYS * PR; x += 128) {
-                const int row = x / PR, c = x % PR;
-                const uint4 code = *reinterpret_cast<const uint4*>(raw + x * 16);
-                const float sc = scale[row];
-                uint32_t out[8];
+              // (a branch for each pair of codes took longer than the conversion itself: tail and
+              // kind of scale are looked at outside)
+              auto piece = [&](int k, int s, auto tail, auto direct, float sc) {
+                const int row = row0 + k * AT_ONCE;
+                const uint4 code =
+                    *reinterpret_cast<const uint4*>(raw + row * D + (group0 ^ s) * LP * 16 + lane % LP * 16);
                 const uint32_t cw[4] = {code.x, code.y, code.z, code.w};
+                const __half2 hs = __float2half2_rn(sc);
+                uint32_t out[8];
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
                   const uint32_t h2 = e4m3x2_to_h2(static_cast<uint16_t>(cw[u >> 1] >> (16 * (u & 1))));
-                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-                  out[u] = row < keep ? pack2(f.x * sc, f.y * sc, static_cast<T*>(nullptr)) : 0u;
+                  if constexpr (direct.value) {
+                    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h2), hs);
+                    out[u] = *reinterpret_cast<const uint32_t*>(&x);
+                  } else {
+                    const float2 f = fmul2(__half22float2(*reinterpret_cast<const __half2*>(&h2)),
+                                           make_float2(sc, sc));
+                    out[u] = pack2(f.x, f.y, static_cast<T*>(nullptr));
+                  }
                 }
-                // the two halves in an order that spreads a row's spans over the banks
+                if constexpr (tail.value) {
+#pragma unroll
+                  for (int u = 0; u < 8; ++u) out[u] = row < keep ? out[u] : 0u;
+                }
+                const int c = (group0 ^ s) * LP + lane % LP;
                 uint8_t* blk = dst + (c * 32 / G::SWZ) * G::KV_BLK;
-                const uint32_t at = row * G::SWZ + (c * 32) % G::SWZ;
-                const bool flip = (c >> 2) & 1;
-                const uint4 lo = make_uint4(out[0], out[1], out[2], out[3]);
-                const uint4 hi = make_uint4(out[4], out[5], out[6], out[7]);
-                *reinterpret_cast<uint4*>(blk + swizzle<G::SWZ>(at + (flip ? 16 : 0))) = flip ? hi : lo;
-                *reinterpret_cast<uint4*>(blk + swizzle<G::SWZ>(at + (flip ? 0 : 16))) = flip ? lo : hi;
+                const uint32_t at = row0 * G::SWZ + (c * 32) % G::SWZ;  // (AT_ONCE keeps the swizzle)
+                uint8_t* to = blk + k * AT_ONCE * G::SWZ;
+                *reinterpret_cast<uint4*>(to + swizzle<G::SWZ>(at)) =
+                    make_uint4(out[0], out[1], out[2], out[3]);
+                *reinterpret_cast<uint4*>(to + swizzle<G::SWZ>(at + 16)) =
+                    make_uint4(out[4], out[5], out[6], out[7]);
+              };
+              auto convert = [&](auto tail) {
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) {
+                  const float sc = scale[row0 + k * AT_ONCE];
+                  // a scale that fp16 holds: the product is rounded once either way
+                  if (kHalf && __all_sync(0xffffffffu, __half2float(__float2half_rn(sc)) == sc)) {
+#pragma unroll
+                    for (int s = 0; s < NG; ++s) piece(k, s, tail, std::true_type{}, sc);
+                  } else {
+#pragma unroll
+                    for (int s = 0; s < NG; ++s) piece(k, s, tail, std::false_type{}, sc);
+                  }
+                }
+              };
+              if (row0 >= AT_ONCE) {
+              } else if (keep >= KEYS) {
+                convert(std::false_type{});
+              } else {
+                convert(std::true_type{});
               }
               fence_proxy_async_smem();
               __syncwarp();
@@ -690,7 +750,7 @@ __global__ void __launch_bounds__(512, 1)
   // ---- teardown: every thread arrives here exactly once
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == G::MMA_WARP) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
