@@ -162,12 +162,14 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   p.causal = a->causal ? 1 : 0;
   p.scale_log2 = a->sm_scale * fa::kLog2e;
   const bool tile = c.rows == 0;
-  p.min_steps_log2 = tile ? 2 : 1;
   // Sequences of at most kWholeTiles tiles are not cut: the joining launch costs more (3 .. 10 us)
   // than the tiles that a CTA then takes one after the other (~0.5 us each in the row kernel,
   // ~1.3 us in the tile kernel).
   constexpr int64_t kWholeTiles = 8;
   p.whole_items = kv.table_cols * kv.page_size <= kWholeTiles * info.keys;
+  p.min_steps_log2 = p.whole_items ? 0 : tile ? 2 : 1;
+  p.item_cost = tile ? 3 : 1;
+  p.pair_from = plan.fp8 ? 6 : 3;
   p.tile_toks = tile ? 128 / p.group : 0;
   p.tile_live = tile ? p.tile_toks * p.group : info.rows;
   char* ws = static_cast<char*>(a->workspace);

@@ -1,7 +1,8 @@
 // Division of a paged attention call among CTAs, shared by its kernels.
 //
 // An item is one (sequence, kv head, block of query rows); it has one step per tile of keys (and
-// one if there is no key, so that its rows are written).  All steps of a call, in the order
+// one if there is no key, so that its rows are written), behind `item_cost` empty steps that stand
+// for what an item costs besides its tiles (fetching the queries, joining, writing).  All steps of a call, in the order
 // sequence - kv head - row block - key tile, form one line that is cut into equal ranges, one per
 // CTA: ragged lengths, few sequences and long contexts all load the SMs alike, and only the two
 // items at a CTA's ends can be shared with a neighbour.  Lengths are device data, so each CTA
@@ -60,9 +61,11 @@ struct PagedAttnParams {
   int causal;
   float scale_log2;  // sm_scale * log2(e)
   int min_steps_log2;  // steps of a CTA's range, at least
+  int item_cost;     // empty steps before an item's tiles
   int whole_items;   // a CTA takes the items that begin in its range, whole: nothing is shared
   int tile_live;     // rows of a tile that are used: a multiple of `group` in the tile kernel
   int tile_toks;     // tokens of a tile (tile kernel)
+  int pair_from;     // steps from which a part of one tile is worked on by both sides, at least 2
   PagedPart* parts;  // [gridDim.x]
   float* part_o;     // [gridDim.x][2][block rows][head_dim]
   float* part_lse;   // [gridDim.x][2][block rows]
@@ -85,7 +88,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
   const int rows = s.count * p.group;  // at most total * heads_q, which the host bounds
   s.blocks = (rows + ROWS - 1) / ROWS;
   s.tiles = max(1, (s.len + KEYS - 1) / KEYS);
-  s.steps = static_cast<int64_t>(p.heads_kv) * s.blocks * s.tiles;
+  s.steps = static_cast<int64_t>(p.heads_kv) * s.blocks * (s.tiles + p.item_cost);
   return s;
 }
 
@@ -161,55 +164,60 @@ template <int ROWS, int KEYS>
 struct PagedWalk {
   const PagedAttnParams& p;
   const PagedRange& range;
-  int64_t pos;
+  int64_t pos;       // next step of the line
+  int at;            // ... and of the item
   int b;
   PagedSeq s;
   // the current part
   int head, block;
   int tile0, tile1;  // key tiles [tile0, tile1) of the item
-  int64_t item;      // its first step
+  int64_t item;      // the item's first step
 
-  // (the walk stands before tile `tile1` of the current item)
   __device__ __forceinline__ PagedWalk(const PagedAttnParams& params, const PagedRange& r)
       : p(params), range(r), pos(r.lo), b(r.seq) {
     if (pos >= range.hi) return;
     s = paged_seq<ROWS, KEYS>(p, b);
-    const int64_t at = pos - r.base;
-    const int64_t n = quot(at, s.tiles);
-    tile1 = static_cast<int>(at - n * s.tiles);
+    const int64_t in_seq = pos - r.base;
+    const int64_t n = quot(in_seq, s.tiles + p.item_cost);
+    at = static_cast<int>(in_seq - n * (s.tiles + p.item_cost));
     head = static_cast<int>(s.blocks == 1 ? n : quot(n, s.blocks));
     block = static_cast<int>(n - static_cast<int64_t>(head) * s.blocks);
-    if (p.whole_items && tile1 > 0) {
-      pos += s.tiles - tile1;
-      tile1 = s.tiles;
+    if (p.whole_items && at > 0) {
+      pos += s.tiles + p.item_cost - at;
+      at = s.tiles + p.item_cost;
     }
   }
   __device__ __forceinline__ bool next() {
-    if (pos >= range.hi) return false;
-    if (tile1 == s.tiles) {
-      tile1 = 0;
-      if (++block == s.blocks) {
-        block = 0;
-        if (++head == p.heads_kv) {
-          head = 0;
-          do s = paged_seq<ROWS, KEYS>(p, ++b);
-          while (s.blocks == 0);
+    do {
+      if (pos >= range.hi) return false;
+      if (at == s.tiles + p.item_cost) {
+        at = 0;
+        if (++block == s.blocks) {
+          block = 0;
+          if (++head == p.heads_kv) {
+            head = 0;
+            do s = paged_seq<ROWS, KEYS>(p, ++b);
+            while (s.blocks == 0);
+          }
         }
       }
-    }
-    tile0 = tile1;
-    const int64_t left = range.hi - pos;
-    tile1 = static_cast<int>(!p.whole_items && left < s.tiles - tile0 ? tile0 + left : s.tiles);
-    item = pos - tile0;
-    pos += tile1 - tile0;
+      const int end = s.tiles + p.item_cost;
+      const int64_t left = range.hi - pos;
+      const int to = static_cast<int>(!p.whole_items && left < end - at ? at + left : end);
+      tile0 = max(0, at - p.item_cost);
+      tile1 = max(0, to - p.item_cost);
+      item = pos - at;
+      pos += to - at;
+      at = to;
+    } while (tile0 == tile1);  // empty steps only
     return true;
   }
   __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == s.tiles; }
   __device__ __forceinline__ int slot() const { return tile0 == 0 ? 1 : 0; }
   // What the combine kernel has to know of the current part (slot 0).
   __device__ __forceinline__ PagedPart note() const {
-    return PagedPart{range.cta_of(item), range.cta_of(item + s.tiles - 1), s.first, s.count,
-                     head, block};
+    return PagedPart{range.cta_of(item + p.item_cost),
+                     range.cta_of(item + p.item_cost + s.tiles - 1), s.first, s.count, head, block};
   }
 };
 
@@ -234,9 +242,9 @@ struct PagedTiles {
     seq_rows(p.seqs, b, first, count);
     len = seq_len(p.seqs, b);
     blocks = (count + TILES * p.tile_toks - 1) / (TILES * p.tile_toks);
-    per_head = 0;
+    per_head = static_cast<int64_t>(blocks) * p.item_cost;
     if (!p.causal) {
-      per_head = static_cast<int64_t>(blocks) * block_tiles(p, 0);
+      per_head += static_cast<int64_t>(blocks) * block_tiles(p, 0);
     } else {
       for (int m = 0; m < blocks; ++m) per_head += block_tiles(p, m);
     }
@@ -249,7 +257,8 @@ struct PagedTiles {
 // (plain data: it lives in shared memory)
 template <int TILES, int KEYS>
 struct PagedTileWalk {
-  int64_t pos;
+  int64_t pos;       // next step of the line
+  int at;            // ... and of the item
   int b;
   PagedTiles<TILES, KEYS> s;
   // the current part
@@ -263,38 +272,43 @@ struct PagedTileWalk {
       : pos(r.lo), b(r.seq) {
     if (pos >= r.hi) return;
     s = PagedTiles<TILES, KEYS>(p, b);
-    int64_t at = pos - r.base;
-    head = static_cast<int>(s.per_head >> 31 ? at / s.per_head
-                                             : quot(at, static_cast<int>(s.per_head)));
-    at -= head * s.per_head;
+    int64_t in_seq = pos - r.base;
+    head = static_cast<int>(s.per_head >> 31 ? in_seq / s.per_head
+                                             : quot(in_seq, static_cast<int>(s.per_head)));
+    in_seq -= head * s.per_head;
     block = 0;
-    for (n = s.block_tiles(p, 0); at >= n; n = s.block_tiles(p, ++block)) at -= n;
-    tile1 = static_cast<int>(at);
+    for (n = s.block_tiles(p, 0); in_seq >= n + p.item_cost; n = s.block_tiles(p, ++block))
+      in_seq -= n + p.item_cost;
+    at = static_cast<int>(in_seq);
     if (p.whole_items && at > 0) {
-      pos += n - at;
-      tile1 = n;
+      pos += n + p.item_cost - at;
+      at = n + p.item_cost;
     }
   }
-  // (the walk stands before tile `tile1` of the current item)
   __device__ __forceinline__ bool next(const PagedAttnParams& p, int64_t hi) {
-    if (pos >= hi) return false;
-    if (tile1 == n) {
-      tile1 = 0;
-      if (++block == s.blocks) {
-        block = 0;
-        if (++head == p.heads_kv) {
-          head = 0;
-          do s = PagedTiles<TILES, KEYS>(p, ++b);
-          while (s.blocks == 0);
+    do {
+      if (pos >= hi) return false;
+      if (at == n + p.item_cost) {
+        at = 0;
+        if (++block == s.blocks) {
+          block = 0;
+          if (++head == p.heads_kv) {
+            head = 0;
+            do s = PagedTiles<TILES, KEYS>(p, ++b);
+            while (s.blocks == 0);
+          }
         }
+        n = s.block_tiles(p, block);
       }
-      n = s.block_tiles(p, block);
-    }
-    tile0 = tile1;
-    const int64_t left = hi - pos;
-    tile1 = static_cast<int>(!p.whole_items && left < n - tile0 ? tile0 + left : n);
-    item = pos - tile0;
-    pos += tile1 - tile0;
+      const int end = n + p.item_cost;
+      const int64_t left = hi - pos;
+      const int to = static_cast<int>(!p.whole_items && left < end - at ? at + left : end);
+      tile0 = max(0, at - p.item_cost);
+      tile1 = max(0, to - p.item_cost);
+      item = pos - at;
+      pos += to - at;
+      at = to;
+    } while (tile0 == tile1);  // empty steps only
     return true;
   }
   // First token of tile i of the block, and the steps of this part that the tile takes part in.
@@ -305,12 +319,16 @@ struct PagedTileWalk {
     if (tok0(p, i) >= s.count) return 0;
     return min(max(s.tiles(p, tok0(p, i) + p.tile_toks) - tile0, 0), tile1 - tile0);
   }
+  // Only the block's first tile has tokens: both sides of the CTA work on it, key tiles in turn.
+  __device__ __forceinline__ bool paired(const PagedAttnParams& p) const {
+    return TILES == 2 && tok0(p, 1) >= s.count && tile1 - tile0 >= p.pair_from;
+  }
   // The part's last tile goes past the sequence's end.
   __device__ __forceinline__ bool tail() const { return tile1 * KEYS > s.len; }
   __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == n; }
   __device__ __forceinline__ int slot() const { return tile0 == 0 ? 1 : 0; }
-  __device__ __forceinline__ PagedPart note(const PagedRange& r) const {
-    return PagedPart{r.cta_of(item), r.cta_of(item + n - 1), s.first, s.count, head, block};
+  __device__ __forceinline__ PagedPart note(const PagedRange& r, int cost) const {
+    return PagedPart{r.cta_of(item + cost), r.cta_of(item + cost + n - 1), s.first, s.count, head, block};
   }
 };
 

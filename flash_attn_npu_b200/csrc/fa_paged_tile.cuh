@@ -1,6 +1,11 @@
 // Paged attention of many query rows per kv head (prompts, chunks): bound by the tensor cores and
 // the exponentials.
 //
+// Where a block has rows for one tile only, both sides (softmax warps, issuers, S and O in TMEM) work
+// on that tile, each on every other key tile, and join their (m, l, O) at the part's end: a single
+// side is a chain of MMA, exponentials, MMA that leaves the units idle more than half the time
+// (~2900 cycles a step of 128 keys, where two sides take ~3700 for twice the work).
+//
 // A query tile is 128 rows of TMEM: `tile_toks` tokens times the `group` query heads that share a
 // kv head (as many whole tokens as fit), so that grouped heads fill the tensor cores and share
 // every key and value.  A CTA works on TILES tiles (two up to head_dim 128, one at 256) over the
@@ -53,7 +58,7 @@ struct TileGeo {
   static constexpr int KV_TILE = KEYS * ROW_BYTES;
   static constexpr int RAW = FP8 ? KEYS * (D + 4) : 0;  // codes, scales
   static constexpr int RAW_STAGES = FP8 ? 3 : 0;
-  static constexpr int FIXED = 1024 + TILES * Q_TILE + RAW_STAGES * RAW + 3072;
+  static constexpr int FIXED = 1024 + TILES * Q_TILE + RAW_STAGES * RAW + 5120;
   static constexpr int FIT = (227 * 1024 - FIXED) / KV_TILE;
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   // More than half of an SM's shared memory in any case: one CTA per SM, which takes all its TMEM.
@@ -86,6 +91,7 @@ struct TileShared {
   uint64_t raw_full[4], raw_empty[4];
   uint64_t s_full[2], p_ready[2], o_full[2], o_empty[2];
   uint64_t mma_done;
+  float2 pair[2][128];  // (m, l) of the two sides' rows
   int issued[2];
   Walk walks[20];  // one per warp: kept out of the registers of the roles' loops
   int more[20];
@@ -124,7 +130,7 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
   using G = TileGeo<D, FP8>;
   using Walk = PagedTileWalk<G::TILES, G::KEYS>;
   using Sh = TileShared<G::STAGES, Walk>;
-  static_assert(sizeof(Sh) <= 3072, "barrier block");
+  static_assert(sizeof(Sh) <= 5120, "barrier block");
   constexpr int TILES = G::TILES, KEYS = G::KEYS, STAGES = G::STAGES;
   constexpr bool kHalf = std::is_same_v<T, __half>;
   constexpr float kPOffset = kHalf ? G::P_OFFSET : 0.f;
@@ -232,7 +238,7 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
             report(status, kStatusPageTable);
 #pragma unroll
           for (int i = 0; i < TILES; ++i) {
-            if (!ok || w.steps(p, i) == 0) continue;
+            if (!ok || (w.steps(p, i) == 0 && !w.paired(p))) continue;
             ok = wait(sh->q_empty[i], qe_ph[i] ^ 1u);
             if (!ok) continue;
             qe_ph[i] ^= 1u;
@@ -244,7 +250,8 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
 #pragma unroll
               for (int c = 0; c < G::NBLK; ++c)
                 tma_load_3d(smem_u32(q_smem + i * G::Q_TILE + c * G::Q_BLK), &tmQ, bar,
-                            c * (G::SWZ / 2), w.head * p.group, w.s.first + w.tok0(p, i));
+                            c * (G::SWZ / 2), w.head * p.group,
+                            w.s.first + w.tok0(p, w.paired(p) ? 0 : i));
             }
           }
         }
@@ -363,6 +370,55 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
         const int n = w.tile1 - w.tile0;
         const int mine = w.steps(p, ti);
         const bool tail = !FP8 && w.tail();
+        if (w.paired(p)) {
+          // Both issuers work on the one query tile, on every other key tile each and without
+          // turns.  A slot is given back by both: by the one that uses it once its MMAs are done,
+          // by the other as soon as the slot is full.
+          if (ok) ok = wait(sh->q_full[ti], q_ph);
+          q_ph ^= 1u;
+          for (int j = 0; j < n; ++j) {
+            const bool act = (j & 1) == ti;
+            if (ok) ok = wait(sh->kv_full[slot], ph);
+            if (ok && lead) {
+              if (act) {
+                tc_fence_after();
+                issue_s(slot);
+                mma_commit(s_bar);
+                if (j + 2 >= n) mma_commit(smem_u32(&sh->q_empty[ti]));
+                mma_commit(smem_u32(&sh->kv_empty[slot]));
+              } else {
+                mbar_arrive(smem_u32(&sh->kv_empty[slot]));
+              }
+            }
+            if (++slot == STAGES) { slot = 0; ph ^= 1u; }
+            if (ok) ok = wait(sh->kv_full[slot], ph);
+            if (tail && j + 1 == n) {
+              if (ok) ok = wait(sh->v_clean[slot], (clean_ph >> slot) & 1u);
+              clean_ph ^= 1u << slot;
+            }
+            if (act) {
+              if (ok) ok = wait(sh->p_ready[ti], p_ph);
+              p_ph ^= 1u;
+              if (j < 2) {
+                if (ok) ok = wait(sh->o_empty[ti], oe_ph ^ 1u);
+                oe_ph ^= 1u;
+              }
+            }
+            if (ok && lead) {
+              if (act) {
+                tc_fence_after();
+                issue_pv(slot, j >= 2 ? 1u : 0u);
+                if (j + 2 >= n) mma_commit(smem_u32(&sh->o_full[ti]));
+                mma_commit(smem_u32(&sh->kv_empty[slot]));
+              } else {
+                mbar_arrive(smem_u32(&sh->kv_empty[slot]));
+              }
+            }
+            __syncwarp();
+            if (++slot == STAGES) { slot = 0; ph ^= 1u; }
+          }
+          continue;
+        }
         const int k0 = slot;
         if (ok) ok = wait(sh->kv_full[slot], ph);
         if (++slot == STAGES) { slot = 0; ph ^= 1u; }
@@ -608,16 +664,21 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
       };
       constexpr float kBound = kHalf ? P_SUM_BOUND * 128.f : P_SUM_BOUND;  // 2^P_OFFSET
 
-      while (ok && next_part()) {
-        const int n = w.steps(p, i);
-        const int tok = w.tok0(p, i) + r_tok;
+      // (a wait that gave up does not end the loop: the two sides still meet where they are paired)
+      while (next_part()) {
+        const bool paired = w.paired(p);
+        const int tile = paired ? 0 : i;  // of the block
+        // key tiles of this side: first, first + stride, ..
+        const int first = paired ? i : 0, stride = paired ? 2 : 1;
+        const int n = paired ? (w.tile1 - w.tile0 - i + 1) / 2 : w.steps(p, i);
+        const int tok = w.tok0(p, tile) + r_tok;
         const bool live = r < p.tile_live && tok < w.s.count;
         const int64_t row = w.s.first + tok;
         const int head = w.head * p.group + r_head;
         const int64_t part_row = (static_cast<int64_t>(blockIdx.x) * 2 + w.slot()) * (128 * TILES) +
-                                 i * 128 + r;
+                                 tile * 128 + r;
         const bool whole = w.whole();
-        if (threadIdx.x == 0 && !whole && w.slot() == 0) p.parts[blockIdx.x] = w.note(range);
+        if (threadIdx.x == 0 && !whole && w.slot() == 0) p.parts[blockIdx.x] = w.note(range, p.item_cost);
         if (n == 0) {
           // nothing of this part concerns the tile (no token, or keys behind all of them)
           if (live && !whole) p.part_lse[part_row] = -INFINITY;
@@ -625,17 +686,17 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
         }
         const int past = w.s.len - w.s.count;
         const int lim = p.causal ? min(w.s.len, past + tok + 1) : w.s.len;  // keys of this row
-        const int lim_all = p.causal ? min(w.s.len, past + w.tok0(p, i) + 1) : w.s.len;
-        const int key_first = w.tile0 * KEYS;
+        const int lim_all = p.causal ? min(w.s.len, past + w.tok0(p, tile) + 1) : w.s.len;
+        const int key_first = (w.tile0 + first) * KEYS;
         float m = -INFINITY;  // the row's base, log2 units
         float l = 0.f;
         float s[KEYS];
-        for (int j = 0; j < n; ++j) {
+        for (int j = 0; j < n && ok; ++j) {
           ok = wait(sh->s_full[i], s_ph);
           if (!ok) break;
           s_ph ^= 1u;
           tc_fence_after();
-          const int key0 = key_first + j * KEYS;
+          const int key0 = key_first + j * stride * KEYS;
           const bool masked = key0 + KEYS > lim_all;
           // the first step and masked ones take the whole row at once
           const bool upper = j > 0 && !masked;
@@ -701,29 +762,54 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
           if (lane == 0) mbar_arrive(smem_u32(&sh->p_ready[i]));
         }
         if (ok) ok = wait(sh->o_full[i], of_ph);
-        if (!ok) break;
         of_ph ^= 1u;
         tc_fence_after();
+        float w_own = 1.f, w_other = 0.f;  // weights of the two sides' O
+        if (paired) {
+          sh->pair[i][r] = make_float2(m, l);
+          tc_fence_before();
+          named_barrier_sync(4, 256);
+          tc_fence_after();
+          const float2 other = sh->pair[i ^ 1][r];
+          const float top = fmaxf(m, other.x);
+          w_own = m == top ? 1.f : ex2_approx(m - top);
+          w_other = other.x == top ? 1.f : ex2_approx(other.x - top);
+          m = top;
+          l = l * w_own + other.y * w_other;
+        }
         const float inv = l == 0.f ? 0.f : 1.f / l;
+        w_own *= inv;
+        w_other *= inv;
         __syncwarp();
-        if (live) {
+        if (live && ok && (i == 0 || !paired)) {
           const float lse2 = l == 0.f ? -INFINITY : m + (log2f(l) - kPOffset);
           if (whole) p.lse[row * (p.heads_kv * p.group) + head] = lse2 * kLn2;
           else p.part_lse[part_row] = lse2;
         }
         T* out = static_cast<T*>(p.o) + row * p.o_stride[0] + head * p.o_stride[1];
         float* part = p.part_o + part_row * D;
+        const uint32_t tO_other = tmem + lane_off + G::TMEM_O + (i ^ 1) * D;
+        // (a pair's sides write every other 16 columns)
 #pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
+        for (int c = first; c < D / 16 && ok; c += stride) {
           uint32_t o[16];
+          float f[16];
           __syncwarp();
           tmem_ld16(tO + c * 16, o);
           tmem_wait_ld();
-          float f[16];
 #pragma unroll
           for (int u = 0; u < 16; ++u) {
             asm volatile("" : "+r"(o[u]));
-            f[u] = __uint_as_float(o[u]) * inv;
+            f[u] = __uint_as_float(o[u]) * w_own;
+          }
+          if (paired) {
+            tmem_ld16(tO_other + c * 16, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+              asm volatile("" : "+r"(o[u]));
+              f[u] = fmaf(__uint_as_float(o[u]), w_other, f[u]);
+            }
           }
           if (live && whole) {
             uint32_t pk[8];
@@ -739,6 +825,10 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
             st_global_v8(part + c * 16, b);
             st_global_v8(part + c * 16 + 8, b + 8);
           }
+        }
+        if (paired) {  // both sides have read both O
+          tc_fence_before();
+          named_barrier_sync(4, 256);
         }
         __syncwarp();
         tc_fence_before();
