@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
   let_next_launch();
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::STAGES; ++s) {
-      mbar_init(smem_u32(&s_full[s]), 1);
+      mbar_init(smem_u32(&s_full[s]), G::NP);
       mbar_init(smem_u32(&s_empty[s]), NW);
     }
     s_abort = 0u;
@@ -231,12 +231,6 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
           if (issued >= meet.limit) break;
         }
         const uint32_t bar = smem_u32(&s_full[slot]);
-        // (the other warps' copies may land before this arrival: the phase waits for it)
-        if (pw == 0 && lane == 0) {
-          const int live = min(boxes, max(0, (w.s.len - key0 + box - 1) / box));  // with a key
-          mbar_arrive_expect_tx(bar, live * box * (2 * G::ROW_BYTES + (FP8 ? 8 : 0)));
-        }
-        __syncwarp();
         if (page >= 0) {
           const uint32_t dst = smem_u32(smem + slot * G::STAGE) + to;
           const int row = (key0 + my_box * box) & ((1 << p.seqs.page_log2) - 1);
@@ -246,6 +240,13 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
             tma_load_4d(dst, map, bar, span * (FP8 ? G::SPAN : G::SPAN / 2), row, w.head, page);
         }
         __syncwarp();
+        // (Copies may land before their bytes are announced: the phase waits for all arrivals.  A
+        // warp without copies arrives too, so that it cannot fall phases behind.)
+        if (lane == 0) {
+          const int live = min(boxes, max(0, (w.s.len - key0 + box - 1) / box));  // with a key
+          if (pw == 0) mbar_arrive_expect_tx(bar, live * box * (2 * G::ROW_BYTES + (FP8 ? 8 : 0)));
+          else mbar_arrive(bar);
+        }
         ++issued;
         if (++slot == G::STAGES) {
           slot = 0;

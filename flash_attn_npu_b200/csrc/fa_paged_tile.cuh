@@ -150,13 +150,13 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
   let_next_launch();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&sh->kv_full[s]), FP8 ? G::AUX : 1);  // converting warps, or the producer
+      mbar_init(smem_u32(&sh->kv_full[s]), FP8 ? G::AUX : 2);  // converting warps, or the producers
       mbar_init(smem_u32(&sh->kv_empty[s]), TILES);       // one commit per issuer
       mbar_init(smem_u32(&sh->v_go[s]), 1);
       mbar_init(smem_u32(&sh->v_clean[s]), 4);
     }
     for (int s = 0; s < 4; ++s) {
-      mbar_init(smem_u32(&sh->raw_full[s]), 1);
+      mbar_init(smem_u32(&sh->raw_full[s]), 2);
       mbar_init(smem_u32(&sh->raw_empty[s]), G::AUX);
     }
     for (int i = 0; i < 2; ++i) {
@@ -279,12 +279,6 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
               if (stop) break;
             }
             const uint32_t bar = smem_u32(&full[slot]);
-            // (the other warp's copies may land before this arrival: the phase waits for it)
-            if (pw == 0 && lane == 0) {
-              const int live = min(boxes, max(0, (w.s.len - key0 + box - 1) / box));  // with a key
-              mbar_arrive_expect_tx(bar, live * box * (FP8 ? D + 4 : G::ROW_BYTES));
-            }
-            __syncwarp();
             if (page >= 0) {
               const CUtensorMap* map = kv ? &tmV : &tmK;
               if constexpr (FP8) {
@@ -302,6 +296,12 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
               }
             }
             __syncwarp();
+            // (as in the row kernel: copies may land before this, and both warps arrive)
+            if (lane == 0) {
+              const int live = min(boxes, max(0, (w.s.len - key0 + box - 1) / box));  // with a key
+              if (pw == 0) mbar_arrive_expect_tx(bar, live * box * (FP8 ? D + 4 : G::ROW_BYTES));
+              else mbar_arrive(bar);
+            }
             if (!FP8 && kv == 1 && t + 1 == w.tile1 && w.tail() && pw == 0 && lane == 0)
               mbar_arrive(smem_u32(&sh->v_go[slot]));
             ++issued;
