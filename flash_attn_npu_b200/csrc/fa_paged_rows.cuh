@@ -605,7 +605,9 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
       }
       if (t + 1 == w.tile1) break;  // the last stage is kept for joining
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s_empty[slot]));
+      // (a stage is given back only if it was seen full: a second fill on top of one that is still
+      // landing would upset the barrier)
+      if (ok && lane == 0) mbar_arrive(smem_u32(&s_empty[slot]));
       if (++slot == G::STAGES) {
         slot = 0;
         ph ^= 1u;
@@ -719,7 +721,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
     // the stage goes back to the producers, whose copies are ordered behind these accesses
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&s_empty[slot]));
+    if (ok && lane == 0) mbar_arrive(smem_u32(&s_empty[slot]));
     if (++slot == G::STAGES) {
       slot = 0;
       ph ^= 1u;
