@@ -139,7 +139,7 @@ def _aligned(t) -> bool:
     if any(t.shape[d] > 1 and (t.stride(d) <= 0 or (t.stride(d) * eb) % 16)
            for d in range(t.ndim - 1)):
         return False
-    return t.device.type == "meta" or t.data_ptr() % 16 == 0
+    return t.device.type == "meta" or hasattr(t, "fake_device") or t.data_ptr() % 16 == 0
 
 
 def _require_cuda(t) -> None:
