@@ -22,6 +22,10 @@
 
 namespace fa {
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 // Programmatic dependent launch: a kernel of the paged calls is brought up while the one before it
 // in the stream still runs, and waits here for its end (and its memory) before it reads anything.
 __device__ __forceinline__ void wait_for_launch_before() {

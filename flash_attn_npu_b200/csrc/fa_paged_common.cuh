@@ -44,6 +44,17 @@ __device__ __forceinline__ int seq_len(const PagedSeqs& s, int b) {
   return n < 0 ? 0 : static_cast<int>(n < cap ? n : cap);
 }
 
+// Entry of the page table for a position inside sequence b, not looked at yet, and what it names: a
+// page of the cache (0, and a report, where it is none).
+__device__ __forceinline__ int page_entry(const PagedSeqs& s, int b, int pos) {
+  return __ldg(s.page_table + b * s.table_stride + (pos >> s.page_log2));
+}
+__device__ __forceinline__ int checked_page(const PagedSeqs& s, int entry) {
+  if (static_cast<uint32_t>(entry) < static_cast<uint32_t>(s.num_pages)) return entry;
+  report(s.status, kStatusPageTable);
+  return 0;
+}
+
 // Page that holds position `pos` of sequence b, or -1 where there is none.
 __device__ __forceinline__ int page_of(const PagedSeqs& s, int b, int pos) {
   const int col = pos >> s.page_log2;

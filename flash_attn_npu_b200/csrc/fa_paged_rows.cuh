@@ -209,19 +209,16 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
             __ldg(p.seqs.offsets + w.b + 1) - __ldg(p.seqs.offsets + w.b) != w.s.count)
           report(status, kStatusPageTable);
       }
-      // the page of this lane's copy for a tile; looked up one tile ahead
-      auto look_up = [&](int t) -> int {
-        const int key = t * KEYS + my_box * box;
-        if (my_box >= boxes || t >= w.tile1 || key >= w.s.len) return -1;
-        const int page = page_of(p.seqs, w.b, key);
-        if (page < 0) report(status, kStatusPageTable);
-        return max(page, 0);
+      // the page of this lane's copy for a tile: its entry is fetched one tile ahead
+      const int tile1 = my_box < boxes ? min(w.tile1, (w.s.len - my_box * box + KEYS - 1) / KEYS) : 0;
+      auto fetch = [&](int t) -> int {
+        return t < tile1 ? page_entry(p.seqs, w.b, t * KEYS + my_box * box) : 0;
       };
-      int next_page = look_up(w.tile0);
+      int entry = fetch(w.tile0);
       for (int t = w.tile0; t < w.tile1; ++t) {
         const int key0 = t * KEYS;
-        const int page = next_page;
-        next_page = look_up(t + 1);
+        const int page = t < tile1 ? checked_page(p.seqs, entry) : -1;
+        entry = fetch(t + 1);
         if (ok) {
           ok = wait_bar_flag(&s_abort, smem_u32(&s_empty[slot]), ph ^ 1u, status);
           ok = __all_sync(0xffffffffu, ok);

@@ -93,6 +93,9 @@ struct TileShared {
   uint64_t mma_done;
   float2 pair[2][128];  // (m, l) of the two sides' rows
   int issued[2];
+  PagedRange range;
+  Walk first_walk;  // at the CTA's first part, if there is one
+  int first_more;
   Walk walks[20];  // one per warp: kept out of the registers of the roles' loops
   int more[20];
   uint32_t tmem_base;
@@ -148,6 +151,11 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
   int* const status = p.seqs.status;
 
   let_next_launch();
+  if (threadIdx.x == 32) {
+    prefetch_map(&tmQ);
+    prefetch_map(&tmK);
+    prefetch_map(&tmV);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&sh->kv_full[s]), FP8 ? G::AUX : 2);  // converting warps, or the producers
@@ -188,8 +196,18 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
   const uint32_t tmem = sh->tmem_base;
   wait_for_launch_before();
   if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
-  const PagedRange range =
-      paged_range(p, [&](int b) { return PagedTiles<TILES, KEYS>(p, b).steps(p); });
+  if (warp == 0) {
+    const PagedRange r =
+        paged_range(p, [&](int b) { return PagedTiles<TILES, KEYS>(p, b).steps(p); });
+    if (lane == 0) {
+      sh->range = r;
+      Walk x(p, r);
+      sh->first_more = x.next(p, r.hi);
+      sh->first_walk = x;
+    }
+  }
+  __syncthreads();
+  const PagedRange& range = sh->range;
 
   auto wait1 = [&](uint64_t& bar, uint32_t parity) {
     return wait_bar_flag(&sh->abort_flag, smem_u32(&bar), parity, status);
@@ -198,10 +216,15 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
     return static_cast<bool>(__all_sync(0xffffffffu, wait1(bar, parity)));
   };
   Walk& w = sh->walks[warp];
-  if (lane == 0) w = Walk(p, range);
+  bool begun = false;
   auto next_part = [&]() -> bool {
     __syncwarp();  // the warp is done with the last part
-    if (lane == 0) sh->more[warp] = w.next(p, range.hi);
+    if (lane == 0) {
+      Walk x = begun ? w : sh->first_walk;
+      sh->more[warp] = begun ? x.next(p, range.hi) : sh->first_more;
+      w = x;
+    }
+    begun = true;
     __syncwarp();
     return sh->more[warp] != 0;
   };
@@ -221,9 +244,9 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
       const uint32_t to = !FP8        ? part * G::KV_BLK + my_box * box * G::SWZ
                           : part == 0 ? my_box * box * D
                                       : KEYS * D + my_box * box * 4;
-      uint32_t qe_ph[2] = {0u, 0u};    // q_empty
-      uint32_t q_par[2] = {1u, 1u};    // parity of the last Q load's q_full phase
-      bool q_loaded[2] = {false, false};
+      uint32_t qe_ph = 0u;   // q_empty
+      uint32_t q_par = 1u;   // parity of the last Q load's q_full phase
+      bool q_loaded = false;
       constexpr int RING = FP8 ? G::RAW_STAGES : STAGES;
       uint64_t* const full = FP8 ? sh->raw_full : sh->kv_full;
       uint64_t* const empty = FP8 ? sh->raw_empty : sh->kv_empty;
@@ -232,43 +255,36 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
       bool ok = true;
       ProducersMeet<2> meet{sh->issued, 3};
       while (issued < meet.limit && next_part()) {
-        if (pw == 0) {
-          if (lane == 0 && (__ldg(p.seqs.kv_lens + w.b) != w.s.len ||
-                            __ldg(p.seqs.offsets + w.b + 1) - __ldg(p.seqs.offsets + w.b) != w.s.count))
-            report(status, kStatusPageTable);
+        // the page of this lane's copies for a tile: its entry is fetched one tile ahead
+        const int tile1 = my_box < boxes ? min(w.tile1, (w.s.len - my_box * box + KEYS - 1) / KEYS) : 0;
+        auto fetch = [&](int t) -> int {
+          return t < tile1 ? page_entry(p.seqs, w.b, t * KEYS + my_box * box) : 0;
+        };
+        int entry = fetch(w.tile0);
+        // The warps load a query tile each.
 #pragma unroll
-          for (int i = 0; i < TILES; ++i) {
-            if (!ok || (w.steps(p, i) == 0 && !w.paired(p))) continue;
-            ok = wait(sh->q_empty[i], qe_ph[i] ^ 1u);
-            if (!ok) continue;
-            qe_ph[i] ^= 1u;
-            q_par[i] ^= 1u;
-            q_loaded[i] = true;
-            if (lane == 0) {
-              const uint32_t bar = smem_u32(&sh->q_full[i]);
-              mbar_arrive_expect_tx(bar, p.tile_live * G::ROW_BYTES);
+        for (int i = 0; i < TILES; ++i) {
+          if (!ok || i != pw || (w.steps(p, i) == 0 && !w.paired(p))) continue;
+          ok = wait(sh->q_empty[i], qe_ph ^ 1u);
+          if (!ok) continue;
+          qe_ph ^= 1u;
+          q_par ^= 1u;
+          q_loaded = true;
+          if (lane == 0) {
+            const uint32_t bar = smem_u32(&sh->q_full[i]);
+            mbar_arrive_expect_tx(bar, p.tile_live * G::ROW_BYTES);
 #pragma unroll
-              for (int c = 0; c < G::NBLK; ++c)
-                tma_load_3d(smem_u32(q_smem + i * G::Q_TILE + c * G::Q_BLK), &tmQ, bar,
-                            c * (G::SWZ / 2), w.head * p.group,
-                            w.s.first + w.tok0(p, w.paired(p) ? 0 : i));
-            }
+            for (int c = 0; c < G::NBLK; ++c)
+              tma_load_3d(smem_u32(q_smem + i * G::Q_TILE + c * G::Q_BLK), &tmQ, bar,
+                          c * (G::SWZ / 2), w.head * p.group,
+                          w.s.first + w.tok0(p, w.paired(p) ? 0 : i));
           }
         }
-        // the page of this lane's copies for a tile; looked up one tile ahead
-        auto look_up = [&](int t) -> int {
-          const int key = t * KEYS + my_box * box;
-          if (my_box >= boxes || t >= w.tile1 || key >= w.s.len) return -1;
-          const int page = page_of(p.seqs, w.b, key);
-          if (page < 0) report(status, kStatusPageTable);
-          return max(page, 0);
-        };
-        int next_page = look_up(w.tile0);
         bool stop = false;
         for (int t = w.tile0; t < w.tile1 && !stop; ++t) {
           const int key0 = t * KEYS;
-          const int page = next_page;
-          next_page = look_up(t + 1);
+          const int page = t < tile1 ? checked_page(p.seqs, entry) : -1;
+          entry = fetch(t + 1);
           const int row = (key0 + my_box * box) & (size - 1);
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
@@ -311,12 +327,14 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
             }
           }
         }
+        if (pw == 0 && lane == 0 &&
+            (__ldg(p.seqs.kv_lens + w.b) != w.s.len ||
+             __ldg(p.seqs.offsets + w.b + 1) - __ldg(p.seqs.offsets + w.b) != w.s.count))
+          report(status, kStatusPageTable);
       }
       meet(pw, issued);
       // the copies issued last land before shared memory goes away
-#pragma unroll
-      for (int i = 0; i < TILES; ++i)
-        if (q_loaded[i]) drain_bar(smem_u32(&sh->q_full[i]), q_par[i]);
+      if (q_loaded) drain_bar(smem_u32(&sh->q_full[pw]), q_par);
       for (int u = 0; u < min(issued, RING); ++u) {
         const int x = issued - 1 - u;
         drain_bar(smem_u32(&full[x % RING]), static_cast<uint32_t>((x / RING) & 1));
@@ -630,6 +648,7 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
       const float sl2 = p.scale_log2;
       const float2 sc = make_float2(sl2, sl2);
       const int r_tok = r / p.group, r_head = r % p.group;  // of the tile
+      const bool wide = (reinterpret_cast<uintptr_t>(p.o) | p.o_stride[0] * 2 | p.o_stride[1] * 2) % 32 == 0;
       uint32_t s_ph = 0, of_ph = 0;
       bool ok = true;
 
@@ -815,10 +834,15 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
             uint32_t pk[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) pk[u] = pack2(f[2 * u], f[2 * u + 1], static_cast<T*>(nullptr));
-            *reinterpret_cast<uint4*>(out + c * 16) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            *reinterpret_cast<uint4*>(out + c * 16 + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+            // (lanes are a row apart, so a store takes a cycle a lane: 32 bytes at a time if the
+            // layout allows)
+            if (wide) {
+              st_global_v8(out + c * 16, pk);
+            } else {
+              *reinterpret_cast<uint4*>(out + c * 16) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              *reinterpret_cast<uint4*>(out + c * 16 + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+            }
           } else if (live) {
-            // whole 32-byte sectors: a thread owns a row, so lanes are a row apart
             uint32_t b[16];
 #pragma unroll
             for (int u = 0; u < 16; ++u) b[u] = __float_as_uint(f[u]);
