@@ -46,7 +46,7 @@ __device__ __forceinline__ int find_seq(const PagedSeqs& s, int t, int lane) {
   while (lo < hi) {
     const int step = (hi - lo + 31) / 32;
     const int probe = min(lo + (lane + 1) * step, hi);  // is the answer >= probe?
-    const bool past = __ldg(s.offsets + probe) <= t;
+    const bool past = fresh(s.offsets + probe) <= t;
     const int n = __popc(__ballot_sync(0xffffffffu, past));
     const int next = min(lo + n * step, hi);
     hi = n == 32 ? hi : min(lo + (n + 1) * step, hi) - 1;
@@ -108,10 +108,10 @@ __global__ void __launch_bounds__(kThreads, 4) paged_copy_kernel(const CopyParam
       const int t = t0 + i;
       const int b = find_seq(p.seqs, t, lane);
       if (lane == 0) {
-        const int end = __ldg(p.seqs.offsets + b + 1);
+        const int end = fresh(p.seqs.offsets + b + 1);
         int page = -2, pos = 0;  // -2: of no sequence
-        if (t < end && t >= __ldg(p.seqs.offsets + b)) {
-          pos = __ldg(p.seqs.kv_lens + b) - (end - t);
+        if (t < end && t >= fresh(p.seqs.offsets + b)) {
+          pos = fresh(p.seqs.kv_lens + b) - (end - t);
           page = page_of(p.seqs, b, pos);
           if (page < 0) report(p.seqs.status, kStatusPageTable);
         }
@@ -137,14 +137,14 @@ __global__ void __launch_bounds__(kThreads, 4) paged_copy_kernel(const CopyParam
         const Place q = place(i);
         if (WRITE) {
 #pragma unroll
-          for (int k = 0; k < WORDS; ++k) x[u][k] = __ldg(reinterpret_cast<const uint4*>(packed(q)) + k);
+          for (int k = 0; k < WORDS; ++k) x[u][k] = fresh(reinterpret_cast<const uint4*>(packed(q)) + k);
         } else if (s_page[q.tok] >= 0) {
           const int64_t c = cached(q);
           if (FP8) {
-            x[u][0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.cache[q.kv]) + c));
-            sc[u] = __ldg(scale_of(q));
+            x[u][0] = fresh(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.cache[q.kv]) + c));
+            sc[u] = fresh(scale_of(q));
           } else {
-            x[u][0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.cache[q.kv]) + c));
+            x[u][0] = fresh(reinterpret_cast<const uint4*>(static_cast<const T*>(p.cache[q.kv]) + c));
           }
         }
       }

@@ -26,13 +26,21 @@ struct PagedSeqs {
   int* status;
 };
 
+// A load of what an earlier kernel may have written.  Not through the read-only path: this kernel may
+// have been brought up before that one ended (programmatic dependent launch), so the data may change
+// within its lifetime.
+template <typename T>
+__device__ __forceinline__ T fresh(const T* p) {
+  return *p;
+}
+
 __device__ __forceinline__ void report(int* status, int code) {
   if (status) atomicCAS(status, 0, code);
 }
 
 // Rows of sequence b in the packed tensors, kept inside [0, total].
 __device__ __forceinline__ void seq_rows(const PagedSeqs& s, int b, int& first, int& count) {
-  const int a = __ldg(s.offsets + b), z = __ldg(s.offsets + b + 1);
+  const int a = fresh(s.offsets + b), z = fresh(s.offsets + b + 1);
   first = min(max(a, 0), s.total);
   count = max(min(z, s.total) - first, 0);
 }
@@ -40,14 +48,14 @@ __device__ __forceinline__ void seq_rows(const PagedSeqs& s, int b, int& first, 
 // Length of sequence b in the cache, kept inside what its table row can name.
 __device__ __forceinline__ int seq_len(const PagedSeqs& s, int b) {
   const int64_t cap = static_cast<int64_t>(s.table_cols) << s.page_log2;
-  const int n = __ldg(s.kv_lens + b);
+  const int n = fresh(s.kv_lens + b);
   return n < 0 ? 0 : static_cast<int>(n < cap ? n : cap);
 }
 
 // Entry of the page table for a position inside sequence b, not looked at yet, and what it names: a
 // page of the cache (0, and a report, where it is none).
 __device__ __forceinline__ int page_entry(const PagedSeqs& s, int b, int pos) {
-  return __ldg(s.page_table + b * s.table_stride + (pos >> s.page_log2));
+  return fresh(s.page_table + b * s.table_stride + (pos >> s.page_log2));
 }
 __device__ __forceinline__ int checked_page(const PagedSeqs& s, int entry) {
   if (static_cast<uint32_t>(entry) < static_cast<uint32_t>(s.num_pages)) return entry;
@@ -59,7 +67,7 @@ __device__ __forceinline__ int checked_page(const PagedSeqs& s, int entry) {
 __device__ __forceinline__ int page_of(const PagedSeqs& s, int b, int pos) {
   const int col = pos >> s.page_log2;
   if (pos < 0 || col >= s.table_cols) return -1;
-  const int page = __ldg(s.page_table + b * s.table_stride + col);
+  const int page = fresh(s.page_table + b * s.table_stride + col);
   return page >= 0 && page < s.num_pages ? page : -1;
 }
 

@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
     ProducersMeet<G::NP> meet{s_issued, 2};
     while (issued < meet.limit && w.next()) {
       if (pw == 0 && lane == 0) {
-        if (__ldg(p.seqs.kv_lens + w.b) != w.s.len ||
-            __ldg(p.seqs.offsets + w.b + 1) - __ldg(p.seqs.offsets + w.b) != w.s.count)
+        if (fresh(p.seqs.kv_lens + w.b) != w.s.len ||
+            fresh(p.seqs.offsets + w.b + 1) - fresh(p.seqs.offsets + w.b) != w.s.count)
           report(status, kStatusPageTable);
       }
       // the page of this lane's copy for a tile: its entry is fetched one tile ahead
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
       const int tok = tok_of(r), h = row0 + r - tok * p.group;
       uint4 x = make_uint4(0, 0, 0, 0);
       if (row0 + r < rows && p.scale_log2 != 0.f)
-        x = __ldg(reinterpret_cast<const uint4*>(
+        x = fresh(reinterpret_cast<const uint4*>(
             static_cast<const T*>(p.q) + static_cast<int64_t>(w.s.first + tok) * p.q_stride[0] +
             static_cast<int64_t>(w.head * p.group + h) * p.q_stride[1] + piece * 8));
       *reinterpret_cast<uint4*>(s_q + r * G::Q_PITCH + piece * 16) = x;

@@ -328,8 +328,8 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
           }
         }
         if (pw == 0 && lane == 0 &&
-            (__ldg(p.seqs.kv_lens + w.b) != w.s.len ||
-             __ldg(p.seqs.offsets + w.b + 1) - __ldg(p.seqs.offsets + w.b) != w.s.count))
+            (fresh(p.seqs.kv_lens + w.b) != w.s.len ||
+             fresh(p.seqs.offsets + w.b + 1) - fresh(p.seqs.offsets + w.b) != w.s.count))
           report(status, kStatusPageTable);
       }
       meet(pw, issued);
