@@ -11,7 +11,12 @@
 // bytes of a 16-bit row or 16 codes of a float8 row (32 bytes of the packed one), head_dim / PIECE
 // threads to a row, so that a row's largest magnitude is a few shuffles.  Each CTA takes a run of
 // tokens, whose sequences and pages its warps look up (a 32-way search of the offsets).  A write has
-// its packed rows on their way before that; a read cannot, so its CTAs are small and many to an SM.
+// its packed rows on their way before that; a read cannot.  What hides the lookups, and the loads
+// where a CTA starts, are other CTAs: two pieces a thread and six (write) or eight (read) CTAs to an
+// SM took 24.4 and 61 us where four pieces and four CTAs took 25.3 and 65 (9 prompts of 16700 tokens
+// in all, 8 heads of 128, to float8; 56700 tokens back to bf16); one piece and eight: 25.1 and 72.
+// These are 4.2 and 5.8 TB/s.  The rest of the shorter one is its start and end: 3 us is what a call
+// of 16 tokens takes.
 #include <cmath>
 
 #include "../../include/fa_paged_sm100.h"
@@ -23,7 +28,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 64;  // tokens of one CTA's run
-constexpr int kUnroll = 4;      // pieces of a thread in flight
+constexpr int kUnroll = 2;      // pieces of a thread in flight
 
 struct CopyParams {
   PagedSeqs seqs;
@@ -63,11 +68,12 @@ constexpr int kPiece = FP8 ? 16 : 8;
 // T: type of the packed rows.  FP8: the cache holds e4m3 codes and scales, else T.  WRITE: rows
 // go to the cache, else from it.
 template <typename T, bool FP8, bool WRITE>
-__global__ void __launch_bounds__(kThreads, 4) paged_copy_kernel(const CopyParams p) {
+__global__ void __launch_bounds__(kThreads, WRITE ? 6 : 8) paged_copy_kernel(const CopyParams p) {
   constexpr int PIECE = kPiece<FP8>;
   constexpr int WORDS = PIECE / 8;  // 16-byte words of a packed piece
-  __shared__ int s_page[kMaxTokens];
-  __shared__ int s_slot[kMaxTokens];
+  __shared__ int s_page[kMaxTokens];            // < 0: the token has no place
+  __shared__ int64_t s_row[2][kMaxTokens];      // its rows in K and V, of head 0
+  __shared__ int64_t s_scale[2][kMaxTokens];
   let_next_launch();
   wait_for_launch_before();
   const int t0 = blockIdx.x * p.tokens;
@@ -96,18 +102,16 @@ __global__ void __launch_bounds__(kThreads, 4) paged_copy_kernel(const CopyParam
            x.head * p.row_stride[x.kv][1] + x.elem;
   };
   auto cached = [&](const Place& x) -> int64_t {
-    return s_page[x.tok] * p.cache_stride[x.kv][0] + x.head * p.cache_stride[x.kv][1] +
-           s_slot[x.tok] * p.cache_stride[x.kv][2] + x.elem;
+    return s_row[x.kv][x.tok] + x.head * p.cache_stride[x.kv][1] + x.elem;
   };
   auto scale_of = [&](const Place& x) -> float* {
-    return p.scale[x.kv] + s_page[x.tok] * p.scale_stride[x.kv][0] +
-           x.head * p.scale_stride[x.kv][1] + s_slot[x.tok];
+    return p.scale[x.kv] + s_scale[x.kv][x.tok] + x.head * p.scale_stride[x.kv][1];
   };
   auto look_up = [&]() {
     for (int i = warp; i < count; i += kThreads / 32) {
       const int t = t0 + i;
       const int b = find_seq(p.seqs, t, lane);
-      if (lane == 0) {
+      if (lane < 2) {  // K, V
         const int end = fresh(p.seqs.offsets + b + 1);
         int page = -2, pos = 0;  // -2: of no sequence
         if (t < end && t >= fresh(p.seqs.offsets + b)) {
@@ -115,8 +119,10 @@ __global__ void __launch_bounds__(kThreads, 4) paged_copy_kernel(const CopyParam
           page = page_of(p.seqs, b, pos);
           if (page < 0) report(p.seqs.status, kStatusPageTable);
         }
-        s_page[i] = page;
-        s_slot[i] = pos & ((1 << p.seqs.page_log2) - 1);
+        const int slot = pos & ((1 << p.seqs.page_log2) - 1);
+        if (lane == 0) s_page[i] = page;
+        s_row[lane][i] = page * p.cache_stride[lane][0] + slot * p.cache_stride[lane][2];
+        s_scale[lane][i] = page * p.scale_stride[lane][0] + slot;
       }
     }
     __syncthreads();
@@ -159,22 +165,29 @@ __global__ void __launch_bounds__(kThreads, 4) paged_copy_kernel(const CopyParam
       if constexpr (!FP8) {
         if (on) *reinterpret_cast<uint4*>(WRITE ? static_cast<T*>(p.cache[q.kv]) + cached(q) : packed(q)) = x[u][0];
       } else if constexpr (WRITE) {
-        float e[16];
+        uint32_t w[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float2 f = Cvt16<T>::unpack(k < 4 ? (&x[u][0].x)[k] : (&x[u][WORDS - 1].x)[k - 4]);
-          e[2 * k] = f.x;
-          e[2 * k + 1] = f.y;
-        }
-        float top = 0.f;
+        for (int k = 0; k < 8; ++k) w[k] = k < 4 ? (&x[u][0].x)[k] : (&x[u][WORDS - 1].x)[k - 4];
+        // The row's largest magnitude: without their signs the bits of 16-bit floats are ordered as
+        // their values are, two to a word.  What is not finite is rare: it becomes NaN and does not
+        // count.  (Float by float this was half of the kernel's instructions, which bound it.)
+        constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
+        uint32_t m = 0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float a = fabsf(e[k]);
-          if (a < INFINITY) top = fmaxf(top, a);
-          else e[k] = NAN;
+        for (int k = 0; k < 8; ++k) m = __vmaxu2(m, w[k] & 0x7fff7fffu);
+        if (__any_sync(0xffffffffu, (m & 0xffffu) >= kInf || m >> 16 >= kInf)) {
+          m = 0;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            uint32_t keep = 0xffffffffu;
+            if ((w[k] & 0x7fffu) >= kInf) keep &= 0xffff0000u;
+            if ((w[k] >> 16 & 0x7fffu) >= kInf) keep &= 0x0000ffffu;
+            m = __vmaxu2(m, w[k] & keep & 0x7fff7fffu);
+            w[k] |= ~keep;
+          }
         }
-        for (int d = 1; d < lanes; d <<= 1)
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        for (int d = 1; d < lanes; d <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
+        const float top = Cvt16<T>::unpack(max(m & 0xffffu, m >> 16)).x;
         // top = (1 + man / 2^23) * 2^(ex - 127); 448 = 1.75 * 2^8.  (A subnormal top has ex = 0
         // and takes the smallest scale.)
         const uint32_t bits = __float_as_uint(top);
@@ -183,9 +196,11 @@ __global__ void __launch_bounds__(kThreads, 4) paged_copy_kernel(const CopyParam
         const float inv = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
         uint32_t c[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          c[k] = pack2_e4m3(e[4 * k] * inv, e[4 * k + 1] * inv) |
-                 (pack2_e4m3(e[4 * k + 2] * inv, e[4 * k + 3] * inv) << 16);
+        for (int k = 0; k < 4; ++k) {
+          const float2 a = fmul2(Cvt16<T>::unpack(w[2 * k]), make_float2(inv, inv));
+          const float2 b = fmul2(Cvt16<T>::unpack(w[2 * k + 1]), make_float2(inv, inv));
+          c[k] = pack2_e4m3(a.x, a.y) | (pack2_e4m3(b.x, b.y) << 16);
+        }
         if (on) {
           *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.cache[q.kv]) + cached(q)) =
               make_uint4(c[0], c[1], c[2], c[3]);
@@ -198,7 +213,8 @@ __global__ void __launch_bounds__(kThreads, 4) paged_copy_kernel(const CopyParam
           const uint32_t w = (&x[u][0].x)[k >> 1];
           const uint32_t h2 = e4m3x2_to_h2(static_cast<uint16_t>(w >> (16 * (k & 1))));
           const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-          out[k] = pack2(v.x * sc[u], v.y * sc[u], static_cast<T*>(nullptr));
+          const float2 y = fmul2(v, make_float2(sc[u], sc[u]));
+          out[k] = pack2(y.x, y.y, static_cast<T*>(nullptr));
         }
         if (on) {
           uint4* dst = reinterpret_cast<uint4*>(packed(q));

@@ -16,9 +16,9 @@ mix them.  Packed rows behind offsets[-1] are padding: they are not read, and ou
 left as they were.  Pages behind a sequence's length may hold anything, NaN included.
 
 A float8 cache holds code = round_e4m3(x / scale) with one power of two per (token, kv head); any
-positive scale can be read.  page_size is a power of two, 8 .. 1024.  Two sequences may share pages (a
-common prefix), but a call to `write` must not be given the same place twice: which of the rows
-stays there is open.
+positive, normal scale can be read.  page_size is a power of two, 8 .. 1024.  Two sequences may share
+pages (a common prefix), but a call to `write` must not be given the same place twice: which of the
+rows stays there is open.
 
 `page_table`, `kv_lens` and `offsets` are device data, which a launch does not wait for.  Entries outside
 the cache or the table are never followed: the call reports them through the device status word
@@ -219,6 +219,11 @@ def attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scal
     natural-log logsumexp; a row with no key to attend to gets 0 and -inf.  `max_q_len`: an upper
     bound of a sequence's new tokens that the kernel choice goes by (default: total).  `out` and
     `lse` may be given; rows that belong to no sequence are not written.
+
+    Every value inside a sequence takes part in the products, with a probability of 0 where the
+    causal mask hides it: a NaN or an infinity among them may show in any row of the sequence.  Over
+    a float8 cache, calls of more than 32 query rows a kv head round code * scale to q's type
+    (exact for `write`'s scales; with float16 queries it has to be within 65504).
     """
     res = None
     if _binding is not None:

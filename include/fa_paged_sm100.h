@@ -100,7 +100,10 @@ FA_API int fa_paged_write_sm100(const FaPagedCopyArgs* args, void* stream);
 FA_API int fa_paged_read_sm100(const FaPagedCopyArgs* args, void* stream);
 
 /* Attention of the packed queries over the cache: out, and the natural-log logsumexp.  A row
- * with no key to attend to gets out = 0 and lse = -inf. */
+ * with no key to attend to gets out = 0 and lse = -inf.  Every value inside a sequence takes part, with
+ * a probability of 0 where the causal mask hides it, so a NaN or an infinity among them may show in any
+ * row of the sequence.  Over a float8 cache, calls of more than 32 query rows (new tokens times
+ * heads_q / heads_kv) round code * scale to q's type; with fp16 it has to be within 65504. */
 FA_API int fa_paged_attn_sm100(const FaPagedAttnArgs* args, void* stream);
 
 /* Workspace of fa_paged_attn_sm100 for these arguments (pointers are not looked at), on the
