@@ -82,7 +82,9 @@ Choice choose(const FaPagedAttnArgs* a) {
   const int64_t longest = a->max_q_len ? std::min(a->max_q_len, a->total) : a->total;
   // Up to 32 rows a kv head every sequence is one block of the row kernel, which reads the cache
   // once; above that the tile kernel does so for 128 or 256 rows.  It needs a positive scale, and
-  // a group that fits a tile.
+  // a group that fits a tile.  At 32 rows (8 kv heads) the row kernel takes 44 us and the tile kernel
+  // 59 for 16 sequences of 4096 tokens at head_dim 64, 65 and 66 at 128, 63 and 88 at 128 from float8,
+  // 10.7 and 11.6 for one of 512; only 40 of 2048 in 16 bits go the other way (85 and 77).
   const int64_t most = longest * group;
   if (most > 32 && group <= 128 && a->sm_scale > 0.f) c.rows = 0;
   else if (most <= 8) c.rows = 8;

@@ -67,7 +67,7 @@ __device__ __forceinline__ int checked_page(const PagedSeqs& s, int entry) {
 __device__ __forceinline__ int page_of(const PagedSeqs& s, int b, int pos) {
   const int col = pos >> s.page_log2;
   if (pos < 0 || col >= s.table_cols) return -1;
-  const int page = fresh(s.page_table + b * s.table_stride + col);
+  const int page = page_entry(s, b, pos);
   return page >= 0 && page < s.num_pages ? page : -1;
 }
 
