@@ -3,13 +3,17 @@ CTAs at any length, tiles worked on by one or both sides, many sequences shorter
 outputs of odd alignment, caches beyond 32-bit offsets.  Tolerances are those of tests/paged_ref.py."""
 from __future__ import annotations
 
+import os
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import flash_attention_forward as fam
 import paged_ref as ref
+from conftest import REPO
 from flash_attn_npu_b200 import build, ops
 
 pytestmark = pytest.mark.gpu
@@ -144,3 +148,40 @@ def test_cache_beyond_32_bit_offsets(fp8, cuda_device):
     plain, _, tol, _ = ref.attention(one, small.k_cache, small.v_cache, small.table, each, small.lens, True,
                                      head_dim ** -0.5, **small.scales)
     assert ((got.double() - plain).abs() <= tol).all()
+
+
+_FIRST_CALL = """
+import sys
+sys.path[:0] = [{repo!r}, {repo!r} + "/tests"]
+import torch
+import flash_attention_forward as fam
+import paged_ref as ref
+from flash_attn_npu_b200 import ops
+dev = torch.device("cuda", 0)
+b = ref.Batch([{count}, 1], [3000, 200], heads_q=8, heads_kv=2, head_dim=128, fp8={fp8}, device=dev)
+args = (b.q, b.k_cache, b.v_cache, *b.where, True, 0.1)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    fam.paged_cache_write(*b.rows, b.k_cache, b.v_cache, *b.where, **b.scales)
+    out, lse = fam.paged_attention(*args, **b.scales, return_lse=True)
+    k, v = fam.paged_cache_read(b.k_cache, b.v_cache, *b.where, b.total, **b.scales)
+graph.replay()
+torch.cuda.synchronize()
+want, _, tol, _ = ref.attention(*args, **b.scales)
+assert ((out.double() - want).abs() <= tol).all()
+again, _ = fam.paged_attention(*args, **b.scales, return_lse=True)
+assert torch.equal(again, out)
+ops.check_device_status(dev)
+del graph
+"""
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("count", [1, 100])
+def test_first_calls_of_a_process_are_captured(count, fp8, cuda_device):
+    """Nothing ran before the capture: no kernel was loaded, the device has no status word yet."""
+    code = _FIRST_CALL.format(repo=str(REPO), count=count, fp8=fp8)
+    res = subprocess.run([sys.executable, "-c", code], cwd=str(REPO), env=dict(os.environ), capture_output=True, text=True,
+                         timeout=300)
+    assert res.returncode == 0, res.stderr[-3000:]
