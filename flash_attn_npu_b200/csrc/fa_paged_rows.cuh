@@ -19,8 +19,8 @@
 // cache in bf16, pages of 16: 189 us, 6.5 TB/s, what a plain copy reaches; 40 sequences, 410,000 tokens
 // in float8: 137 us, 6.3 TB/s (ncu: DRAM 78 to 80 % of its nominal rate, tensor pipe 10 and 18 %).  One
 // sequence of 131,000 tokens in fp16, 4 kv heads of 64: 32.5 us, 4.1 TB/s, of which start, cut and joining
-// are ~10 us.  Two to eight drafted tokens of 16 sequences: 61 us, 3.8 TB/s, bound by the 32-row
-// block's mma.sync and softmax.  A call of one sequence of 777 tokens: 8.2 us.
+// are ~10 us.  Two to eight drafted tokens of 16 sequences: 57 us, 4.1 TB/s, bound by the 32-row
+// block's chain of mma.sync and softmax (issue slots 30 %, tensor pipe 24 %).  A call of one sequence of 777 tokens: 8.2 us.
 //
 // Float8 caches: codes convert exactly to fp16, so the products run in fp16.  Queries in bf16 are
 // scaled per row by a power of two into fp16's range first (exact but for values 2^-24 below the
