@@ -172,8 +172,10 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   p.min_steps_log2 = p.whole_items ? 0 : tile ? 2 : 1;
   // What an item costs besides its tiles, in tiles: with blocks of 32 rows 6500 cycles where a tile
   // takes 2000 to 2800, with 16 rows 5000.  Counted as one for all of them, drafts of 16 sequences
-  // took 61.9 us instead of 56.7, single tokens of 64 and 40 sequences the same time.
-  p.item_cost = tile ? 3 : c.rows == 32 ? 4 : c.rows == 16 ? 2 : 1;
+  // took 61.9 us instead of 56.7, single tokens of 64 and 40 sequences the same time.  In the tile
+  // kernel 2 took 102 to 104 us and 3 took 105 to 108 for the mixed batch of fa_paged_tile.cuh; other
+  // chunks differ by 2 % either way.
+  p.item_cost = tile ? 2 : c.rows == 32 ? 4 : c.rows == 16 ? 2 : 1;
   p.pair_from = plan.fp8 ? 6 : 3;
   p.tile_toks = tile ? 128 / p.group : 0;
   p.tile_live = tile ? p.tile_toks * p.group : info.rows;
