@@ -25,12 +25,16 @@
 // Float8 caches: codes convert exactly to fp16, so the products run in fp16.  Queries in bf16 are
 // scaled per row by a power of two into fp16's range first (exact but for values 2^-24 below the
 // row's largest).  The key scale multiplies S.  The value scale multiplies p before it is rounded
-// to fp16, relative to the largest scale met so far (mv): O and mv are kept apart.
+// to fp16, relative to a scale mv that O is kept apart from.  Scales may lie far apart (a row of zeros has
+// scale 1), and a ratio of scales must not push p out of fp16's range.  So mv follows the tiles, up and
+// down, where a tile's scales are not all within 2^8 below it, and a tile whose scales spread over more is
+// taken in turns, each with the keys of one such band (the others' logits are -inf in it).
 //
 // p in fp16 (fp16 caches, float8 caches) carries the factor 2^kPOffset, which l carries too: fp16
 // keeps full precision down to 2^-14, and so p does down to 2^-(14 + kPOffset) of the row's
-// largest.  Rounding p to 16 bits costs a relative 2^-8 (bf16) or 2^-11 (fp16) per term at most, as
-// much as rounding the output once; l sums the unrounded p.
+// largest, over a float8 cache times a ratio of at least 2^-8: down to 2^-16 in any case, and what is below
+// that is off by at most 2^-27 of it.  Rounding p to 16 bits costs a relative 2^-8 (bf16) or 2^-11 (fp16)
+// per term at most, as much as rounding the output once; l sums the unrounded p.
 #pragma once
 
 #include <type_traits>
@@ -149,6 +153,11 @@ __device__ __forceinline__ uint32_t swizzled(int row, int piece) {
 }
 
 constexpr float kRescale = 4.f;  // a row's base moves once its max passes it by 2^4
+// Value scales that are taken together, relative to the largest of them, and what is left out of account
+// relative to the largest of all (O, kept in units of mv, has to stay within fp32's range).
+constexpr uint32_t kBandBits = 8;
+constexpr float kBand = 1.f / (1 << kBandBits);
+constexpr float kLeastScale = 1.f / (1ull << 40) / (1ull << 40);
 
 // T: type of q and the output (and of a 16-bit cache).
 template <typename T, int D, bool FP8, int ROWS>
@@ -382,7 +391,9 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
 
     float o[KSTEPS][WN][4];
     float m[WN][2], l[WN][2];
-    float mv = 0.f, inv_mv = 0.f;  // float8: largest value scale so far, and its inverse
+    // float8: what O is relative to, its inverse, the largest value scale so far, and the bound below
+    // which this tile's are left
+    float mv = 0.f, inv_mv = 0.f, top_mv = 0.f, below = INFINITY;
 #pragma unroll
     for (int n = 0; n < WN; ++n) {
 #pragma unroll
@@ -476,34 +487,60 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
         float vs[KN][2];
         if constexpr (FP8) {
           const float* sk = reinterpret_cast<const float*>(smem + slot * G::STAGE + 2 * G::TILE) + key_w + g;
-          float top = 0.f;
+          const bool hides = key0 + 16 * KN > lim_any;
+          uint32_t far = 0;  // of positive floats the bits are ordered, a step of 1 << 23 a power of two
 #pragma unroll
           for (int kn = 0; kn < KN; ++kn)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float ks = sk[16 * kn + 8 * h];
               vs[kn][h] = sk[KEYS + 16 * kn + 8 * h];
-              // a scale behind the last key may be any bits
-              if (tail && key0 + 16 * kn + 8 * h + g >= w.s.len) vs[kn][h] = 0.f;
-              top = fmaxf(top, vs[kn][h]);
+              // that of a key which no row attends to does not count (behind the last key it may be
+              // any bits)
+              if (hides && key0 + 16 * kn + 8 * h + g >= lim_any) vs[kn][h] = 0.f;
+              far = max(far, __float_as_uint(mv) - __float_as_uint(vs[kn][h]));  // (above mv: wraps)
 #pragma unroll
               for (int n = 0; n < WN; ++n) {
                 s[kn][n][2 * h] *= ks;
                 s[kn][n][2 * h + 1] *= ks;
               }
             }
-          if (__any_sync(0xffffffffu, top > mv)) {
+          if (__any_sync(0xffffffffu, far > kBandBits << 23)) {
+            float top = 0.f;
+#pragma unroll
+            for (int kn = 0; kn < KN; ++kn)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) top = vs[kn][h] < below ? fmaxf(top, vs[kn][h]) : top;
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float f = mv / top;  // the same in every lane
+            top_mv = fmaxf(top_mv, top);
+            const float to = fmaxf(top, kLeastScale * top_mv);
+            if (to > mv || (top > 0.f && to < kBand * mv)) {  // the same in every lane
+              const float f = mv / to;
 #pragma unroll
-            for (int d = 0; d < KSTEPS; ++d)
+              for (int d = 0; d < KSTEPS; ++d)
 #pragma unroll
-              for (int n = 0; n < WN; ++n)
+                for (int n = 0; n < WN; ++n)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) o[d][n][c] *= f;
-            mv = top;
-            inv_mv = 1.f / top;
+                  for (int c = 0; c < 4; ++c) o[d][n][c] *= f;
+              mv = to;
+              inv_mv = 1.f / to;
+            }
+            // the keys of this turn, and whether any are left
+            bool more = false;
+            const float from = top < kBand * mv ? 0.f : kBand * mv;  // (of the least there is no other turn)
+#pragma unroll
+            for (int kn = 0; kn < KN; ++kn)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                more |= vs[kn][h] < from && vs[kn][h] > 0.f;
+                if (vs[kn][h] >= below || (vs[kn][h] < from && vs[kn][h] > 0.f)) {
+                  vs[kn][h] = 0.f;
+#pragma unroll
+                  for (int n = 0; n < WN; ++n) s[kn][n][2 * h] = s[kn][n][2 * h + 1] = -INFINITY;
+                }
+              }
+            below = __any_sync(0xffffffffu, more) ? from : INFINITY;
           }
 #pragma unroll
           for (int kn = 0; kn < KN; ++kn)
@@ -606,6 +643,10 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
               mma16816(o[d][n], a, pf[kn][n][0], pf[kn][n][1], (C*)nullptr);
           }
         }
+      }
+      if (FP8 && ok && below != INFINITY) {  // once more, with the keys that are left: fewer each time
+        --t;
+        continue;
       }
       if (t + 1 == w.tile1) break;  // the last stage is kept for joining
       __syncwarp();
