@@ -23,8 +23,8 @@
 // block's chain of mma.sync and softmax (issue slots 30 %, tensor pipe 24 %).  A call of one sequence of 777 tokens: 8.2 us.
 //
 // Float8 caches: codes convert exactly to fp16, so the products run in fp16.  Queries in bf16 are
-// scaled per row by a power of two into fp16's range first (exact but for values 2^-24 below the
-// row's largest).  The key scale multiplies S.  The value scale multiplies p before it is rounded
+// scaled per row by a power of two to the top of fp16's range first (exact but for values below 2^-29 of
+// the row's largest, which are off by at most 2^-40 of it).  The key scale multiplies S.  The value scale multiplies p before it is rounded
 // to fp16, relative to a scale mv that O is kept apart from.  Scales may lie far apart (a row of zeros has
 // scale 1), and a ratio of scales must not push p out of fp16's range.  So mv follows the tiles, up and
 // down, where a tile's scales are not all within 2^8 below it, and a tile whose scales spread over more is
@@ -168,6 +168,8 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
   using C = std::conditional_t<FP8, __half, T>;  // type of the products
   constexpr bool kHalf = std::is_same_v<C, __half>;
   constexpr float kPOffset = kHalf ? 10.f : 0.f;  // p <= 2^(kPOffset + kRescale) < 65504
+  // of a scaled query row (bf16 queries over float8)
+  constexpr float kQueryUnit = std::is_same_v<T, __nv_bfloat16> ? 1.f / 32768.f : 1.f;
   constexpr int NW = G::NW, KEYS = G::KEYS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t s_full[G::STAGES], s_empty[G::STAGES];
@@ -368,9 +370,10 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^-x brings the row's largest into [1, 2)
-        const int x = min(max(static_cast<int>(__float_as_uint(top) >> 23), 2), 252);
-        const float inv = __uint_as_float(static_cast<uint32_t>(254 - x) << 23);
+        // 2^(15 - x) brings the row's largest into [2^15, 2^16), the top of fp16's range (the 2^15 go
+        // back with the key scales, so that no product leaves fp32's range sooner)
+        const int x = min(max(static_cast<int>(__float_as_uint(top) >> 23), 16), 254);
+        const float inv = __uint_as_float(static_cast<uint32_t>(254 + 15 - x) << 23);
         const float back = __uint_as_float(static_cast<uint32_t>(x) << 23);
 #pragma unroll
         for (int k = 0; k < KSTEPS; ++k)
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
           for (int kn = 0; kn < KN; ++kn)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float ks = sk[16 * kn + 8 * h];
+              const float ks = sk[16 * kn + 8 * h] * kQueryUnit;
               vs[kn][h] = sk[KEYS + 16 * kn + 8 * h];
               // that of a key which no row attends to does not count (behind the last key it may be
               // any bits)

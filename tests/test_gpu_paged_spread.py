@@ -1,4 +1,5 @@
-"""Paged attention over float8 caches whose scales lie far apart, or are no powers of two.
+"""Paged attention over float8 caches whose scales lie far apart, or are no powers of two, and bf16 queries of
+unequal channels.
 
 The tolerance is that of tests/paged_ref.py without its allowance in units of the sequence's largest value, which
 would hide what is looked for here: values that a few large rows make small.  With u = eps / 2,
@@ -166,3 +167,19 @@ def test_scales_that_are_no_powers_of_two(count, dtype, causal, cuda_device):
         for s in (b.k_scale, b.v_scale):
             s.mul_(torch.exp(0.5 * torch.randn(s.shape, generator=g)).to(cuda_device))
         _check(b, causal, rounded=True)
+
+@pytest.mark.parametrize("count", COUNTS)
+@pytest.mark.parametrize("low", [2.0 ** -10, 2.0 ** -18])
+def test_queries_of_unequal_channels(low, count, cuda_device):
+    """One channel of the queries is 2^20 or 2^28 times the others, and meets keys that are 0 there."""
+    b = _batch([count], [300], 1.0, head_dim=64, dtype=BF16, device=cuda_device)
+    g = torch.Generator().manual_seed(5)
+    q = low * torch.randn(b.q.shape, generator=g)
+    q[..., 7] = 2.0 ** 10
+    b.q = q.to(BF16).to(cuda_device)
+    k = torch.randn(300, 2, 64, generator=g) / low
+    k[..., 7] = 0
+    _set(b, "k", 0, list(range(300)), k)
+    _check(b, scale=0.25)
+    b.q[..., 7] = 0  # every channel small
+    _check(b, scale=0.25)
