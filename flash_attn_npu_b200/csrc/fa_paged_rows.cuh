@@ -37,6 +37,7 @@
 // per term at most, as much as rounding the output once; l sums the unrounded p.
 #pragma once
 
+#include <cfloat>
 #include <type_traits>
 
 #include "fa_paged_attn.cuh"
@@ -383,8 +384,9 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
             qf[n][k][c] = pack2(a.x * inv, a.y * inv, static_cast<__half*>(nullptr));
           }
         // this lane's fragment is of row g, its logits are of rows 2 t4 and 2 t4 + 1
-        qs[n][0] = scale * __shfl_sync(0xffffffffu, back, 8 * t4);
-        qs[n][1] = scale * __shfl_sync(0xffffffffu, back, 8 * t4 + 4);
+        // (at least FLT_MIN: a factor of 0 would make NaN of masked logits)
+        qs[n][0] = fmaxf(scale * __shfl_sync(0xffffffffu, back, 8 * t4), FLT_MIN);
+        qs[n][1] = fmaxf(scale * __shfl_sync(0xffffffffu, back, 8 * t4 + 4), FLT_MIN);
       }
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k)

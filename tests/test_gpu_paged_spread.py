@@ -183,3 +183,11 @@ def test_queries_of_unequal_channels(low, count, cuda_device):
     _check(b, scale=0.25)
     b.q[..., 7] = 0  # every channel small
     _check(b, scale=0.25)
+
+
+@pytest.mark.parametrize("count", COUNTS)
+def test_queries_of_zeros_and_a_small_scale(count, cuda_device):
+    """The logits are 0 however small the scale is, and what the mask hides stays hidden."""
+    b = _batch([count], [300], 1.0, head_dim=64, dtype=BF16, device=cuda_device)
+    b.q.zero_()
+    _check(b, scale=1e-30)
