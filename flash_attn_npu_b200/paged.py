@@ -131,15 +131,24 @@ def validate_copy(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale=
         _validate_rows(name, t, k_cache, k_cache.shape[1])
 
 
-def _aligned(t) -> bool:
-    """Unit inner stride, and 16-byte strides and address (of a tensor that has one)."""
-    eb = t.element_size()
+def _strided(t) -> bool:
+    """Unit inner stride and 16-byte strides."""
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         return False
-    if any(t.shape[d] > 1 and (t.stride(d) <= 0 or (t.stride(d) * eb) % 16)
-           for d in range(t.ndim - 1)):
-        return False
-    return t.device.type == "meta" or hasattr(t, "fake_device") or t.data_ptr() % 16 == 0
+    return all(t.shape[d] <= 1 or (t.stride(d) > 0 and (t.stride(d) * t.element_size()) % 16 == 0)
+               for d in range(t.ndim - 1))
+
+
+def _aligned(t) -> bool:
+    """... and a 16-byte address (of a tensor that has one)."""
+    return _strided(t) and (t.device.type == "meta" or hasattr(t, "fake_device")
+                            or t.data_ptr() % 16 == 0)
+
+
+def empty_rows(t):
+    """Rows like `t`, not initialised: in its layout where the strides are 16-byte aligned, else
+    contiguous (whatever the address, which a traced call does not know)."""
+    return torch.empty_like(t) if _strided(t) else t.new_empty(t.shape)
 
 
 def _require_cuda(t) -> None:
@@ -206,8 +215,8 @@ def _check(res, device) -> None:
 
 
 def _rows_like(t):
-    """`t`, or a contiguous copy where its rows are not 16-byte aligned."""
-    return t if _aligned(t) else t.contiguous()
+    """`t`, or a copy where its rows are not 16-byte aligned."""
+    return t if _aligned(t) else empty_rows(t).copy_(t.detach())
 
 
 def attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scale, k_scale=None,

@@ -66,7 +66,7 @@ def _paged_attention_fake(q, k_cache, v_cache, page_table, offsets, kv_lens, cau
                           k_scale=None, v_scale=None, max_q_len=None):
     paged.validate_attention(q, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale,
                              max_q_len)
-    return _out_like(q), q.new_empty(q.shape[:2], dtype=torch.float32)
+    return paged.empty_rows(q), q.new_empty(q.shape[:2], dtype=torch.float32)
 
 
 @torch.library.custom_op("flash_attn_b200::paged_cache_write",

@@ -1,0 +1,80 @@
+"""Paged calls that a user may make of the arguments as they come: rows at any address, in any layout."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import flash_attention_forward as fam
+import paged_ref as ref
+from flash_attn_npu_b200 import build, ops, paged, torch_op  # noqa: F401  (registers the operators)
+
+OPS = torch.ops.flash_attn_b200
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def binding(native_lib):
+    build.build_binding()
+
+
+def _off(t, by=1):
+    """The same values, contiguous, `by` elements behind an aligned address."""
+    flat = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)
+    out = flat[by:by + t.numel()].view(t.shape)
+    out.copy_(t)
+    return out
+
+
+def _permuted(t, by=0):
+    """The same values with the heads outside the tokens, `by` elements behind an aligned address."""
+    return _off(t.transpose(0, 1).contiguous(), by).transpose(0, 1)
+
+
+def _layouts(t):
+    wide = torch.empty(*t.shape[:2], t.shape[2] + 3, dtype=t.dtype, device=t.device)[..., 1:1 + t.shape[2]]
+    return {"contiguous, odd address": _off(t), "permuted": _permuted(t), "permuted, odd address": _permuted(t, 3),
+            "odd strides": wide.copy_(t), "shared by the heads": t[:, :1].expand(t.shape)}
+
+
+def test_rows_of_any_layout_become_aligned():
+    t = torch.randn(5, 4, 64).to(BF16)
+    for name, x in _layouts(t).items():
+        y = paged._rows_like(x)
+        assert paged._aligned(y), name
+        assert torch.equal(x, y), name
+        assert y.stride() == paged.empty_rows(x).stride(), name
+    assert paged._rows_like(t) is t
+    assert paged._rows_like(_permuted(t, 3)).stride() == _permuted(t).stride()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_rows_of_any_layout(fp8, cuda_device):
+    b = ref.Batch([1, 30, 140], [500, 77, 300], heads_q=4, heads_kv=2, head_dim=64, fp8=fp8, device=cuda_device, garbage=0.0)
+    given = {n: getattr(b, n).clone() for n in ("k_cache", "v_cache") + (("k_scale", "v_scale") if fp8 else ())}
+    for name, q in _layouts(b.q).items():
+        want, want_lse = fam.paged_attention(q.contiguous().clone(), b.k_cache, b.v_cache, *b.where, True, 0.1, **b.scales,
+                                             return_lse=True)
+        out, lse = fam.paged_attention(q, b.k_cache, b.v_cache, *b.where, True, 0.1, **b.scales, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse), name
+        assert out.stride() == paged.empty_rows(q).stride(), name
+    for name in _layouts(b.rows[0]):
+        held = []
+        for rows in (_layouts, lambda t: {name: _layouts(t)[name].contiguous().clone()}):
+            for n, x in given.items():
+                getattr(b, n).copy_(x)
+            k, v = (rows(x)[name] for x in b.rows)
+            fam.paged_cache_write(k, v, b.k_cache, b.v_cache, *b.where, **b.scales)
+            held.append([getattr(b, n).view(torch.uint8).clone() for n in given])
+        for x, y in zip(*held):
+            assert torch.equal(x, y), name
+    ops.check_device_status(cuda_device)
+
+
+@pytest.mark.gpu
+def test_registered_operator_in_any_layout(cuda_device):
+    """The traced call foresees the output's layout whatever the address is."""
+    b = ref.Batch([1, 30], [50, 77], heads_q=4, heads_kv=2, head_dim=64, device=cuda_device, garbage=0.0)
+    for q in _layouts(b.q).values():
+        torch.library.opcheck(OPS.paged_attention, (q, b.k_cache, b.v_cache, *b.where, True, 0.1),
+                              test_utils=("test_schema", "test_faketensor"))
