@@ -27,6 +27,8 @@ the cache or the table are never followed: the call reports them through the dev
 from __future__ import annotations
 
 import ctypes
+import math
+import operator
 
 import torch
 
@@ -64,9 +66,13 @@ def validate_cache(k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_sc
         raise ValueError("page_size must be a power of two, 8 .. 1024")
     if pages < 1 or heads < 1:
         raise ValueError("a cache needs at least one page and one head")
+    if pages > 1 << 30 or heads > 65536:
+        raise ValueError("a cache has at most 2^30 pages and 65536 heads")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if not _aligned(t):
             raise ValueError(f"{name} needs a unit inner stride and 16-byte aligned strides")
+        if any(t.shape[d] > 1 and t.stride(d) >= 1 << 38 for d in range(3)):
+            raise ValueError(f"{name} needs strides below 2^38")
     if (k_scale is None) != (v_scale is None) or (k_scale is None) == (k_cache.dtype == FP8):
         raise ValueError("k_scale and v_scale go with a float8_e4m3fn cache, and with no other")
     if k_scale is not None:
@@ -198,7 +204,7 @@ def _call(name, device, *args):
         finally:
             binding.set_status(index, 0, False)
     if res is None:
-        raise ValueError("paged calls take plain CUDA tensors")
+        raise ValueError("paged calls take dense CUDA tensors with memory of their own, no subclasses")
     return res
 
 
@@ -212,6 +218,27 @@ def _check(res, device) -> None:
         raise exc
     if ops._CHECK_EVERY_CALL:
         ops.check_device_status(device)
+
+
+def _max_len(n):
+    """An upper bound given as any kind of integer, or None."""
+    if n is None:
+        return None
+    try:
+        n = operator.index(n)
+    except TypeError:
+        raise ValueError(f"max_q_len must be an integer or None (got {n!r})") from None
+    return min(n, 1 << 30)  # (there are no more rows)
+
+
+def _scale(x) -> float:
+    try:
+        x = float(x)
+    except (TypeError, ValueError):
+        raise ValueError(f"sm_scale must be a number (got {x!r})") from None
+    if not math.isfinite(ctypes.c_float(x).value):
+        raise ValueError(f"sm_scale must be finite in float32 (got {x})")
+    return x
 
 
 def _rows_like(t):
@@ -239,6 +266,7 @@ def attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scal
         res = _binding.attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scale,
                                  k_scale, v_scale, max_q_len, out, lse)
     if res is None:
+        sm_scale, max_q_len = _scale(sm_scale), _max_len(max_q_len)
         validate_attention(q, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale,
                            max_q_len)
         _require_cuda(q)
@@ -250,7 +278,7 @@ def attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scal
                                 or lse.device != q.device or not lse.is_contiguous()):
             raise ValueError("lse must be a contiguous float32 tensor [total, heads_q]")
         res = _call("attention", q.device, _rows_like(q), k_cache, v_cache, page_table, offsets,
-                    kv_lens, bool(causal), float(sm_scale), k_scale, v_scale, max_q_len, out, lse)
+                    kv_lens, bool(causal), sm_scale, k_scale, v_scale, max_q_len, out, lse)
     if type(res) is int or ops._CHECK_EVERY_CALL:
         _check(res, q.device)
     return res

@@ -1,8 +1,10 @@
 """Paged calls that a user may make of the arguments as they come: rows at any address, in any layout."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 import flash_attention_forward as fam
 import paged_ref as ref
@@ -78,3 +80,52 @@ def test_registered_operator_in_any_layout(cuda_device):
     for q in _layouts(b.q).values():
         torch.library.opcheck(OPS.paged_attention, (q, b.k_cache, b.v_cache, *b.where, True, 0.1),
                               test_utils=("test_schema", "test_faketensor"))
+
+
+# ------------------------------------------------------------------------------ refusals and their reasons
+def _attend(b, **kw):
+    a = dict(q=b.q, k_cache=b.k_cache, v_cache=b.v_cache, page_table=b.table, offsets=b.offsets, kv_lens=b.lens,
+             causal=True, sm_scale=0.1, **b.scales)
+    a.update(kw)
+    return fam.paged_attention(**a)
+
+
+BAD = [(dict(sm_scale=float("inf")), "sm_scale"), (dict(sm_scale=float("nan")), "sm_scale"), (dict(sm_scale=1e300), "sm_scale"),
+       (dict(sm_scale=None), "sm_scale"), (dict(max_q_len=2.0), "max_q_len"), (dict(max_q_len="2"), "max_q_len"),
+       (dict(max_q_len=np.int64(-1)), "max_q_len")]
+
+
+def test_scales_and_lengths_are_refused_for_what_they_are():
+    b = ref.Batch([2, 3], [20, 30])
+    for change, text in BAD:
+        with pytest.raises(ValueError, match=text):
+            _attend(b, **change)
+
+
+def test_sizes_beyond_the_library():
+    b = ref.Batch([2, 3], [20, 30], device="meta")
+    shape = list(b.k_cache.shape)
+    for at, n, text in ((0, (1 << 30) + 1, "pages"), (1, 65537, "heads")):
+        many = [*shape[:at], n, *shape[at + 1:]]
+        k = torch.empty_strided(many, b.k_cache.stride(), dtype=BF16, device="meta")
+        with pytest.raises(ValueError, match=text):
+            paged.validate_cache(k, k, *b.where, None, None)
+    k = torch.empty_strided(shape, (1 << 38, *b.k_cache.stride()[1:]), dtype=BF16, device="meta")
+    with pytest.raises(ValueError, match="2\\^38"):
+        paged.validate_cache(k, k, *b.where, None, None)
+
+
+@pytest.mark.gpu
+def test_reasons_and_integers_on_the_device(cuda_device):
+    b = ref.Batch([1, 30], [50, 77], heads_q=4, heads_kv=2, head_dim=64, device=cuda_device)
+    want = _attend(b)
+    for n in (30, np.int64(30), np.int32(30), torch.tensor(30), 1 << 70):
+        assert torch.equal(_attend(b, max_q_len=n), want)
+    for scale in (np.float32(0.1), torch.tensor(0.1)):
+        assert torch.allclose(_attend(b, sm_scale=scale).float(), want.float())
+    for change, text in BAD:
+        with pytest.raises(ValueError, match=text):
+            _attend(b, **change)
+    with FakeTensorMode() as mode, pytest.raises(ValueError, match="subclass"):
+        fake = [mode.from_tensor(x) for x in (b.q, b.k_cache, b.v_cache, *b.where)]
+        paged.attention(*fake, True, 0.1)
