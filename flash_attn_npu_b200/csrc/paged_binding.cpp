@@ -36,10 +36,11 @@ const Tensor* tensor_of(PyObject* x) {
   return THPVariable_Check(x) ? &THPVariable_Unpack(x) : nullptr;
 }
 
-// A tensor with memory of its own on device `index`.
+// A tensor on device `index` with memory of its own that holds its values (not their negatives, which
+// the imaginary part of a conjugate view is).
 bool plain(const Tensor& t, int index) {
   return t.is_cuda() && t.get_device() == index && t.layout() == c10::kStrided &&
-         t.unsafeGetTensorImpl()->has_storage() &&
+         t.unsafeGetTensorImpl()->has_storage() && !t.is_neg() &&
          !t.unsafeGetTensorImpl()->key_set().has(c10::DispatchKey::Python);
 }
 

@@ -93,9 +93,11 @@ def validate_cache(k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_sc
         raise ValueError("offsets, kv_lens and the rows of page_table must be contiguous")
     if page_table.shape[1] * size > 1 << 30:
         raise ValueError("page_table names more than 2^30 positions a sequence")
-    for t in (v_cache, page_table, offsets, kv_lens, k_scale, v_scale):
+    for t in (k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale):
         if t is not None and t.device != k_cache.device:
             raise ValueError("all tensors of a paged call must be on the same device")
+        if t is not None and t.is_neg():
+            raise ValueError("a cache, its scales and its sequences must not be negated views")
 
 
 def _validate_rows(name, t, k_cache, heads) -> None:
@@ -242,8 +244,8 @@ def _scale(x) -> float:
 
 
 def _rows_like(t):
-    """`t`, or a copy where its rows are not 16-byte aligned."""
-    return t if _aligned(t) else empty_rows(t).copy_(t.detach())
+    """`t`, or a copy where its rows are not 16-byte aligned or its memory holds their negatives."""
+    return t if _aligned(t) and not t.is_neg() else empty_rows(t).copy_(t.detach())
 
 
 def attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scale, k_scale=None,
@@ -271,11 +273,11 @@ def attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scal
                            max_q_len)
         _require_cuda(q)
         if out is not None and (out.shape != q.shape or out.dtype != q.dtype
-                                or out.device != q.device or not _aligned(out)):
+                                or out.device != q.device or not _aligned(out) or out.is_neg()):
             raise ValueError("out must match q in shape, dtype and device, with a unit inner stride "
                              "and 16-byte aligned strides")
         if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32
-                                or lse.device != q.device or not lse.is_contiguous()):
+                                or lse.device != q.device or not lse.is_contiguous() or lse.is_neg()):
             raise ValueError("lse must be a contiguous float32 tensor [total, heads_q]")
         res = _call("attention", q.device, _rows_like(q), k_cache, v_cache, page_table, offsets,
                     kv_lens, bool(causal), sm_scale, k_scale, v_scale, max_q_len, out, lse)
@@ -336,7 +338,7 @@ def read(k_cache, v_cache, page_table, offsets, kv_lens, total, k_scale=None, v_
         k, v = out
         if k.shape[0] != total or (dtype is not None and k.dtype != dtype):
             raise ValueError("out must have `total` rows of the given dtype")
-        if not (_aligned(k) and _aligned(v)):
+        if not (_aligned(k) and _aligned(v)) or k.is_neg() or v.is_neg():
             raise ValueError("out needs a unit inner stride and 16-byte aligned strides")
     _copy(False, k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale)
     return k, v

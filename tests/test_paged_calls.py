@@ -129,3 +129,31 @@ def test_reasons_and_integers_on_the_device(cuda_device):
     with FakeTensorMode() as mode, pytest.raises(ValueError, match="subclass"):
         fake = [mode.from_tensor(x) for x in (b.q, b.k_cache, b.v_cache, *b.where)]
         paged.attention(*fake, True, 0.1)
+
+
+# ------------------------------------------------------------------------------ negated views
+def test_negated_views_are_copied_or_refused():
+    b = ref.Batch([2, 3], [20, 30])
+    x = paged._rows_like(torch._neg_view(b.q))
+    assert not x.is_neg() and torch.equal(x, -b.q)
+    for name in ("k_cache", "v_cache"):
+        with pytest.raises(ValueError, match="negated"):
+            _attend(b, **{name: torch._neg_view(getattr(b, name))})
+
+
+@pytest.mark.gpu
+def test_negated_views(cuda_device):
+    """Their memory holds the values with the other sign."""
+    b = ref.Batch([1, 30], [50, 77], heads_q=4, heads_kv=2, head_dim=64, device=cuda_device, garbage=0.0)
+    want = _attend(b)
+    assert torch.equal(_attend(b, q=torch._neg_view(-b.q)), want)
+    with pytest.raises(ValueError, match="out"):
+        _attend(b, out=torch._neg_view(torch.empty_like(b.q)))
+    with pytest.raises(ValueError, match="negated"):
+        _attend(b, v_cache=torch._neg_view(b.v_cache))
+    k, v = b.rows
+    fam.paged_cache_write(k, v, b.k_cache, b.v_cache, *b.where)
+    held = b.k_cache.clone(), b.v_cache.clone()
+    fam.paged_cache_write(torch._neg_view(-k), torch._neg_view(-v), b.k_cache, b.v_cache, *b.where)
+    assert torch.equal(held[0], b.k_cache) and torch.equal(held[1], b.v_cache)
+    ops.check_device_status(cuda_device)
