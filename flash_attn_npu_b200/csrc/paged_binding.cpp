@@ -139,6 +139,11 @@ bool rows_ok(const Tensor* t, const FaPagedCache& c, int index) {
          (code == c.dtype || c.dtype == FA_DTYPE_FP8_E4M3);
 }
 
+// A tensor given by the caller was written: autograd has to know, as of any operation in place.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 PyObject* none() { Py_RETURN_NONE; }
 
 // attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scale, k_scale, v_scale,
@@ -208,6 +213,8 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int rc = g_attn(&x, c10::cuda::getCurrentCUDAStream(index).stream());
     if (rc != FA_OK) return PyLong_FromLong(rc);
   }
+  if (a[11] != Py_None) written(out);
+  if (a[12] != Py_None) written(lse);
   PyObject* r = PyTuple_New(2);
   if (!r) return nullptr;
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(out)));
@@ -277,7 +284,12 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   x.dev_status = g_status[index];
   const c10::cuda::OptionalCUDAGuard guard(k->device());
   void* stream = c10::cuda::getCurrentCUDAStream(index).stream();
-  return PyLong_FromLong(a[0] == Py_True ? g_write(&x, stream) : g_read(&x, stream));
+  const bool write = a[0] == Py_True;
+  const int rc = write ? g_write(&x, stream) : g_read(&x, stream);
+  if (rc == FA_OK)
+    for (int i : {write ? 3 : 1, write ? 4 : 2, write ? 8 : 0, write ? 9 : 0})
+      if (i > 0 && a[i] != Py_None) written(*tensor_of(a[i]));
+  return PyLong_FromLong(rc);
   END_HANDLE_TH_ERRORS
 }
 

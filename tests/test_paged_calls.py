@@ -157,3 +157,47 @@ def test_negated_views(cuda_device):
     fam.paged_cache_write(torch._neg_view(-k), torch._neg_view(-v), b.k_cache, b.v_cache, *b.where)
     assert torch.equal(held[0], b.k_cache) and torch.equal(held[1], b.v_cache)
     ops.check_device_status(cuda_device)
+
+
+# ------------------------------------------------------------------------------ what autograd sees
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_tensors_written_in_place_have_a_new_version(fp8, cuda_device):
+    b = ref.Batch([1, 30], [50, 77], heads_q=4, heads_kv=2, head_dim=64, fp8=fp8, device=cuda_device, garbage=0.0)
+    held = [b.k_cache, b.v_cache] + ([b.k_scale, b.v_scale] if fp8 else [])
+    out, lse = torch.empty_like(b.q), torch.empty(b.q.shape[:2], device=cuda_device)
+    back = [torch.empty_like(x) for x in b.rows]
+
+    def versions(ts):
+        return [t._version for t in ts]
+
+    before = versions(held + [out, lse] + back)
+    fam.paged_cache_write(*b.rows, b.k_cache, b.v_cache, *b.where, **b.scales)
+    _attend(b, out=out, lse=lse)
+    fam.paged_cache_read(b.k_cache, b.v_cache, *b.where, b.total, **b.scales, out=tuple(back))
+    assert all(x > y for x, y in zip(versions(held + [out, lse] + back), before))
+    now = versions([b.q, b.table, b.offsets, b.lens, *b.rows] + held)
+    _attend(b)
+    fam.paged_cache_read(b.k_cache, b.v_cache, *b.where, b.total, **b.scales)
+    assert versions([b.q, b.table, b.offsets, b.lens, *b.rows] + held) == now
+
+
+@pytest.mark.gpu
+def test_backward_over_a_cache_written_meanwhile_is_refused(cuda_device):
+    b = ref.Batch([3], [20], heads_kv=2, head_dim=64, device=cuda_device, garbage=0.0)
+    w = torch.ones((), device=cuda_device, requires_grad=True)
+    loss = (w * b.k_cache).sum()
+    fam.paged_cache_write(*b.rows, b.k_cache, b.v_cache, *b.where)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.gpu
+def test_inference_tensors_may_be_written(cuda_device):
+    with torch.inference_mode():
+        b = ref.Batch([3], [20], heads_kv=2, head_dim=64, device=cuda_device, garbage=0.0)
+        fam.paged_cache_write(*b.rows, b.k_cache, b.v_cache, *b.where)
+    fam.paged_cache_write(*b.rows, b.k_cache, b.v_cache, *b.where)
+    out = torch.zeros_like(b.q)
+    _attend(b, out=out)
+    assert (out != 0).any()
