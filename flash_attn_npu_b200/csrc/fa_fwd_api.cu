@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -44,33 +45,35 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 // Per-device "is this an sm_100 part" cache (16 devices is plenty for one node).
 int device_ok(int dev) {
-  static int cache[16] = {0};  // 0 unknown, 1 ok, -1 not ok
+  static std::atomic<int> cache[16] = {};  // 0 unknown, 1 ok, -1 not ok
   if (dev < 0 || dev >= 16) return 0;
-  if (cache[dev] == 0) {
+  int known = cache[dev].load(std::memory_order_relaxed);
+  if (known == 0) {
     int major = 0, minor = 0;
     if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
         cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess) {
       (void)cudaGetLastError();
       return 0;
     }
-    cache[dev] = (major == 10 && minor == 0) ? 1 : -1;
+    known = (major == 10 && minor == 0) ? 1 : -1;
+    cache[dev].store(known, std::memory_order_relaxed);
   }
-  return cache[dev] == 1;
+  return known == 1;
 }
 
 // Streaming multiprocessors of a device (cached; 148 on B200).
 int sm_count(int dev) {
-  static int cache[16] = {0};
+  static std::atomic<int> cache[16] = {};
   if (dev < 0 || dev >= 16) return 148;
-  if (cache[dev] == 0) {
-    int n = 0;
+  int n = cache[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
       (void)cudaGetLastError();
       n = 148;
     }
-    cache[dev] = n;
+    cache[dev].store(n, std::memory_order_relaxed);
   }
-  return cache[dev];
+  return n;
 }
 
 // Element type of a tensor map: an FaDtype, or one byte (fp8 V).

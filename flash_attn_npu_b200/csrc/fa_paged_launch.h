@@ -2,6 +2,8 @@
 // translation units that hold the kernel instantiations (fa_paged_rows_d*.cu).
 #pragma once
 
+#include <atomic>
+
 #include "fa_paged_attn.cuh"
 
 namespace fa {
@@ -35,20 +37,40 @@ int launch_rows_d64(const PagedPlan& plan);
 int launch_rows_d128(const PagedPlan& plan);
 int launch_rows_d256(const PagedPlan& plan);
 
+// (Calls of several threads may meet in the two below: what they remember is atomic, and only successes
+// are remembered.)
+
 // A kernel's opt-in to more than 48 KB of shared memory, made once per device: the call costs as
 // much as a small part of a launch.
 struct SmemOptIn {
-  bool done[16] = {};
+  std::atomic<bool> done[16] = {};
   bool operator()(const void* kernel, int bytes) {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
-    if (dev >= 0 && dev < 16 && done[dev]) return true;
+    if (dev >= 0 && dev < 16 && done[dev].load(std::memory_order_acquire)) return true;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
         cudaSuccess) {
       (void)cudaGetLastError();
       return false;
     }
-    if (dev >= 0 && dev < 16) done[dev] = true;
+    if (dev >= 0 && dev < 16) done[dev].store(true, std::memory_order_release);
+    return true;
+  }
+};
+
+// Whether a kernel was built with `regs` registers a thread: setmaxnreg redistributes exactly the launch
+// allocation, so a build that differs is refused.
+struct RegsMatch {
+  std::atomic<bool> known{false};
+  bool operator()(const void* kernel, int regs) {
+    if (known.load(std::memory_order_relaxed)) return true;
+    cudaFuncAttributes attr{};
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return false;
+    }
+    if (attr.numRegs != regs) return false;
+    known.store(true, std::memory_order_relaxed);
     return true;
   }
 };

@@ -19,16 +19,8 @@ int launch_rows(const PagedPlan& plan) {
   using G = RowsGeo<FA_HEAD_DIM, FP8, ROWS>;
   auto kernel = paged_rows_kernel<T, FA_HEAD_DIM, FP8, ROWS>;
   if constexpr (G::SPLIT) {
-    // the split redistributes exactly the launch allocation: refuse a build that differs
-    static int regs_ok = 0;  // 0 unknown, 1 ok, -1 mismatch
-    if (regs_ok == 0) {
-      cudaFuncAttributes attr{};
-      regs_ok = cudaFuncGetAttributes(&attr, kernel) == cudaSuccess && attr.numRegs == G::REG_LAUNCH
-                    ? 1
-                    : -1;
-      (void)cudaGetLastError();
-    }
-    if (regs_ok != 1) return -7;
+    static RegsMatch regs_match;
+    if (!regs_match(reinterpret_cast<const void*>(kernel), G::REG_LAUNCH)) return -7;
   }
   static SmemOptIn opt_in;
   if (!opt_in(reinterpret_cast<const void*>(kernel), G::SMEM)) return -7;
