@@ -331,7 +331,13 @@ def read(k_cache, v_cache, page_table, offsets, kv_lens, total, k_scale=None, v_
                 if type(res) is int or ops._CHECK_EVERY_CALL:
                     _check(res, k_cache.device)
                 return res
-        shape = (int(total), k_cache.shape[1], k_cache.shape[-1])
+        try:
+            total = operator.index(total)
+        except TypeError:
+            total = -1
+        if total < 0:
+            raise ValueError("total must be an integer that is not negative")
+        shape = (total, k_cache.shape[1], k_cache.shape[-1])
         k = torch.empty(shape, dtype=dtype, device=k_cache.device)
         v = torch.empty_like(k)
     else:

@@ -201,3 +201,123 @@ def test_inference_tensors_may_be_written(cuda_device):
     out = torch.zeros_like(b.q)
     _attend(b, out=out)
     assert (out != 0).any()
+
+
+# ------------------------------------------------------------------------------ caches and sequences as they come
+def _cut(b, how):
+    """The batch's cache, its scales too, as views of larger tensors."""
+    for names in (("k_cache", "v_cache"), ("k_scale", "v_scale")):
+        k, v = (getattr(b, n) for n in names)
+        if k is None:
+            continue
+        raw = [x.view(torch.uint8) if x.dtype == ref.FP8 else x for x in (k, v)]
+        if how == "joint":            # [pages, K and V, heads, ..]
+            both = torch.stack(raw, 1)
+            cut = both[:, 0], both[:, 1]
+        elif how == "pages inside":   # [heads, pages, ..]
+            cut = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in raw]
+        else:                         # some of the heads and pages of a larger cache
+            cut = []
+            for x in raw:
+                big = torch.zeros(x.shape[0] + 4, x.shape[1] + 3, *x.shape[2:], dtype=x.dtype, device=x.device)
+                cut.append(big[3:-1, 1:-2].copy_(x))
+        for n, x in zip(names, cut):
+            setattr(b, n, x.view(ref.FP8) if k.dtype == ref.FP8 else x)
+    return b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("how", ["joint", "pages inside", "some"])
+@pytest.mark.parametrize("counts", [[1, 2, 1], [30, 140, 1]])
+def test_caches_cut_from_larger_tensors(counts, how, fp8, cuda_device):
+    a, b = (ref.Batch(counts, [500, 177, 300], heads_q=8, heads_kv=2, head_dim=64, page=32, fp8=fp8, device=cuda_device,
+                      garbage=0.0) for _ in range(2))
+    _cut(b, how)
+    most = max(counts)
+    assert torch.equal(_attend(a, max_q_len=most), _attend(b, max_q_len=most))
+    for x in (a, b):
+        fam.paged_cache_write(*x.rows, x.k_cache, x.v_cache, *x.where, **x.scales)
+    for n in ("k_cache", "v_cache") + (("k_scale", "v_scale") if fp8 else ()):
+        assert torch.equal(getattr(a, n).float(), getattr(b, n).float()), n
+    for x, y in zip(*(fam.paged_cache_read(z.k_cache, z.v_cache, *z.where, z.total, **z.scales) for z in (a, b))):
+        assert torch.equal(x, y)
+    ops.check_device_status(cuda_device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("count", [1, 50])
+def test_sequences_that_share_a_row_of_the_table(count, fp8, cuda_device):
+    """One row of the table for all, expanded: the same tokens seen at different lengths."""
+    b = ref.Batch([count] * 3, [300] * 3, heads_q=8, heads_kv=2, head_dim=64, fp8=fp8, device=cuda_device, garbage=0.0)
+    b.lens = torch.tensor([300, 211, 64], dtype=torch.int32, device=cuda_device)
+    b.table = b.table[:1].expand(3, b.table.shape[1])
+    assert b.table.stride(0) == 0
+    out = _attend(b, max_q_len=count)
+    b.table = b.table.contiguous()
+    assert torch.equal(out, _attend(b, max_q_len=count))
+    want, _, tol, _ = ref.attention(b.q, b.k_cache, b.v_cache, *b.where, True, 0.1, **b.scales, max_q_len=count)
+    assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("counts", [[1, 2], [30, 140]])
+def test_rows_before_the_first_sequence_are_padding(counts, fp8, cuda_device):
+    b = ref.Batch(counts, [500, 177], heads_q=4, heads_kv=2, head_dim=64, fp8=fp8, device=cuda_device, garbage=0.0, pad=7)
+    n, most = int(b.offsets[-1]), max(counts)
+    want = _attend(b, max_q_len=most)
+    caches = [b.k_cache, b.v_cache] + ([b.k_scale, b.v_scale] if fp8 else [])
+    held = [x.clone() for x in caches]
+    fam.paged_cache_write(*b.rows, b.k_cache, b.v_cache, *b.where, **b.scales)
+    read = fam.paged_cache_read(b.k_cache, b.v_cache, *b.where, b.total, **b.scales)
+    written = [x.clone() for x in caches]
+    for x, y in zip(caches, held):
+        x.copy_(y)
+    b.offsets += 5
+    q = torch.full_like(b.q, 7.0)
+    q[5:5 + n] = b.q[:n]
+    out, lse = torch.full_like(b.q, 7.0), torch.full(b.q.shape[:2], 7.0, device=cuda_device)
+    _attend(b, q=q, out=out, lse=lse, max_q_len=most)
+    assert torch.equal(out[5:5 + n], want[:n])
+    for x in (out, lse):
+        assert (x[:5] == 7).all() and (x[5 + n:] == 7).all()
+    rows = [torch.full_like(x, 7.0) for x in b.rows]
+    for x, y in zip(rows, b.rows):
+        x[5:5 + n] = y[:n]
+    fam.paged_cache_write(*rows, b.k_cache, b.v_cache, *b.where, **b.scales)
+    for x, y in zip(caches, written):
+        assert torch.equal(x.float(), y.float())
+    back = tuple(torch.full_like(x, 7.0) for x in b.rows)
+    fam.paged_cache_read(b.k_cache, b.v_cache, *b.where, b.total, **b.scales, out=back)
+    for x, y in zip(back, read):
+        assert torch.equal(x[5:5 + n], y[:n]) and (x[:5] == 7).all() and (x[5 + n:] == 7).all()
+    ops.check_device_status(cuda_device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_table_without_columns(fp8, cuda_device):
+    for counts in ([1, 1], [40, 2]):
+        b = ref.Batch(counts, [40, 2], heads_q=4, heads_kv=2, head_dim=64, fp8=fp8, device=cuda_device)
+        b.table, b.lens = b.table[:, :0], torch.zeros_like(b.lens)
+        out, lse = _attend(b, return_lse=True, max_q_len=max(counts))
+        assert (out == 0).all() and torch.isneginf(lse).all()
+    ops.check_device_status(cuda_device)
+
+
+@pytest.mark.gpu
+def test_the_output_may_be_the_queries(cuda_device):
+    for counts in ([1, 2], [30, 300]):
+        b = ref.Batch(counts, [5000, 777], heads_q=8, heads_kv=2, head_dim=128, device=cuda_device)
+        want = _attend(b, max_q_len=max(counts))
+        q = b.q.clone()
+        assert torch.equal(_attend(b, q=q, out=q, max_q_len=max(counts)), want)
+
+
+def test_totals_that_are_none():
+    b = ref.Batch([2, 3], [20, 30])
+    for total, text in ((-1, "total"), (2.5, "total"), ("5", "total")):
+        with pytest.raises(ValueError, match=text):
+            fam.paged_cache_read(b.k_cache, b.v_cache, *b.where, total)
