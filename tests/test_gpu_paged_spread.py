@@ -191,3 +191,18 @@ def test_queries_of_zeros_and_a_small_scale(count, cuda_device):
     b = _batch([count], [300], 1.0, head_dim=64, dtype=BF16, device=cuda_device)
     b.q.zero_()
     _check(b, scale=1e-30)
+
+
+@pytest.mark.parametrize("count", COUNTS)
+@pytest.mark.parametrize("power", [-126, -100, 60, 100])
+def test_scales_at_the_ends_of_their_range(power, count, cuda_device):
+    """Values at either end, and keys there too, with queries that bring the logits back."""
+    b = ref.Batch([count] * 2, [500, 77], heads_q=8, heads_kv=2, head_dim=64, dtype=BF16, fp8=True, garbage=0.0,
+                  device=cuda_device, seed=6)
+    g = torch.Generator().manual_seed(7)
+    b.v_scale = (2.0 ** power * (1 + torch.rand(b.v_scale.shape, generator=g))).to(cuda_device)
+    _check(b, rounded=True)
+    if power > -126:
+        b.k_scale *= 2.0 ** power
+        b.q *= 2.0 ** -power
+        _check(b, rounded=True)
