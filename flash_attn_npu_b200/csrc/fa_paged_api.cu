@@ -85,6 +85,9 @@ Choice choose(const FaPagedAttnArgs* a) {
   // a group that fits a tile.  At 32 rows (8 kv heads) the row kernel takes 44 us and the tile kernel
   // 59 for 16 sequences of 4096 tokens at head_dim 64, 65 and 66 at 128, 63 and 88 at 128 from float8,
   // 10.7 and 11.6 for one of 512; only 40 of 2048 in 16 bits go the other way (85 and 77).
+  // At head_dim 256 that does not hold: blocks have 16 rows, so 17 to 32 rows are two of them, which
+  // read the cache one after the other.  There 16 sequences of 4096 tokens take 216 us and 110 (float8: 239
+  // and 129), 40 of 2048 270 and 137, one of 512 17 and 17.
   const int64_t most = longest * group;
   if (most > 32 && group <= 128 && a->sm_scale > 0.f) c.rows = 0;
   else if (most <= 8) c.rows = 8;
@@ -166,12 +169,17 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   const bool tile = c.rows == 0;
   // Sequences of at most kWholeTiles tiles are not cut: the joining launch costs more (3 .. 10 us)
   // than the tiles that a CTA then takes one after the other (~0.5 us each in the row kernel,
-  // ~1.3 us in the tile kernel).
+  // ~1.3 us in the tile kernel), however many SMs have nothing to do.  (What is known here is the table's
+  // width, so the same lengths behind a wider table are cut.)  Not cut, and cut, at head_dim 128: one token of
+  // one sequence of 777 with 16 kv heads 8.3 and 10.2 us, with 8 kv heads 8.4 and 9.8; of 8 such sequences 9.1
+  // and 12.1, of 64 40.6 and 43.4; 100 tokens of 4 sequences of 900 25 and 35, of 16 50 and 77 (float8: 64 and
+  // 94); a prompt of 500 17 and 26.
   constexpr int64_t kWholeTiles = 8;
   p.whole_items = kv.table_cols * kv.page_size <= kWholeTiles * info.keys;
   p.min_steps_log2 = p.whole_items ? 0 : tile ? 2 : 1;
-  // What an item costs besides its tiles, in tiles: with blocks of 32 rows 6500 cycles where a tile
-  // takes 2000 to 2800, with 16 rows 5000.  Counted as one for all of them, drafts of 16 sequences
+  // What an item costs besides its tiles, in tiles: at head_dim 128 with blocks of 32 rows 6500 cycles
+  // where a tile takes 2000 to 2800, with 16 rows 5000 (other head dims go by the same counts, unmeasured).
+  // Counted as one for all of them, drafts of 16 sequences
   // took 61.9 us instead of 56.7, single tokens of 64 and 40 sequences the same time.  In the tile
   // kernel 2 took 102 to 104 us and 3 took 105 to 108 for the mixed batch of fa_paged_tile.cuh; other
   // chunks differ by 2 % either way.

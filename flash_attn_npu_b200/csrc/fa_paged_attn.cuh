@@ -39,7 +39,7 @@ __device__ __forceinline__ void let_next_launch() {
 
 // What a CTA notes about its slot 0 for the combine kernel.
 struct PagedPart {
-  int first_cta; // CTA that holds the item's first part, in its slot 1; -1: slot 0 is empty
+  int first_cta; // CTA that holds the item's first part, in its slot 1; negative: slot 0 is empty
   int last_cta;  // CTA that holds its last part
   int first_row; // packed row of the sequence's first query
   int count;     // queries of the sequence

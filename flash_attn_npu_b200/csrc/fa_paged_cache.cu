@@ -15,8 +15,9 @@
 // where a CTA starts, are other CTAs: two pieces a thread and six (write) or eight (read) CTAs to an
 // SM took 24.4 and 61 us where four pieces and four CTAs took 25.3 and 65 (9 prompts of 16700 tokens
 // in all, 8 heads of 128, to float8; 56700 tokens back to bf16); one piece and eight: 25.1 and 72.
-// These are 4.2 and 5.8 TB/s.  The rest of the shorter one is its start and end: 3 us is what a call
-// of 16 tokens takes.
+// (From a graph; 24.7 and 66 called one by one.)  These are 4.2 and 5.5 TB/s, where a plain copy reaches 6.5.  3 us
+// of the shorter one is what a call of 16 tokens takes; the rest is that no CTA has its next run's rows on
+// their way (issue slots 65 %).
 #include <cmath>
 
 #include "../../include/fa_paged_sm100.h"

@@ -15,20 +15,26 @@
 // here (measured), a warp ~1000 cycles for 16 keys at head_dim 128: 8 warps take in ~65 bytes a
 // cycle, and an SM's share of the measured memory bandwidth is 23.
 //
-// Measured (head_dim 128, 8 kv heads of 4 query heads): one new token of 64 sequences, 300,000 in the
-// cache in bf16, pages of 16: 189 us, 6.5 TB/s, what a plain copy reaches; 40 sequences, 410,000 tokens
-// in float8: 137 us, 6.3 TB/s (ncu: DRAM 78 to 80 % of its nominal rate, tensor pipe 10 and 18 %).  One
-// sequence of 131,000 tokens in fp16, 4 kv heads of 64: 32.5 us, 4.1 TB/s, of which start, cut and joining
-// are ~10 us.  Two to eight drafted tokens of 16 sequences: 57 us, 4.1 TB/s, bound by the 32-row
-// block's chain of mma.sync and softmax (issue slots 30 %, tensor pipe 24 %).  A call of one sequence of 777 tokens: 8.2 us.
+// Measured (head_dim 128, 8 kv heads of 4 query heads; the first figure of calls from a graph, the second of
+// calls one by one): one new token of 64 sequences, 300,000 in the cache in bf16, pages of 16: 190 to 194 us,
+// 6.4 TB/s, what a plain copy reaches; 40 sequences, 410,000 tokens in float8: 140 to 148 us, 5.9 to 6.2 TB/s
+// (ncu: DRAM 74 to 80 % of its nominal rate, tensor pipe 17 and 10 %).  One sequence of 131,000 tokens in
+// fp16, 4 kv heads of 64: 33 us, 4.1 TB/s, of which start, cut and joining are ~10 us.  Two to eight drafted
+// tokens of 16 sequences: 56 us, 4.1 TB/s, bound by the 32-row block's chain of mma.sync and softmax (issue
+// slots 30 %, tensor pipe 24 %); in float8 55 us, half the bytes in nearly the same time.  One sequence of 777
+// tokens and 16 kv heads: 8.3 us, in which 16 SMs take 7 tiles one after the other.
 //
 // Float8 caches: codes convert exactly to fp16, so the products run in fp16.  Queries in bf16 are
 // scaled per row by a power of two to the top of fp16's range first (exact but for values below 2^-29 of
-// the row's largest, which are off by at most 2^-40 of it).  The key scale multiplies S.  The value scale multiplies p before it is rounded
-// to fp16, relative to a scale mv that O is kept apart from.  Scales may lie far apart (a row of zeros has
-// scale 1), and a ratio of scales must not push p out of fp16's range.  So mv follows the tiles, up and
-// down, where a tile's scales are not all within 2^8 below it, and a tile whose scales spread over more is
-// taken in turns, each with the keys of one such band (the others' logits are -inf in it).
+// the row's largest, which are off by at most 2^-40 of it).  The key scale multiplies S.  The value scale
+// multiplies p before it is rounded to fp16, relative to a scale mv that O is kept apart from.  Scales may
+// lie far apart (a row of zeros has scale 1), and a ratio of scales must not push p out of fp16's range.  So
+// mv follows the tiles, up and down, where a tile's scales are not all within 2^8 below it, and a tile whose
+// scales spread over more is taken in turns, each with the keys of one such band (the others' logits are
+// -inf in it).  The batch above takes 141 us; where each sequence begins with a row of zeros and the other
+// scales are below 2^-8, 145; where every 16th row is one, so that every tile takes two turns, 259.  (A second
+// product for the keys left out, instead of a second turn, took the registers of the first: 94 us against 88 for
+// groups of 16 heads.)
 //
 // p in fp16 (fp16 caches, float8 caches) carries the factor 2^kPOffset, which l carries too: fp16
 // keeps full precision down to 2^-14, and so p does down to 2^-(14 + kPOffset) of the row's

@@ -37,8 +37,9 @@
 //
 // Measured (head_dim 128, 4 query heads a kv head, all SMs busy on caches of their own): a key tile
 // takes two sides 2.0 us (16-bit cache) or 2.5 (float8), one side's rows on both sides 1.35 or 1.75.
-// Four chunks of 3400 tokens in all over 50,000 in the cache, 8 kv heads: 660 to 750 us by the power limit,
-// 895 to 1020 TFLOP/s (ncu: tensor pipe 56 %, exponentials 56 %).  Twelve sequences of 1 to 226 new tokens
+// Four chunks of 3400 tokens in all over 50,000 in the cache, 8 kv heads: 670 us in a short run, 730 to 775 under
+// the power limit, 1005 to 870 TFLOP/s (ncu: tensor pipe 56 %, exponentials 56 %); the persistent dense kernel
+// with as many pairs, in turn with it, 640 to 700 and 646 to 674.  Twelve sequences of 1 to 226 new tokens
 // over 59,000 in a float8 cache, 4 kv heads: 103 us; tiles of few rows leave the units idle (tensor pipe
 // 20 %).  148 blocks of 256 rows over one key tile each: 12.6 us, most of it start and output.
 //

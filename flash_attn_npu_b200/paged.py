@@ -12,8 +12,9 @@ Sequences share caches of pages,
 Row i of sequence b is row offsets[b] + i of the packed tensors [total, heads, head_dim], and the
 token at position kv_lens[b] - (offsets[b + 1] - offsets[b]) + i of the sequence.  A decoding step
 has one row per sequence (offsets = 0, 1, 2, ...), a prompt or a chunk of one has many; a call may
-mix them.  Packed rows behind offsets[-1] are padding: they are not read, and outputs there are
-left as they were.  Pages behind a sequence's length may hold anything, NaN included.
+mix them.  Packed rows of no sequence (behind offsets[-1], or before offsets[0]) are padding: what
+they hold does not matter, and outputs there are left as they were.  Pages behind a sequence's length
+may hold anything, NaN included.
 
 A float8 cache holds code = round_e4m3(x / scale) with one power of two per (token, kv head); any
 positive, normal scale can be read.  page_size is a power of two, 8 .. 1024.  Two sequences may share
@@ -260,8 +261,12 @@ def attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scal
 
     Every value inside a sequence takes part in the products, with a probability of 0 where the
     causal mask hides it: a NaN or an infinity among them may show in any row of the sequence.  Over
-    a float8 cache, calls of more than 32 query rows a kv head round code * scale to q's type
-    (exact for `write`'s scales; with float16 queries it has to be within 65504).
+    a float8 cache, calls of more than 32 query rows a kv head (`max_q_len` counts) round code *
+    scale to q's type: exact for scales that `write` left for rows of that type (up to 63488 in
+    float16), else one rounding more, and infinite beyond 65504 with float16 queries.
+
+    Rows that are not 16-byte aligned are copied first.  There is no backward pass: `out` and `lse`
+    do not require gradients.
     """
     res = None
     if _binding is not None:

@@ -11,8 +11,10 @@
  * entries behind a sequence's last page are not read.  `kv_lens` [seqs] is each sequence's length
  * in the cache, its new tokens included.  `offsets` [seqs + 1] gives its rows in the packed
  * tensors [total, heads, head_dim]: row i of sequence b is row offsets[b] + i there and the token
- * at position kv_lens[b] - (offsets[b + 1] - offsets[b]) + i of the sequence.  Packed rows behind
- * offsets[seqs] are neither read nor written.  All three are int32 device arrays.
+ * at position kv_lens[b] - (offsets[b + 1] - offsets[b]) + i of the sequence.  Packed rows of no
+ * sequence (behind offsets[seqs], or before offsets[0]) are padding: outputs there are not written, and
+ * what inputs hold there does not matter, but it may be read, so all `total` rows have to be there.  All
+ * three are int32 device arrays.
  *
  * Lengths, offsets and pages are device data, so they are checked by the kernels: what lies
  * outside the table or the cache is not accessed, FA_ERR_PAGE_TABLE is written to *dev_status,
@@ -103,7 +105,11 @@ FA_API int fa_paged_read_sm100(const FaPagedCopyArgs* args, void* stream);
  * with no key to attend to gets out = 0 and lse = -inf.  Every value inside a sequence takes part, with
  * a probability of 0 where the causal mask hides it, so a NaN or an infinity among them may show in any
  * row of the sequence.  Over a float8 cache, calls of more than 32 query rows (new tokens times
- * heads_q / heads_kv) round code * scale to q's type; with fp16 it has to be within 65504. */
+ * heads_q / heads_kv; max_q_len counts) round code * scale to q's type.  That is exact for scales that
+ * fa_paged_write_sm100 left for rows of q's type, up to 63488 in fp16 (which e4m3 does not round up to
+ * 65536); otherwise it is a rounding more, and with fp16 queries what lies beyond 65504 becomes infinite.
+ * Scales: positive, normal numbers; up to 32 query rows, values 2^-80 below the largest that a row's
+ * sequence holds may be left out of account. */
 FA_API int fa_paged_attn_sm100(const FaPagedAttnArgs* args, void* stream);
 
 /* Workspace of fa_paged_attn_sm100 for these arguments (pointers are not looked at), on the
