@@ -516,7 +516,9 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
                 s[kn][n][2 * h + 1] *= ks;
               }
             }
-          if (__any_sync(0xffffffffu, far > kBandBits << 23)) {
+          // (A turn that takes up what was left always comes here, whatever the bits of the scales are:
+          // it takes the largest below the last turn's bound, so that the bound falls and the turns end.)
+          if (__any_sync(0xffffffffu, far > kBandBits << 23 || below != INFINITY)) {
             float top = 0.f;
 #pragma unroll
             for (int kn = 0; kn < KN; ++kn)
@@ -544,8 +546,9 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
             for (int kn = 0; kn < KN; ++kn)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                more |= vs[kn][h] < from && vs[kn][h] > 0.f;
-                if (vs[kn][h] >= below || (vs[kn][h] < from && vs[kn][h] > 0.f)) {
+                const bool later = vs[kn][h] < from && vs[kn][h] > 0.f;
+                more |= later;
+                if (later || (below != INFINITY && !(vs[kn][h] > 0.f && vs[kn][h] < below))) {
                   vs[kn][h] = 0.f;
 #pragma unroll
                   for (int n = 0; n < WN; ++n) s[kn][n][2 * h] = s[kn][n][2 * h + 1] = -INFINITY;

@@ -206,3 +206,35 @@ def test_scales_at_the_ends_of_their_range(power, count, cuda_device):
         b.k_scale *= 2.0 ** power
         b.q *= 2.0 ** -power
         _check(b, rounded=True)
+
+
+@pytest.mark.parametrize("count", COUNTS)
+def test_scales_of_0_count_as_values_of_0(count, cuda_device):
+    """Once each, also in tiles that are taken in several turns."""
+    b = _batch([count], [500], 1e-5, head_dim=64, dtype=BF16, device=cuda_device)
+    _set(b, "v", 0, list(range(5, 500, 16)), torch.zeros(31, 2, 64))
+    at = torch.arange(0, 500, 7)
+    page, row = b.table.cpu()[0, at // b.page].long(), at % b.page
+    b.v_scale[page.to(cuda_device), :, row.to(cuda_device)] = 0
+    _check(b)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("kind", ["subnormal", "any bits"])
+@pytest.mark.parametrize("count", COUNTS)
+def test_scales_outside_their_range_stay_within_their_sequence(count, kind, head_dim, cuda_device):
+    """Whatever is found in place of scales, the call ends, and the other sequences are as they were."""
+    b = ref.Batch([count] * 3, [300, 700, 129], heads_q=8, heads_kv=2, head_dim=head_dim, dtype=BF16, fp8=True, garbage=0.0,
+                  device=cuda_device, seed=8)
+    call = lambda: fam.paged_attention(b.q, b.k_cache, b.v_cache, *b.where, True, 0.1, **b.scales, max_q_len=count)  # noqa: E731
+    want = call()
+    g = torch.Generator().manual_seed(9)
+    pages = b.table[1][b.table[1] >= 0].long()
+    for s in (b.k_scale, b.v_scale):
+        bits = torch.randint(1, 1 << 23, (len(pages), *s.shape[1:]), generator=g, dtype=torch.int64)
+        if kind == "any bits":
+            bits = torch.randint(-2 ** 31, 2 ** 31, bits.shape, generator=g, dtype=torch.int64)
+        s[pages] = bits.to(torch.int32).view(torch.float32).to(cuda_device)
+    out = call()
+    ops.check_device_status(cuda_device)
+    assert torch.equal(out[:count], want[:count]) and torch.equal(out[2 * count:], want[2 * count:])
