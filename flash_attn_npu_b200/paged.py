@@ -21,8 +21,9 @@ positive, normal scale can be read.  page_size is a power of two, 8 .. 1024.  Tw
 pages (a common prefix), but a call to `write` must not be given the same place twice: which of the
 rows stays there is open.
 
-`page_table`, `kv_lens` and `offsets` are device data, which a launch does not wait for.  Entries outside
-the cache or the table are never followed: the call reports them through the device status word
+`page_table`, `kv_lens` and `offsets` (which do not decrease) are device data, which a launch does not
+wait for: a kernel on another stream must not change them while a call runs.  Entries outside the cache
+or the table are never followed: the call reports them through the device status word
 (`ops.check_device_status` raises), and the results of that sequence are undefined.
 """
 from __future__ import annotations

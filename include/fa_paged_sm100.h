@@ -16,9 +16,10 @@
  * what inputs hold there does not matter, but it may be read, so all `total` rows have to be there.  All
  * three are int32 device arrays.
  *
- * Lengths, offsets and pages are device data, so they are checked by the kernels: what lies
- * outside the table or the cache is not accessed, FA_ERR_PAGE_TABLE is written to *dev_status,
- * and the results of the sequence concerned are undefined.
+ * Lengths, offsets (which do not decrease) and pages are device data that must not change while a call
+ * runs: a kernel reads them more than once.  They are checked by the kernels: what lies outside the table
+ * or the cache is not accessed, FA_ERR_PAGE_TABLE is written to *dev_status, and the results of the
+ * sequence concerned are undefined.
  *
  * Conventions as in fa_fwd_sm100.h: the caller owns every buffer, the library allocates no device
  * memory, launches are asynchronous on `stream`, errors seen on the host come back before
