@@ -226,6 +226,18 @@ def paged_attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, s
     return out
 
 
+def paged_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, prefix_lens, page_table,
+                           offsets, kv_lens, causal, sm_scale, k_scale=None, v_scale=None,
+                           max_q_len=None, max_prefix_q_len=None, return_lse=False, out=None, lse=None):
+    """`paged_attention` of sequences that share prefixes, which are read and multiplied once for all."""
+    out, lse = _paged.prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, prefix_lens,
+                                       page_table, offsets, kv_lens, causal, sm_scale, k_scale, v_scale,
+                                       max_q_len, max_prefix_q_len, out, lse)
+    if return_lse:
+        return out, lse
+    return out
+
+
 # ----------------------------------------------------------------------------- profiling
 def profile_once(z, h, n_ctx, head_dim, causal, q, k, v, sm_scale):
     out = attention(q, k, v, causal, sm_scale)
@@ -446,6 +458,7 @@ __all__ = [
     "paged_cache_empty",
     "paged_cache_read",
     "paged_cache_write",
+    "paged_prefix_attention",
     "profile_once",
     "profiling",
 ]

@@ -48,6 +48,8 @@ EXPORTED_SYMBOLS = (
     "fa_paged_read_sm100",
     "fa_paged_attn_sm100",
     "fa_paged_workspace_bytes",
+    "fa_paged_prefix_sm100",
+    "fa_paged_prefix_workspace_bytes",
 )
 
 
@@ -187,12 +189,15 @@ def load() -> ctypes.CDLL:
         lib.fa_fwd_sm100_max_stages.restype = ctypes.c_int
         lib.fa_fwd_sm100_grid_size.argtypes = [ctypes.POINTER(FaFwdArgs)]
         lib.fa_fwd_sm100_grid_size.restype = ctypes.c_int64
-        for name in ("fa_paged_write_sm100", "fa_paged_read_sm100", "fa_paged_attn_sm100"):
+        for name in ("fa_paged_write_sm100", "fa_paged_read_sm100", "fa_paged_attn_sm100",
+                     "fa_paged_prefix_sm100"):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
             fn.restype = ctypes.c_int
-        lib.fa_paged_workspace_bytes.argtypes = [ctypes.c_void_p]
-        lib.fa_paged_workspace_bytes.restype = ctypes.c_int64
+        for name in ("fa_paged_workspace_bytes", "fa_paged_prefix_workspace_bytes"):
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.c_void_p]
+            fn.restype = ctypes.c_int64
         lib.fa_fwd_sm100_status_string.argtypes = [ctypes.c_int]
         lib.fa_fwd_sm100_status_string.restype = ctypes.c_char_p
         lib.fa_fwd_sm100_version.argtypes = []

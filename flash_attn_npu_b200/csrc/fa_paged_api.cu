@@ -52,15 +52,7 @@ PagedInfo info_for(int64_t head_dim, bool fp8, int rows) {
   }
 }
 
-int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
-
-// What a call runs with, from its arguments alone.
-struct Choice {
-  int rows;  // of a block of the row kernel; 0: the tile kernel
-  PagedInfo info;
-  int grid;
-  int64_t parts, lse, o, bytes;  // workspace offsets
-};
+}  // namespace
 
 int check_attn(const FaPagedAttnArgs* a) {
   if (!a || a->struct_size != static_cast<int32_t>(sizeof(FaPagedAttnArgs)))
@@ -76,8 +68,8 @@ int check_attn(const FaPagedAttnArgs* a) {
   return FA_OK;
 }
 
-Choice choose(const FaPagedAttnArgs* a) {
-  Choice c{};
+PagedChoice choose_attn(const FaPagedAttnArgs* a) {
+  PagedChoice c{};
   const int64_t group = a->heads_q / a->cache.heads_kv;
   const int64_t longest = a->max_q_len ? std::min(a->max_q_len, a->total) : a->total;
   // Up to 32 rows a kv head every sequence is one block of the row kernel, which reads the cache
@@ -102,22 +94,7 @@ Choice choose(const FaPagedAttnArgs* a) {
   return c;
 }
 
-}  // namespace
-
-}  // namespace fa
-
-extern "C" {
-
-int64_t fa_paged_workspace_bytes(const FaPagedAttnArgs* a) {
-  const int rc = fa::check_attn(a);
-  return rc != FA_OK ? rc : fa::choose(a).bytes;
-}
-
-int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
-  int rc = fa::check_attn(a);
-  if (rc == FA_OK) rc = fa::check_cache(a->cache, a->dtype, a->total);
-  if (rc != FA_OK) return rc;
-  if (a->total == 0 || a->cache.seqs == 0) return FA_OK;
+int check_attn_pointers(const FaPagedAttnArgs* a) {
   if (!a->q || !a->o || !a->lse || !a->workspace) return FA_ERR_INVALID_ARG;
   for (const void* x : {a->q, static_cast<const void*>(a->o)})
     if (reinterpret_cast<uintptr_t>(x) % 16) return FA_ERR_MISALIGNED;
@@ -126,29 +103,28 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   if (reinterpret_cast<uintptr_t>(a->lse) % 4 ||
       reinterpret_cast<uintptr_t>(a->workspace) % 256)
     return FA_ERR_MISALIGNED;
-  rc = fa::check_device();
-  if (rc != FA_OK) return rc;
-  const fa::Choice c = fa::choose(a);
-  if (a->workspace_bytes < c.bytes) return FA_ERR_INVALID_ARG;
+  return FA_OK;
+}
 
+int plan_attn(const FaPagedAttnArgs* a, const PagedChoice& c, char* ws, cudaStream_t stream, PagedPlan& plan) {
   const FaPagedCache& kv = a->cache;
-  fa::PagedPlan plan{};
+  int rc = FA_OK;
   plan.half = a->dtype == FA_DTYPE_FP16;
   plan.fp8 = kv.dtype == FA_DTYPE_FP8_E4M3;
   plan.rows = c.rows;
   plan.grid = c.grid;
-  plan.stream = static_cast<cudaStream_t>(stream);
-  const fa::PagedInfo& info = c.info;
+  plan.stream = stream;
+  const PagedInfo& info = c.info;
   const int box = static_cast<int>(std::min<int64_t>(kv.page_size, info.keys));
-  rc = fa::encode_cache_map(&plan.tmK, kv.k, kv.dtype, kv.num_pages, kv.heads_kv, kv.page_size,
-                            kv.head_dim, kv.k_stride, info.cols, box, info.span);
+  rc = encode_cache_map(&plan.tmK, kv.k, kv.dtype, kv.num_pages, kv.heads_kv, kv.page_size,
+                        kv.head_dim, kv.k_stride, info.cols, box, info.span);
   if (rc == FA_OK)
-    rc = fa::encode_cache_map(&plan.tmV, kv.v, kv.dtype, kv.num_pages, kv.heads_kv, kv.page_size,
-                              kv.head_dim, kv.v_stride, info.cols, box, info.span);
+    rc = encode_cache_map(&plan.tmV, kv.v, kv.dtype, kv.num_pages, kv.heads_kv, kv.page_size,
+                          kv.head_dim, kv.v_stride, info.cols, box, info.span);
   if (rc != FA_OK) return rc;
 
-  fa::PagedAttnParams& p = plan.params;
-  p.seqs = fa::seqs_of(kv, a->total, a->dev_status);
+  PagedAttnParams& p = plan.params;
+  p.seqs = seqs_of(kv, a->total, a->dev_status);
   p.q = a->q;
   p.o = a->o;
   p.lse = a->lse;
@@ -165,7 +141,7 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   p.group_inv = static_cast<uint32_t>((int64_t{1} << 32) / p.group + 1);
   p.head_dim = static_cast<int>(kv.head_dim);
   p.causal = a->causal ? 1 : 0;
-  p.scale_log2 = a->sm_scale * fa::kLog2e;
+  p.scale_log2 = a->sm_scale * kLog2e;
   const bool tile = c.rows == 0;
   // Sequences of at most kWholeTiles tiles are not cut: the joining launch costs more (3 .. 10 us)
   // than the tiles that a CTA then takes one after the other (~0.5 us each in the row kernel,
@@ -187,31 +163,60 @@ int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
   p.pair_from = plan.fp8 ? 6 : 3;
   p.tile_toks = tile ? 128 / p.group : 0;
   p.tile_live = tile ? p.tile_toks * p.group : info.rows;
-  char* ws = static_cast<char*>(a->workspace);
-  p.parts = reinterpret_cast<fa::PagedPart*>(ws + c.parts);
+  p.lse_unit = kLn2;
+  p.parts = reinterpret_cast<PagedPart*>(ws + c.parts);
   p.part_lse = reinterpret_cast<float*>(ws + c.lse);
   p.part_o = reinterpret_cast<float*>(ws + c.o);
 
   if (tile) {
-    rc = fa::encode_query_map(&plan.tmQ, a->q, a->dtype, a->total, a->heads_q, kv.head_dim,
-                              a->q_stride, static_cast<int>(std::min<int64_t>(kv.head_dim, 64)),
-                              p.group, p.tile_toks, static_cast<int>(std::min<int64_t>(2 * kv.head_dim, 128)));
-    if (rc != FA_OK) return rc;
-    switch (kv.head_dim) {
-      case 16: return fa::launch_tile_d16(plan);
-      case 32: return fa::launch_tile_d32(plan);
-      case 64: return fa::launch_tile_d64(plan);
-      case 128: return fa::launch_tile_d128(plan);
-      default: return fa::launch_tile_d256(plan);
+    rc = encode_query_map(&plan.tmQ, a->q, a->dtype, a->total, a->heads_q, kv.head_dim,
+                          a->q_stride, static_cast<int>(std::min<int64_t>(kv.head_dim, 64)),
+                          p.group, p.tile_toks, static_cast<int>(std::min<int64_t>(2 * kv.head_dim, 128)));
+  }
+  return rc;
+}
+
+int launch_attn(const PagedPlan& plan) {
+  if (plan.rows == 0) {
+    switch (plan.params.head_dim) {
+      case 16: return launch_tile_d16(plan);
+      case 32: return launch_tile_d32(plan);
+      case 64: return launch_tile_d64(plan);
+      case 128: return launch_tile_d128(plan);
+      default: return launch_tile_d256(plan);
     }
   }
-  switch (kv.head_dim) {
-    case 16: return fa::launch_rows_d16(plan);
-    case 32: return fa::launch_rows_d32(plan);
-    case 64: return fa::launch_rows_d64(plan);
-    case 128: return fa::launch_rows_d128(plan);
-    default: return fa::launch_rows_d256(plan);
+  switch (plan.params.head_dim) {
+    case 16: return launch_rows_d16(plan);
+    case 32: return launch_rows_d32(plan);
+    case 64: return launch_rows_d64(plan);
+    case 128: return launch_rows_d128(plan);
+    default: return launch_rows_d256(plan);
   }
+}
+
+}  // namespace fa
+
+extern "C" {
+
+int64_t fa_paged_workspace_bytes(const FaPagedAttnArgs* a) {
+  const int rc = fa::check_attn(a);
+  return rc != FA_OK ? rc : fa::choose_attn(a).bytes;
+}
+
+int fa_paged_attn_sm100(const FaPagedAttnArgs* a, void* stream) {
+  int rc = fa::check_attn(a);
+  if (rc == FA_OK) rc = fa::check_cache(a->cache, a->dtype, a->total);
+  if (rc != FA_OK) return rc;
+  if (a->total == 0 || a->cache.seqs == 0) return FA_OK;
+  rc = fa::check_attn_pointers(a);
+  if (rc == FA_OK) rc = fa::check_device();
+  if (rc != FA_OK) return rc;
+  const fa::PagedChoice c = fa::choose_attn(a);
+  if (a->workspace_bytes < c.bytes) return FA_ERR_INVALID_ARG;
+  fa::PagedPlan plan{};
+  rc = fa::plan_attn(a, c, static_cast<char*>(a->workspace), static_cast<cudaStream_t>(stream), plan);
+  return rc != FA_OK ? rc : fa::launch_attn(plan);
 }
 
 }  // extern "C"

@@ -47,6 +47,23 @@ struct PagedPart {
   int block;     // row block
 };
 
+// What a level of a call behind shared prefixes weighs, for the division of the CTAs among the two.
+struct PagedLevel {
+  PagedSeqs seqs;
+  int rows, keys;  // of a block and a tile
+  int cost;        // of an item, in tiles
+  int unit;        // of a tile
+};
+
+// A row's parts in the workspace of a level: n CTAs from `first` on hold one each, in row `row` of their
+// slots; n = 0: the item was held whole.
+struct PagedWhere {
+  static constexpr int kMostCtas = 1023;
+  static __device__ __forceinline__ uint32_t pack(int n, int first, int row) {
+    return static_cast<uint32_t>(n | first << 10 | row << 20);
+  }
+};
+
 struct PagedAttnParams {
   PagedSeqs seqs;
   const void* q;
@@ -74,7 +91,56 @@ struct PagedAttnParams {
   PagedPart* parts;  // [gridDim.x]
   float* part_o;     // [gridDim.x][2][block rows][head_dim]
   float* part_lse;   // [gridDim.x][2][block rows]
+  // Calls behind shared prefixes (fa_paged_prefix.cu): 1 the prefixes, 2 the sequences' own tokens, 0 any
+  // other call.  There no row is finished here: whole items go to `whole_o` in fp32, `lse` is of base 2,
+  // and `where` tells where a row's parts are.
+  int level;
+  float lse_unit;    // what a base-2 logsumexp is multiplied by on its way to `lse`
+  float* whole_o;    // [total, heads_q, head_dim]
+  uint32_t* where;   // [total, heads_q]
+  PagedLevel levels[2];
 };
+
+// Steps of one kv head of a level, weighted.  An estimate (a causal triangle counts as a rectangle): both
+// kernels divide the CTAs by it, and nothing but their balance depends on it.
+__device__ __forceinline__ int64_t level_weight(const PagedLevel& v, int group) {
+  const int lane = threadIdx.x & 31;
+  int64_t sum = 0;
+  for (int b = lane; b < v.seqs.seqs; b += 32) {
+    int first, count;
+    seq_rows(v.seqs, b, first, count);
+    const int len = seq_len(v.seqs, b);
+    const int64_t blocks = (static_cast<int64_t>(count) * group + v.rows - 1) / v.rows;
+    sum += blocks * ((len + v.keys - 1) / v.keys + v.cost);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  return sum * v.unit;
+}
+
+// CTAs that a kernel may use: all, or its level's share of them.
+__device__ __forceinline__ int ctas_for(const PagedAttnParams& p) {
+  const int all = static_cast<int>(gridDim.x);
+  if (p.level == 0) return all;
+  const float a = static_cast<float>(level_weight(p.levels[0], p.group));
+  const float b = static_cast<float>(level_weight(p.levels[1], p.group));
+  if (a == 0.f || b == 0.f || all < 2) return all;
+  const int n = min(max(__float2int_rn(all * (a / (a + b))), 1), all - 1);
+  return p.level == 1 ? n : all - n;
+}
+
+// The two kernels of such a call run at the same time: the second is brought up once every CTA of the
+// first has seen the end of what was before it, reads nothing that the first writes, and ends behind it.
+__device__ __forceinline__ void level_begin_before_sync(const PagedAttnParams& p) {
+  if (p.level != 1) let_next_launch();
+}
+__device__ __forceinline__ void level_begin(const PagedAttnParams& p) {
+  if (p.level != 2) wait_for_launch_before();
+  if (p.level == 1) let_next_launch();
+}
+__device__ __forceinline__ void level_end(const PagedAttnParams& p) {
+  if (p.level == 2 && blockIdx.x == 0) wait_for_launch_before();
+}
 
 // One sequence's share of the line.
 struct PagedSeq {
@@ -143,7 +209,8 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttnParams& p, Step
   }
   PagedRange r{0, 0, 0, __shfl_sync(0xffffffffu, upto, 31), 1, 0, 0, 0};
   const int64_t most = (r.all + (1 << p.min_steps_log2) - 1) >> p.min_steps_log2;
-  r.ctas = static_cast<int>(most < gridDim.x ? most : gridDim.x);
+  const int ctas = ctas_for(p);
+  r.ctas = static_cast<int>(most < ctas ? most : ctas);
   const int c = static_cast<int>(blockIdx.x);
   if (c >= r.ctas) return r;
   // the first `rest` CTAs take a step more than the others
@@ -219,6 +286,11 @@ struct PagedWalk {
   }
   __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == s.tiles; }
   __device__ __forceinline__ int slot() const { return tile0 == 0 ? 1 : 0; }
+  // For a row of an item that begins with this part (row `row` of the block).
+  __device__ __forceinline__ uint32_t where(int row) const {
+    const int first = static_cast<int>(blockIdx.x);
+    return whole() ? 0u : PagedWhere::pack(range.cta_of(item + p.item_cost + s.tiles - 1) - first + 1, first, row);
+  }
   // What the combine kernel has to know of the current part (slot 0).
   __device__ __forceinline__ PagedPart note() const {
     return PagedPart{range.cta_of(item + p.item_cost),
@@ -332,6 +404,10 @@ struct PagedTileWalk {
   __device__ __forceinline__ bool tail() const { return tile1 * KEYS > s.len; }
   __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == n; }
   __device__ __forceinline__ int slot() const { return tile0 == 0 ? 1 : 0; }
+  __device__ __forceinline__ uint32_t where(const PagedRange& r, int cost, int row) const {
+    const int first = static_cast<int>(blockIdx.x);
+    return whole() ? 0u : PagedWhere::pack(r.cta_of(item + cost + n - 1) - first + 1, first, row);
+  }
   __device__ __forceinline__ PagedPart note(const PagedRange& r, int cost) const {
     return PagedPart{r.cta_of(item + cost), r.cta_of(item + cost + n - 1), s.first, s.count, head, block};
   }

@@ -4,6 +4,7 @@
 
 #include <atomic>
 
+#include "../../include/fa_paged_sm100.h"
 #include "fa_paged_attn.cuh"
 
 namespace fa {
@@ -25,6 +26,24 @@ struct PagedPlan {
   int grid;
   cudaStream_t stream;
 };
+
+// What a call runs with, from its arguments alone.
+struct PagedChoice {
+  int rows;  // of a block of the row kernel; 0: the tile kernel
+  PagedInfo info;
+  int grid;
+  int64_t parts, lse, o, bytes;  // workspace offsets
+};
+
+inline int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+
+// fa_paged_api.cu: sizes and types; pointers; the kernel for a call; the launch that it takes (the
+// workspace at `ws`); and that launch.
+int check_attn(const FaPagedAttnArgs* a);
+int check_attn_pointers(const FaPagedAttnArgs* a);
+PagedChoice choose_attn(const FaPagedAttnArgs* a);
+int plan_attn(const FaPagedAttnArgs* a, const PagedChoice& c, char* ws, cudaStream_t stream, PagedPlan& plan);
+int launch_attn(const PagedPlan& plan);
 
 int launch_tile_d16(const PagedPlan& plan);
 int launch_tile_d32(const PagedPlan& plan);

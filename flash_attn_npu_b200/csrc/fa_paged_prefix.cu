@@ -1,0 +1,272 @@
+// Attention of a batch whose sequences share long prefixes (fa_paged_prefix_sm100 of
+// include/fa_paged_sm100.h).  A row attends to the keys P of its group's prefix and to the keys S of its
+// own sequence; with l_X = log2 sum_{j in X} 2^(s_j) and O_X the softmax average of the values over X,
+//   l = log2(2^l_P + 2^l_S),   O = 2^(l_P - l) O_P + 2^(l_S - l) O_S ,
+// which holds for any division of the keys, down to the parts that CTAs hold.
+//
+// A prefix is attended to by all rows of its group at once, as one sequence without a causal mask: its
+// keys and values are read once for the group, and its products have rows enough for the tensor cores.
+// So a call is two launches of the paged attention kernels over the same packed rows, the prefixes (level
+// 1, mostly the tile kernel, bound by its products) and the sequences' own tokens (level 2, in decoding
+// the row kernel, bound by memory), and one that joins a row's parts.  The first two run side by side
+// (programmatic dependent launch; level_begin in fa_paged_attn.cuh): each takes its share of the SMs by
+// what the levels weigh, which the kernels work out from the lengths, as these are device data.
+#include <algorithm>
+
+#include "fa_paged_host.h"
+#include "fa_paged_launch.h"
+
+namespace fa {
+namespace {
+
+struct JoinLevel {
+  const float* part_o;
+  const float* part_lse;
+  const float* whole_o;
+  const float* lse;
+  const uint32_t* where;
+  const int* offsets;
+  int seqs;
+  int slot_rows;  // rows of a slot
+  int ctas;
+};
+
+struct JoinParams {
+  JoinLevel level[2];
+  void* o;
+  float* lse;
+  int64_t o_stride[2];
+  int rows;  // total * heads_q
+  int total;
+  int heads_q;
+};
+
+constexpr int kJoinThreads = 128;
+
+// D / 4 threads to a row, four columns each, times PS groups of them that take every PS-th part.
+template <typename T, int D, int PS>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ JoinParams p) {
+  constexpr int TPR = D / 4;
+  constexpr int ROWS = kJoinThreads / (TPR * PS);
+  __shared__ float4 s_o[PS > 1 ? kJoinThreads : 1];
+  __shared__ float2 s_ml[PS > 1 ? PS * ROWS : 1];
+  const int col = threadIdx.x % TPR, split = threadIdx.x / TPR % PS, r = threadIdx.x / (TPR * PS);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + r;
+  let_next_launch();
+  wait_for_launch_before();
+  const int tok = static_cast<int>(min(row, static_cast<int64_t>(p.rows - 1)) / p.heads_q);
+  int n[2], at[2];      // parts of each level, and the slot of the first
+  uint32_t in_slot[2];
+  bool live = row < p.rows;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const JoinLevel& v = p.level[x];
+    const bool in = tok >= fresh(v.offsets) && tok < fresh(v.offsets + v.seqs);
+    if (x == 1) live = live && in;
+    const uint32_t w = in && live ? fresh(v.where + row) : 0u;
+    // (what a kernel that gave up has left may be any bits)
+    const int first = min(static_cast<int>(w >> 10 & 1023), v.ctas - 1);
+    n[x] = !in ? 0 : (w & 1023) == 0 ? 1 : min(static_cast<int>(w & 1023), v.ctas - first);
+    at[x] = (w & 1023) == 0 ? -1 : first;
+    in_slot[x] = min(w >> 20, static_cast<uint32_t>(v.slot_rows - 1));
+  }
+  const int count = live ? n[0] + n[1] : 0;
+  // part i: its logsumexp, and its O
+  auto part = [&](int i, const float*& o) -> float {
+    const int x = i >= n[0];
+    const JoinLevel& v = p.level[x];
+    if (x) i -= n[0];
+    if (at[x] < 0) {
+      o = v.whole_o + row * D;
+      return fresh(v.lse + row);
+    }
+    const int64_t slot = i == 0 ? 2 * static_cast<int64_t>(at[x]) + 1 : 2 * static_cast<int64_t>(at[x] + i);
+    const int64_t y = slot * v.slot_rows + in_slot[x];
+    o = v.part_o + y * D;
+    return fresh(v.part_lse + y);
+  };
+  const float* from;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int i = split; i < count; i += PS) top = fmaxf(top, part(i, from));
+  const float base = top == -INFINITY ? 0.f : top;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = split; i < count; i += PS) {
+    const float w = exp2f(part(i, from) - base);
+    if (w == 0.f) continue;  // a part without keys for the row may have left no values
+    const float4 v = fresh(reinterpret_cast<const float4*>(from) + col);
+    sum += w;
+    acc.x += w * v.x;
+    acc.y += w * v.y;
+    acc.z += w * v.z;
+    acc.w += w * v.w;
+  }
+  if constexpr (PS > 1) {
+    s_o[threadIdx.x] = acc;
+    if (col == 0) s_ml[r * PS + split] = make_float2(top, sum);
+    __syncthreads();
+    if (split != 0) return;
+    top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PS; ++i) top = fmaxf(top, s_ml[r * PS + i].x);
+    sum = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < PS; ++i) {
+      const float2 ml = s_ml[r * PS + i];
+      const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - top);
+      const float4 v = s_o[threadIdx.x + i * TPR];
+      sum += w * ml.y;
+      acc.x += w * v.x;
+      acc.y += w * v.y;
+      acc.z += w * v.z;
+      acc.w += w * v.w;
+    }
+  }
+  if (!live) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int head = static_cast<int>(row - static_cast<int64_t>(tok) * p.heads_q);
+  T* out = static_cast<T*>(p.o) + tok * p.o_stride[0] + head * p.o_stride[1] + 4 * col;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack2(acc.x * inv, acc.y * inv, static_cast<T*>(nullptr)),
+                                              pack2(acc.z * inv, acc.w * inv, static_cast<T*>(nullptr)));
+  if (col == 0) p.lse[row] = (top + log2f(sum)) * kLn2;  // (no key: -inf)
+}
+
+template <typename T, int D, int PS>
+int launch_join(const JoinParams& p, cudaStream_t stream) {
+  constexpr int ROWS = kJoinThreads / (D / 4 * PS);
+  const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(p.rows) + ROWS - 1) / ROWS);
+  return launch_dependent(paged_join_kernel<T, D, PS>, dim3(blocks), kJoinThreads, 0, stream, p);
+}
+
+template <typename T>
+int join(const JoinParams& p, int64_t head_dim, bool split, cudaStream_t stream) {
+  switch (head_dim) {
+    case 16: return split ? launch_join<T, 16, 4>(p, stream) : launch_join<T, 16, 1>(p, stream);
+    case 32: return split ? launch_join<T, 32, 4>(p, stream) : launch_join<T, 32, 1>(p, stream);
+    case 64: return split ? launch_join<T, 64, 4>(p, stream) : launch_join<T, 64, 1>(p, stream);
+    case 128: return split ? launch_join<T, 128, 4>(p, stream) : launch_join<T, 128, 1>(p, stream);
+    default: return split ? launch_join<T, 256, 2>(p, stream) : launch_join<T, 256, 1>(p, stream);
+  }
+}
+
+// The prefixes as the sequences of a call of their own.
+FaPagedAttnArgs of_prefixes(const FaPagedPrefixArgs* a) {
+  FaPagedAttnArgs x = a->attn;
+  x.cache.page_table = a->prefix_table;
+  x.cache.offsets = a->prefix_offsets;
+  x.cache.kv_lens = a->prefix_lens;
+  x.cache.table_stride = a->prefix_stride;
+  x.cache.table_cols = a->prefix_cols;
+  x.cache.seqs = a->prefixes;
+  x.max_q_len = a->max_prefix_q_len;
+  x.causal = 0;
+  return x;
+}
+
+int check_prefix(const FaPagedPrefixArgs* a) {
+  if (!a || a->struct_size != static_cast<int32_t>(sizeof(FaPagedPrefixArgs))) return FA_ERR_INVALID_ARG;
+  const int rc = check_attn(&a->attn);
+  if (rc != FA_OK) return rc;
+  const FaPagedAttnArgs x = of_prefixes(a);
+  return check_attn(&x);
+}
+
+// Workspace: per level the kernel's own, whole rows, their logsumexps and where a row's parts are.
+struct PrefixChoice {
+  PagedChoice level[2];
+  int64_t own[2], whole_o[2], lse[2], where[2], bytes;
+};
+
+PrefixChoice choose(const FaPagedPrefixArgs* a) {
+  PrefixChoice c{};
+  const FaPagedAttnArgs x[2] = {of_prefixes(a), a->attn};
+  const int64_t rows = a->attn.total * a->attn.heads_q;
+  for (int i = 0; i < 2; ++i) {
+    c.level[i] = choose_attn(&x[i]);
+    c.level[i].grid = std::min(c.level[i].grid, PagedWhere::kMostCtas);
+    c.own[i] = c.bytes;
+    c.whole_o[i] = c.own[i] + c.level[i].bytes;
+    c.lse[i] = up256(c.whole_o[i] + 4 * rows * a->attn.cache.head_dim);
+    c.where[i] = up256(c.lse[i] + 4 * rows);
+    c.bytes = up256(c.where[i] + 4 * rows);
+  }
+  return c;
+}
+
+// Weight of a tile of each kernel, in 10 ns of one SM (measured at head_dim 128): 128 keys take the tile
+// kernel 2.0 us for two query tiles (float8 2.5); the row kernel takes 64 KB in 1.0 us.
+int unit_of(const PagedPlan& plan, const PagedInfo& info) {
+  if (plan.rows == 0) return plan.fp8 ? 250 : 200;
+  const int bytes = 2 * info.keys * plan.params.head_dim * (plan.fp8 ? 1 : 2);
+  return std::max(40, bytes / 655);
+}
+
+int prefix_attention(const FaPagedPrefixArgs* a, void* stream) {
+  int rc = check_prefix(a);
+  if (rc != FA_OK) return rc;
+  const FaPagedAttnArgs x[2] = {of_prefixes(a), a->attn};
+  for (int i = 0; i < 2 && rc == FA_OK; ++i) rc = check_cache(x[i].cache, x[i].dtype, x[i].total);
+  if (rc != FA_OK) return rc;
+  if (a->attn.total == 0 || a->attn.cache.seqs == 0) return FA_OK;
+  rc = check_attn_pointers(&a->attn);
+  if (rc == FA_OK) rc = check_device();
+  if (rc != FA_OK) return rc;
+  const PrefixChoice c = choose(a);
+  if (a->attn.workspace_bytes < c.bytes) return FA_ERR_INVALID_ARG;
+
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(a->attn.workspace);
+  PagedPlan plan[2] = {};
+  JoinParams join_params{};
+  for (int i = 0; i < 2; ++i) {
+    rc = plan_attn(&x[i], c.level[i], ws + c.own[i], s, plan[i]);
+    if (rc != FA_OK) return rc;
+    PagedAttnParams& p = plan[i].params;
+    const PagedInfo& info = c.level[i].info;
+    p.level = i + 1;
+    p.whole_items = 0;
+    p.min_steps_log2 = plan[i].rows == 0 ? 2 : 1;
+    p.lse_unit = 1.f;
+    p.lse = reinterpret_cast<float*>(ws + c.lse[i]);
+    p.whole_o = reinterpret_cast<float*>(ws + c.whole_o[i]);
+    p.where = reinterpret_cast<uint32_t*>(ws + c.where[i]);
+    const int rows = plan[i].rows == 0 ? info.rows / 128 * p.tile_live : info.rows;
+    const PagedLevel v{p.seqs, rows, info.keys, p.item_cost, unit_of(plan[i], info)};
+    plan[0].params.levels[i] = plan[1].params.levels[i] = v;
+    join_params.level[i] = JoinLevel{p.part_o, p.part_lse, p.whole_o, p.lse, p.where, p.seqs.offsets,
+                                     p.seqs.seqs, info.rows, c.level[i].grid};
+  }
+  for (int i = 0; i < 2; ++i) {
+    rc = launch_attn(plan[i]);
+    if (rc != 0) return rc;
+  }
+  join_params.o = a->attn.o;
+  join_params.lse = a->attn.lse;
+  for (int d = 0; d < 2; ++d) join_params.o_stride[d] = a->attn.o_stride[d];
+  join_params.total = static_cast<int>(a->attn.total);
+  join_params.heads_q = static_cast<int>(a->attn.heads_q);
+  join_params.rows = join_params.total * join_params.heads_q;
+  // Parts are shared among threads while that leaves few enough blocks to be on the SMs at once.
+  const int64_t blocks = static_cast<int64_t>(join_params.rows) * a->attn.cache.head_dim / 4 * 4 / kJoinThreads;
+  const bool split = blocks <= 16 * c.level[0].grid;
+  return plan[0].half ? join<__half>(join_params, a->attn.cache.head_dim, split, s)
+                      : join<__nv_bfloat16>(join_params, a->attn.cache.head_dim, split, s);
+}
+
+}  // namespace
+}  // namespace fa
+
+extern "C" {
+
+int64_t fa_paged_prefix_workspace_bytes(const FaPagedPrefixArgs* a) {
+  const int rc = fa::check_prefix(a);
+  return rc != FA_OK ? rc : fa::choose(a).bytes;
+}
+
+int fa_paged_prefix_sm100(const FaPagedPrefixArgs* a, void* stream) {
+  return fa::prefix_attention(a, stream);
+}
+
+}  // extern "C"

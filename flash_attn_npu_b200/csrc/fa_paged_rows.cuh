@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
   uint8_t* s_q = smem + G::STAGES * G::STAGE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  let_next_launch();
+  level_begin_before_sync(p);
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::STAGES; ++s) {
       mbar_init(smem_u32(&s_full[s]), G::NP);
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
     fence_mbar_init();
   }
   __syncthreads();
-  wait_for_launch_before();
+  level_begin(p);
   if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
   const PagedRange range =
       paged_range(p, [&](int b) { return paged_seq<ROWS, KEYS>(p, b).steps; });
@@ -745,8 +745,10 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
         inv = sum == 0.f ? 0.f : 1.f / sum;
         if (threadIdx.x % TPR == 0) {
           const float lse2 = sum == 0.f ? -INFINITY : top + (log2f(sum) - kPOffset);
-          if (whole) p.lse[static_cast<int64_t>(w.s.first + my_tok) * p.heads_kv * p.group + my_head] = lse2 * kLn2;
+          const int64_t at = static_cast<int64_t>(w.s.first + my_tok) * p.heads_kv * p.group + my_head;
+          if (whole) p.lse[at] = lse2 * p.lse_unit;
           else p.part_lse[part_row] = lse2;
+          if (p.level && w.tile0 == 0) p.where[at] = w.where(my_r);
         }
       }
       named_barrier_sync(1, NW * 32);
@@ -766,7 +768,11 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
           a.z += v.z;
           a.w += v.w;
         }
-        if (whole)
+        if (whole && p.level)
+          *reinterpret_cast<float4*>(
+              p.whole_o + (static_cast<int64_t>(w.s.first + my_tok) * p.heads_kv * p.group + my_head) * D + c0 + c) =
+              make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+        else if (whole)
           *reinterpret_cast<uint2*>(static_cast<T*>(p.o) +
                                     static_cast<int64_t>(w.s.first + my_tok) * p.o_stride[0] +
                                     my_head * p.o_stride[1] + c0 + c) =
@@ -786,6 +792,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
       ph ^= 1u;
     }
   }
+  level_end(p);
 }
 
 }  // namespace fa

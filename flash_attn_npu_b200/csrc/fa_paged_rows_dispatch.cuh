@@ -27,7 +27,7 @@ int launch_rows(const PagedPlan& plan) {
   const int rc = launch_dependent(kernel, dim3(plan.grid), G::THREADS, G::SMEM, plan.stream,
                                   plan.tmK, plan.tmV, plan.params);
   if (rc != 0) return rc;
-  if (plan.grid == 1 || plan.params.whole_items) return 0;  // no shared item
+  if (plan.grid == 1 || plan.params.whole_items || plan.params.level) return 0;  // no item to join here
   const int64_t most = static_cast<int64_t>(plan.params.seqs.total) * plan.params.group;
   const unsigned rows = static_cast<unsigned>(most < G::ROWS ? most : G::ROWS);
   constexpr int kWarps = 4;

@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
   const int lane = threadIdx.x & 31;
   int* const status = p.seqs.status;
 
-  let_next_launch();
+  level_begin_before_sync(p);
   if (threadIdx.x == 32) {
     prefetch_map(&tmQ);
     prefetch_map(&tmK);
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  wait_for_launch_before();
+  level_begin(p);
   if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
   if (warp == 0) {
     const PagedRange r =
@@ -815,11 +815,14 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
         __syncwarp();
         if (live && ok && (i == 0 || !paired)) {
           const float lse2 = l == 0.f ? -INFINITY : m + (log2f(l) - kPOffset);
-          if (whole) p.lse[row * (p.heads_kv * p.group) + head] = lse2 * kLn2;
+          const int64_t at = row * (p.heads_kv * p.group) + head;
+          if (whole) p.lse[at] = lse2 * p.lse_unit;
           else p.part_lse[part_row] = lse2;
+          if (p.level && w.tile0 == 0) p.where[at] = w.where(range, p.item_cost, tile * 128 + r);
         }
         T* out = static_cast<T*>(p.o) + row * p.o_stride[0] + head * p.o_stride[1];
-        float* part = p.part_o + part_row * D;
+        const bool last = whole && p.level == 0;  // the row is finished here
+        float* part = whole ? p.whole_o + (row * (p.heads_kv * p.group) + head) * D : p.part_o + part_row * D;
         const uint32_t tO_other = tmem + lane_off + G::TMEM_O + (i ^ 1) * D;
         // (a pair's sides write every other 16 columns)
 #pragma unroll 1
@@ -843,7 +846,7 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
               f[u] = fmaf(__uint_as_float(o[u]), w_other, f[u]);
             }
           }
-          if (live && whole) {
+          if (live && last) {
             uint32_t pk[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) pk[u] = pack2(f[2 * u], f[2 * u + 1], static_cast<T*>(nullptr));
@@ -881,6 +884,7 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  level_end(p);
 }
 
 }  // namespace fa

@@ -23,7 +23,7 @@ int launch_tile(const PagedPlan& plan) {
   const int rc = launch_dependent(kernel, dim3(plan.grid), G::THREADS, G::SMEM, plan.stream,
                                   plan.tmQ, plan.tmK, plan.tmV, plan.params);
   if (rc != 0) return rc;
-  if (plan.grid == 1 || plan.params.whole_items) return 0;  // no shared item
+  if (plan.grid == 1 || plan.params.whole_items || plan.params.level) return 0;  // no item to join here
   // a warp to a row: shared items mostly have two or three parts
   constexpr int kRows = 8;
   return launch_dependent(paged_combine_kernel<T, 128, G::TILES, 1, kRows>, dim3(plan.grid - 1, 16),

@@ -26,6 +26,8 @@ int (*g_attn)(const FaPagedAttnArgs*, void*) = nullptr;
 int (*g_write)(const FaPagedCopyArgs*, void*) = nullptr;
 int (*g_read)(const FaPagedCopyArgs*, void*) = nullptr;
 int64_t (*g_workspace)(const FaPagedAttnArgs*) = nullptr;
+int (*g_prefix)(const FaPagedPrefixArgs*, void*) = nullptr;
+int64_t (*g_prefix_workspace)(const FaPagedPrefixArgs*) = nullptr;
 
 constexpr int kDevices = 64;
 // Devices that paged.py has prepared, and their status words.
@@ -76,21 +78,12 @@ struct CacheArgs {
   PyObject *k, *v, *table, *offsets, *lens, *k_scale, *v_scale;
 };
 
-// The cache and its sequences; false if they are not in order (the sizes are left to the library).
-bool fill_cache(const CacheArgs& a, FaPagedCache& c, int& index) {
-  const Tensor *k = tensor_of(a.k), *v = tensor_of(a.v), *table = tensor_of(a.table),
-               *offsets = tensor_of(a.offsets), *lens = tensor_of(a.lens);
-  if (!k || !v || !table || !offsets || !lens || !k->is_cuda()) return false;
-  index = k->get_device();
-  if (index < 0 || index >= kDevices || !g_ready[index]) return false;
-  for (const Tensor* t : {k, v, table, offsets, lens})
-    if (!plain(*t, index)) return false;
-  c.dtype = code_of(k->scalar_type());
-  if (c.dtype < 0 || k->scalar_type() != v->scalar_type() || k->dim() != 4 ||
-      k->sizes() != v->sizes() || !aligned(*k) || !aligned(*v))
-    return false;
+// The sequences of a cache on device `index`; false if they are not in order.
+bool fill_seqs(const CacheArgs& a, FaPagedCache& c, int index) {
+  const Tensor *table = tensor_of(a.table), *offsets = tensor_of(a.offsets), *lens = tensor_of(a.lens);
+  if (!table || !offsets || !lens) return false;
   for (const Tensor* t : {table, offsets, lens})
-    if (t->scalar_type() != at::kInt) return false;
+    if (!plain(*t, index) || t->scalar_type() != at::kInt) return false;
   if (table->dim() != 2 || offsets->dim() != 1 || lens->dim() != 1) return false;
   c.seqs = table->size(0);
   c.table_cols = table->size(1);
@@ -98,6 +91,25 @@ bool fill_cache(const CacheArgs& a, FaPagedCache& c, int& index) {
       !lens->is_contiguous() || (c.table_cols > 1 && table->stride(1) != 1))
     return false;
   c.table_stride = c.seqs > 1 ? table->stride(0) : c.table_cols;
+  c.page_table = static_cast<const int32_t*>(table->const_data_ptr());
+  c.offsets = static_cast<const int32_t*>(offsets->const_data_ptr());
+  c.kv_lens = static_cast<const int32_t*>(lens->const_data_ptr());
+  return true;
+}
+
+// The cache and its sequences; false if they are not in order (the sizes are left to the library).
+bool fill_cache(const CacheArgs& a, FaPagedCache& c, int& index) {
+  const Tensor *k = tensor_of(a.k), *v = tensor_of(a.v);
+  if (!k || !v || !k->is_cuda()) return false;
+  index = k->get_device();
+  if (index < 0 || index >= kDevices || !g_ready[index]) return false;
+  for (const Tensor* t : {k, v})
+    if (!plain(*t, index)) return false;
+  if (!fill_seqs(a, c, index)) return false;
+  c.dtype = code_of(k->scalar_type());
+  if (c.dtype < 0 || k->scalar_type() != v->scalar_type() || k->dim() != 4 ||
+      k->sizes() != v->sizes() || !aligned(*k) || !aligned(*v))
+    return false;
   c.num_pages = k->size(0);
   c.heads_kv = k->size(1);
   c.page_size = k->size(2);
@@ -109,9 +121,6 @@ bool fill_cache(const CacheArgs& a, FaPagedCache& c, int& index) {
   strides(*v, c.v_stride);
   c.k = const_cast<void*>(k->const_data_ptr());
   c.v = const_cast<void*>(v->const_data_ptr());
-  c.page_table = static_cast<const int32_t*>(table->const_data_ptr());
-  c.offsets = static_cast<const int32_t*>(offsets->const_data_ptr());
-  c.kv_lens = static_cast<const int32_t*>(lens->const_data_ptr());
   if ((c.dtype == FA_DTYPE_FP8_E4M3) != (a.k_scale != Py_None) ||
       (a.k_scale != Py_None) != (a.v_scale != Py_None))
     return false;
@@ -146,53 +155,52 @@ void written(const Tensor& t) {
 
 PyObject* none() { Py_RETURN_NONE; }
 
-// attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scale, k_scale, v_scale,
-//           max_q_len, out, lse) -> (out, lse), a status code, or None
-PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (n != 13) return none();
-  FaPagedAttnArgs x{};
+// An upper bound given as an integer or None (0).
+bool fill_bound(PyObject* a, int64_t& out) {
+  if (a == Py_None) return true;
+  out = PyLong_Check(a) ? PyLong_AsLongLong(a) : -1;
+  if (out >= 0) return true;
+  PyErr_Clear();
+  return false;
+}
+
+// What attention calls have in common; false if it is not in order.
+bool fill_attention(const Tensor* q, const CacheArgs& cache, PyObject* causal, PyObject* sm_scale,
+                    PyObject* max_q_len, FaPagedAttnArgs& x, int& index) {
   x.struct_size = sizeof(x);
-  int index = -1;
-  const Tensor* q = tensor_of(a[0]);
-  if (!fill_cache({a[1], a[2], a[3], a[4], a[5], a[8], a[9]}, x.cache, index) ||
-      !rows_ok(q, x.cache, index))
-    return none();
+  if (!fill_cache(cache, x.cache, index) || !rows_ok(q, x.cache, index)) return false;
   x.total = q->size(0);
   x.heads_q = q->size(1);
-  if (x.heads_q < 1 || x.heads_q % x.cache.heads_kv) return none();
+  if (x.heads_q < 1 || x.heads_q % x.cache.heads_kv) return false;
   x.dtype = code_of(q->scalar_type());
-  x.causal = PyObject_IsTrue(a[6]);
-  const double scale = PyFloat_AsDouble(a[7]);
+  x.causal = PyObject_IsTrue(causal);
+  const double scale = PyFloat_AsDouble(sm_scale);
   if (x.causal < 0 || (scale == -1.0 && PyErr_Occurred())) {
     PyErr_Clear();
-    return none();
+    return false;
   }
   x.sm_scale = static_cast<float>(scale);
-  if (a[10] != Py_None) {
-    x.max_q_len = PyLong_Check(a[10]) ? PyLong_AsLongLong(a[10]) : -1;
-    if (x.max_q_len < 0) {
-      PyErr_Clear();
-      return none();
-    }
-  }
-  const c10::cuda::OptionalCUDAGuard guard(q->device());
-  Tensor out, lse;
-  if (a[11] != Py_None) {
-    const Tensor* t = tensor_of(a[11]);
+  return fill_bound(max_q_len, x.max_q_len);
+}
+
+// The tensors that an attention call writes: given (not None) or new; false if they are not in order.
+bool fill_outputs(const Tensor* q, PyObject* out_arg, PyObject* lse_arg, FaPagedAttnArgs& x, int index,
+                  Tensor& out, Tensor& lse) {
+  if (out_arg != Py_None) {
+    const Tensor* t = tensor_of(out_arg);
     if (!t || !plain(*t, index) || t->sizes() != q->sizes() ||
         t->scalar_type() != q->scalar_type() || !aligned(*t))
-      return none();
+      return false;
     out = *t;
   } else {
     out = at::empty_like(*q);
-    if (!aligned(out)) return none();
+    if (!aligned(out)) return false;
   }
-  if (a[12] != Py_None) {
-    const Tensor* t = tensor_of(a[12]);
+  if (lse_arg != Py_None) {
+    const Tensor* t = tensor_of(lse_arg);
     if (!t || !plain(*t, index) || t->dim() != 2 || t->size(0) != x.total ||
         t->size(1) != x.heads_q || t->scalar_type() != at::kFloat || !t->is_contiguous())
-      return none();
+      return false;
     lse = *t;
   } else {
     lse = at::empty({x.total, x.heads_q}, q->options().dtype(at::kFloat));
@@ -203,6 +211,32 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   x.o = out.mutable_data_ptr();
   x.lse = static_cast<float*>(lse.mutable_data_ptr());
   x.dev_status = g_status[index];
+  return true;
+}
+
+PyObject* outputs(PyObject* out_arg, PyObject* lse_arg, Tensor& out, Tensor& lse) {
+  if (out_arg != Py_None) written(out);
+  if (lse_arg != Py_None) written(lse);
+  PyObject* r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(out)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(lse)));
+  return r;
+}
+
+// attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scale, k_scale, v_scale,
+//           max_q_len, out, lse) -> (out, lse), a status code, or None
+PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 13) return none();
+  FaPagedAttnArgs x{};
+  int index = -1;
+  const Tensor* q = tensor_of(a[0]);
+  if (!fill_attention(q, {a[1], a[2], a[3], a[4], a[5], a[8], a[9]}, a[6], a[7], a[10], x, index))
+    return none();
+  const c10::cuda::OptionalCUDAGuard guard(q->device());
+  Tensor out, lse;
+  if (!fill_outputs(q, a[11], a[12], x, index, out, lse)) return none();
   if (x.total > 0 && x.cache.seqs > 0) {
     x.workspace_bytes = g_workspace(&x);
     if (x.workspace_bytes < 0) return none();
@@ -213,13 +247,47 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int rc = g_attn(&x, c10::cuda::getCurrentCUDAStream(index).stream());
     if (rc != FA_OK) return PyLong_FromLong(rc);
   }
-  if (a[11] != Py_None) written(out);
-  if (a[12] != Py_None) written(lse);
-  PyObject* r = PyTuple_New(2);
-  if (!r) return nullptr;
-  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(out)));
-  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(lse)));
-  return r;
+  return outputs(a[11], a[12], out, lse);
+  END_HANDLE_TH_ERRORS
+}
+
+// prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, prefix_lens, page_table, offsets,
+//                  kv_lens, causal, sm_scale, k_scale, v_scale, max_q_len, max_prefix_q_len, out, lse)
+//   -> (out, lse), a status code, or None
+PyObject* prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 17) return none();
+  FaPagedPrefixArgs x{};
+  x.struct_size = sizeof(x);
+  int index = -1;
+  const Tensor* q = tensor_of(a[0]);
+  // the prefixes first: they are sequences of the same cache
+  if (!fill_attention(q, {a[1], a[2], a[3], a[4], a[5], a[11], a[12]}, a[9], a[10], a[14], x.attn, index))
+    return none();
+  x.prefix_table = x.attn.cache.page_table;
+  x.prefix_offsets = x.attn.cache.offsets;
+  x.prefix_lens = x.attn.cache.kv_lens;
+  x.prefix_stride = x.attn.cache.table_stride;
+  x.prefix_cols = x.attn.cache.table_cols;
+  x.prefixes = x.attn.cache.seqs;
+  x.max_prefix_q_len = x.attn.max_q_len;
+  x.attn.max_q_len = 0;
+  if (!fill_seqs({a[1], a[2], a[6], a[7], a[8], a[11], a[12]}, x.attn.cache, index) ||
+      !fill_bound(a[13], x.attn.max_q_len))
+    return none();
+  const c10::cuda::OptionalCUDAGuard guard(q->device());
+  Tensor out, lse;
+  if (!fill_outputs(q, a[15], a[16], x.attn, index, out, lse)) return none();
+  if (x.attn.total > 0 && x.attn.cache.seqs > 0) {
+    x.attn.workspace_bytes = g_prefix_workspace(&x);
+    if (x.attn.workspace_bytes < 0) return none();
+    const c10::DataPtr workspace =
+        c10::cuda::CUDACachingAllocator::get()->allocate(x.attn.workspace_bytes);
+    x.attn.workspace = workspace.get();
+    const int rc = g_prefix(&x, c10::cuda::getCurrentCUDAStream(index).stream());
+    if (rc != FA_OK) return PyLong_FromLong(rc);
+  }
+  return outputs(a[15], a[16], out, lse);
   END_HANDLE_TH_ERRORS
 }
 
@@ -295,9 +363,10 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // setup(attention, workspace_bytes, write, read): addresses of the C ABI
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* p[4];
-  if (n != 4) return none();
-  for (int i = 0; i < 4; ++i) {
+  constexpr int kCalls = 4;
+  void* p[kCalls];
+  if (n != kCalls) return none();
+  for (int i = 0; i < kCalls; ++i) {
     p[i] = PyLong_AsVoidPtr(a[i]);
     if (!p[i]) return PyErr_Occurred() ? nullptr : none();
   }
@@ -305,6 +374,20 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g_workspace = reinterpret_cast<decltype(g_workspace)>(p[1]);
   g_write = reinterpret_cast<decltype(g_write)>(p[2]);
   g_read = reinterpret_cast<decltype(g_read)>(p[3]);
+  return PyBool_FromLong(1);
+}
+
+// setup_more(prefix attention, its workspace_bytes): those of the other calls
+PyObject* setup_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  constexpr int kCalls = 2;
+  void* p[kCalls];
+  if (n != kCalls) return none();
+  for (int i = 0; i < kCalls; ++i) {
+    p[i] = PyLong_AsVoidPtr(a[i]);
+    if (!p[i]) return PyErr_Occurred() ? nullptr : none();
+  }
+  g_prefix = reinterpret_cast<decltype(g_prefix)>(p[0]);
+  g_prefix_workspace = reinterpret_cast<decltype(g_prefix_workspace)>(p[1]);
   return PyBool_FromLong(1);
 }
 
@@ -323,9 +406,11 @@ PyObject* set_status(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attention)), METH_FASTCALL, nullptr},
+    {"prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(prefix_attention)), METH_FASTCALL, nullptr},
     {"read_new", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(read_new)), METH_FASTCALL, nullptr},
     {"copy", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(copy)), METH_FASTCALL, nullptr},
     {"setup", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(setup)), METH_FASTCALL, nullptr},
+    {"setup_more", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(setup_more)), METH_FASTCALL, nullptr},
     {"set_status", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(set_status)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_binding", nullptr, -1, methods,

@@ -83,23 +83,29 @@ def validate_cache(k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_sc
                 raise ValueError(f"{name} must be float32 [num_pages, heads_kv, page_size]")
             if not _aligned(t):
                 raise ValueError(f"{name} needs a unit inner stride and 16-byte aligned strides")
-    if page_table.ndim != 2 or offsets.ndim != 1 or kv_lens.ndim != 1:
-        raise ValueError("page_table must be [seqs, columns], offsets [seqs + 1], kv_lens [seqs]")
-    seqs = page_table.shape[0]
-    if offsets.shape[0] != seqs + 1 or kv_lens.shape[0] != seqs:
-        raise ValueError("page_table must be [seqs, columns], offsets [seqs + 1], kv_lens [seqs]")
-    if any(t.dtype != torch.int32 for t in (page_table, offsets, kv_lens)):
-        raise ValueError("page_table, offsets and kv_lens must be int32")
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1 or not (
-            offsets.is_contiguous() and kv_lens.is_contiguous()):
-        raise ValueError("offsets, kv_lens and the rows of page_table must be contiguous")
-    if page_table.shape[1] * size > 1 << 30:
-        raise ValueError("page_table names more than 2^30 positions a sequence")
+    validate_sequences(page_table, offsets, kv_lens, size)
     for t in (k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale):
         if t is not None and t.device != k_cache.device:
             raise ValueError("all tensors of a paged call must be on the same device")
         if t is not None and t.is_neg():
             raise ValueError("a cache, its scales and its sequences must not be negated views")
+
+
+def validate_sequences(page_table, offsets, kv_lens, page_size,
+                       names=("page_table", "offsets", "kv_lens"), rows="seqs") -> None:
+    """Shapes, types and layout of a page table and what goes with it."""
+    table, offs, lens = names
+    if (page_table.ndim != 2 or offsets.ndim != 1 or kv_lens.ndim != 1
+            or offsets.shape[0] != page_table.shape[0] + 1
+            or kv_lens.shape[0] != page_table.shape[0]):
+        raise ValueError(f"{table} must be [{rows}, columns], {offs} [{rows} + 1], {lens} [{rows}]")
+    if any(t.dtype != torch.int32 for t in (page_table, offsets, kv_lens)):
+        raise ValueError(f"{table}, {offs} and {lens} must be int32")
+    if page_table.shape[1] > 1 and page_table.stride(1) != 1 or not (
+            offsets.is_contiguous() and kv_lens.is_contiguous()):
+        raise ValueError(f"{offs}, {lens} and the rows of {table} must be contiguous")
+    if page_table.shape[1] * page_size > 1 << 30:
+        raise ValueError(f"{table} names more than 2^30 positions a sequence")
 
 
 def _validate_rows(name, t, k_cache, heads) -> None:
@@ -129,6 +135,22 @@ def validate_attention(q, k_cache, v_cache, page_table, offsets, kv_lens, k_scal
         raise ValueError("q has more than 2^30 - 1 (token, head) rows")
     if max_q_len is not None and max_q_len < 0:
         raise ValueError("max_q_len must not be negative")
+
+
+def validate_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, prefix_lens, page_table,
+                              offsets, kv_lens, k_scale=None, v_scale=None, max_q_len=None,
+                              max_prefix_q_len=None) -> None:
+    """The rules of `prefix_attention`, on tensors of any device."""
+    validate_attention(q, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale, max_q_len)
+    prefix = (prefix_table, prefix_offsets, prefix_lens)
+    validate_sequences(*prefix, k_cache.shape[2], ("prefix_table", "prefix_offsets", "prefix_lens"),
+                       "prefixes")
+    if any(t.device != k_cache.device for t in prefix):
+        raise ValueError("all tensors of a paged call must be on the same device")
+    if any(t.is_neg() for t in prefix):
+        raise ValueError("a cache, its scales and its sequences must not be negated views")
+    if max_prefix_q_len is not None and max_prefix_q_len < 0:
+        raise ValueError("max_prefix_q_len must not be negative")
 
 
 def validate_copy(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale=None,
@@ -182,9 +204,14 @@ def _native_binding():
             raise RuntimeError(f"the paged calls need {exc.name or '_paged_binding'}; build it with "
                                "`python -m flash_attn_npu_b200.build`") from None
         lib = _native.load()
-        _paged_binding.setup(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+        def addresses(*calls):
+            return (ctypes.cast(fn, ctypes.c_void_p).value for fn in calls)
+
+        _paged_binding.setup(*addresses(
             lib.fa_paged_attn_sm100, lib.fa_paged_workspace_bytes, lib.fa_paged_write_sm100,
-            lib.fa_paged_read_sm100)))
+            lib.fa_paged_read_sm100))
+        _paged_binding.setup_more(*addresses(
+            lib.fa_paged_prefix_sm100, lib.fa_paged_prefix_workspace_bytes))
         _binding = _paged_binding
     return _binding
 
@@ -224,14 +251,14 @@ def _check(res, device) -> None:
         ops.check_device_status(device)
 
 
-def _max_len(n):
+def _max_len(n, name="max_q_len"):
     """An upper bound given as any kind of integer, or None."""
     if n is None:
         return None
     try:
         n = operator.index(n)
     except TypeError:
-        raise ValueError(f"max_q_len must be an integer or None (got {n!r})") from None
+        raise ValueError(f"{name} must be an integer or None (got {n!r})") from None
     return min(n, 1 << 30)  # (there are no more rows)
 
 
@@ -248,6 +275,16 @@ def _scale(x) -> float:
 def _rows_like(t):
     """`t`, or a copy where its rows are not 16-byte aligned or its memory holds their negatives."""
     return t if _aligned(t) and not t.is_neg() else empty_rows(t).copy_(t.detach())
+
+
+def _validate_outputs(q, out, lse) -> None:
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype
+                            or out.device != q.device or not _aligned(out) or out.is_neg()):
+        raise ValueError("out must match q in shape, dtype and device, with a unit inner stride "
+                         "and 16-byte aligned strides")
+    if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32
+                            or lse.device != q.device or not lse.is_contiguous() or lse.is_neg()):
+        raise ValueError("lse must be a contiguous float32 tensor [total, heads_q]")
 
 
 def attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scale, k_scale=None,
@@ -278,15 +315,44 @@ def attention(q, k_cache, v_cache, page_table, offsets, kv_lens, causal, sm_scal
         validate_attention(q, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale,
                            max_q_len)
         _require_cuda(q)
-        if out is not None and (out.shape != q.shape or out.dtype != q.dtype
-                                or out.device != q.device or not _aligned(out) or out.is_neg()):
-            raise ValueError("out must match q in shape, dtype and device, with a unit inner stride "
-                             "and 16-byte aligned strides")
-        if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32
-                                or lse.device != q.device or not lse.is_contiguous() or lse.is_neg()):
-            raise ValueError("lse must be a contiguous float32 tensor [total, heads_q]")
+        _validate_outputs(q, out, lse)
         res = _call("attention", q.device, _rows_like(q), k_cache, v_cache, page_table, offsets,
                     kv_lens, bool(causal), sm_scale, k_scale, v_scale, max_q_len, out, lse)
+    if type(res) is int or ops._CHECK_EVERY_CALL:
+        _check(res, q.device)
+    return res
+
+
+def prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, prefix_lens, page_table, offsets,
+                     kv_lens, causal, sm_scale, k_scale=None, v_scale=None, max_q_len=None,
+                     max_prefix_q_len=None, out=None, lse=None):
+    """Attention of sequences that share prefixes, which are read and multiplied once for all; (out, lse).
+
+    Prefix g is the `prefix_lens[g]` tokens in the pages `prefix_table[g]` of the same cache.  The packed
+    rows prefix_offsets[g] .. prefix_offsets[g + 1] attend to all of it, and behind it to their own
+    sequence: `page_table`, `offsets`, `kv_lens` and `causal` as for `attention`, of the sequences' own
+    tokens alone (`kv_lens` does not count the prefix, whose last page no sequence continues).  Rows of no
+    group have no prefix, and rows of no sequence are not written.  `lse` is over both.
+
+    `max_prefix_q_len`: an upper bound of the rows that share one prefix, which the kernel choice goes by
+    (default: total); `max_q_len`, `out`, `lse` and what values may do as in `attention`.
+    """
+    res = None
+    if _binding is not None:
+        res = _binding.prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, prefix_lens,
+                                        page_table, offsets, kv_lens, causal, sm_scale, k_scale, v_scale,
+                                        max_q_len, max_prefix_q_len, out, lse)
+    if res is None:
+        sm_scale, max_q_len = _scale(sm_scale), _max_len(max_q_len)
+        max_prefix_q_len = _max_len(max_prefix_q_len, "max_prefix_q_len")
+        validate_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, prefix_lens,
+                                  page_table, offsets, kv_lens, k_scale, v_scale, max_q_len,
+                                  max_prefix_q_len)
+        _require_cuda(q)
+        _validate_outputs(q, out, lse)
+        res = _call("prefix_attention", q.device, _rows_like(q), k_cache, v_cache, prefix_table,
+                    prefix_offsets, prefix_lens, page_table, offsets, kv_lens, bool(causal), sm_scale,
+                    k_scale, v_scale, max_q_len, max_prefix_q_len, out, lse)
     if type(res) is int or ops._CHECK_EVERY_CALL:
         _check(res, q.device)
     return res

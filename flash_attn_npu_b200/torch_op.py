@@ -11,8 +11,8 @@ the C ABI, no host synchronisation), so it can be recorded into a CUDA graph.
 Arguments follow `ops.forward`: the last four are BLOCK_M, BLOCK_N, NUM_STAGES,
 PERSISTENT_CTAS, each 0 for the library default.
 
-`paged_attention`, `paged_cache_write` and `paged_cache_read` are the calls of `paged` in the same
-way.  The write is registered as one that mutates the cache (and the scales of a float8 one), and
+`paged_attention`, `paged_prefix_attention`, `paged_cache_write` and `paged_cache_read` are the calls of
+`paged` in the same way.  The write is registered as one that mutates the cache (and the scales of a float8 one), and
 returns nothing; its scales have no default (a mutated argument must be there), None for a 16-bit
 cache.
 
@@ -66,6 +66,29 @@ def _paged_attention_fake(q, k_cache, v_cache, page_table, offsets, kv_lens, cau
                           k_scale=None, v_scale=None, max_q_len=None):
     paged.validate_attention(q, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale,
                              max_q_len)
+    return paged.empty_rows(q), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+@torch.library.custom_op("flash_attn_b200::paged_prefix_attention", mutates_args=())
+def paged_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           prefix_table: torch.Tensor, prefix_offsets: torch.Tensor,
+                           prefix_lens: torch.Tensor, page_table: torch.Tensor, offsets: torch.Tensor,
+                           kv_lens: torch.Tensor, causal: bool, sm_scale: float,
+                           k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                           max_q_len: int | None = None,
+                           max_prefix_q_len: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    return paged.prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, prefix_lens,
+                                  page_table, offsets, kv_lens, causal, sm_scale, k_scale, v_scale,
+                                  max_q_len, max_prefix_q_len)
+
+
+@paged_prefix_attention.register_fake
+def _paged_prefix_attention_fake(q, k_cache, v_cache, prefix_table, prefix_offsets, prefix_lens, page_table,
+                                 offsets, kv_lens, causal, sm_scale, k_scale=None, v_scale=None,
+                                 max_q_len=None, max_prefix_q_len=None):
+    paged.validate_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, prefix_lens,
+                                    page_table, offsets, kv_lens, k_scale, v_scale, max_q_len,
+                                    max_prefix_q_len)
     return paged.empty_rows(q), q.new_empty(q.shape[:2], dtype=torch.float32)
 
 

@@ -117,6 +117,31 @@ FA_API int fa_paged_attn_sm100(const FaPagedAttnArgs* args, void* stream);
  * current device; negative: a FaStatus. */
 FA_API int64_t fa_paged_workspace_bytes(const FaPagedAttnArgs* args);
 
+/* Attention behind shared prefixes: a row attends to a prefix that its group shares, and to its own
+ * sequence behind that.  Prefix g is `prefix_lens[g]` tokens in the pages `prefix_table[g]` of the same
+ * cache, and its group the packed rows prefix_offsets[g] .. prefix_offsets[g + 1], which may cut sequences
+ * anywhere; rows of no group have no prefix.  `attn` is as for fa_paged_attn_sm100: its cache's page_table,
+ * kv_lens and offsets are those of the sequences' own tokens, and `causal` concerns these alone.  Its
+ * workspace takes fa_paged_prefix_workspace_bytes() bytes. */
+typedef struct FaPagedPrefixArgs {
+  int32_t struct_size; /* sizeof(FaPagedPrefixArgs) */
+  FaPagedAttnArgs attn;
+  const int32_t* prefix_table;   /* [prefixes, prefix_cols] */
+  const int32_t* prefix_offsets; /* [prefixes + 1] */
+  const int32_t* prefix_lens;    /* [prefixes] */
+  int64_t prefix_stride;         /* elements between the rows of prefix_table */
+  int64_t prefix_cols;
+  int64_t prefixes;
+  int64_t max_prefix_q_len; /* upper bound of a group's rows that the kernel choice goes by (0: total) */
+} FaPagedPrefixArgs;
+
+/* Attention of the packed queries over their prefixes and sequences: out, and the logsumexp over both.
+ * All else as in fa_paged_attn_sm100. */
+FA_API int fa_paged_prefix_sm100(const FaPagedPrefixArgs* args, void* stream);
+
+/* Its workspace, as fa_paged_workspace_bytes. */
+FA_API int64_t fa_paged_prefix_workspace_bytes(const FaPagedPrefixArgs* args);
+
 #ifdef __cplusplus
 }
 #endif
