@@ -60,6 +60,16 @@ SOURCES = [
     "fa_paged_tile_d64.cu",
     "fa_paged_tile_d128.cu",
     "fa_paged_tile_d256.cu",
+    "fa_paged_levels_rows_d16.cu",
+    "fa_paged_levels_rows_d32.cu",
+    "fa_paged_levels_rows_d64.cu",
+    "fa_paged_levels_rows_d128.cu",
+    "fa_paged_levels_rows_d256.cu",
+    "fa_paged_levels_tile_d16.cu",
+    "fa_paged_levels_tile_d32.cu",
+    "fa_paged_levels_tile_d64.cu",
+    "fa_paged_levels_tile_d128.cu",
+    "fa_paged_levels_tile_d256.cu",
 ]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

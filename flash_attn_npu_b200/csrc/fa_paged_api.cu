@@ -69,7 +69,6 @@ int check_attn(const FaPagedAttnArgs* a) {
 }
 
 PagedChoice choose_attn(const FaPagedAttnArgs* a) {
-  PagedChoice c{};
   const int64_t group = a->heads_q / a->cache.heads_kv;
   const int64_t longest = a->max_q_len ? std::min(a->max_q_len, a->total) : a->total;
   // Up to 32 rows a kv head every sequence is one block of the row kernel, which reads the cache
@@ -80,8 +79,16 @@ PagedChoice choose_attn(const FaPagedAttnArgs* a) {
   // At head_dim 256 that does not hold: blocks have 16 rows, so 17 to 32 rows are two of them, which
   // read the cache one after the other.  There 16 sequences of 4096 tokens take 216 us and 110 (float8: 239
   // and 129), 40 of 2048 270 and 137, one of 512 17 and 17.
-  const int64_t most = longest * group;
-  if (most > 32 && group <= 128 && a->sm_scale > 0.f) c.rows = 0;
+  return choose_for_rows(a, longest * group);
+}
+
+bool tile_kernel_takes(const FaPagedAttnArgs* a) {
+  return a->heads_q / a->cache.heads_kv <= 128 && a->sm_scale > 0.f;
+}
+
+PagedChoice choose_for_rows(const FaPagedAttnArgs* a, int64_t most) {
+  PagedChoice c{};
+  if (most > 32 && tile_kernel_takes(a)) c.rows = 0;
   else if (most <= 8) c.rows = 8;
   else c.rows = most <= 16 || a->cache.head_dim > 128 ? 16 : 32;
   c.info = info_for(a->cache.head_dim, a->cache.dtype == FA_DTYPE_FP8_E4M3, c.rows);
@@ -163,7 +170,6 @@ int plan_attn(const FaPagedAttnArgs* a, const PagedChoice& c, char* ws, cudaStre
   p.pair_from = plan.fp8 ? 6 : 3;
   p.tile_toks = tile ? 128 / p.group : 0;
   p.tile_live = tile ? p.tile_toks * p.group : info.rows;
-  p.lse_unit = kLn2;
   p.parts = reinterpret_cast<PagedPart*>(ws + c.parts);
   p.part_lse = reinterpret_cast<float*>(ws + c.lse);
   p.part_o = reinterpret_cast<float*>(ws + c.o);

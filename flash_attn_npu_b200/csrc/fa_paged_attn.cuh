@@ -17,6 +17,7 @@
 #pragma once
 
 #include <climits>
+#include <type_traits>
 
 #include "fa_fwd_kernel.cuh"
 #include "fa_paged_common.cuh"
@@ -91,55 +92,95 @@ struct PagedAttnParams {
   PagedPart* parts;  // [gridDim.x]
   float* part_o;     // [gridDim.x][2][block rows][head_dim]
   float* part_lse;   // [gridDim.x][2][block rows]
-  // Calls behind shared prefixes (fa_paged_prefix.cu): 1 the prefixes, 2 the sequences' own tokens, 0 any
-  // other call.  There no row is finished here: whole items go to `whole_o` in fp32, `lse` is of base 2,
-  // and `where` tells where a row's parts are.
-  int level;
-  float lse_unit;    // what a base-2 logsumexp is multiplied by on its way to `lse`
-  float* whole_o;    // [total, heads_q, head_dim]
-  uint32_t* where;   // [total, heads_q]
+};
+
+// A call behind shared prefixes (fa_paged_prefix.cu) has two levels: the prefixes, which are the sequences
+// of `seqs` and have no causal mask, and the sequences' own tokens, which follow in the line as those of
+// `own`.  A kernel may hold both or (the other has no sequence in it) one of them.  No row is finished here:
+// whole items go to `whole_o` in fp32 and `lse` in base 2, and `where` tells where a row's parts are.
+struct PagedLevelParams : PagedAttnParams {
+  PagedSeqs own;
+  float* whole_o;    // [2][total, heads_q, head_dim]
+  uint32_t* where;   // [2][total, heads_q]
+  int64_t rows;      // total * heads_q
+  int place;         // of two kernels that run side by side: 1 the first, 2 the second; 0: alone
   PagedLevel levels[2];
 };
 
-// Steps of one kv head of a level, weighted.  An estimate (a causal triangle counts as a rectangle): both
-// kernels divide the CTAs by it, and nothing but their balance depends on it.
-__device__ __forceinline__ int64_t level_weight(const PagedLevel& v, int group) {
+template <bool LV>
+using PagedParams = std::conditional_t<LV, PagedLevelParams, PagedAttnParams>;
+
+// Sequence b of the line: whose it is, and which one there.
+__device__ __forceinline__ const PagedSeqs& seqs_of_line(const PagedAttnParams& p, int) { return p.seqs; }
+__device__ __forceinline__ const PagedSeqs& seqs_of_line(const PagedLevelParams& p, int b) {
+  return b >= p.seqs.seqs ? p.own : p.seqs;
+}
+__device__ __forceinline__ int seq_of_line(const PagedAttnParams&, int b) { return b; }
+__device__ __forceinline__ int seq_of_line(const PagedLevelParams& p, int b) {
+  return b >= p.seqs.seqs ? b - p.seqs.seqs : b;
+}
+__device__ __forceinline__ int line_seqs(const PagedAttnParams& p) { return p.seqs.seqs; }
+__device__ __forceinline__ int line_seqs(const PagedLevelParams& p) { return p.seqs.seqs + p.own.seqs; }
+__device__ __forceinline__ bool is_causal(const PagedAttnParams& p, int) { return p.causal; }
+__device__ __forceinline__ bool is_causal(const PagedLevelParams& p, int b) {
+  return p.causal && b >= p.seqs.seqs;
+}
+// First of the level's rows in `lse`, `where` and `whole_o`.
+__device__ __forceinline__ int64_t level_row(const PagedLevelParams& p, int b) {
+  return b >= p.seqs.seqs ? p.rows : 0;
+}
+
+// Weights of the levels: steps of one kv head, times what a step takes.  An estimate (a causal triangle
+// counts as a rectangle): both kernels divide the CTAs by it, and nothing but their balance depends on it.
+__device__ __forceinline__ void level_weights(const PagedLevelParams& p, float (&weight)[2]) {
   const int lane = threadIdx.x & 31;
-  int64_t sum = 0;
-  for (int b = lane; b < v.seqs.seqs; b += 32) {
-    int first, count;
-    seq_rows(v.seqs, b, first, count);
-    const int len = seq_len(v.seqs, b);
-    const int64_t blocks = (static_cast<int64_t>(count) * group + v.rows - 1) / v.rows;
-    sum += blocks * ((len + v.keys - 1) / v.keys + v.cost);
+  int64_t sum[2] = {0, 0};
+  for (int b = lane; b < max(p.levels[0].seqs.seqs, p.levels[1].seqs.seqs); b += 32) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const PagedLevel& v = p.levels[i];
+      if (b >= v.seqs.seqs) continue;
+      int first, count;
+      seq_rows(v.seqs, b, first, count);
+      const int64_t blocks = (static_cast<int64_t>(count) * p.group + v.rows - 1) / v.rows;
+      sum[i] += blocks * ((seq_len(v.seqs, b) + v.keys - 1) / v.keys + v.cost);
+    }
   }
 #pragma unroll
-  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  return sum * v.unit;
+  for (int i = 0; i < 2; ++i) {
+    weight[i] = static_cast<float>(sum[i]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) weight[i] += __shfl_xor_sync(0xffffffffu, weight[i], d);
+    weight[i] *= p.levels[i].unit;
+  }
 }
 
-// CTAs that a kernel may use: all, or its level's share of them.
-__device__ __forceinline__ int ctas_for(const PagedAttnParams& p) {
+// CTAs that a kernel may use: all, or its share of them.
+__device__ __forceinline__ int ctas_for(const PagedAttnParams&) { return static_cast<int>(gridDim.x); }
+__device__ __forceinline__ int ctas_for(const PagedLevelParams& p) {
   const int all = static_cast<int>(gridDim.x);
-  if (p.level == 0) return all;
-  const float a = static_cast<float>(level_weight(p.levels[0], p.group));
-  const float b = static_cast<float>(level_weight(p.levels[1], p.group));
-  if (a == 0.f || b == 0.f || all < 2) return all;
-  const int n = min(max(__float2int_rn(all * (a / (a + b))), 1), all - 1);
-  return p.level == 1 ? n : all - n;
+  if (p.place == 0) return all;
+  float w[2];
+  level_weights(p, w);
+  if (w[0] == 0.f || w[1] == 0.f || all < 2) return all;
+  const int n = min(max(__float2int_rn(all * (w[0] / (w[0] + w[1]))), 1), all - 1);
+  return p.place == 1 ? n : all - n;
 }
 
-// The two kernels of such a call run at the same time: the second is brought up once every CTA of the
-// first has seen the end of what was before it, reads nothing that the first writes, and ends behind it.
-__device__ __forceinline__ void level_begin_before_sync(const PagedAttnParams& p) {
-  if (p.level != 1) let_next_launch();
+// Two kernels side by side: the second is brought up once every CTA of the first has seen the end of what
+// was before it, reads nothing that the first writes, and ends behind it.
+__device__ __forceinline__ void begin_early(const PagedAttnParams&) { let_next_launch(); }
+__device__ __forceinline__ void begin_early(const PagedLevelParams& p) {
+  if (p.place != 1) let_next_launch();
 }
-__device__ __forceinline__ void level_begin(const PagedAttnParams& p) {
-  if (p.level != 2) wait_for_launch_before();
-  if (p.level == 1) let_next_launch();
+__device__ __forceinline__ void begin(const PagedAttnParams&) { wait_for_launch_before(); }
+__device__ __forceinline__ void begin(const PagedLevelParams& p) {
+  if (p.place != 2) wait_for_launch_before();
+  if (p.place == 1) let_next_launch();
 }
-__device__ __forceinline__ void level_end(const PagedAttnParams& p) {
-  if (p.level == 2 && blockIdx.x == 0) wait_for_launch_before();
+__device__ __forceinline__ void end(const PagedAttnParams&) {}
+__device__ __forceinline__ void end(const PagedLevelParams& p) {
+  if (p.place == 2 && blockIdx.x == 0) wait_for_launch_before();
 }
 
 // One sequence's share of the line.
@@ -151,11 +192,11 @@ struct PagedSeq {
 };
 
 // Work of the row kernel: blocks of ROWS rows, each over all key tiles of its sequence.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnParams& p, int b) {
+template <int ROWS, int KEYS, typename P>
+__device__ __forceinline__ PagedSeq paged_seq(const P& p, int b) {
   PagedSeq s;
-  seq_rows(p.seqs, b, s.first, s.count);
-  s.len = seq_len(p.seqs, b);
+  seq_rows(seqs_of_line(p, b), seq_of_line(p, b), s.first, s.count);
+  s.len = seq_len(seqs_of_line(p, b), seq_of_line(p, b));
   const int rows = s.count * p.group;  // at most total * heads_q, which the host bounds
   s.blocks = (rows + ROWS - 1) / ROWS;
   s.tiles = max(1, (s.len + KEYS - 1) / KEYS);
@@ -193,10 +234,10 @@ struct PagedRange {
 // steps_of(b): steps of sequence b.  Every warp of the CTA finds the range by itself, a lane for
 // each 32nd of the sequences: two sums with a block barrier between them took longer than reading
 // the same few lines in every warp.
-template <typename Steps>
-__device__ __forceinline__ PagedRange paged_range(const PagedAttnParams& p, Steps steps_of) {
+template <typename P, typename Steps>
+__device__ __forceinline__ PagedRange paged_range(const P& p, Steps steps_of) {
   const int lane = threadIdx.x & 31;
-  const int seqs = p.seqs.seqs;
+  const int seqs = line_seqs(p);
   const int each = (seqs + 31) / 32;
   const int b0 = min(lane * each, seqs), b1 = min(b0 + each, seqs);
   int64_t own = 0;
@@ -232,9 +273,9 @@ __device__ __forceinline__ PagedRange paged_range(const PagedAttnParams& p, Step
 }
 
 // Walks the items of a CTA's range; every role of the kernel walks the same ones.
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, typename P>
 struct PagedWalk {
-  const PagedAttnParams& p;
+  const P& p;
   const PagedRange& range;
   int64_t pos;       // next step of the line
   int at;            // ... and of the item
@@ -245,7 +286,7 @@ struct PagedWalk {
   int tile0, tile1;  // key tiles [tile0, tile1) of the item
   int64_t item;      // the item's first step
 
-  __device__ __forceinline__ PagedWalk(const PagedAttnParams& params, const PagedRange& r)
+  __device__ __forceinline__ PagedWalk(const P& params, const PagedRange& r)
       : p(params), range(r), pos(r.lo), b(r.seq) {
     if (pos >= range.hi) return;
     s = paged_seq<ROWS, KEYS>(p, b);
@@ -298,46 +339,60 @@ struct PagedWalk {
   }
 };
 
+// Whether a sequence of the line has a causal mask, kept with its share of the line where they differ.
+template <typename P>
+struct LineMask {
+  __device__ __forceinline__ void set(const P&, int) {}
+  __device__ __forceinline__ bool causal(const P& p) const { return p.causal; }
+};
+template <>
+struct LineMask<PagedLevelParams> {
+  bool mask;
+  __device__ __forceinline__ void set(const PagedLevelParams& p, int b) { mask = is_causal(p, b); }
+  __device__ __forceinline__ bool causal(const PagedLevelParams&) const { return mask; }
+};
+
 // Work of the tile kernel: blocks of TILES tiles of `tile_toks` tokens with all their heads, each
 // over the key tiles up to its last token's position (causal) or the sequence's end.
-template <int TILES, int KEYS>
-struct PagedTiles {
+template <int TILES, int KEYS, typename P>
+struct PagedTiles : LineMask<P> {
   int first, count, len;
   int blocks;
   int64_t per_head;  // steps of one kv head
 
   // Key tiles that the tokens before `tok_end` attend to; 1 if there is none.
-  __device__ __forceinline__ int tiles(const PagedAttnParams& p, int tok_end) const {
-    const int end = p.causal ? min(len, len - count + min(tok_end, count)) : len;
+  __device__ __forceinline__ int tiles(const P& p, int tok_end) const {
+    const int end = this->causal(p) ? min(len, len - count + min(tok_end, count)) : len;
     return max(1, (end + KEYS - 1) / KEYS);
   }
-  __device__ __forceinline__ int block_tiles(const PagedAttnParams& p, int block) const {
+  __device__ __forceinline__ int block_tiles(const P& p, int block) const {
     return tiles(p, (block + 1) * TILES * p.tile_toks);
   }
   PagedTiles() = default;
-  __device__ __forceinline__ PagedTiles(const PagedAttnParams& p, int b) {
-    seq_rows(p.seqs, b, first, count);
-    len = seq_len(p.seqs, b);
+  __device__ __forceinline__ PagedTiles(const P& p, int b) {
+    seq_rows(seqs_of_line(p, b), seq_of_line(p, b), first, count);
+    len = seq_len(seqs_of_line(p, b), seq_of_line(p, b));
+    this->set(p, b);
     blocks = (count + TILES * p.tile_toks - 1) / (TILES * p.tile_toks);
     per_head = static_cast<int64_t>(blocks) * p.item_cost;
-    if (!p.causal) {
+    if (!this->causal(p)) {
       per_head += static_cast<int64_t>(blocks) * block_tiles(p, 0);
     } else {
       for (int m = 0; m < blocks; ++m) per_head += block_tiles(p, m);
     }
   }
-  __device__ __forceinline__ int64_t steps(const PagedAttnParams& p) const {
+  __device__ __forceinline__ int64_t steps(const P& p) const {
     return per_head * p.heads_kv;
   }
 };
 
 // (plain data: it lives in shared memory)
-template <int TILES, int KEYS>
+template <int TILES, int KEYS, typename P>
 struct PagedTileWalk {
   int64_t pos;       // next step of the line
   int at;            // ... and of the item
   int b;
-  PagedTiles<TILES, KEYS> s;
+  PagedTiles<TILES, KEYS, P> s;
   // the current part
   int head, block;
   int n;             // key tiles of the item
@@ -345,10 +400,10 @@ struct PagedTileWalk {
   int64_t item;      // the item's first step
 
   PagedTileWalk() = default;
-  __device__ __forceinline__ PagedTileWalk(const PagedAttnParams& p, const PagedRange& r)
+  __device__ __forceinline__ PagedTileWalk(const P& p, const PagedRange& r)
       : pos(r.lo), b(r.seq) {
     if (pos >= r.hi) return;
-    s = PagedTiles<TILES, KEYS>(p, b);
+    s = PagedTiles<TILES, KEYS, P>(p, b);
     int64_t in_seq = pos - r.base;
     head = static_cast<int>(s.per_head >> 31 ? in_seq / s.per_head
                                              : quot(in_seq, static_cast<int>(s.per_head)));
@@ -362,7 +417,7 @@ struct PagedTileWalk {
       at = n + p.item_cost;
     }
   }
-  __device__ __forceinline__ bool next(const PagedAttnParams& p, int64_t hi) {
+  __device__ __forceinline__ bool next(const P& p, int64_t hi) {
     do {
       if (pos >= hi) return false;
       if (at == n + p.item_cost) {
@@ -371,7 +426,7 @@ struct PagedTileWalk {
           block = 0;
           if (++head == p.heads_kv) {
             head = 0;
-            do s = PagedTiles<TILES, KEYS>(p, ++b);
+            do s = PagedTiles<TILES, KEYS, P>(p, ++b);
             while (s.blocks == 0);
           }
         }
@@ -389,15 +444,15 @@ struct PagedTileWalk {
     return true;
   }
   // First token of tile i of the block, and the steps of this part that the tile takes part in.
-  __device__ __forceinline__ int tok0(const PagedAttnParams& p, int i) const {
+  __device__ __forceinline__ int tok0(const P& p, int i) const {
     return (block * TILES + i) * p.tile_toks;
   }
-  __device__ __forceinline__ int steps(const PagedAttnParams& p, int i) const {
+  __device__ __forceinline__ int steps(const P& p, int i) const {
     if (tok0(p, i) >= s.count) return 0;
     return min(max(s.tiles(p, tok0(p, i) + p.tile_toks) - tile0, 0), tile1 - tile0);
   }
   // Only the block's first tile has tokens: both sides of the CTA work on it, key tiles in turn.
-  __device__ __forceinline__ bool paired(const PagedAttnParams& p) const {
+  __device__ __forceinline__ bool paired(const P& p) const {
     return TILES == 2 && tok0(p, 1) >= s.count && tile1 - tile0 >= p.pair_from;
   }
   // The part's last tile goes past the sequence's end.

@@ -19,7 +19,7 @@ struct PagedInfo {
 
 struct PagedPlan {
   CUtensorMap tmQ, tmK, tmV;  // tmQ: tile kernel
-  PagedAttnParams params;
+  PagedLevelParams params;  // (its own part: calls behind shared prefixes)
   bool half;  // q and the output are fp16 (else bf16)
   bool fp8;
   int rows;   // row kernel: rows of a block (8, 16 or 32)
@@ -37,11 +37,14 @@ struct PagedChoice {
 
 inline int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
-// fa_paged_api.cu: sizes and types; pointers; the kernel for a call; the launch that it takes (the
-// workspace at `ws`); and that launch.
+// fa_paged_api.cu: sizes and types; pointers; the kernel for a call, or for that many rows a kv head of a
+// sequence; whether the tile kernel can take it; the launch that it takes (the workspace at `ws`); and that
+// launch.
 int check_attn(const FaPagedAttnArgs* a);
 int check_attn_pointers(const FaPagedAttnArgs* a);
 PagedChoice choose_attn(const FaPagedAttnArgs* a);
+PagedChoice choose_for_rows(const FaPagedAttnArgs* a, int64_t most);
+bool tile_kernel_takes(const FaPagedAttnArgs* a);
 int plan_attn(const FaPagedAttnArgs* a, const PagedChoice& c, char* ws, cudaStream_t stream, PagedPlan& plan);
 int launch_attn(const PagedPlan& plan);
 
@@ -55,6 +58,16 @@ int launch_rows_d32(const PagedPlan& plan);
 int launch_rows_d64(const PagedPlan& plan);
 int launch_rows_d128(const PagedPlan& plan);
 int launch_rows_d256(const PagedPlan& plan);
+int launch_levels_tile_d16(const PagedPlan& plan);
+int launch_levels_tile_d32(const PagedPlan& plan);
+int launch_levels_tile_d64(const PagedPlan& plan);
+int launch_levels_tile_d128(const PagedPlan& plan);
+int launch_levels_tile_d256(const PagedPlan& plan);
+int launch_levels_rows_d16(const PagedPlan& plan);
+int launch_levels_rows_d32(const PagedPlan& plan);
+int launch_levels_rows_d64(const PagedPlan& plan);
+int launch_levels_rows_d128(const PagedPlan& plan);
+int launch_levels_rows_d256(const PagedPlan& plan);
 
 // (Calls of several threads may meet in the two below: what they remember is atomic, and only successes
 // are remembered.)

@@ -1,0 +1,8 @@
+// Paged row kernel of calls behind shared prefixes, head_dim = 128 (see fa_paged_rows_dispatch.cuh).
+#define FA_HEAD_DIM 128
+#define FA_LEVELS true
+#include "fa_paged_rows_dispatch.cuh"
+
+namespace fa {
+int launch_levels_rows_d128(const PagedPlan& plan) { return launch_any(plan); }
+}  // namespace fa

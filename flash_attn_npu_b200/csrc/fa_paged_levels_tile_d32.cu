@@ -1,0 +1,8 @@
+// Paged tile kernel of calls behind shared prefixes, head_dim = 32 (see fa_paged_tile_dispatch.cuh).
+#define FA_HEAD_DIM 32
+#define FA_LEVELS true
+#include "fa_paged_tile_dispatch.cuh"
+
+namespace fa {
+int launch_levels_tile_d32(const PagedPlan& plan) { return launch_any(plan); }
+}  // namespace fa

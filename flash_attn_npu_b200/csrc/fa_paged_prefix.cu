@@ -6,11 +6,12 @@
 //
 // A prefix is attended to by all rows of its group at once, as one sequence without a causal mask: its
 // keys and values are read once for the group, and its products have rows enough for the tensor cores.
-// So a call is two launches of the paged attention kernels over the same packed rows, the prefixes (level
-// 1, mostly the tile kernel, bound by its products) and the sequences' own tokens (level 2, in decoding
-// the row kernel, bound by memory), and one that joins a row's parts.  The first two run side by side
-// (programmatic dependent launch; level_begin in fa_paged_attn.cuh): each takes its share of the SMs by
-// what the levels weigh, which the kernels work out from the lengths, as these are device data.
+// So a call runs the paged attention kernels over the same packed rows twice, for the prefixes and for the
+// sequences' own tokens (the levels), and joins a row's parts.  In decoding the first is work for the tile
+// kernel, bound by its products, and the second for the row kernel, bound by memory: two launches that run
+// side by side (programmatic dependent launch; `begin` in fa_paged_attn.cuh), each on its share of the SMs
+// by what the levels weigh, which the kernels work out from the lengths, as these are device data.  Where
+// one kernel suits both levels, one launch has the prefixes and the sequences in one line.
 #include <algorithm>
 
 #include "fa_paged_host.h"
@@ -19,12 +20,10 @@
 namespace fa {
 namespace {
 
+// A level's parts, as the kernel that held it left them.
 struct JoinLevel {
   const float* part_o;
   const float* part_lse;
-  const float* whole_o;
-  const float* lse;
-  const uint32_t* where;
   const int* offsets;
   int seqs;
   int slot_rows;  // rows of a slot
@@ -33,11 +32,13 @@ struct JoinLevel {
 
 struct JoinParams {
   JoinLevel level[2];
+  const float* whole_o;   // as in PagedLevelParams
+  const float* whole_lse;
+  const uint32_t* where;
   void* o;
   float* lse;
   int64_t o_stride[2];
   int rows;  // total * heads_q
-  int total;
   int heads_q;
 };
 
@@ -63,7 +64,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     const JoinLevel& v = p.level[x];
     const bool in = tok >= fresh(v.offsets) && tok < fresh(v.offsets + v.seqs);
     if (x == 1) live = live && in;
-    const uint32_t w = in && live ? fresh(v.where + row) : 0u;
+    const uint32_t w = in && live ? fresh(p.where + x * static_cast<int64_t>(p.rows) + row) : 0u;
     // (what a kernel that gave up has left may be any bits)
     const int first = min(static_cast<int>(w >> 10 & 1023), v.ctas - 1);
     n[x] = !in ? 0 : (w & 1023) == 0 ? 1 : min(static_cast<int>(w & 1023), v.ctas - first);
@@ -77,8 +78,9 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     const JoinLevel& v = p.level[x];
     if (x) i -= n[0];
     if (at[x] < 0) {
-      o = v.whole_o + row * D;
-      return fresh(v.lse + row);
+      const int64_t y = x * static_cast<int64_t>(p.rows) + row;
+      o = p.whole_o + y * D;
+      return fresh(p.whole_lse + y);
     }
     const int64_t slot = i == 0 ? 2 * static_cast<int64_t>(at[x]) + 1 : 2 * static_cast<int64_t>(at[x] + i);
     const int64_t y = slot * v.slot_rows + in_slot[x];
@@ -173,34 +175,55 @@ int check_prefix(const FaPagedPrefixArgs* a) {
   return check_attn(&x);
 }
 
-// Workspace: per level the kernel's own, whole rows, their logsumexps and where a row's parts are.
+// One kernel for both levels, where both have few rows or the own tokens have many, else the tile kernel
+// for the prefixes beside the row kernel for the own tokens.
 struct PrefixChoice {
-  PagedChoice level[2];
-  int64_t own[2], whole_o[2], lse[2], where[2], bytes;
+  int launches;
+  PagedChoice kernel[2];
+  int64_t own[2], whole_o, whole_lse, where, bytes;  // workspace: the kernels' own, and what the join reads
 };
 
 PrefixChoice choose(const FaPagedPrefixArgs* a) {
   PrefixChoice c{};
-  const FaPagedAttnArgs x[2] = {of_prefixes(a), a->attn};
-  const int64_t rows = a->attn.total * a->attn.heads_q;
-  for (int i = 0; i < 2; ++i) {
-    c.level[i] = choose_attn(&x[i]);
-    c.level[i].grid = std::min(c.level[i].grid, PagedWhere::kMostCtas);
+  const FaPagedAttnArgs& x = a->attn;
+  const int64_t group = x.heads_q / x.cache.heads_kv, total = x.total;
+  int64_t most[2] = {a->max_prefix_q_len, x.max_q_len};
+  for (int64_t& m : most) m = (m ? std::min(m, total) : total) * group;
+  c.launches = most[0] > 32 && most[1] <= 32 && tile_kernel_takes(&x) ? 2 : 1;
+  if (c.launches == 1) most[0] = std::max(most[0], most[1]);
+  for (int i = 0; i < c.launches; ++i) {
+    c.kernel[i] = choose_for_rows(&x, most[i]);
+    c.kernel[i].grid = std::min(c.kernel[i].grid, +PagedWhere::kMostCtas);
     c.own[i] = c.bytes;
-    c.whole_o[i] = c.own[i] + c.level[i].bytes;
-    c.lse[i] = up256(c.whole_o[i] + 4 * rows * a->attn.cache.head_dim);
-    c.where[i] = up256(c.lse[i] + 4 * rows);
-    c.bytes = up256(c.where[i] + 4 * rows);
+    c.bytes += c.kernel[i].bytes;
   }
+  const int64_t rows = 2 * total * x.heads_q;
+  c.whole_o = c.bytes;
+  c.whole_lse = up256(c.whole_o + 4 * rows * x.cache.head_dim);
+  c.where = up256(c.whole_lse + 4 * rows);
+  c.bytes = up256(c.where + 4 * rows);
   return c;
 }
 
-// Weight of a tile of each kernel, in 10 ns of one SM (measured at head_dim 128): 128 keys take the tile
-// kernel 2.0 us for two query tiles (float8 2.5); the row kernel takes 64 KB in 1.0 us.
+int launch_levels(const PagedPlan& plan) {
+  const bool tile = plan.rows == 0;
+  switch (plan.params.head_dim) {
+    case 16: return tile ? launch_levels_tile_d16(plan) : launch_levels_rows_d16(plan);
+    case 32: return tile ? launch_levels_tile_d32(plan) : launch_levels_rows_d32(plan);
+    case 64: return tile ? launch_levels_tile_d64(plan) : launch_levels_rows_d64(plan);
+    case 128: return tile ? launch_levels_tile_d128(plan) : launch_levels_rows_d128(plan);
+    default: return tile ? launch_levels_tile_d256(plan) : launch_levels_rows_d256(plan);
+  }
+}
+
+// What a tile takes of an SM, in 10 ns (measured at head_dim 128, both kernels at work): 128 keys of two
+// query tiles 3.0 us in the tile kernel, 64 KB 1.05 us in the row kernel with blocks of 8 rows; blocks of
+// 32 rows are bound by their chain, 1.2 us a tile.
 int unit_of(const PagedPlan& plan, const PagedInfo& info) {
-  if (plan.rows == 0) return plan.fp8 ? 250 : 200;
+  if (plan.rows == 0) return 300;
+  if (plan.rows == 32) return 120;
   const int bytes = 2 * info.keys * plan.params.head_dim * (plan.fp8 ? 1 : 2);
-  return std::max(40, bytes / 655);
+  return std::max(60, bytes * 105 / 65536);
 }
 
 int prefix_attention(const FaPagedPrefixArgs* a, void* stream) {
@@ -218,41 +241,50 @@ int prefix_attention(const FaPagedPrefixArgs* a, void* stream) {
 
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(a->attn.workspace);
+  const PagedSeqs seqs[2] = {seqs_of(x[0].cache, x[0].total, x[0].dev_status),
+                             seqs_of(x[1].cache, x[1].total, x[1].dev_status)};
   PagedPlan plan[2] = {};
-  JoinParams join_params{};
-  for (int i = 0; i < 2; ++i) {
-    rc = plan_attn(&x[i], c.level[i], ws + c.own[i], s, plan[i]);
+  JoinParams j{};
+  for (int i = 0; i < c.launches; ++i) {
+    rc = plan_attn(&a->attn, c.kernel[i], ws + c.own[i], s, plan[i]);
     if (rc != FA_OK) return rc;
-    PagedAttnParams& p = plan[i].params;
-    const PagedInfo& info = c.level[i].info;
-    p.level = i + 1;
-    p.whole_items = 0;
+    PagedLevelParams& p = plan[i].params;
+    const PagedInfo& info = c.kernel[i].info;
+    p.whole_items = 0;  // (there is a join in any case)
     p.min_steps_log2 = plan[i].rows == 0 ? 2 : 1;
-    p.lse_unit = 1.f;
-    p.lse = reinterpret_cast<float*>(ws + c.lse[i]);
-    p.whole_o = reinterpret_cast<float*>(ws + c.whole_o[i]);
-    p.where = reinterpret_cast<uint32_t*>(ws + c.where[i]);
-    const int rows = plan[i].rows == 0 ? info.rows / 128 * p.tile_live : info.rows;
-    const PagedLevel v{p.seqs, rows, info.keys, p.item_cost, unit_of(plan[i], info)};
-    plan[0].params.levels[i] = plan[1].params.levels[i] = v;
-    join_params.level[i] = JoinLevel{p.part_o, p.part_lse, p.whole_o, p.lse, p.where, p.seqs.offsets,
-                                     p.seqs.seqs, info.rows, c.level[i].grid};
+    p.seqs = seqs[0];
+    p.own = seqs[1];
+    p.lse = reinterpret_cast<float*>(ws + c.whole_lse);
+    p.whole_o = reinterpret_cast<float*>(ws + c.whole_o);
+    p.where = reinterpret_cast<uint32_t*>(ws + c.where);
+    p.rows = a->attn.total * a->attn.heads_q;
+    if (c.launches == 2) {
+      p.place = i + 1;
+      (i == 0 ? p.own : p.seqs).seqs = 0;
+      const int rows = plan[i].rows == 0 ? info.rows / 128 * p.tile_live : info.rows;
+      const PagedLevel v{seqs[i], rows, info.keys, p.item_cost, unit_of(plan[i], info)};
+      plan[0].params.levels[i] = plan[1].params.levels[i] = v;
+    }
+    for (int k = c.launches == 2 ? i : 0; k < (c.launches == 2 ? i + 1 : 2); ++k)
+      j.level[k] = JoinLevel{p.part_o, p.part_lse, seqs[k].offsets, seqs[k].seqs, info.rows, c.kernel[i].grid};
   }
-  for (int i = 0; i < 2; ++i) {
-    rc = launch_attn(plan[i]);
+  for (int i = 0; i < c.launches; ++i) {
+    rc = launch_levels(plan[i]);
     if (rc != 0) return rc;
   }
-  join_params.o = a->attn.o;
-  join_params.lse = a->attn.lse;
-  for (int d = 0; d < 2; ++d) join_params.o_stride[d] = a->attn.o_stride[d];
-  join_params.total = static_cast<int>(a->attn.total);
-  join_params.heads_q = static_cast<int>(a->attn.heads_q);
-  join_params.rows = join_params.total * join_params.heads_q;
+  j.whole_o = plan[0].params.whole_o;
+  j.whole_lse = plan[0].params.lse;
+  j.where = plan[0].params.where;
+  j.o = a->attn.o;
+  j.lse = a->attn.lse;
+  for (int d = 0; d < 2; ++d) j.o_stride[d] = a->attn.o_stride[d];
+  j.heads_q = static_cast<int>(a->attn.heads_q);
+  j.rows = static_cast<int>(plan[0].params.rows);
   // Parts are shared among threads while that leaves few enough blocks to be on the SMs at once.
-  const int64_t blocks = static_cast<int64_t>(join_params.rows) * a->attn.cache.head_dim / 4 * 4 / kJoinThreads;
-  const bool split = blocks <= 16 * c.level[0].grid;
-  return plan[0].half ? join<__half>(join_params, a->attn.cache.head_dim, split, s)
-                      : join<__nv_bfloat16>(join_params, a->attn.cache.head_dim, split, s);
+  const int64_t blocks = static_cast<int64_t>(j.rows) * a->attn.cache.head_dim / kJoinThreads;
+  const bool split = blocks <= 16 * c.kernel[0].grid;
+  return plan[0].half ? join<__half>(j, a->attn.cache.head_dim, split, s)
+                      : join<__nv_bfloat16>(j, a->attn.cache.head_dim, split, s);
 }
 
 }  // namespace

@@ -166,11 +166,11 @@ constexpr uint32_t kBandBits = 8;
 constexpr float kBand = 1.f / (1 << kBandBits);
 constexpr float kLeastScale = 1.f / (1ull << 40) / (1ull << 40);
 
-// T: type of q and the output (and of a 16-bit cache).
-template <typename T, int D, bool FP8, int ROWS>
+// T: type of q and the output (and of a 16-bit cache).  LV: a call behind shared prefixes.
+template <typename T, int D, bool FP8, int ROWS, bool LV>
 __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
     paged_rows_kernel(const __grid_constant__ CUtensorMap tmK,
-                      const __grid_constant__ CUtensorMap tmV, const PagedAttnParams p) {
+                      const __grid_constant__ CUtensorMap tmV, const PagedParams<LV> p) {
   using G = RowsGeo<D, FP8, ROWS>;
   using C = std::conditional_t<FP8, __half, T>;  // type of the products
   constexpr bool kHalf = std::is_same_v<C, __half>;
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
   uint8_t* s_q = smem + G::STAGES * G::STAGE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  level_begin_before_sync(p);
+  begin_early(p);
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::STAGES; ++s) {
       mbar_init(smem_u32(&s_full[s]), G::NP);
@@ -198,11 +198,11 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
     fence_mbar_init();
   }
   __syncthreads();
-  level_begin(p);
+  begin(p);
   if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
   const PagedRange range =
       paged_range(p, [&](int b) { return paged_seq<ROWS, KEYS>(p, b).steps; });
-  PagedWalk<ROWS, KEYS> w(p, range);
+  PagedWalk<ROWS, KEYS, PagedParams<LV>> w(p, range);
   int* const status = p.seqs.status;
 
   if (warp >= NW) {
@@ -230,14 +230,15 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
     ProducersMeet<G::NP> meet{s_issued, 2};
     while (issued < meet.limit && w.next()) {
       if (pw == 0 && lane == 0) {
-        if (fresh(p.seqs.kv_lens + w.b) != w.s.len ||
-            fresh(p.seqs.offsets + w.b + 1) - fresh(p.seqs.offsets + w.b) != w.s.count)
+        const PagedSeqs& from = seqs_of_line(p, w.b);
+        const int b = seq_of_line(p, w.b);
+        if (fresh(from.kv_lens + b) != w.s.len || fresh(from.offsets + b + 1) - fresh(from.offsets + b) != w.s.count)
           report(status, kStatusPageTable);
       }
       // the page of this lane's copy for a tile: its entry is fetched one tile ahead
       const int tile1 = my_box < boxes ? min(w.tile1, (w.s.len - my_box * box + KEYS - 1) / KEYS) : 0;
       auto fetch = [&](int t) -> int {
-        return t < tile1 ? page_entry(p.seqs, w.b, t * KEYS + my_box * box) : 0;
+        return t < tile1 ? page_entry(seqs_of_line(p, w.b), seq_of_line(p, w.b), t * KEYS + my_box * box) : 0;
       };
       int entry = fetch(w.tile0);
       for (int t = w.tile0; t < w.tile1; ++t) {
@@ -337,6 +338,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
     const bool my_live = row0 + my_r < rows;
     const int my_tok = tok_of(my_r);
     const int64_t my_head = w.head * p.group + row0 + my_r - my_tok * p.group;
+    const bool causal = is_causal(p, w.b);
     // this thread's logits belong to rows first + 8 n + 2 t4 + {0, 1}
     int lim[WN][2];       // keys that the row may attend to
     float qs[WN][2];      // factor of the row's logits
@@ -345,13 +347,13 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = first + 8 * n + 2 * t4 + e;
-        lim[n][e] = p.causal && row0 + r < rows ? min(w.s.len, past + tok_of(r) + 1) : w.s.len;
+        lim[n][e] = causal && row0 + r < rows ? min(w.s.len, past + tok_of(r) + 1) : w.s.len;
         qs[n][e] = scale;
       }
     // keys that every row of the warp may attend to, and that any row may
     const int last = min(rows - row0, first + 8 * WN) - 1;
-    const int lim_all = p.causal ? min(w.s.len, past + tok_of(first) + 1) : w.s.len;
-    const int lim_any = last < first ? 0 : p.causal ? min(w.s.len, past + tok_of(last) + 1) : w.s.len;
+    const int lim_all = causal ? min(w.s.len, past + tok_of(first) + 1) : w.s.len;
+    const int lim_any = last < first ? 0 : causal ? min(w.s.len, past + tok_of(last) + 1) : w.s.len;
     named_barrier_sync(1, NW * 32);
     uint32_t qf[WN][KSTEPS][2];
 #pragma unroll
@@ -746,9 +748,13 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
         if (threadIdx.x % TPR == 0) {
           const float lse2 = sum == 0.f ? -INFINITY : top + (log2f(sum) - kPOffset);
           const int64_t at = static_cast<int64_t>(w.s.first + my_tok) * p.heads_kv * p.group + my_head;
-          if (whole) p.lse[at] = lse2 * p.lse_unit;
-          else p.part_lse[part_row] = lse2;
-          if (p.level && w.tile0 == 0) p.where[at] = w.where(my_r);
+          if constexpr (LV) {
+            if (whole) p.lse[level_row(p, w.b) + at] = lse2;
+            if (w.tile0 == 0) p.where[level_row(p, w.b) + at] = w.where(my_r);
+          } else if (whole) {
+            p.lse[at] = lse2 * kLn2;
+          }
+          if (!whole) p.part_lse[part_row] = lse2;
         }
       }
       named_barrier_sync(1, NW * 32);
@@ -768,11 +774,12 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
           a.z += v.z;
           a.w += v.w;
         }
-        if (whole && p.level)
-          *reinterpret_cast<float4*>(
-              p.whole_o + (static_cast<int64_t>(w.s.first + my_tok) * p.heads_kv * p.group + my_head) * D + c0 + c) =
+        if constexpr (LV) {
+          const int64_t at =
+              level_row(p, w.b) + static_cast<int64_t>(w.s.first + my_tok) * p.heads_kv * p.group + my_head;
+          *reinterpret_cast<float4*>((whole ? p.whole_o + at * D : p.part_o + part_row * D) + c0 + c) =
               make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-        else if (whole)
+        } else if (whole)
           *reinterpret_cast<uint2*>(static_cast<T*>(p.o) +
                                     static_cast<int64_t>(w.s.first + my_tok) * p.o_stride[0] +
                                     my_head * p.o_stride[1] + c0 + c) =
@@ -792,7 +799,7 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
       ph ^= 1u;
     }
   }
-  level_end(p);
+  end(p);
 }
 
 }  // namespace fa

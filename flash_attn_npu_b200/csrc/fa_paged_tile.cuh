@@ -138,13 +138,14 @@ __device__ __forceinline__ void st_global_v8(void* to, const uint32_t* r) {
                : "memory");
 }
 
-template <typename T, int D, bool FP8>
+// LV: a call behind shared prefixes.
+template <typename T, int D, bool FP8, bool LV>
 __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ,
                       const __grid_constant__ CUtensorMap tmK,
-                      const __grid_constant__ CUtensorMap tmV, const PagedAttnParams p) {
+                      const __grid_constant__ CUtensorMap tmV, const PagedParams<LV> p) {
   using G = TileGeo<D, FP8>;
-  using Walk = PagedTileWalk<G::TILES, G::KEYS>;
+  using Walk = PagedTileWalk<G::TILES, G::KEYS, PagedParams<LV>>;
   using Sh = TileShared<G::STAGES, Walk>;
   static_assert(sizeof(Sh) <= 5120, "barrier block");
   constexpr int TILES = G::TILES, KEYS = G::KEYS, STAGES = G::STAGES;
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
   const int lane = threadIdx.x & 31;
   int* const status = p.seqs.status;
 
-  level_begin_before_sync(p);
+  begin_early(p);
   if (threadIdx.x == 32) {
     prefetch_map(&tmQ);
     prefetch_map(&tmK);
@@ -207,11 +208,11 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  level_begin(p);
+  begin(p);
   if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
   if (warp == 0) {
     const PagedRange r =
-        paged_range(p, [&](int b) { return PagedTiles<TILES, KEYS>(p, b).steps(p); });
+        paged_range(p, [&](int b) { return PagedTiles<TILES, KEYS, PagedParams<LV>>(p, b).steps(p); });
     if (lane == 0) {
       sh->range = r;
       Walk x(p, r);
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
         // the page of this lane's copies for a tile: its entry is fetched one tile ahead
         const int tile1 = my_box < boxes ? min(w.tile1, (w.s.len - my_box * box + KEYS - 1) / KEYS) : 0;
         auto fetch = [&](int t) -> int {
-          return t < tile1 ? page_entry(p.seqs, w.b, t * KEYS + my_box * box) : 0;
+          return t < tile1 ? page_entry(seqs_of_line(p, w.b), seq_of_line(p, w.b), t * KEYS + my_box * box) : 0;
         };
         int entry = fetch(w.tile0);
         // The warps load a query tile each.
@@ -340,10 +341,12 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
             }
           }
         }
-        if (pw == 0 && lane == 0 &&
-            (fresh(p.seqs.kv_lens + w.b) != w.s.len ||
-             fresh(p.seqs.offsets + w.b + 1) - fresh(p.seqs.offsets + w.b) != w.s.count))
-          report(status, kStatusPageTable);
+        if (pw == 0 && lane == 0) {
+          const PagedSeqs& from = seqs_of_line(p, w.b);
+          const int b = seq_of_line(p, w.b);
+          if (fresh(from.kv_lens + b) != w.s.len || fresh(from.offsets + b + 1) - fresh(from.offsets + b) != w.s.count)
+            report(status, kStatusPageTable);
+        }
       }
       meet(pw, issued);
       // the copies issued last land before shared memory goes away
@@ -717,8 +720,8 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
           continue;
         }
         const int past = w.s.len - w.s.count;
-        const int lim = p.causal ? min(w.s.len, past + tok + 1) : w.s.len;  // keys of this row
-        const int lim_all = p.causal ? min(w.s.len, past + w.tok0(p, tile) + 1) : w.s.len;
+        const int lim = w.s.causal(p) ? min(w.s.len, past + tok + 1) : w.s.len;  // keys of this row
+        const int lim_all = w.s.causal(p) ? min(w.s.len, past + w.tok0(p, tile) + 1) : w.s.len;
         const int key_first = (w.tile0 + first) * KEYS;
         float m = -INFINITY;  // the row's base, log2 units
         float l = 0.f;
@@ -816,13 +819,20 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
         if (live && ok && (i == 0 || !paired)) {
           const float lse2 = l == 0.f ? -INFINITY : m + (log2f(l) - kPOffset);
           const int64_t at = row * (p.heads_kv * p.group) + head;
-          if (whole) p.lse[at] = lse2 * p.lse_unit;
-          else p.part_lse[part_row] = lse2;
-          if (p.level && w.tile0 == 0) p.where[at] = w.where(range, p.item_cost, tile * 128 + r);
+          if constexpr (LV) {
+            if (whole) p.lse[level_row(p, w.b) + at] = lse2;
+            if (w.tile0 == 0) p.where[level_row(p, w.b) + at] = w.where(range, p.item_cost, tile * 128 + r);
+          } else if (whole) {
+            p.lse[at] = lse2 * kLn2;
+          }
+          if (!whole) p.part_lse[part_row] = lse2;
         }
         T* out = static_cast<T*>(p.o) + row * p.o_stride[0] + head * p.o_stride[1];
-        const bool last = whole && p.level == 0;  // the row is finished here
-        float* part = whole ? p.whole_o + (row * (p.heads_kv * p.group) + head) * D : p.part_o + part_row * D;
+        const bool last = whole && !LV;  // the row is finished here
+        float* part = p.part_o + part_row * D;
+        if constexpr (LV) {
+          if (whole) part = p.whole_o + (level_row(p, w.b) + row * (p.heads_kv * p.group) + head) * D;
+        }
         const uint32_t tO_other = tmem + lane_off + G::TMEM_O + (i ^ 1) * D;
         // (a pair's sides write every other 16 columns)
 #pragma unroll 1
@@ -884,7 +894,7 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  level_end(p);
+  end(p);
 }
 
 }  // namespace fa
