@@ -238,6 +238,17 @@ def paged_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, pr
     return out
 
 
+def paged_cache_evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale=None,
+                      v_scale=None, to_table=None, return_kept=False):
+    """Cut sequences to `keep` tokens a kv head, by the attention weight that each token received;
+    their new lengths."""
+    new_lens, kept = _paged.evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale,
+                                  v_scale, to_table)
+    if return_kept:
+        return new_lens, kept
+    return new_lens
+
+
 # ----------------------------------------------------------------------------- profiling
 def profile_once(z, h, n_ctx, head_dim, causal, q, k, v, sm_scale):
     out = attention(q, k, v, causal, sm_scale)
@@ -456,6 +467,7 @@ __all__ = [
     "attention",
     "paged_attention",
     "paged_cache_empty",
+    "paged_cache_evict",
     "paged_cache_read",
     "paged_cache_write",
     "paged_prefix_attention",

@@ -50,6 +50,7 @@ EXPORTED_SYMBOLS = (
     "fa_paged_workspace_bytes",
     "fa_paged_prefix_sm100",
     "fa_paged_prefix_workspace_bytes",
+    "fa_paged_evict_sm100",
 )
 
 
@@ -190,7 +191,7 @@ def load() -> ctypes.CDLL:
         lib.fa_fwd_sm100_grid_size.argtypes = [ctypes.POINTER(FaFwdArgs)]
         lib.fa_fwd_sm100_grid_size.restype = ctypes.c_int64
         for name in ("fa_paged_write_sm100", "fa_paged_read_sm100", "fa_paged_attn_sm100",
-                     "fa_paged_prefix_sm100"):
+                     "fa_paged_prefix_sm100", "fa_paged_evict_sm100"):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
             fn.restype = ctypes.c_int

@@ -49,6 +49,7 @@ SOURCES = [
     "fa_fwd_d256.cu",
     "fa_paged_api.cu",
     "fa_paged_cache.cu",
+    "fa_paged_evict.cu",
     "fa_paged_prefix.cu",
     "fa_paged_rows_d16.cu",
     "fa_paged_rows_d32.cu",

@@ -28,6 +28,7 @@ int (*g_read)(const FaPagedCopyArgs*, void*) = nullptr;
 int64_t (*g_workspace)(const FaPagedAttnArgs*) = nullptr;
 int (*g_prefix)(const FaPagedPrefixArgs*, void*) = nullptr;
 int64_t (*g_prefix_workspace)(const FaPagedPrefixArgs*) = nullptr;
+int (*g_evict)(const FaPagedEvictArgs*, void*) = nullptr;
 
 constexpr int kDevices = 64;
 // Devices that paged.py has prepared, and their status words.
@@ -78,21 +79,28 @@ struct CacheArgs {
   PyObject *k, *v, *table, *offsets, *lens, *k_scale, *v_scale;
 };
 
-// The sequences of a cache on device `index`; false if they are not in order.
+bool ints(const Tensor* t, int index) {
+  return t && plain(*t, index) && t->scalar_type() == at::kInt;
+}
+
+// The sequences of a cache on device `index` (a call without packed rows has no offsets: null); false if
+// they are not in order.
 bool fill_seqs(const CacheArgs& a, FaPagedCache& c, int index) {
-  const Tensor *table = tensor_of(a.table), *offsets = tensor_of(a.offsets), *lens = tensor_of(a.lens);
-  if (!table || !offsets || !lens) return false;
-  for (const Tensor* t : {table, offsets, lens})
-    if (!plain(*t, index) || t->scalar_type() != at::kInt) return false;
-  if (table->dim() != 2 || offsets->dim() != 1 || lens->dim() != 1) return false;
+  const Tensor *table = tensor_of(a.table), *lens = tensor_of(a.lens);
+  if (!ints(table, index) || !ints(lens, index) || table->dim() != 2 || lens->dim() != 1) return false;
   c.seqs = table->size(0);
   c.table_cols = table->size(1);
-  if (offsets->size(0) != c.seqs + 1 || lens->size(0) != c.seqs || !offsets->is_contiguous() ||
-      !lens->is_contiguous() || (c.table_cols > 1 && table->stride(1) != 1))
+  if (lens->size(0) != c.seqs || !lens->is_contiguous() || (c.table_cols > 1 && table->stride(1) != 1))
     return false;
+  if (a.offsets) {
+    const Tensor* offsets = tensor_of(a.offsets);
+    if (!ints(offsets, index) || offsets->dim() != 1 || offsets->size(0) != c.seqs + 1 ||
+        !offsets->is_contiguous())
+      return false;
+    c.offsets = static_cast<const int32_t*>(offsets->const_data_ptr());
+  }
   c.table_stride = c.seqs > 1 ? table->stride(0) : c.table_cols;
   c.page_table = static_cast<const int32_t*>(table->const_data_ptr());
-  c.offsets = static_cast<const int32_t*>(offsets->const_data_ptr());
   c.kv_lens = static_cast<const int32_t*>(lens->const_data_ptr());
   return true;
 }
@@ -361,6 +369,62 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// One float for each (page, head, row) of the cache.
+bool per_token(const Tensor* t, const Tensor& cache, int index) {
+  return t && plain(*t, index) && t->scalar_type() == at::kFloat &&
+         t->sizes() == cache.sizes().slice(0, 3) && aligned(*t);
+}
+
+// evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale, v_scale, to_table)
+//   -> (new_lens, kept), a status code, or None
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10 || !PyLong_Check(a[5]) || !PyLong_Check(a[6])) return none();
+  FaPagedEvictArgs x{};
+  x.struct_size = sizeof(x);
+  int index = -1;
+  if (!fill_cache({a[0], a[1], a[3], nullptr, a[4], a[7], a[8]}, x.cache, index)) return none();
+  const Tensor& cache = *tensor_of(a[0]);
+  const Tensor* weights = tensor_of(a[2]);
+  if (!per_token(weights, cache, index)) return none();
+  x.keep = PyLong_AsLongLong(a[5]);
+  x.recent = PyLong_AsLongLong(a[6]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  if (x.keep < 0 || x.keep > (1 << 30) || x.recent < 0 || x.recent > x.keep) return none();
+  x.in_place = a[9] == Py_None;
+  if (!x.in_place) {
+    const Tensor* to = tensor_of(a[9]);
+    if (!ints(to, index) || to->dim() != 2 || to->size(0) != x.cache.seqs ||
+        (to->size(1) > 1 && to->stride(1) != 1))
+      return none();
+    x.to_cols = to->size(1);
+    x.to_stride = x.cache.seqs > 1 ? to->stride(0) : x.to_cols;
+    x.to_table = static_cast<const int32_t*>(to->const_data_ptr());
+  }
+  const c10::cuda::OptionalCUDAGuard guard(cache.device());
+  const auto options = cache.options().dtype(at::kInt);
+  Tensor lens = at::empty({x.cache.seqs}, options);
+  Tensor kept = at::empty({x.cache.seqs, x.cache.heads_kv, x.keep}, options);
+  strides(*weights, x.weights_stride);
+  x.weights = static_cast<float*>(const_cast<void*>(weights->const_data_ptr()));
+  x.new_lens = static_cast<int32_t*>(lens.mutable_data_ptr());
+  x.kept = static_cast<int32_t*>(kept.mutable_data_ptr());
+  x.dev_status = g_status[index];
+  const int rc = g_evict(&x, c10::cuda::getCurrentCUDAStream(index).stream());
+  if (rc != FA_OK) return PyLong_FromLong(rc);
+  for (int i : {0, 1, 2, 7, 8})
+    if (a[i] != Py_None) written(*tensor_of(a[i]));
+  PyObject* r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(lens)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(kept)));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
 // setup(attention, workspace_bytes, write, read): addresses of the C ABI
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   constexpr int kCalls = 4;
@@ -377,9 +441,9 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyBool_FromLong(1);
 }
 
-// setup_more(prefix attention, its workspace_bytes): those of the other calls
+// setup_more(prefix attention, its workspace_bytes, evict): those of the other calls
 PyObject* setup_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  constexpr int kCalls = 2;
+  constexpr int kCalls = 3;
   void* p[kCalls];
   if (n != kCalls) return none();
   for (int i = 0; i < kCalls; ++i) {
@@ -388,6 +452,7 @@ PyObject* setup_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   g_prefix = reinterpret_cast<decltype(g_prefix)>(p[0]);
   g_prefix_workspace = reinterpret_cast<decltype(g_prefix_workspace)>(p[1]);
+  g_evict = reinterpret_cast<decltype(g_evict)>(p[2]);
   return PyBool_FromLong(1);
 }
 
@@ -407,6 +472,7 @@ PyObject* set_status(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attention)), METH_FASTCALL, nullptr},
     {"prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(prefix_attention)), METH_FASTCALL, nullptr},
+    {"evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(evict)), METH_FASTCALL, nullptr},
     {"read_new", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(read_new)), METH_FASTCALL, nullptr},
     {"copy", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(copy)), METH_FASTCALL, nullptr},
     {"setup", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(setup)), METH_FASTCALL, nullptr},

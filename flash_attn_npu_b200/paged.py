@@ -55,7 +55,8 @@ def empty_cache(num_pages: int, page_size: int, heads_kv: int, head_dim: int, dt
 
 # ------------------------------------------------------------------------------------- checks
 def validate_cache(k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale) -> None:
-    """Shapes, types and layout of a cache and its sequences, on tensors of any device."""
+    """Shapes, types and layout of a cache and its sequences, on tensors of any device (`offsets` None:
+    a call without packed rows)."""
     if k_cache.ndim != 4 or k_cache.shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must have the same shape [num_pages, heads_kv, "
                          "page_size, head_dim]")
@@ -95,6 +96,8 @@ def validate_sequences(page_table, offsets, kv_lens, page_size,
                        names=("page_table", "offsets", "kv_lens"), rows="seqs") -> None:
     """Shapes, types and layout of a page table and what goes with it."""
     table, offs, lens = names
+    if offsets is None:
+        offsets = kv_lens.new_empty(kv_lens.shape[0] + 1 if kv_lens.ndim == 1 else 0, dtype=torch.int32)
     if (page_table.ndim != 2 or offsets.ndim != 1 or kv_lens.ndim != 1
             or offsets.shape[0] != page_table.shape[0] + 1
             or kv_lens.shape[0] != page_table.shape[0]):
@@ -151,6 +154,37 @@ def validate_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets,
         raise ValueError("a cache, its scales and its sequences must not be negated views")
     if max_prefix_q_len is not None and max_prefix_q_len < 0:
         raise ValueError("max_prefix_q_len must not be negative")
+
+
+def _validate_weights(weights, k_cache) -> None:
+    if weights.shape != k_cache.shape[:3] or weights.dtype != torch.float32:
+        raise ValueError("weights must be float32 [num_pages, heads_kv, page_size]")
+    if not _aligned(weights):
+        raise ValueError("weights needs a unit inner stride and 16-byte aligned strides")
+    if weights.device != k_cache.device:
+        raise ValueError("all tensors of a paged call must be on the same device")
+    if weights.is_neg():
+        raise ValueError("weights must not be a negated view")
+
+
+def validate_evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale=None, v_scale=None,
+                   to_table=None) -> None:
+    """The rules of `evict`, on tensors of any device."""
+    validate_cache(k_cache, v_cache, page_table, None, kv_lens, k_scale, v_scale)
+    _validate_weights(weights, k_cache)
+    if not 0 <= recent <= keep <= 1 << 30:
+        raise ValueError("keep and recent must be 0 <= recent <= keep <= 2^30")
+    if to_table is not None:
+        if to_table.ndim != 2 or to_table.shape[0] != page_table.shape[0] or to_table.dtype != torch.int32:
+            raise ValueError("to_table must be int32 [seqs, columns]")
+        if to_table.shape[1] > 1 and to_table.stride(1) != 1:
+            raise ValueError("the rows of to_table must be contiguous")
+        if to_table.shape[1] * k_cache.shape[2] > 1 << 30:
+            raise ValueError("to_table names more than 2^30 positions a sequence")
+        if to_table.device != k_cache.device:
+            raise ValueError("all tensors of a paged call must be on the same device")
+        if to_table.is_neg():
+            raise ValueError("a cache, its scales and its sequences must not be negated views")
 
 
 def validate_copy(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale=None,
@@ -211,7 +245,7 @@ def _native_binding():
             lib.fa_paged_attn_sm100, lib.fa_paged_workspace_bytes, lib.fa_paged_write_sm100,
             lib.fa_paged_read_sm100))
         _paged_binding.setup_more(*addresses(
-            lib.fa_paged_prefix_sm100, lib.fa_paged_prefix_workspace_bytes))
+            lib.fa_paged_prefix_sm100, lib.fa_paged_prefix_workspace_bytes, lib.fa_paged_evict_sm100))
         _binding = _paged_binding
     return _binding
 
@@ -260,6 +294,13 @@ def _max_len(n, name="max_q_len"):
     except TypeError:
         raise ValueError(f"{name} must be an integer or None (got {n!r})") from None
     return min(n, 1 << 30)  # (there are no more rows)
+
+
+def _count(n, name) -> int:
+    try:
+        return operator.index(n)
+    except TypeError:
+        raise ValueError(f"{name} must be an integer (got {n!r})") from None
 
 
 def _scale(x) -> float:
@@ -420,3 +461,34 @@ def read(k_cache, v_cache, page_table, offsets, kv_lens, total, k_scale=None, v_
             raise ValueError("out needs a unit inner stride and 16-byte aligned strides")
     _copy(False, k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale)
     return k, v
+
+
+def evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale=None, v_scale=None,
+          to_table=None):
+    """Cut long sequences to `keep` tokens by the attention weight that each received; (new_lens, kept).
+
+    `weights` [num_pages, heads_kv, page_size] float32 is what `attention_weights` accumulates.  Of a
+    sequence longer than `keep` each kv head keeps its last `recent` tokens and, of the others, the
+    keep - recent with the largest weights (of equal ones the earlier; NaN counts as the largest).  They
+    keep their order and move to positions 0 .. keep - 1, with their scales and weights: in place, or into
+    the pages of `to_table` [seqs, columns], which also receive the sequences that are not longer, and must
+    not be among those of `page_table`.  What lies behind the new length is left as it was.  Pages that
+    receive tokens must not belong to another sequence too (a shared prefix among them).
+
+    new_lens [seqs] int32 is min(kv_lens, keep); kept [seqs, heads_kv, keep] int32 the positions that
+    stayed, -1 behind them.  Both stay on the device, and nothing waits for it.
+    """
+    res = None
+    if _binding is not None:
+        res = _binding.evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale, v_scale,
+                             to_table)
+    if res is None:
+        keep, recent = _count(keep, "keep"), _count(recent, "recent")
+        validate_evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale, v_scale,
+                       to_table)
+        _require_cuda(k_cache)
+        res = _call("evict", k_cache.device, k_cache, v_cache, weights, page_table, kv_lens, keep, recent,
+                    k_scale, v_scale, to_table)
+    if type(res) is int or ops._CHECK_EVERY_CALL:
+        _check(res, k_cache.device)
+    return res

@@ -123,3 +123,20 @@ def _paged_cache_read_fake(k_cache, v_cache, page_table, offsets, kv_lens, total
     v = torch.empty_like(k)
     paged.validate_copy(k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale)
     return k, v
+
+
+@torch.library.custom_op("flash_attn_b200::paged_cache_evict",
+                         mutates_args=("k_cache", "v_cache", "weights", "k_scale", "v_scale"))
+def paged_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor,
+                      page_table: torch.Tensor, kv_lens: torch.Tensor, keep: int, recent: int,
+                      k_scale: torch.Tensor | None, v_scale: torch.Tensor | None,
+                      to_table: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    return paged.evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale, v_scale, to_table)
+
+
+@paged_cache_evict.register_fake
+def _paged_cache_evict_fake(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale, v_scale,
+                            to_table=None):
+    paged.validate_evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale, v_scale, to_table)
+    seqs = page_table.shape[0]
+    return (kv_lens.new_empty((seqs,)), kv_lens.new_empty((seqs, k_cache.shape[1], keep)))

@@ -142,6 +142,32 @@ FA_API int fa_paged_prefix_sm100(const FaPagedPrefixArgs* args, void* stream);
 /* Its workspace, as fa_paged_workspace_bytes. */
 FA_API int64_t fa_paged_prefix_workspace_bytes(const FaPagedPrefixArgs* args);
 
+/* Eviction by accumulated attention weight, per sequence and kv head.  `weights` [num_pages, heads_kv,
+ * page_size] has one float for each (token, kv head) of the cache.  The offsets of `cache` are not read. */
+typedef struct FaPagedEvictArgs {
+  int32_t struct_size;     /* sizeof(FaPagedEvictArgs) */
+  float* weights;          /* moved along with the tokens */
+  int32_t* new_lens;       /* [seqs]: min(kv_lens, keep) */
+  int32_t* kept;           /* [seqs, heads_kv, keep]: the positions that stay, in order, -1 behind them */
+  int32_t* dev_status;     /* optional device int, 0 on success */
+  FaPagedCache cache;
+  int64_t weights_stride[2]; /* element strides of (page, head); multiples of 16 bytes */
+  const int32_t* to_table;   /* [seqs, to_cols]: pages that receive what stays, unless in_place */
+  int64_t to_stride;
+  int64_t to_cols;
+  int64_t keep;     /* tokens that stay of a longer sequence */
+  int64_t recent;   /* the last ones, which stay whatever their weight; at most keep */
+  int32_t in_place; /* what stays goes to the front of the sequence's own pages */
+} FaPagedEvictArgs;
+
+/* Of each sequence longer than `keep` every kv head keeps its last `recent` tokens and, of the others, the
+ * keep - recent with the largest weights: of equal ones the earlier, and NaN before all.  They keep their
+ * order and go to positions 0 .. keep - 1, in K, V, the scales of a float8 cache and the weights.  What
+ * lies behind the new length is left as it was.  Shorter sequences stay as they are (not in place: they
+ * are copied).  Pages that receive tokens must not belong to another sequence too; those of to_table must
+ * not be among those of page_table. */
+FA_API int fa_paged_evict_sm100(const FaPagedEvictArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
