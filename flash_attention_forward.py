@@ -238,6 +238,9 @@ def paged_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_offsets, pr
     return out
 
 
+paged_attention_weights = _paged.attention_weights
+
+
 def paged_cache_evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale=None,
                       v_scale=None, to_table=None, return_kept=False):
     """Cut sequences to `keep` tokens a kv head, by the attention weight that each token received;
@@ -466,6 +469,7 @@ __all__ = [
     "get_tile_config",
     "attention",
     "paged_attention",
+    "paged_attention_weights",
     "paged_cache_empty",
     "paged_cache_evict",
     "paged_cache_read",

@@ -50,6 +50,8 @@ EXPORTED_SYMBOLS = (
     "fa_paged_workspace_bytes",
     "fa_paged_prefix_sm100",
     "fa_paged_prefix_workspace_bytes",
+    "fa_paged_weights_sm100",
+    "fa_paged_weights_workspace_bytes",
     "fa_paged_evict_sm100",
 )
 
@@ -191,11 +193,12 @@ def load() -> ctypes.CDLL:
         lib.fa_fwd_sm100_grid_size.argtypes = [ctypes.POINTER(FaFwdArgs)]
         lib.fa_fwd_sm100_grid_size.restype = ctypes.c_int64
         for name in ("fa_paged_write_sm100", "fa_paged_read_sm100", "fa_paged_attn_sm100",
-                     "fa_paged_prefix_sm100", "fa_paged_evict_sm100"):
+                     "fa_paged_prefix_sm100", "fa_paged_weights_sm100", "fa_paged_evict_sm100"):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
             fn.restype = ctypes.c_int
-        for name in ("fa_paged_workspace_bytes", "fa_paged_prefix_workspace_bytes"):
+        for name in ("fa_paged_workspace_bytes", "fa_paged_prefix_workspace_bytes",
+                     "fa_paged_weights_workspace_bytes"):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.c_void_p]
             fn.restype = ctypes.c_int64

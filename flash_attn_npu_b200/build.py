@@ -50,6 +50,12 @@ SOURCES = [
     "fa_paged_api.cu",
     "fa_paged_cache.cu",
     "fa_paged_evict.cu",
+    "fa_paged_weights.cu",
+    "fa_paged_weights_d16.cu",
+    "fa_paged_weights_d32.cu",
+    "fa_paged_weights_d64.cu",
+    "fa_paged_weights_d128.cu",
+    "fa_paged_weights_d256.cu",
     "fa_paged_prefix.cu",
     "fa_paged_rows_d16.cu",
     "fa_paged_rows_d32.cu",

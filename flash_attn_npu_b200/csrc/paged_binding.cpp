@@ -28,6 +28,8 @@ int (*g_read)(const FaPagedCopyArgs*, void*) = nullptr;
 int64_t (*g_workspace)(const FaPagedAttnArgs*) = nullptr;
 int (*g_prefix)(const FaPagedPrefixArgs*, void*) = nullptr;
 int64_t (*g_prefix_workspace)(const FaPagedPrefixArgs*) = nullptr;
+int (*g_weights)(const FaPagedWeightsArgs*, void*) = nullptr;
+int64_t (*g_weights_workspace)(const FaPagedWeightsArgs*) = nullptr;
 int (*g_evict)(const FaPagedEvictArgs*, void*) = nullptr;
 
 constexpr int kDevices = 64;
@@ -375,6 +377,52 @@ bool per_token(const Tensor* t, const Tensor& cache, int index) {
          t->sizes() == cache.sizes().slice(0, 3) && aligned(*t);
 }
 
+// weights(q, lse, k_cache, page_table, offsets, kv_lens, weights, causal, sm_scale, k_scale, max_q_len,
+//         reset_new) -> status code, or None
+PyObject* weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12) return none();
+  FaPagedAttnArgs y{};
+  int index = -1;
+  const Tensor *q = tensor_of(a[0]), *lse = tensor_of(a[1]), *out = tensor_of(a[6]);
+  // (there are no values: the keys stand for them)
+  if (!fill_attention(q, {a[2], a[2], a[3], a[4], a[5], a[9], a[9]}, a[7], a[8], a[10], y, index) ||
+      !per_token(out, *tensor_of(a[2]), index))
+    return none();
+  if (!lse || !plain(*lse, index) || lse->dim() != 2 || lse->size(0) != y.total || lse->size(1) != y.heads_q ||
+      lse->scalar_type() != at::kFloat || !lse->is_contiguous())
+    return none();
+  FaPagedWeightsArgs x{};
+  x.struct_size = sizeof(x);
+  x.q = q->const_data_ptr();
+  x.lse = static_cast<const float*>(lse->const_data_ptr());
+  x.weights = static_cast<float*>(const_cast<void*>(out->const_data_ptr()));
+  x.dev_status = g_status[index];
+  x.cache = y.cache;
+  strides(*q, x.q_stride);
+  strides(*out, x.weights_stride);
+  x.total = y.total;
+  x.heads_q = y.heads_q;
+  x.max_q_len = y.max_q_len;
+  x.dtype = y.dtype;
+  x.causal = y.causal;
+  x.reset_new = a[11] == Py_True;
+  x.sm_scale = y.sm_scale;
+  if (x.total > 0 && x.cache.seqs > 0) {
+    const c10::cuda::OptionalCUDAGuard guard(q->device());
+    x.workspace_bytes = g_weights_workspace(&x);
+    if (x.workspace_bytes < 0) return none();
+    const c10::DataPtr workspace =
+        c10::cuda::CUDACachingAllocator::get()->allocate(x.workspace_bytes);
+    x.workspace = workspace.get();
+    const int rc = g_weights(&x, c10::cuda::getCurrentCUDAStream(index).stream());
+    if (rc != FA_OK) return PyLong_FromLong(rc);
+    written(*out);
+  }
+  return PyLong_FromLong(FA_OK);
+  END_HANDLE_TH_ERRORS
+}
+
 // evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale, v_scale, to_table)
 //   -> (new_lens, kept), a status code, or None
 PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -441,9 +489,10 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyBool_FromLong(1);
 }
 
-// setup_more(prefix attention, its workspace_bytes, evict): those of the other calls
+// setup_more(prefix attention, its workspace_bytes, weights, its workspace_bytes, evict): those of the
+// other calls
 PyObject* setup_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  constexpr int kCalls = 3;
+  constexpr int kCalls = 5;
   void* p[kCalls];
   if (n != kCalls) return none();
   for (int i = 0; i < kCalls; ++i) {
@@ -452,7 +501,9 @@ PyObject* setup_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   g_prefix = reinterpret_cast<decltype(g_prefix)>(p[0]);
   g_prefix_workspace = reinterpret_cast<decltype(g_prefix_workspace)>(p[1]);
-  g_evict = reinterpret_cast<decltype(g_evict)>(p[2]);
+  g_weights = reinterpret_cast<decltype(g_weights)>(p[2]);
+  g_weights_workspace = reinterpret_cast<decltype(g_weights_workspace)>(p[3]);
+  g_evict = reinterpret_cast<decltype(g_evict)>(p[4]);
   return PyBool_FromLong(1);
 }
 
@@ -472,6 +523,7 @@ PyObject* set_status(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(attention)), METH_FASTCALL, nullptr},
     {"prefix_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(prefix_attention)), METH_FASTCALL, nullptr},
+    {"weights", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(weights)), METH_FASTCALL, nullptr},
     {"evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(evict)), METH_FASTCALL, nullptr},
     {"read_new", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(read_new)), METH_FASTCALL, nullptr},
     {"copy", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(copy)), METH_FASTCALL, nullptr},

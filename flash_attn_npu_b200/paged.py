@@ -167,6 +167,17 @@ def _validate_weights(weights, k_cache) -> None:
         raise ValueError("weights must not be a negated view")
 
 
+def validate_attention_weights(q, lse, k_cache, page_table, offsets, kv_lens, weights, k_scale=None,
+                               max_q_len=None) -> None:
+    """The rules of `attention_weights`, on tensors of any device."""
+    if (k_scale is None) == (k_cache.dtype == FP8):
+        raise ValueError("k_scale goes with a float8_e4m3fn cache, and with no other")
+    validate_attention(q, k_cache, k_cache, page_table, offsets, kv_lens, k_scale, k_scale, max_q_len)
+    _validate_weights(weights, k_cache)
+    if lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != q.device:
+        raise ValueError("lse must be float32 [total, heads_q]")
+
+
 def validate_evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale=None, v_scale=None,
                    to_table=None) -> None:
     """The rules of `evict`, on tensors of any device."""
@@ -245,7 +256,8 @@ def _native_binding():
             lib.fa_paged_attn_sm100, lib.fa_paged_workspace_bytes, lib.fa_paged_write_sm100,
             lib.fa_paged_read_sm100))
         _paged_binding.setup_more(*addresses(
-            lib.fa_paged_prefix_sm100, lib.fa_paged_prefix_workspace_bytes, lib.fa_paged_evict_sm100))
+            lib.fa_paged_prefix_sm100, lib.fa_paged_prefix_workspace_bytes, lib.fa_paged_weights_sm100,
+            lib.fa_paged_weights_workspace_bytes, lib.fa_paged_evict_sm100))
         _binding = _paged_binding
     return _binding
 
@@ -461,6 +473,37 @@ def read(k_cache, v_cache, page_table, offsets, kv_lens, total, k_scale=None, v_
             raise ValueError("out needs a unit inner stride and 16-byte aligned strides")
     _copy(False, k, v, k_cache, v_cache, page_table, offsets, kv_lens, k_scale, v_scale)
     return k, v
+
+
+def attention_weights(q, lse, k_cache, page_table, offsets, kv_lens, weights, causal, sm_scale, k_scale=None,
+                      max_q_len=None, reset_new=True) -> None:
+    """Add the attention weight that each cached token gets from these rows to `weights`, in place.
+
+    `weights` [num_pages, heads_kv, page_size] float32, a number for each (token, kv head) of the cache,
+    grows by the sum of the probabilities exp(sm_scale q k - lse) of all rows and query heads that attend to
+    it: `q`, `causal`, `sm_scale` and the sequences are those of the attention call that `lse` [total,
+    heads_q] float32 comes from.  With `reset_new` the places of the sequences' new tokens (the last
+    offsets[b + 1] - offsets[b]) start from 0, so pages need no clearing.  Rows with lse = -inf give nothing.
+
+    With the joint `lse` of `prefix_attention`, one call over the sequences' own tokens, and one over the
+    prefixes (prefix_table, prefix_offsets, prefix_lens, causal=False, reset_new=False) give the weights of
+    both.  Pages that get weight must not belong to two sequences of a call.  What a key or row holds shows
+    in its own weight only, and in those that a row attends to.
+    """
+    res = None
+    if _binding is not None:
+        res = _binding.weights(q, lse, k_cache, page_table, offsets, kv_lens, weights, causal, sm_scale, k_scale,
+                               max_q_len, bool(reset_new))
+    if res is None:
+        sm_scale, max_q_len = _scale(sm_scale), _max_len(max_q_len)
+        validate_attention_weights(q, lse, k_cache, page_table, offsets, kv_lens, weights, k_scale, max_q_len)
+        _require_cuda(q)
+        if not lse.is_contiguous() or lse.is_neg():
+            lse = torch.empty_like(lse, memory_format=torch.contiguous_format).copy_(lse.detach())
+        res = _call("weights", q.device, _rows_like(q), lse, k_cache, page_table, offsets, kv_lens, weights,
+                    bool(causal), sm_scale, k_scale, max_q_len, bool(reset_new))
+    if res != _native.FA_OK or ops._CHECK_EVERY_CALL:
+        _check(res, q.device)
 
 
 def evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale=None, v_scale=None,

@@ -140,3 +140,18 @@ def _paged_cache_evict_fake(k_cache, v_cache, weights, page_table, kv_lens, keep
     paged.validate_evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale, v_scale, to_table)
     seqs = page_table.shape[0]
     return (kv_lens.new_empty((seqs,)), kv_lens.new_empty((seqs, k_cache.shape[1], keep)))
+
+
+@torch.library.custom_op("flash_attn_b200::paged_attention_weights", mutates_args=("weights",))
+def paged_attention_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, page_table: torch.Tensor,
+                            offsets: torch.Tensor, kv_lens: torch.Tensor, weights: torch.Tensor, causal: bool,
+                            sm_scale: float, k_scale: torch.Tensor | None = None, max_q_len: int | None = None,
+                            reset_new: bool = True) -> None:
+    paged.attention_weights(q, lse, k_cache, page_table, offsets, kv_lens, weights, causal, sm_scale, k_scale,
+                            max_q_len, reset_new)
+
+
+@paged_attention_weights.register_fake
+def _paged_attention_weights_fake(q, lse, k_cache, page_table, offsets, kv_lens, weights, causal, sm_scale,
+                                  k_scale=None, max_q_len=None, reset_new=True):
+    paged.validate_attention_weights(q, lse, k_cache, page_table, offsets, kv_lens, weights, k_scale, max_q_len)

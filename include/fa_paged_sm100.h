@@ -142,6 +142,37 @@ FA_API int fa_paged_prefix_sm100(const FaPagedPrefixArgs* args, void* stream);
 /* Its workspace, as fa_paged_workspace_bytes. */
 FA_API int64_t fa_paged_prefix_workspace_bytes(const FaPagedPrefixArgs* args);
 
+/* The attention weight that cached tokens received.  `weights` [num_pages, heads_kv, page_size] has one
+ * float for each (token, kv head) of the cache.  The values of `cache` (v, v_scale) are not read. */
+typedef struct FaPagedWeightsArgs {
+  int32_t struct_size;     /* sizeof(FaPagedWeightsArgs) */
+  const void* q;           /* [total, heads_q, head_dim] */
+  const float* lse;        /* [total, heads_q], contiguous: what the attention call over these rows left */
+  float* weights;
+  void* workspace;         /* fa_paged_weights_workspace_bytes() bytes, 256-byte aligned; needs no clearing */
+  int32_t* dev_status;     /* optional device int, 0 on success */
+  FaPagedCache cache;
+  int64_t q_stride[2];       /* element strides of (row, head); multiples of 16 bytes */
+  int64_t weights_stride[2]; /* element strides of (page, head); multiples of 16 bytes */
+  int64_t total;
+  int64_t heads_q;   /* a multiple of heads_kv */
+  int64_t max_q_len; /* upper bound of a sequence's new tokens that the tiling goes by (0: total); a longer
+                        sequence is computed all the same */
+  int64_t workspace_bytes;
+  int32_t dtype;     /* of q: the cache's own, or fp16 / bf16 with a float8 cache */
+  int32_t causal;    /* a token gives weight to positions up to its own; 0: to the whole sequence */
+  int32_t reset_new; /* the weights of the sequences' new tokens start from 0 */
+  float sm_scale;
+} FaPagedWeightsArgs;
+
+/* For each sequence, kv head and position: weights += the sum of exp(sm_scale q k - lse) over the rows
+ * that attend to it and share the head.  A row with lse = -inf gives nothing.  Sequences with new tokens
+ * only; pages must not belong to two sequences of a call. */
+FA_API int fa_paged_weights_sm100(const FaPagedWeightsArgs* args, void* stream);
+
+/* Its workspace, as fa_paged_workspace_bytes. */
+FA_API int64_t fa_paged_weights_workspace_bytes(const FaPagedWeightsArgs* args);
+
 /* Eviction by accumulated attention weight, per sequence and kv head.  `weights` [num_pages, heads_kv,
  * page_size] has one float for each (token, kv head) of the cache.  The offsets of `cache` are not read. */
 typedef struct FaPagedEvictArgs {
