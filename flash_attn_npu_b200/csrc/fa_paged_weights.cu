@@ -40,6 +40,12 @@ int check_weights(const FaPagedWeightsArgs* a) {
   return FA_OK;
 }
 
+int query_rows(int64_t head_dim, bool fp8) {
+  if (head_dim <= 64) return WeightsGeo<64, false>::QN;
+  if (head_dim == 128) return fp8 ? WeightsGeo<128, true>::QN : WeightsGeo<128, false>::QN;
+  return fp8 ? WeightsGeo<256, true>::QN : WeightsGeo<256, false>::QN;
+}
+
 struct WeightsChoice {
   int grid;
   int64_t parts, bytes;  // workspace: notes, parts
@@ -88,12 +94,13 @@ int weights(const FaPagedWeightsArgs* a, void* stream) {
   p.reset_new = a->reset_new ? 1 : 0;
   p.heads_kv = static_cast<int>(kv.heads_kv);
   p.group = static_cast<int>(a->heads_q / kv.heads_kv);
+  p.group_inv = static_cast<uint32_t>((int64_t{1} << 32) / p.group + 1);
   p.head_dim = static_cast<int>(kv.head_dim);
   p.causal = a->causal ? 1 : 0;
   p.scale_log2 = a->sm_scale * kLog2e;
   // A query tile has as many whole tokens as fit, but no more than a sequence has (their rows are loaded
   // and multiplied); a larger group has its heads in several tiles.
-  const int most = kv.head_dim <= 128 ? 128 : plan.fp8 ? 32 : 64;
+  const int most = query_rows(kv.head_dim, plan.fp8);
   const int64_t longest = a->max_q_len ? std::min(a->max_q_len, a->total) : a->total;
   p.tile_heads = std::min(p.group, most);
   p.chunks = (p.group + most - 1) / most;

@@ -20,12 +20,18 @@
 // Float8: the codes are exact in q's type and are converted as they are; the row's scale multiplies the
 // thread's logits.
 //
-// Warps (16-bit 12, float8 20):
-//   0-3, 4-7  epilogue of key tile 0, 1
-//   8         MMA issuer (owns TMEM)
-//   9, 10     TMA producers of K
-//   11        TMA producer of Q, and the logsumexps of its rows
-//   12-19     float8: convert the key tiles
+// Each key tile has two warpgroups, which take every other step (and TMEM buffer): the latency of a step is
+// a few times its work.  What they add up is joined at the item's end.
+//
+// Warps (16-bit 20, float8 28):
+//   0-3, 4-7, 8-11, 12-15  epilogue: key tile 0 and 1 of even steps, key tile 0 and 1 of odd ones
+//   16, 17    MMA issuers of key tile 0 and 1 (the first owns TMEM)
+//   18        TMA producer of K
+//   19        walks the line and tells the others the parts (a ring of descriptions: every warp walking
+//             by itself took 1500 cycles an item); TMA producer of Q, and the logsumexps of its rows
+//   20-27     float8: convert the key tiles
+// What a ring holds is waited for and given back by all warps that read from it, in order, though not all
+// look at each fill: a warp that passed over fills could take an older one for its own.
 #pragma once
 
 #include <type_traits>
@@ -54,7 +60,7 @@ constexpr int kWeightsBlock = 256;  // keys of an item
 
 template <int D, bool FP8>
 struct WeightsGeo {
-  static constexpr int QN = D <= 128 ? 128 : FP8 ? 32 : 64;  // rows of a query tile
+  static constexpr int QN = D <= 64 ? 128 : D == 128 ? (FP8 ? 64 : 128) : (FP8 ? 32 : 64);  // rows of a query tile
   static constexpr int ROW_BYTES = 2 * D;
   static constexpr int SWZ = ROW_BYTES >= 128 ? 128 : ROW_BYTES;
   static constexpr int NBLK = ROW_BYTES / SWZ;
@@ -63,16 +69,18 @@ struct WeightsGeo {
   static constexpr int Q_BLK = QN * SWZ;
   static constexpr int Q_TILE = QN * ROW_BYTES;
   static constexpr int RAW = FP8 ? 128 * (D + 4) : 0;  // codes, scales
-  static constexpr int K_SLOTS = D == 256 ? 2 : FP8 ? 3 : 4;
-  static constexpr int Q_SLOTS = D <= 64 ? 4 : 2;
+  static constexpr int K_SLOTS = D <= 64 ? (FP8 ? 3 : 4) : D == 128 ? 2 : 1;  // of each key tile of an item
+  static constexpr int Q_SLOTS = D <= 64 && !FP8 ? 4 : 2;
+  static constexpr int RAW_SLOTS = !FP8 ? 0 : D == 256 ? 1 : D == 128 ? 3 : 6;
   static constexpr int L_SLOTS = 4;  // logsumexps of query tiles
-  static constexpr int RAW_SLOTS = !FP8 ? 0 : D == 256 ? 1 : 3;
-  static constexpr int SHARED = 8192;
-  static constexpr int TILES = K_SLOTS * K_TILE + Q_SLOTS * Q_TILE + RAW_SLOTS * RAW;
+  static constexpr int I_SLOTS = 8;  // pages and scales of key tiles
+  static constexpr int P_SLOTS = 8;  // parts
+  static constexpr int SHARED = 11 * 1024;
+  static constexpr int TILES = 2 * K_SLOTS * K_TILE + Q_SLOTS * Q_TILE + RAW_SLOTS * RAW;
   // more than half of an SM's shared memory in any case: one CTA per SM, which takes all its TMEM
   static constexpr int SMEM = 1024 + TILES + SHARED > 120 * 1024 ? 1024 + TILES + SHARED : 120 * 1024;
   static constexpr int AUX = FP8 ? 8 : 0;
-  static constexpr int THREADS = (12 + AUX) * 32;
+  static constexpr int THREADS = (20 + AUX) * 32;
   static constexpr uint32_t LAYOUT = SWZ == 128 ? 2u : SWZ == 64 ? 4u : 6u;
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -105,7 +113,6 @@ struct WeightsSeq {
   }
 };
 
-// (plain data: it lives in shared memory)
 struct WeightsWalk {
   int64_t pos;  // next step of the line
   int at;       // ... and of the item
@@ -162,39 +169,49 @@ struct WeightsWalk {
     q0 = s.first_q(p, block);
     return true;
   }
-  __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == n; }
+};
+
+// A part as the warps see it: its sequence, what they need to know of it, and its steps.
+struct alignas(16) WeightsPart {
+  int tiles;   // key tiles with a key; 0: there is no further part
+  int seq, head, block;
+  int first, count, len;
+  int qtile;   // first query tile
+  int steps;
+  int qtiles;  // of the sequence
+  int slot;    // -1: a whole item, else that of the CTA's parts that its sums go to
+  int note;    // this CTA holds an item's last part, and this one its first (-1: nothing to note)
+
   __device__ __forceinline__ int key0() const { return block * kWeightsBlock; }
-  __device__ __forceinline__ int tiles() const { return key0() + 128 < s.len ? 2 : 1; }
   // A step's query tile: its first token, its first head of the group, and its rows.
   __device__ __forceinline__ int tok0(const PagedWeightsParams& p, int t) const {
-    return (q0 + t) / p.chunks * p.tile_toks;
+    return (p.chunks == 1 ? qtile + t : (qtile + t) / p.chunks) * p.tile_toks;
   }
   __device__ __forceinline__ int head0(const PagedWeightsParams& p, int t) const {
-    return (q0 + t) % p.chunks * p.tile_heads;
+    return p.chunks == 1 ? 0 : (qtile + t) % p.chunks * p.tile_heads;
   }
   __device__ __forceinline__ int rows(const PagedWeightsParams& p, int t) const {
-    return min(s.count - tok0(p, t), p.tile_toks) * min(p.group - head0(p, t), p.tile_heads);
+    return min(count - tok0(p, t), p.tile_toks) * min(p.group - head0(p, t), p.tile_heads);
   }
 };
 
 template <typename G>
 struct WeightsShared {
-  uint64_t k_full[G::K_SLOTS], k_empty[G::K_SLOTS];
+  uint64_t k_full[2][G::K_SLOTS], k_empty[2][G::K_SLOTS];
   uint64_t q_full[G::Q_SLOTS], q_empty[G::Q_SLOTS];
   uint64_t l_full[G::L_SLOTS], l_empty[G::L_SLOTS];
-  uint64_t raw_full[4], raw_empty[4];
+  uint64_t i_full[G::I_SLOTS], i_empty[G::I_SLOTS];
+  uint64_t p_full[G::P_SLOTS], p_empty[G::P_SLOTS];
+  uint64_t raw_full[8], raw_empty[8];
   uint64_t s_full[2][2], s_empty[2][2];
-  uint64_t mma_done;
-  int page[4][16];       // of a key tile's boxes, -1: none
-  int raw_page[4][16];
-  float scale[4][128];   // float8: of a key tile's rows
+  uint64_t sum_full[2][4], sum_empty[2][4];  // of a key tile, for each 32 of its keys
+  uint64_t mma_done[2];
+  WeightsPart parts[G::P_SLOTS];
+  int page[G::I_SLOTS][16];       // of a key tile's boxes, -1: none
+  int raw_page[8][16];
+  float scale[G::I_SLOTS][128];   // float8: of a key tile's rows
+  float sum[2][128];              // of the steps of the other warpgroup
   alignas(16) float neg_lse[G::L_SLOTS][G::QN];  // -l of a query tile's rows
-  int issued[2];
-  PagedRange range;
-  WeightsWalk first_walk;
-  int first_more;
-  WeightsWalk walks[20];
-  int more[20];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
@@ -210,8 +227,8 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* k_smem = smem;
-  uint8_t* q_smem = k_smem + K_SLOTS * G::K_TILE;
+  uint8_t* k_smem = smem;  // [2][K_SLOTS]
+  uint8_t* q_smem = k_smem + 2 * K_SLOTS * G::K_TILE;
   uint8_t* raw_smem = q_smem + Q_SLOTS * G::Q_TILE;
   Sh* sh = reinterpret_cast<Sh*>(raw_smem + G::RAW_SLOTS * G::RAW);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -219,29 +236,30 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
 
   let_next_launch();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < K_SLOTS; ++s) {
-      mbar_init(smem_u32(&sh->k_full[s]), FP8 ? G::AUX : 2);
-      mbar_init(smem_u32(&sh->k_empty[s]), 1 + 8);  // the MMAs, the epilogue
-    }
-    for (int s = 0; s < Q_SLOTS; ++s) {
-      mbar_init(smem_u32(&sh->q_full[s]), 1);
-      mbar_init(smem_u32(&sh->q_empty[s]), 1);
-    }
-    for (int s = 0; s < G::L_SLOTS; ++s) {
-      mbar_init(smem_u32(&sh->l_full[s]), 1);
-      mbar_init(smem_u32(&sh->l_empty[s]), 8);
-    }
-    for (int s = 0; s < 4; ++s) {
-      mbar_init(smem_u32(&sh->raw_full[s]), 2);
-      mbar_init(smem_u32(&sh->raw_empty[s]), 8);
-      mbar_init(smem_u32(&sh->s_full[s >> 1][s & 1]), 1);
-      mbar_init(smem_u32(&sh->s_empty[s >> 1][s & 1]), 4);
-    }
-    mbar_init(smem_u32(&sh->mma_done), 1);
+    auto init = [](uint64_t* bars, int n, uint32_t count) {
+      for (int s = 0; s < n; ++s) mbar_init(smem_u32(bars + s), count);
+    };
+    init(sh->k_full[0], 2 * K_SLOTS, FP8 ? G::AUX : 1);
+    init(sh->k_empty[0], 2 * K_SLOTS, 1);
+    init(sh->q_full, Q_SLOTS, 1);
+    init(sh->q_empty, Q_SLOTS, 2);  // the issuers
+    init(sh->l_full, G::L_SLOTS, 1);
+    init(sh->l_empty, G::L_SLOTS, 16);  // the epilogue
+    init(sh->i_full, G::I_SLOTS, FP8 ? G::AUX : 1);
+    init(sh->i_empty, G::I_SLOTS, 16);
+    init(sh->p_full, G::P_SLOTS, 1);
+    init(sh->p_empty, G::P_SLOTS, 19 + G::AUX);  // all other warps
+    init(sh->raw_full, 8, 1);
+    init(sh->raw_empty, 8, 8);
+    init(sh->s_full[0], 4, 1);
+    init(sh->s_empty[0], 4, 4);
+    init(sh->sum_full[0], 8, 1);
+    init(sh->sum_empty[0], 8, 1);
+    init(sh->mma_done, 2, 1);
     sh->abort_flag = 0u;
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == 16) {
     tmem_alloc(smem_u32(&sh->tmem_base), 512);
     tmem_relinquish();
   }
@@ -250,163 +268,227 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
   wait_for_launch_before();
-  if (threadIdx.x == 0) p.notes[blockIdx.x].first_cta = -1;
-  if (warp == 0) {
-    const PagedRange r =
-        paged_range(p, [&](int b) { const WeightsSeq s(p, b); return s.per_head * p.heads_kv; });
-    if (lane == 0) {
-      sh->range = r;
-      WeightsWalk x(p, r);
-      sh->first_more = x.next(p, r.hi);
-      sh->first_walk = x;
-    }
-  }
-  __syncthreads();
-  const PagedRange& range = sh->range;
 
   auto wait = [&](uint64_t& bar, uint32_t parity) {
     const bool ok = wait_bar_flag(&sh->abort_flag, smem_u32(&bar), parity, status);
     return static_cast<bool>(__all_sync(0xffffffffu, ok));
   };
-  WeightsWalk& w = sh->walks[warp];
-  bool begun = false;
+  // The next part, in the order of the line; false: there is none, or a wait gave up.
+  WeightsPart w;
+  int pslot = 0;
+  uint32_t pph = 0;
   auto next_part = [&]() -> bool {
+    if (!wait(sh->p_full[pslot], pph)) return false;
+    w = sh->parts[pslot];
     __syncwarp();
-    if (lane == 0) {
-      WeightsWalk x = begun ? w : sh->first_walk;
-      sh->more[warp] = begun ? x.next(p, range.hi) : sh->first_more;
-      w = x;
+    if (lane == 0) mbar_arrive(smem_u32(&sh->p_empty[pslot]));
+    if (++pslot == G::P_SLOTS) {
+      pslot = 0;
+      pph ^= 1u;
     }
-    begun = true;
-    __syncwarp();
-    return sh->more[warp] != 0;
+    return w.tiles > 0;
   };
   // The query tile in use; a lone one stays from item to item of the same sequence and head.
   int q_seq = -1, q_head = -1;
-  auto same_q = [&]() { return w.s.qtiles == 1 && q_seq == w.b && q_head == w.head; };
+  auto same_q = [&]() { return w.qtiles == 1 && q_seq == w.seq && q_head == w.head; };
   auto now_q = [&]() {
-    q_seq = w.b;
+    q_seq = w.seq;
     q_head = w.head;
   };
 
-  if (warp == 9 || warp == 10) {
-    // ------------------------------------------------------------------ producers of K
-    const int pw = warp - 9;
-    const int op = lane * 2 + pw;
+  if (warp == 18) {
+    // ------------------------------------------------------------------ producer of K
+    // The copies of a key tile, a lane each (two where the smallest pages have long rows).
     constexpr int COPIES = FP8 ? 2 : G::NBLK;  // of one page
+    constexpr int OPS = (16 * COPIES + 31) / 32;
     const int size = 1 << p.seqs.page_log2;
     const int box = min(size, 128);
     const int boxes = 128 / box;
-    const int my_box = op / COPIES, part = op % COPIES;
-    const uint32_t to = !FP8        ? part * G::K_BLK + my_box * box * G::SWZ
-                        : part == 0 ? my_box * box * D
-                                    : 128 * D + my_box * box * 4;
-    constexpr int RING = FP8 ? G::RAW_SLOTS : K_SLOTS;
-    uint64_t* const full = FP8 ? sh->raw_full : sh->k_full;
-    uint64_t* const empty = FP8 ? sh->raw_empty : sh->k_empty;
-    int(*const pages)[16] = FP8 ? sh->raw_page : sh->page;
-    int slot = 0, issued = 0;
-    uint32_t ph = 0;
+    int slot[2] = {0, 0}, islot = 0, rslot = 0;  // (rings of the two key tiles)
+    uint32_t ph[2] = {0, 0}, iph = 0, rph = 0;
+    int issued[2] = {0, 0};  // (float8: all of them in the first)
     bool ok = true;
-    ProducersMeet<2> meet{sh->issued, 3};
-    while (issued < meet.limit && next_part()) {
-      const int tiles = w.tiles();
-      int entry[2];
+    // the pages of an item, fetched an item ahead where that is the next block of the same sequence
+    int entry[2][OPS], ahead[2][OPS], ahead_seq = -1, ahead_block = -1, checked = -1;
+    auto fetch = [&](int block, int (&e)[2][OPS]) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int pos = w.key0() + i * 128 + my_box * box;
-        entry[i] = my_box < boxes && pos < w.s.len ? page_entry(p.seqs, w.b, pos) : -1;
-      }
-      bool stop = false;
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (i >= tiles || stop) continue;
-        const int key0 = w.key0() + i * 128;
-        const int pos = key0 + my_box * box;
-        const bool in = my_box < boxes && pos < w.s.len;
-        const int page = in ? checked_page(p.seqs, entry[i]) : -1;
-        if (ok) ok = wait(empty[slot], ph ^ 1u);
-        if (!ok) {
-          meet(pw, issued);
-          stop = issued >= meet.limit;
-          if (stop) continue;
+        for (int u = 0; u < OPS; ++u) {
+          const int my_box = (lane + 32 * u) / COPIES;
+          const int pos = block * kWeightsBlock + i * 128 + my_box * box;
+          e[i][u] = my_box < boxes && pos < w.len ? page_entry(p.seqs, w.seq, pos) : -1;
         }
-        const uint32_t bar = smem_u32(&full[slot]);
-        // (what is no page is copied from another one, and gets no weight)
-        if (my_box < boxes && part == 0) pages[slot][my_box] = in && page == entry[i] ? page : -1;
-        if (page >= 0) {
-          const int row = pos & (size - 1);
+    };
+    while (ok && next_part()) {
+      if (ahead_seq == w.seq && ahead_block == w.block) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int u = 0; u < OPS; ++u) entry[i][u] = ahead[i][u];
+      } else {
+        fetch(w.block, entry);
+      }
+      ahead_seq = w.seq;
+      ahead_block = w.key0() + kWeightsBlock < w.len ? w.block + 1 : 0;  // (of the next head)
+      fetch(ahead_block, ahead);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i >= w.tiles || !ok) continue;
+        const int key0 = w.key0() + i * 128;
+        ok = FP8 ? wait(sh->raw_empty[rslot], rph ^ 1u) : wait(sh->k_empty[i][slot[i]], ph[i] ^ 1u);
+        if (!FP8 && ok) ok = wait(sh->i_empty[islot], iph ^ 1u);
+        if (!ok) continue;
+        const uint32_t bar = smem_u32(FP8 ? &sh->raw_full[rslot] : &sh->k_full[i][slot[i]]);
+        const uint32_t dst =
+            smem_u32(FP8 ? raw_smem + rslot * G::RAW : k_smem + (i * K_SLOTS + slot[i]) * G::K_TILE);
+        int page[OPS];
+#pragma unroll
+        for (int u = 0; u < OPS; ++u) {
+          const int my_box = (lane + 32 * u) / COPIES, part = (lane + 32 * u) % COPIES;
+          const bool in = my_box < boxes && key0 + my_box * box < w.len;
+          page[u] = in ? checked_page(p.seqs, entry[i][u]) : -1;
+          // (what is no page is copied from another one, and gets no weight)
+          if (my_box < boxes && part == 0)
+            (FP8 ? sh->raw_page[rslot] : sh->page[islot])[my_box] = in && page[u] == entry[i][u] ? page[u] : -1;
+        }
+        __syncwarp();
+        if (lane == 0) {  // (after the page numbers, which those read who see the barrier complete)
+          const int live = min(boxes, (w.len - key0 + box - 1) / box);  // with a key
+          mbar_arrive_expect_tx(bar, live * box * (FP8 ? D + 4 : G::ROW_BYTES));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < OPS; ++u) {
+          const int my_box = (lane + 32 * u) / COPIES, part = (lane + 32 * u) % COPIES;
+          const int row = (key0 + my_box * box) & (size - 1);
+          if (page[u] < 0) continue;
           if constexpr (FP8) {
-            const uint32_t dst = smem_u32(raw_smem + slot * G::RAW) + to;
-            if (part == 0) tma_load_4d(dst, &tmK, bar, 0, row, w.head, page);
+            if (part == 0) tma_load_4d(dst + my_box * box * D, &tmK, bar, 0, row, w.head, page[u]);
             else
-              bulk_load_tile(dst, p.k_scale + page * p.k_scale_stride[0] + w.head * p.k_scale_stride[1] + row,
+              bulk_load_tile(dst + 128 * D + my_box * box * 4,
+                             p.k_scale + page[u] * p.k_scale_stride[0] + w.head * p.k_scale_stride[1] + row,
                              box * 4, bar);
           } else {
-            tma_load_4d(smem_u32(k_smem + slot * G::K_TILE) + to, &tmK, bar, part * (G::SWZ / 2), row, w.head,
-                        page);
+            tma_load_4d(dst + part * G::K_BLK + my_box * box * G::SWZ, &tmK, bar, part * (G::SWZ / 2), row, w.head,
+                        page[u]);
           }
         }
         __syncwarp();
-        if (lane == 0) {
-          const int live = min(boxes, (w.s.len - key0 + box - 1) / box);  // with a key
-          if (pw == 0) mbar_arrive_expect_tx(bar, live * box * (FP8 ? D + 4 : G::ROW_BYTES));
-          else mbar_arrive(bar);
-        }
-        ++issued;
-        if (++slot == RING) {
-          slot = 0;
-          ph ^= 1u;
+        if constexpr (FP8) {
+          ++issued[0];
+          if (++rslot == G::RAW_SLOTS) {
+            rslot = 0;
+            rph ^= 1u;
+          }
+        } else {
+          if (lane == 0) mbar_arrive(smem_u32(&sh->i_full[islot]));
+          if (++islot == G::I_SLOTS) {
+            islot = 0;
+            iph ^= 1u;
+          }
+          ++issued[i];
+          if (++slot[i] == K_SLOTS) {
+            slot[i] = 0;
+            ph[i] ^= 1u;
+          }
         }
       }
-      if (pw == 0 && lane == 0 &&
-          (fresh(p.seqs.kv_lens + w.b) != w.s.len ||
-           fresh(p.seqs.offsets + w.b + 1) - fresh(p.seqs.offsets + w.b) != w.s.count))
+      if (lane == 0 && checked != w.seq &&
+          (fresh(p.seqs.kv_lens + w.seq) != w.len ||
+           fresh(p.seqs.offsets + w.seq + 1) - fresh(p.seqs.offsets + w.seq) != w.count))
         report(status, kStatusPageTable);
+      checked = w.seq;
     }
-    meet(pw, issued);
-    for (int u = 0; u < min(issued, RING); ++u) {  // the copies issued last land before shared memory goes away
-      const int x = issued - 1 - u;
-      drain_bar(smem_u32(&full[x % RING]), static_cast<uint32_t>((x / RING) & 1));
+    // the copies issued last land before shared memory goes away
+    if constexpr (FP8) {
+      for (int u = 0; u < min(issued[0], G::RAW_SLOTS); ++u) {
+        const int x = issued[0] - 1 - u;
+        drain_bar(smem_u32(&sh->raw_full[x % G::RAW_SLOTS]), static_cast<uint32_t>((x / G::RAW_SLOTS) & 1));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        for (int u = 0; u < min(issued[i], K_SLOTS); ++u) {
+          const int x = issued[i] - 1 - u;
+          drain_bar(smem_u32(&sh->k_full[i][x % K_SLOTS]), static_cast<uint32_t>((x / K_SLOTS) & 1));
+        }
     }
-  } else if (warp == 11) {
-    // ------------------------------------------------------------------ producer of Q
+  } else if (warp == 19) {
+    // ------------------------------------------------------------------ the line, and Q
+    if (lane == 0) p.notes[blockIdx.x].first_cta = -1;
+    const PagedRange range =
+        paged_range(p, [&](int b) { const WeightsSeq s(p, b); return s.per_head * p.heads_kv; });
+    WeightsWalk walk(p, range);
+    bool more = true, ok = true;
+    // Tells the others the next part; it is told one part before its query tiles are loaded, so that its
+    // keys are on their way while the part before is worked on.
+    auto tell = [&](WeightsPart& x) {
+      more = walk.next(p, range.hi);
+      x = WeightsPart{};
+      if (more) {
+        x.tiles = walk.block * kWeightsBlock + 128 < walk.s.len ? 2 : 1;
+        x.seq = walk.b;
+        x.head = walk.head;
+        x.block = walk.block;
+        x.first = walk.s.first;
+        x.count = walk.s.count;
+        x.len = walk.s.len;
+        x.qtile = walk.q0 + walk.t0;
+        x.steps = walk.t1 - walk.t0;
+        x.qtiles = walk.s.qtiles;
+        x.slot = walk.t0 == 0 ? walk.t1 == walk.n ? -1 : 1 : 0;
+        x.note = x.slot == 0 && walk.t1 == walk.n ? range.cta_of(walk.item + p.item_cost) : -1;
+      }
+      ok = wait(sh->p_empty[pslot], pph ^ 1u);
+      if (!ok) return;
+      if (lane == 0) {
+        sh->parts[pslot] = x;
+        mbar_arrive(smem_u32(&sh->p_full[pslot]));
+      }
+      if (++pslot == G::P_SLOTS) {
+        pslot = 0;
+        pph ^= 1u;
+      }
+    };
     int slot = 0, lslot = 0, issued = 0;
     uint32_t ph = 0, lph = 0;
-    bool ok = true;
-    while (ok && next_part()) {
-      for (int t = w.t0; t < w.t1 && ok; ++t) {
+    WeightsPart coming;
+    tell(coming);
+    while (ok && coming.tiles > 0) {
+      w = coming;
+      tell(coming);
+      for (int t = 0; t < w.steps && ok; ++t) {
         if (same_q()) continue;
         now_q();
         const int tok0 = w.tok0(p, t), head0 = w.head0(p, t), rows = w.rows(p, t);
-        const int each = min(p.group - head0, p.tile_heads);  // rows of a token
-        float neg[QN / 32];
+        const float* const from = p.row_lse + static_cast<int64_t>(w.first + tok0) * (p.heads_kv * p.group) +
+                                  w.head * p.group + head0;
+        float l[QN / 32];
 #pragma unroll
         for (int u = 0; u < QN / 32; ++u) {
-          const int c = u * 32 + lane;
-          neg[u] = -INFINITY;
-          if (c < rows) {
-            const int tok = c / each;
-            const float l = fresh(p.row_lse + static_cast<int64_t>(w.s.first + tok0 + tok) * (p.heads_kv * p.group) +
-                                  w.head * p.group + head0 + c - tok * each);
-            if (l != -INFINITY) neg[u] = -l * kLog2e;  // (a row without keys gives nothing)
-          }
+          const int c = min(u * 32 + lane, rows - 1);  // (tile_heads = group unless tiles have one token)
+          const int tok = p.chunks > 1 ? 0 : p.group == 1 ? c : static_cast<int>(__umulhi(c, p.group_inv));
+          l[u] = fresh(from + static_cast<int64_t>(tok) * (p.heads_kv * p.group) + (c - tok * p.group));
         }
         ok = wait(sh->q_empty[slot], ph ^ 1u) && wait(sh->l_empty[lslot], lph ^ 1u);
         if (!ok) break;
-#pragma unroll
-        for (int u = 0; u < QN / 32; ++u) sh->neg_lse[lslot][u * 32 + lane] = neg[u];
-        __syncwarp();
         if (lane == 0) {
-          mbar_arrive(smem_u32(&sh->l_full[lslot]));
           const uint32_t bar = smem_u32(&sh->q_full[slot]);
           mbar_arrive_expect_tx(bar, p.tile_toks * p.tile_heads * G::ROW_BYTES);
 #pragma unroll
           for (int c = 0; c < G::NBLK; ++c)
             tma_load_3d(smem_u32(q_smem + slot * G::Q_TILE + c * G::Q_BLK), &tmQ, bar, c * (G::SWZ / 2),
-                        w.head * p.group + head0, w.s.first + tok0);
+                        w.head * p.group + head0, w.first + tok0);
+        }
+#pragma unroll
+        for (int u = 0; u < QN / 32; ++u) {
+          // (a row without keys gives nothing)
+          const bool none = u * 32 + lane >= rows || l[u] == -INFINITY;
+          sh->neg_lse[lslot][u * 32 + lane] = none ? -INFINITY : -l[u] * kLog2e;
         }
         __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh->l_full[lslot]));
         ++issued;
         if (++slot == Q_SLOTS) {
           slot = 0;
@@ -422,73 +504,63 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
       const int x = issued - 1 - u;
       drain_bar(smem_u32(&sh->q_full[x % Q_SLOTS]), static_cast<uint32_t>((x / Q_SLOTS) & 1));
     }
-  } else if (warp == 8) {
-    // ------------------------------------------------------------------ MMA issuer
+  } else if (warp == 16 || warp == 17) {
+    // ------------------------------------------------------------------ MMA issuers
     constexpr uint32_t hi = ((8u * G::SWZ) >> 4) | (1u << 14) | (G::LAYOUT << 29);
-    const uint32_t k_lo = (smem_u32(k_smem) >> 4) | (1u << 16);
+    const int i = warp - 16;
+    const uint32_t k_lo = (smem_u32(k_smem + i * K_SLOTS * G::K_TILE) >> 4) | (1u << 16);
     const uint32_t q_lo = (smem_u32(q_smem) >> 4) | (1u << 16);
-    int kslot = 0, qslot = -1;
-    uint32_t kph = 0, qph = 1;   // (qph: of the slot in use)
-    bool held = false;           // a lone query tile's slot is given back when the next one comes
-    int buf[2] = {0, 0};
+    int kslot = 0, qslot = -1, buf = 0;  // (buf: of the step)
+    uint32_t kph = 0, qph = 1;           // (qph: of the slot in use)
     uint32_t sph[2] = {0, 0};
+    bool held = false;  // a lone query tile's slot is given back when the next one comes
     bool ok = true;
     while (ok && next_part()) {
-      const int tiles = w.tiles();
-      int ks[2];
-      uint32_t kp[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ks[i] = kslot;
-        kp[i] = kph;
-        if (i < tiles && ++kslot == K_SLOTS) {
-          kslot = 0;
-          kph ^= 1u;
-        }
-      }
-      for (int t = w.t0; t < w.t1 && ok; ++t) {
+      const bool mine = i < w.tiles;
+      for (int t = 0; t < w.steps && ok; ++t) {
         if (!same_q()) {
           now_q();
           if (held && lane == 0) mma_commit(smem_u32(&sh->q_empty[qslot]));
-          held = w.s.qtiles == 1;
+          held = w.qtiles == 1;
           if (++qslot == Q_SLOTS) qslot = 0;
           if (qslot == 0) qph ^= 1u;
           ok = wait(sh->q_full[qslot], qph);
         }
-        const int n = min(QN, (w.rows(p, t) + 15) & ~15);
-        const uint32_t idesc = make_idesc(Elt<T>::kFmt, false, 128, 16) - (2u << 17) + (static_cast<uint32_t>(n >> 3) << 17);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (i >= tiles || !ok) continue;
-          if (t == w.t0) ok = wait(sh->k_full[ks[i]], kp[i]);
-          if (ok) ok = wait(sh->s_empty[i][buf[i]], sph[i] ^ 1u);
-          if (!ok) continue;
+        if (mine) {
+          if (t == 0 && ok) ok = wait(sh->k_full[i][kslot], kph);
+          if (ok) ok = wait(sh->s_empty[i][buf], sph[buf] ^ 1u);
+          if (!ok) break;
+          sph[buf] ^= 1u;
+          const int n = min(QN, (w.rows(p, t) + 15) & ~15);
+          const uint32_t idesc = make_idesc(Elt<T>::kFmt, false, 128, 0) + (static_cast<uint32_t>(n >> 3) << 17);
+          const uint32_t a0 = k_lo + ((kslot * G::K_TILE) >> 4);
+          const uint32_t b0 = q_lo + ((qslot * G::Q_TILE) >> 4);
+          const uint32_t d = tmem + (i * 2 + buf) * QN;
           tc_fence_after();
           if (lane == 0) {
-            const uint32_t a0 = k_lo + ((ks[i] * G::K_TILE) >> 4);
-            const uint32_t b0 = q_lo + ((qslot * G::Q_TILE) >> 4);
-            const uint32_t d = tmem + (i * 2 + buf[i]) * QN;
 #pragma unroll
             for (int c = 0; c < G::NBLK; ++c)
 #pragma unroll
               for (int k = 0; k < G::SWZ / 32; ++k)
                 mma_f16_ss_lo(d, a0 + ((c * G::K_BLK + k * 32) >> 4), b0 + ((c * G::Q_BLK + k * 32) >> 4), hi, idesc,
                               (c | k) ? 1u : 0u);
-            mma_commit(smem_u32(&sh->s_full[i][buf[i]]));
-            if (t + 1 == w.t1) mma_commit(smem_u32(&sh->k_empty[ks[i]]));
+            mma_commit(smem_u32(&sh->s_full[i][buf]));
+            if (t + 1 == w.steps) mma_commit(smem_u32(&sh->k_empty[i][kslot]));
           }
-          __syncwarp();
-          buf[i] ^= 1;
-          if (buf[i] == 0) sph[i] ^= 1u;
         }
         if (ok && !held && lane == 0) mma_commit(smem_u32(&sh->q_empty[qslot]));
         __syncwarp();
+        buf ^= 1;
+      }
+      if (mine && ++kslot == K_SLOTS) {
+        kslot = 0;
+        kph ^= 1u;
       }
     }
-    if (lane == 0) mma_commit(smem_u32(&sh->mma_done));
+    if (lane == 0) mma_commit(smem_u32(&sh->mma_done[i]));
     __syncwarp();
-    drain_bar(smem_u32(&sh->mma_done), 0);
-  } else if (warp >= 12) {
+    drain_bar(smem_u32(&sh->mma_done[i]), 0);
+  } else if (warp >= 20) {
     if constexpr (FP8) {
       // ---------------------------------------------------------------- convert the key tiles
       // (lanes and pieces as in the tile kernel)
@@ -498,20 +570,23 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
       constexpr int NG = PR / LP;
       constexpr int AT_ONCE = G::AUX * RW < 128 ? G::AUX * RW : 128;
       constexpr int STEPS = 128 / AT_ONCE;
-      const int row0 = (warp - 12) * RW + lane / LP;
+      const int row0 = (warp - 20) * RW + lane / LP;
       const int group0 = row0 & (NG - 1);
-      const int tid = threadIdx.x - 12 * 32;
-      int slot = 0, rslot = 0;
-      uint32_t ph = 0, rph = 0;
+      const int tid = threadIdx.x - 20 * 32;
+      int slot[2] = {0, 0}, rslot = 0, islot = 0;
+      uint32_t ph[2] = {0, 0}, rph = 0, iph = 0;
       bool ok = true;
       while (ok && next_part()) {
-        for (int i = 0; i < w.tiles() && ok; ++i) {
-          ok = wait(sh->raw_full[rslot], rph) && wait(sh->k_empty[slot], ph ^ 1u);
-          if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (i >= w.tiles || !ok) continue;
+          ok = wait(sh->raw_full[rslot], rph) && wait(sh->i_empty[islot], iph ^ 1u) &&
+               wait(sh->k_empty[i][slot[i]], ph[i] ^ 1u);
+          if (!ok) continue;
           const uint8_t* raw = raw_smem + rslot * G::RAW;
-          uint8_t* dst = k_smem + slot * G::K_TILE;
-          if (tid < 128) sh->scale[slot][tid] = reinterpret_cast<const float*>(raw + 128 * D)[tid];
-          else if (tid < 144) sh->page[slot][tid - 128] = sh->raw_page[rslot][tid - 128];
+          uint8_t* dst = k_smem + (i * K_SLOTS + slot[i]) * G::K_TILE;
+          if (tid < 128) sh->scale[islot][tid] = reinterpret_cast<const float*>(raw + 128 * D)[tid];
+          else if (tid < 144) sh->page[islot][tid - 128] = sh->raw_page[rslot][tid - 128];
           if (row0 < AT_ONCE) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k)
@@ -541,60 +616,62 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(smem_u32(&sh->k_full[slot]));
+            mbar_arrive(smem_u32(&sh->i_full[islot]));
+            mbar_arrive(smem_u32(&sh->k_full[i][slot[i]]));
             mbar_arrive(smem_u32(&sh->raw_empty[rslot]));
           }
-          if (++slot == K_SLOTS) { slot = 0; ph ^= 1u; }
+          if (++islot == G::I_SLOTS) { islot = 0; iph ^= 1u; }
+          if (++slot[i] == K_SLOTS) { slot[i] = 0; ph[i] ^= 1u; }
           if (++rslot == G::RAW_SLOTS) { rslot = 0; rph ^= 1u; }
         }
       }
     }
   } else {
     // -------------------------------------------------------------------- epilogue
-    const int i = warp >> 2;         // key tile
+    const int i = warp >> 2 & 1;     // key tile
+    const int buf = warp >> 3;       // steps of this parity, and their buffer
+    const int part = warp & 3;       // 32 keys of the tile
     const int r = threadIdx.x & 127; // key of the tile
-    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + (static_cast<uint32_t>(part * 32) << 16) + (i * 2 + buf) * QN;
     const int size = 1 << p.seqs.page_log2;
     const int box_log2 = min(p.seqs.page_log2, 7);
-    int kslot = 0, lslot = -1, buf = 0;
-    uint32_t kph = 0, lph = 1, sph = 0;
+    int islot = 0, lslot = -1, step = 0;  // (step: parity of the next one)
+    uint32_t iph = 0, lph = 1, sph = 0, sum_ph = 0;
     bool ok = true;
     while (ok && next_part()) {
-      const int tiles = w.tiles();
-      const bool mine = i < tiles;
+      // the warpgroup of the last step writes what both have added up
+      const bool last = ((step + w.steps - 1) & 1) == buf;
+      const bool mine = i < w.tiles && (w.steps > 1 || last);
       const int pos = w.key0() + i * 128 + r;
-      const int past = w.s.len - w.s.count;
-      const bool whole = w.whole();
+      const int past = w.len - w.count;
       float old = 0.f, k2 = p.scale_log2;
       float* place = nullptr;
-      // Both tiles' slots are waited for and given back by all warps, though each looks at one: a warp that
-      // passed over fills of a slot could take an older fill for its own.
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        if (x >= tiles) continue;
-        if (ok) ok = wait(sh->k_full[kslot], kph);
+        if (x >= w.tiles) continue;
+        if (ok) ok = wait(sh->i_full[islot], iph);
         if (ok) {
-          if (x == i) {
-            const int page = sh->page[kslot][r >> box_log2];
-            if (FP8) k2 *= sh->scale[kslot][r];
-            if (whole && pos < w.s.len && page >= 0) {
+          if (x == i && mine) {
+            const int page = sh->page[islot][r >> box_log2];
+            if (FP8) k2 *= sh->scale[islot][r];
+            if (last && w.slot < 0 && pos < w.len && page >= 0) {
               place = p.weights + page * p.weights_stride[0] + w.head * p.weights_stride[1] + (pos & (size - 1));
               if (!(p.reset_new && pos >= past)) old = fresh(place);
             }
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sh->k_empty[kslot]));
+          if (lane == 0) mbar_arrive(smem_u32(&sh->i_empty[islot]));
         }
-        if (++kslot == K_SLOTS) {
-          kslot = 0;
-          kph ^= 1u;
+        if (++islot == G::I_SLOTS) {
+          islot = 0;
+          iph ^= 1u;
         }
       }
       const float2 kk = make_float2(k2, k2);
       float2 acc[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) acc[u] = make_float2(0.f, 0.f);
-      for (int t = w.t0; t < w.t1 && ok; ++t) {
+      for (int t = 0; t < w.steps && ok; ++t, step ^= 1) {
         if (!same_q()) {
           now_q();
           if (lslot >= 0 && lane == 0) mbar_arrive(smem_u32(&sh->l_empty[lslot]));
@@ -602,16 +679,17 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
           if (lslot == 0) lph ^= 1u;
           ok = wait(sh->l_full[lslot], lph);
         }
-        if (!mine || !ok) continue;
+        if (i >= w.tiles || step != buf || !ok) continue;
         ok = wait(sh->s_full[i][buf], sph);
         if (!ok) break;
+        sph ^= 1u;
         tc_fence_after();
         const int live = w.rows(p, t);
         // columns before `from` are hidden from this key: of tokens that come before it
-        const int from = p.causal ? max(0, pos - past - w.tok0(p, t)) * p.group : 0;
-        const int from_all = p.causal ? max(0, pos - lane + 31 - past - w.tok0(p, t)) * p.group : 0;
-        const int from_any = p.causal ? max(0, pos - lane - past - w.tok0(p, t)) * p.group : 0;
-        const uint32_t tS = tmem + lane_off + (i * 2 + buf) * QN;
+        const int ahead = pos - past - w.tok0(p, t);
+        const int from = p.causal ? max(0, ahead) * p.group : 0;
+        const int from_all = p.causal ? max(0, ahead - lane + 31) * p.group : 0;
+        const int from_any = p.causal ? max(0, ahead - lane) * p.group : 0;
         const float* neg = sh->neg_lse[lslot];
 #pragma unroll 1
         for (int c0 = from_any & ~31; c0 < live; c0 += 32) {
@@ -645,19 +723,28 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh->s_empty[i][buf]));
-        buf ^= 1;
-        if (buf == 0) sph ^= 1u;
       }
       if (!mine || !ok) continue;
       const float2 a = fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3]));
-      const float sum = a.x + a.y;
-      if (whole) {
+      float sum = a.x + a.y;
+      if (w.steps > 1) {
+        uint64_t& full = sh->sum_full[i][part];
+        uint64_t& empty = sh->sum_empty[i][part];
+        ok = last ? wait(full, sum_ph) : wait(empty, sum_ph ^ 1u);
+        if (!ok) break;
+        sum_ph ^= 1u;
+        if (last) sum += sh->sum[i][r];
+        else sh->sum[i][r] = sum;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(last ? &empty : &full));
+        if (!last) continue;
+      }
+      if (w.slot < 0) {
         if (place) *place = old + sum;
       } else {
-        const int slot = w.t0 == 0 ? 1 : 0;
-        p.parts[(static_cast<int64_t>(blockIdx.x) * 2 + slot) * kWeightsBlock + i * 128 + r] = sum;
-        if (threadIdx.x == 0 && slot == 0 && w.t1 == w.n)
-          p.notes[blockIdx.x] = PagedWeightsNote{range.cta_of(w.item + p.item_cost), w.b, w.head, w.block};
+        p.parts[(static_cast<int64_t>(blockIdx.x) * 2 + w.slot) * kWeightsBlock + i * 128 + r] = sum;
+        if (i == 0 && r == 0 && w.note >= 0)
+          p.notes[blockIdx.x] = PagedWeightsNote{w.note, w.seq, w.head, w.block};
       }
     }
   }
@@ -665,7 +752,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
   // ---- teardown: every thread arrives here exactly once
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
