@@ -26,9 +26,10 @@
 // Warps (16-bit 20, float8 28):
 //   0-3, 4-7, 8-11, 12-15  epilogue: key tile 0 and 1 of even steps, key tile 0 and 1 of odd ones
 //   16, 17    MMA issuers of key tile 0 and 1 (the first owns TMEM)
-//   18        TMA producer of K
+//   18        TMA producer of K (16 bits: of key tile 0)
 //   19        walks the line and tells the others the parts (a ring of descriptions: every warp walking
-//             by itself took 1500 cycles an item); TMA producer of Q, and the logsumexps of its rows
+//             by itself took 1500 cycles an item); TMA producer of Q, and the logsumexps of its rows, and
+//             (16 bits) of K's key tile 1
 //   20-27     float8: convert the key tiles
 // What a ring holds is waited for and given back by all warps that read from it, in order, though not all
 // look at each fill: a warp that passed over fills could take an older one for its own.
@@ -73,7 +74,7 @@ struct WeightsGeo {
   static constexpr int Q_SLOTS = D <= 64 && !FP8 ? 4 : 2;
   static constexpr int RAW_SLOTS = !FP8 ? 0 : D == 256 ? 1 : D == 128 ? 3 : 6;
   static constexpr int L_SLOTS = 4;  // logsumexps of query tiles
-  static constexpr int I_SLOTS = 8;  // pages and scales of key tiles
+  static constexpr int I_SLOTS = 4;  // pages and scales of each key tile of an item
   static constexpr int P_SLOTS = 8;  // parts
   static constexpr int SHARED = 11 * 1024;
   static constexpr int TILES = 2 * K_SLOTS * K_TILE + Q_SLOTS * Q_TILE + RAW_SLOTS * RAW;
@@ -200,21 +201,46 @@ struct WeightsShared {
   uint64_t k_full[2][G::K_SLOTS], k_empty[2][G::K_SLOTS];
   uint64_t q_full[G::Q_SLOTS], q_empty[G::Q_SLOTS];
   uint64_t l_full[G::L_SLOTS], l_empty[G::L_SLOTS];
-  uint64_t i_full[G::I_SLOTS], i_empty[G::I_SLOTS];
+  uint64_t i_full[2][G::I_SLOTS], i_empty[2][G::I_SLOTS];
   uint64_t p_full[G::P_SLOTS], p_empty[G::P_SLOTS];
   uint64_t raw_full[8], raw_empty[8];
   uint64_t s_full[2][2], s_empty[2][2];
   uint64_t sum_full[2][4], sum_empty[2][4];  // of a key tile, for each 32 of its keys
   uint64_t mma_done[2];
   WeightsPart parts[G::P_SLOTS];
-  int page[G::I_SLOTS][16];       // of a key tile's boxes, -1: none
+  int page[2][G::I_SLOTS][16];       // of a key tile's boxes, -1: none
   int raw_page[8][16];
-  float scale[G::I_SLOTS][128];   // float8: of a key tile's rows
+  float scale[2][G::I_SLOTS][128];   // float8: of a key tile's rows
   float sum[2][128];              // of the steps of the other warpgroup
   alignas(16) float neg_lse[G::L_SLOTS][G::QN];  // -l of a query tile's rows
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
+
+// acc + 2^x of a pair on the FMA pipe: 2^n 2^f with n = round(x), f = x - n in [-1/2, 1/2], and a polynomial
+// of degree 5 that minimises the relative error of 2^f there (the fit of exp2_poly_fit.py at degree 5: 2.3e-7,
+// as ex2.approx).  2^-126 below -126, infinite from 128 on; NaN stays NaN.
+__device__ __forceinline__ float2 add_exp2_poly(float2 x, float2 acc) {
+  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the low bits of x + kRound are n
+  constexpr float c0 = 1.000000119e+00f, c1 = 6.931469440e-01f, c2 = 2.402212024e-01f, c3 = 5.550713092e-02f,
+                  c4 = 9.675540961e-03f, c5 = 1.327647129e-03f;
+  auto both = [](float c) { return make_float2(c, c); };
+  auto clamp = [](float v) {
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;\n\tmin.NaN.f32 %0, %0, 0f43000000;" : "+f"(v));  // -126, 128
+    return v;
+  };
+  x = make_float2(clamp(x.x), clamp(x.y));
+  const float2 t = fadd2(x, both(kRound));
+  const float2 f = ffma2(fadd2(t, both(-kRound)), both(-1.f), x);
+  float2 q = ffma2(both(c5), f, both(c4));
+  q = ffma2(q, f, both(c3));
+  q = ffma2(q, f, both(c2));
+  q = ffma2(q, f, both(c1));
+  q = ffma2(q, f, both(c0));
+  const float2 scale = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
+                                   __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
+  return ffma2(q, scale, acc);
+}
 
 template <typename T, int D, bool FP8>
 __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
@@ -245,8 +271,8 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     init(sh->q_empty, Q_SLOTS, 2);  // the issuers
     init(sh->l_full, G::L_SLOTS, 1);
     init(sh->l_empty, G::L_SLOTS, 16);  // the epilogue
-    init(sh->i_full, G::I_SLOTS, FP8 ? G::AUX : 1);
-    init(sh->i_empty, G::I_SLOTS, 16);
+    init(sh->i_full[0], 2 * G::I_SLOTS, FP8 ? G::AUX : 1);
+    init(sh->i_empty[0], 2 * G::I_SLOTS, 8);  // the two warpgroups of the tile
     init(sh->p_full, G::P_SLOTS, 1);
     init(sh->p_empty, G::P_SLOTS, 19 + G::AUX);  // all other warps
     init(sh->raw_full, 8, 1);
@@ -296,124 +322,118 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     q_head = w.head;
   };
 
+  // Producer of key tiles: both of an item, or one of them.
+  // The copies of a tile, a lane each (two where the smallest pages have long rows).
+  constexpr int COPIES = FP8 ? 2 : G::NBLK;  // of one page
+  constexpr int OPS = (16 * COPIES + 31) / 32;
+  struct Keys {
+    int slot = 0, islot = 0;
+    uint32_t ph = 0, iph = 0;
+    int issued = 0;
+    int ahead_seq = -1, ahead_block = -1;  // the item whose pages were fetched ahead
+  };
+  const int size = 1 << p.seqs.page_log2;
+  const int box = min(size, 128);
+  const int boxes = 128 / box;
+  // (float8: `k` of the ring of raw tiles, which both key tiles share)
+  auto load_keys = [&](int i, Keys& k, int (&ahead)[OPS]) -> bool {
+    const int key0 = w.key0() + i * 128;
+    auto fetch = [&](int u, int first) {
+      const int my_box = (lane + 32 * u) / COPIES;
+      const int pos = first + my_box * box;
+      return my_box < boxes && pos < w.len ? page_entry(p.seqs, w.seq, pos) : -1;
+    };
+    const bool known = k.ahead_seq == w.seq && k.ahead_block == w.block;
+    // the next block of the sequence, or the first one, of the next head
+    const int next = w.key0() + kWeightsBlock < w.len ? w.block + 1 : 0;
+    int entry[OPS];
+#pragma unroll
+    for (int u = 0; u < OPS; ++u) {
+      entry[u] = known ? ahead[u] : fetch(u, key0);
+      ahead[u] = fetch(u, next * kWeightsBlock + i * 128);
+    }
+    bool ok = FP8 ? wait(sh->raw_empty[k.slot], k.ph ^ 1u) : wait(sh->k_empty[i][k.slot], k.ph ^ 1u);
+    if (!FP8 && ok) ok = wait(sh->i_empty[i][k.islot], k.iph ^ 1u);
+    if (!ok) return false;
+    const uint32_t bar = smem_u32(FP8 ? &sh->raw_full[k.slot] : &sh->k_full[i][k.slot]);
+    const uint32_t dst = smem_u32(FP8 ? raw_smem + k.slot * G::RAW : k_smem + (i * K_SLOTS + k.slot) * G::K_TILE);
+    int page[OPS];
+#pragma unroll
+    for (int u = 0; u < OPS; ++u) {
+      const int my_box = (lane + 32 * u) / COPIES, part = (lane + 32 * u) % COPIES;
+      const bool in = my_box < boxes && key0 + my_box * box < w.len;
+      page[u] = in ? checked_page(p.seqs, entry[u]) : -1;
+      // (what is no page is copied from another one, and gets no weight)
+      if (my_box < boxes && part == 0)
+        (FP8 ? sh->raw_page[k.slot] : sh->page[i][k.islot])[my_box] = in && page[u] == entry[u] ? page[u] : -1;
+    }
+    __syncwarp();
+    if (lane == 0) {  // (behind the page numbers, which those read who see the barrier complete)
+      const int live = min(boxes, (w.len - key0 + box - 1) / box);  // with a key
+      mbar_arrive_expect_tx(bar, live * box * (FP8 ? D + 4 : G::ROW_BYTES));
+    }
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < OPS; ++u) {
+      const int my_box = (lane + 32 * u) / COPIES, part = (lane + 32 * u) % COPIES;
+      const int row = (key0 + my_box * box) & (size - 1);
+      if (page[u] < 0) continue;
+      if constexpr (FP8) {
+        if (part == 0) tma_load_4d(dst + my_box * box * D, &tmK, bar, 0, row, w.head, page[u]);
+        else
+          bulk_load_tile(dst + 128 * D + my_box * box * 4,
+                         p.k_scale + page[u] * p.k_scale_stride[0] + w.head * p.k_scale_stride[1] + row, box * 4, bar);
+      } else {
+        tma_load_4d(dst + part * G::K_BLK + my_box * box * G::SWZ, &tmK, bar, part * (G::SWZ / 2), row, w.head, page[u]);
+      }
+    }
+    __syncwarp();
+    ++k.issued;
+    if (++k.slot == (FP8 ? G::RAW_SLOTS : K_SLOTS)) {
+      k.slot = 0;
+      k.ph ^= 1u;
+    }
+    if constexpr (!FP8) {
+      if (lane == 0) mbar_arrive(smem_u32(&sh->i_full[i][k.islot]));
+      if (++k.islot == G::I_SLOTS) {
+        k.islot = 0;
+        k.iph ^= 1u;
+      }
+    }
+    return true;
+  };
+  auto fetched = [&](Keys& k) {
+    k.ahead_seq = w.seq;
+    k.ahead_block = w.key0() + kWeightsBlock < w.len ? w.block + 1 : 0;
+  };
+  // The copies issued last land before shared memory goes away.
+  auto drain_keys = [&](int i, const Keys& k) {
+    constexpr int RING = FP8 ? G::RAW_SLOTS : K_SLOTS;
+    for (int u = 0; u < min(k.issued, RING); ++u) {
+      const int x = k.issued - 1 - u;
+      drain_bar(smem_u32(FP8 ? &sh->raw_full[x % RING] : &sh->k_full[i][x % RING]),
+                static_cast<uint32_t>((x / RING) & 1));
+    }
+  };
+
   if (warp == 18) {
     // ------------------------------------------------------------------ producer of K
-    // The copies of a key tile, a lane each (two where the smallest pages have long rows).
-    constexpr int COPIES = FP8 ? 2 : G::NBLK;  // of one page
-    constexpr int OPS = (16 * COPIES + 31) / 32;
-    const int size = 1 << p.seqs.page_log2;
-    const int box = min(size, 128);
-    const int boxes = 128 / box;
-    int slot[2] = {0, 0}, islot = 0, rslot = 0;  // (rings of the two key tiles)
-    uint32_t ph[2] = {0, 0}, iph = 0, rph = 0;
-    int issued[2] = {0, 0};  // (float8: all of them in the first)
+    Keys k;
+    int ahead[2][OPS], checked = -1;
     bool ok = true;
-    // the pages of an item, fetched an item ahead where that is the next block of the same sequence
-    int entry[2][OPS], ahead[2][OPS], ahead_seq = -1, ahead_block = -1, checked = -1;
-    auto fetch = [&](int block, int (&e)[2][OPS]) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int u = 0; u < OPS; ++u) {
-          const int my_box = (lane + 32 * u) / COPIES;
-          const int pos = block * kWeightsBlock + i * 128 + my_box * box;
-          e[i][u] = my_box < boxes && pos < w.len ? page_entry(p.seqs, w.seq, pos) : -1;
-        }
-    };
     while (ok && next_part()) {
-      if (ahead_seq == w.seq && ahead_block == w.block) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int u = 0; u < OPS; ++u) entry[i][u] = ahead[i][u];
-      } else {
-        fetch(w.block, entry);
-      }
-      ahead_seq = w.seq;
-      ahead_block = w.key0() + kWeightsBlock < w.len ? w.block + 1 : 0;  // (of the next head)
-      fetch(ahead_block, ahead);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (i >= w.tiles || !ok) continue;
-        const int key0 = w.key0() + i * 128;
-        ok = FP8 ? wait(sh->raw_empty[rslot], rph ^ 1u) : wait(sh->k_empty[i][slot[i]], ph[i] ^ 1u);
-        if (!FP8 && ok) ok = wait(sh->i_empty[islot], iph ^ 1u);
-        if (!ok) continue;
-        const uint32_t bar = smem_u32(FP8 ? &sh->raw_full[rslot] : &sh->k_full[i][slot[i]]);
-        const uint32_t dst =
-            smem_u32(FP8 ? raw_smem + rslot * G::RAW : k_smem + (i * K_SLOTS + slot[i]) * G::K_TILE);
-        int page[OPS];
-#pragma unroll
-        for (int u = 0; u < OPS; ++u) {
-          const int my_box = (lane + 32 * u) / COPIES, part = (lane + 32 * u) % COPIES;
-          const bool in = my_box < boxes && key0 + my_box * box < w.len;
-          page[u] = in ? checked_page(p.seqs, entry[i][u]) : -1;
-          // (what is no page is copied from another one, and gets no weight)
-          if (my_box < boxes && part == 0)
-            (FP8 ? sh->raw_page[rslot] : sh->page[islot])[my_box] = in && page[u] == entry[i][u] ? page[u] : -1;
-        }
-        __syncwarp();
-        if (lane == 0) {  // (after the page numbers, which those read who see the barrier complete)
-          const int live = min(boxes, (w.len - key0 + box - 1) / box);  // with a key
-          mbar_arrive_expect_tx(bar, live * box * (FP8 ? D + 4 : G::ROW_BYTES));
-        }
-        __syncwarp();
-#pragma unroll
-        for (int u = 0; u < OPS; ++u) {
-          const int my_box = (lane + 32 * u) / COPIES, part = (lane + 32 * u) % COPIES;
-          const int row = (key0 + my_box * box) & (size - 1);
-          if (page[u] < 0) continue;
-          if constexpr (FP8) {
-            if (part == 0) tma_load_4d(dst + my_box * box * D, &tmK, bar, 0, row, w.head, page[u]);
-            else
-              bulk_load_tile(dst + 128 * D + my_box * box * 4,
-                             p.k_scale + page[u] * p.k_scale_stride[0] + w.head * p.k_scale_stride[1] + row,
-                             box * 4, bar);
-          } else {
-            tma_load_4d(dst + part * G::K_BLK + my_box * box * G::SWZ, &tmK, bar, part * (G::SWZ / 2), row, w.head,
-                        page[u]);
-          }
-        }
-        __syncwarp();
-        if constexpr (FP8) {
-          ++issued[0];
-          if (++rslot == G::RAW_SLOTS) {
-            rslot = 0;
-            rph ^= 1u;
-          }
-        } else {
-          if (lane == 0) mbar_arrive(smem_u32(&sh->i_full[islot]));
-          if (++islot == G::I_SLOTS) {
-            islot = 0;
-            iph ^= 1u;
-          }
-          ++issued[i];
-          if (++slot[i] == K_SLOTS) {
-            slot[i] = 0;
-            ph[i] ^= 1u;
-          }
-        }
-      }
+      for (int i = 0; i < (FP8 ? 2 : 1); ++i)
+        if (i < w.tiles && ok) ok = load_keys(i, k, ahead[i]);
+      if (FP8 && w.tiles == 1) k.ahead_block = -1;  // (those of the second tile have not been fetched)
+      else fetched(k);
       if (lane == 0 && checked != w.seq &&
           (fresh(p.seqs.kv_lens + w.seq) != w.len ||
            fresh(p.seqs.offsets + w.seq + 1) - fresh(p.seqs.offsets + w.seq) != w.count))
         report(status, kStatusPageTable);
       checked = w.seq;
     }
-    // the copies issued last land before shared memory goes away
-    if constexpr (FP8) {
-      for (int u = 0; u < min(issued[0], G::RAW_SLOTS); ++u) {
-        const int x = issued[0] - 1 - u;
-        drain_bar(smem_u32(&sh->raw_full[x % G::RAW_SLOTS]), static_cast<uint32_t>((x / G::RAW_SLOTS) & 1));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        for (int u = 0; u < min(issued[i], K_SLOTS); ++u) {
-          const int x = issued[i] - 1 - u;
-          drain_bar(smem_u32(&sh->k_full[i][x % K_SLOTS]), static_cast<uint32_t>((x / K_SLOTS) & 1));
-        }
-    }
+    drain_keys(0, k);
   } else if (warp == 19) {
     // ------------------------------------------------------------------ the line, and Q
     if (lane == 0) p.notes[blockIdx.x].first_cta = -1;
@@ -453,11 +473,17 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     };
     int slot = 0, lslot = 0, issued = 0;
     uint32_t ph = 0, lph = 0;
+    Keys k;
+    int ahead[OPS];
     WeightsPart coming;
     tell(coming);
     while (ok && coming.tiles > 0) {
       w = coming;
       tell(coming);
+      if (!FP8 && w.tiles == 2) {
+        if (ok) ok = load_keys(1, k, ahead);
+        fetched(k);
+      }
       for (int t = 0; t < w.steps && ok; ++t) {
         if (same_q()) continue;
         now_q();
@@ -504,6 +530,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
       const int x = issued - 1 - u;
       drain_bar(smem_u32(&sh->q_full[x % Q_SLOTS]), static_cast<uint32_t>((x / Q_SLOTS) & 1));
     }
+    if constexpr (!FP8) drain_keys(1, k);
   } else if (warp == 16 || warp == 17) {
     // ------------------------------------------------------------------ MMA issuers
     constexpr uint32_t hi = ((8u * G::SWZ) >> 4) | (1u << 14) | (G::LAYOUT << 29);
@@ -573,20 +600,20 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
       const int row0 = (warp - 20) * RW + lane / LP;
       const int group0 = row0 & (NG - 1);
       const int tid = threadIdx.x - 20 * 32;
-      int slot[2] = {0, 0}, rslot = 0, islot = 0;
-      uint32_t ph[2] = {0, 0}, rph = 0, iph = 0;
+      int slot[2] = {0, 0}, islot[2] = {0, 0}, rslot = 0;
+      uint32_t ph[2] = {0, 0}, iph[2] = {0, 0}, rph = 0;
       bool ok = true;
       while (ok && next_part()) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (i >= w.tiles || !ok) continue;
-          ok = wait(sh->raw_full[rslot], rph) && wait(sh->i_empty[islot], iph ^ 1u) &&
+          ok = wait(sh->raw_full[rslot], rph) && wait(sh->i_empty[i][islot[i]], iph[i] ^ 1u) &&
                wait(sh->k_empty[i][slot[i]], ph[i] ^ 1u);
           if (!ok) continue;
           const uint8_t* raw = raw_smem + rslot * G::RAW;
           uint8_t* dst = k_smem + (i * K_SLOTS + slot[i]) * G::K_TILE;
-          if (tid < 128) sh->scale[islot][tid] = reinterpret_cast<const float*>(raw + 128 * D)[tid];
-          else if (tid < 144) sh->page[islot][tid - 128] = sh->raw_page[rslot][tid - 128];
+          if (tid < 128) sh->scale[i][islot[i]][tid] = reinterpret_cast<const float*>(raw + 128 * D)[tid];
+          else if (tid < 144) sh->page[i][islot[i]][tid - 128] = sh->raw_page[rslot][tid - 128];
           if (row0 < AT_ONCE) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k)
@@ -616,11 +643,11 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(smem_u32(&sh->i_full[islot]));
+            mbar_arrive(smem_u32(&sh->i_full[i][islot[i]]));
             mbar_arrive(smem_u32(&sh->k_full[i][slot[i]]));
             mbar_arrive(smem_u32(&sh->raw_empty[rslot]));
           }
-          if (++islot == G::I_SLOTS) { islot = 0; iph ^= 1u; }
+          if (++islot[i] == G::I_SLOTS) { islot[i] = 0; iph[i] ^= 1u; }
           if (++slot[i] == K_SLOTS) { slot[i] = 0; ph[i] ^= 1u; }
           if (++rslot == G::RAW_SLOTS) { rslot = 0; rph ^= 1u; }
         }
@@ -633,7 +660,6 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     const int part = warp & 3;       // 32 keys of the tile
     const int r = threadIdx.x & 127; // key of the tile
     const uint32_t tS = tmem + (static_cast<uint32_t>(part * 32) << 16) + (i * 2 + buf) * QN;
-    const int size = 1 << p.seqs.page_log2;
     const int box_log2 = min(p.seqs.page_log2, 7);
     int islot = 0, lslot = -1, step = 0;  // (step: parity of the next one)
     uint32_t iph = 0, lph = 1, sph = 0, sum_ph = 0;
@@ -646,22 +672,19 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
       const int past = w.len - w.count;
       float old = 0.f, k2 = p.scale_log2;
       float* place = nullptr;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (x >= w.tiles) continue;
-        if (ok) ok = wait(sh->i_full[islot], iph);
-        if (ok) {
-          if (x == i && mine) {
-            const int page = sh->page[islot][r >> box_log2];
-            if (FP8) k2 *= sh->scale[islot][r];
-            if (last && w.slot < 0 && pos < w.len && page >= 0) {
-              place = p.weights + page * p.weights_stride[0] + w.head * p.weights_stride[1] + (pos & (size - 1));
-              if (!(p.reset_new && pos >= past)) old = fresh(place);
-            }
+      if (i < w.tiles) {
+        ok = wait(sh->i_full[i][islot], iph);
+        if (!ok) break;
+        if (mine) {
+          const int page = sh->page[i][islot][r >> box_log2];
+          if (FP8) k2 *= sh->scale[i][islot][r];
+          if (last && w.slot < 0 && pos < w.len && page >= 0) {
+            place = p.weights + page * p.weights_stride[0] + w.head * p.weights_stride[1] + (pos & (size - 1));
+            if (!(p.reset_new && pos >= past)) old = fresh(place);
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&sh->i_empty[islot]));
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh->i_empty[i][islot]));
         if (++islot == G::I_SLOTS) {
           islot = 0;
           iph ^= 1u;
@@ -689,23 +712,31 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
         const int ahead = pos - past - w.tok0(p, t);
         const int from = p.causal ? max(0, ahead) * p.group : 0;
         const int from_all = p.causal ? max(0, ahead - lane + 31) * p.group : 0;
-        const int from_any = p.causal ? max(0, ahead - lane) * p.group : 0;
+        const int from_any = p.causal ? max(0, ahead - lane) * p.group & ~31 : 0;
         const float* neg = sh->neg_lse[lslot];
 #pragma unroll 1
-        for (int c0 = from_any & ~31; c0 < live; c0 += 32) {
+        for (int c0 = from_any; c0 < live; c0 += 32) {
           float s[32];
           tmem_ld32(tS + c0, reinterpret_cast<uint32_t*>(s));
           tmem_wait_ld();
 #pragma unroll
           for (int u = 0; u < 32; ++u) asm volatile("" : "+f"(s[u]));
+          if (c0 + 32 >= live) {  // the last of the buffer is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh->s_empty[i][buf]));
+          }
           if (c0 >= from_all && c0 + 32 <= live) {
 #pragma unroll
             for (int u = 0; u < 32; u += 4) {
               const float4 l = *reinterpret_cast<const float4*>(neg + c0 + u);
               const float2 x = ffma2(make_float2(s[u], s[u + 1]), kk, make_float2(l.x, l.y));
               const float2 y = ffma2(make_float2(s[u + 2], s[u + 3]), kk, make_float2(l.z, l.w));
-              acc[u / 4 & 3] = fadd2(acc[u / 4 & 3], make_float2(ex2_approx(x.x), ex2_approx(x.y)));
-              acc[(u / 4 & 3) ^ 1] = fadd2(acc[(u / 4 & 3) ^ 1], make_float2(ex2_approx(y.x), ex2_approx(y.y)));
+              float2& a = acc[u / 4 & 3];
+              float2& b = acc[(u / 4 & 3) ^ 1];
+              a = fadd2(a, make_float2(ex2_approx(x.x), ex2_approx(x.y)));
+              if (FP8 || u / 4 % 2 != 0) b = fadd2(b, make_float2(ex2_approx(y.x), ex2_approx(y.y)));
+              else b = add_exp2_poly(y, b);
             }
           } else {
 #pragma unroll
@@ -720,9 +751,11 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
             }
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh->s_empty[i][buf]));
+        if (from_any >= live) {  // (nothing to read)
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh->s_empty[i][buf]));
+        }
       }
       if (!mine || !ok) continue;
       const float2 a = fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3]));
