@@ -80,15 +80,26 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
+// COLS: columns of the histogram, lane by lane: with 32 no two lanes of a warp meet in a word, with 4 there is
+// less to clear and add up.  CLUSTER: several CTAs share an item.
+template <int COLS, bool CLUSTER>
 __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __grid_constant__ EvictParams p) {
-  extern __shared__ uint32_t s_key[];
-  __shared__ uint32_t s_hist[kBins * 32];   // a column for each lane: no two of a warp meet
+  extern __shared__ uint32_t s_mem[];
+  uint32_t* const s_hist = s_mem;                                // [kBins][COLS]
+  uint4* const s_key4 = reinterpret_cast<uint4*>(s_mem + kBins * COLS);
+  const uint32_t* const s_key = s_mem + kBins * COLS;
   __shared__ uint32_t s_total[2][kBins];    // read by the cluster
   __shared__ uint32_t s_count[2];           // ... keys above the threshold, keys at it
-  __shared__ uint32_t s_found[2];           // digit, and how many are wanted at it
+  __shared__ uint32_t s_found[3];           // digit, how many are wanted at it, and how many there are
   __shared__ uint32_t s_warp[2][kSelectThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int cs = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_rank());
+  const int cs = CLUSTER ? static_cast<int>(cluster_size()) : 1;
+  const int rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0;
+  auto sync_all = [&]() {
+    if (CLUSTER) cluster_sync();
+    else __syncthreads();
+  };
+  auto of_cta = [&](const uint32_t& x, int c) -> uint32_t { return CLUSTER ? ld_cluster(smem_u32(&x), c) : x; };
   const int item = blockIdx.x / cs;
   const int b = item / p.heads, head = item - b * p.heads;
   let_next_launch();
@@ -110,44 +121,54 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
   for (int i = rank * kSelectThreads + tid; i < p.recent; i += cs * kSelectThreads) kept[want + i] = old + i;
   if (want == 0) return;
 
-  // this CTA's positions
+  // this CTA's positions, four at a time: they lie in one page, 16 bytes together
   const int share = ((old + cs - 1) / cs + 3) & ~3;
   const int lo = min(rank * share, old), count = min(share, old - lo);
-  auto from_memory = [&](int i) -> uint32_t {
-    const int pos = lo + i;
+  const int mask = (1 << p.seqs.page_log2) - 1;
+  auto from_memory = [&](int i4) -> uint4 {
+    const int pos = lo + 4 * i4;
     const int page = checked_page(p.seqs, page_entry(p.seqs, b, pos));
-    return order_of(fresh(p.weights + page * p.weights_stride[0] + head * p.weights_stride[1] +
-                          (pos & ((1 << p.seqs.page_log2) - 1))));
+    const float4 x = fresh(reinterpret_cast<const float4*>(p.weights + page * p.weights_stride[0] +
+                                                           head * p.weights_stride[1] + (pos & mask)));
+    return make_uint4(order_of(x.x), order_of(x.y), order_of(x.z), order_of(x.w));
   };
-  auto key = [&](int i) -> uint32_t { return i < p.cached ? s_key[i] : from_memory(i); };
-  const int in_shared = min(count, p.cached);
+  const int count4 = (count + 3) / 4, cached4 = min(count4, p.cached / 4);
+  auto keys = [&](int i4) -> uint4 { return i4 < cached4 ? s_key4[i4] : from_memory(i4); };
 #pragma unroll 4
-  for (int i = tid; i < in_shared; i += kSelectThreads) s_key[i] = from_memory(i);
+  for (int i = tid; i < cached4; i += kSelectThreads) s_key4[i] = from_memory(i);
 
+  // A key stays if its upper digits are above `found`, and of the keys that have them equal the first `left`.
   uint32_t found = 0, left = want;
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
-    for (int i = tid; i < kBins * 32; i += kSelectThreads) s_hist[i] = 0;
+  int shift = 32;
+  do {
+    shift -= 8;
+    const int turn = shift >> 3 & 1;
+    for (int i = tid; i < kBins * COLS; i += kSelectThreads) s_hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < count; i += kSelectThreads) {
-      const uint32_t k = key(i);
-      if (pass == 0 || (k ^ found) >> (shift + 8) == 0) atomicAdd(&s_hist[(k >> shift & 255) * 32 + lane], 1u);
+    for (int i = tid; i < count4; i += kSelectThreads) {
+      const uint4 k4 = keys(i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t k = (&k4.x)[j];
+        if (4 * i + j < count && (shift == 24 || (k ^ found) >> (shift + 8) == 0))
+          atomicAdd(&s_hist[(k >> shift & 255) * COLS + lane % COLS], 1u);
+      }
     }
     __syncthreads();
     if (tid < kBins) {
       uint32_t sum = 0;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) sum += s_hist[tid * 32 + ((j + lane) & 31)];
-      s_total[pass & 1][tid] = sum;
+      for (int j = 0; j < COLS; ++j) sum += s_hist[tid * COLS + (j + lane) % COLS];
+      s_total[turn][tid] = sum;
     }
-    cluster_sync();
+    sync_all();
     if (warp == 0) {  // a lane for 8 bins, the highest first
       uint32_t bins[8], sum = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int bin = kBins - 1 - (lane * 8 + j);
         bins[j] = 0;
-        for (int c = 0; c < cs; ++c) bins[j] += ld_cluster(smem_u32(&s_total[pass & 1][bin]), c);
+        for (int c = 0; c < cs; ++c) bins[j] += of_cta(s_total[turn][bin], c);
         sum += bins[j];
       }
       uint32_t upto = sum;
@@ -158,51 +179,63 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
       }
       uint32_t before = upto - sum;
       if (before < left && left <= upto) {  // one lane
-        int j = 0;
-        while (before + bins[j] < left) before += bins[j++];
-        s_found[0] = kBins - 1 - (lane * 8 + j);
-        s_found[1] = left - before;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (before < left && left <= before + bins[j]) {
+            s_found[0] = kBins - 1 - (lane * 8 + j);
+            s_found[1] = left - before;
+            s_found[2] = bins[j];
+          }
+          before += bins[j];
+        }
       }
     }
     __syncthreads();
     found |= s_found[0] << shift;
     left = s_found[1];
-  }
-  // `left` of the keys equal to `found` stay, the first ones, and all above it
+  } while (shift > 0 && left < s_found[2]);  // (all of a bin stay: its lower digits do not matter)
+  found >>= shift;
   uint32_t above = 0, equal = 0;
-  for (int i = tid; i < count; i += kSelectThreads) {
-    const uint32_t k = key(i);
-    above += k > found;
-    equal += k == found;
-  }
+  if (CLUSTER) {  // this CTA's numbers of them, for those behind it
+    for (int i = tid; i < count4; i += kSelectThreads) {
+      const uint4 k4 = keys(i);
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    above += __shfl_xor_sync(0xffffffffu, above, d);
-    equal += __shfl_xor_sync(0xffffffffu, equal, d);
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t k = (&k4.x)[j] >> shift;
+        above += 4 * i + j < count && k > found;
+        equal += 4 * i + j < count && k == found;
+      }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      above += __shfl_xor_sync(0xffffffffu, above, d);
+      equal += __shfl_xor_sync(0xffffffffu, equal, d);
+    }
+    if (lane == 0) {
+      s_warp[0][warp] = above;
+      s_warp[1][warp] = equal;
+    }
+    __syncthreads();
+    if (tid < 2) {
+      uint32_t sum = 0;
+      for (int w = 0; w < kSelectThreads / 32; ++w) sum += s_warp[tid][w];
+      s_count[tid] = sum;
+    }
+    cluster_sync();
   }
-  if (lane == 0) {
-    s_warp[0][warp] = above;
-    s_warp[1][warp] = equal;
-  }
-  __syncthreads();
-  if (tid < 2) {
-    uint32_t sum = 0;
-    for (int w = 0; w < kSelectThreads / 32; ++w) sum += s_warp[tid][w];
-    s_count[tid] = sum;
-  }
-  cluster_sync();
   above = equal = 0;  // those of the CTAs before
   for (int c = 0; c < rank; ++c) {
-    above += ld_cluster(smem_u32(&s_count[0]), c);
-    equal += ld_cluster(smem_u32(&s_count[1]), c);
+    above += of_cta(s_count[0], c);
+    equal += of_cta(s_count[1], c);
   }
   constexpr int kEach = 4;  // keys of a thread at a time
   for (int at = 0; at < count; at += kSelectThreads * kEach) {
     uint32_t k[kEach], mine = 0;  // above in the low half, equal in the high one
     const int i0 = at + tid * kEach;
+    const uint4 k4 = i0 < count ? keys(i0 / 4) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      k[j] = i0 + j < count ? key(i0 + j) : 0u;
+      k[j] = (&k4.x)[j] >> shift;
       if (i0 + j < count) mine += (k[j] > found) | (k[j] == found) << 16;
     }
     uint32_t upto = mine;
@@ -230,16 +263,24 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
     above += all & 0xffffu;
     equal += all >> 16;
   }
-  cluster_sync();  // nobody reads this CTA's shared memory any more
+  if (CLUSTER) cluster_sync();  // nobody reads this CTA's shared memory any more
 }
 
 // ------------------------------------------------------------------------------------ moving
 constexpr int kMoveThreads = 512;
 constexpr int kMoveUnroll = 4;
+constexpr int kMostRows = kMoveThreads * kMoveUnroll / 2;  // of a chunk (rows of 16 bytes: half of what they could be)
 
 // One block: (sequence, head), and a column slice of K or V, or the weights and scales.
+//
+// A chunk's ranks go through four stages, one turn of the loop each, so that no turn waits for more than one
+// load: positions, pages, rows into registers, rows into their places.  Positions and pages are looked up
+// once for a row and go through shared memory to the threads that share it.
 __global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __grid_constant__ EvictParams p) {
   constexpr int U = kMoveUnroll;
+  constexpr int EACH = kMostRows / kMoveThreads;  // rows that a thread looks up
+  __shared__ int64_t s_from[3][kMostRows];        // bytes from the head's first; < 0: stays, or has no place
+  __shared__ int s_to[3][kMostRows];              // page
   const int pieces = 2 * p.slices + 1;
   const int piece = blockIdx.x % pieces, item = blockIdx.x / pieces;
   const int b = item / p.heads, head = item - b * p.heads;
@@ -253,61 +294,112 @@ __global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __gri
     from = min(static_cast<int>(blockIdx.y) * each, stay);
     stay = min(from + each, stay);
   }
+  if (from >= stay) return;
   const int* const kept = p.kept + static_cast<int64_t>(item) * p.keep;
   const int mask = (1 << p.seqs.page_log2) - 1;
-  // source and destination of rank i: pages and slots; false: stays where it is, or has no place
-  auto place = [&](int i, int& page, int& slot, int& to_page) -> bool {
-    if (i >= stay) return false;
+  // position of rank i; -1: stays where it is
+  auto position = [&](int i) -> int {
+    if (i >= stay) return -1;
     const int pos = fresh(kept + i);
-    if (p.in_place && pos == i) return false;
+    if (static_cast<uint32_t>(pos) >= static_cast<uint32_t>(n)) {
+      report(p.seqs.status, kStatusPageTable);
+      return -1;
+    }
+    return p.in_place && pos == i ? -1 : pos;
+  };
+  // page that rank i goes to, or -1
+  auto page_to = [&](int i) -> int {
     const int col = i >> p.seqs.page_log2;
-    if (static_cast<uint32_t>(pos) >= static_cast<uint32_t>(n) || col >= p.to_cols) {
-      report(p.seqs.status, kStatusPageTable);
-      return false;
-    }
-    page = page_entry(p.seqs, b, pos);
-    to_page = fresh(p.to_table + b * p.to_stride + col);
-    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.seqs.num_pages) ||
-        static_cast<uint32_t>(to_page) >= static_cast<uint32_t>(p.seqs.num_pages)) {
-      report(p.seqs.status, kStatusPageTable);
-      return false;
-    }
-    slot = pos & mask;
-    return true;
+    return col < p.to_cols ? fresh(p.to_table + b * p.to_stride + col) : -1;
+  };
+  auto is_page = [&](int page) -> bool {
+    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.seqs.num_pages)) return true;
+    report(p.seqs.status, kStatusPageTable);
+    return false;
   };
   if (piece < 2 * p.slices) {
     const int kv = piece / p.slices, lanes = 1 << p.lanes_log2;
+    const int64_t st_page = p.cache_stride[kv][0], st_row = p.cache_stride[kv][2];
     char* const cache = static_cast<char*>(p.cache[kv]) + head * p.cache_stride[kv][1] +
                         ((piece % p.slices) * lanes + (threadIdx.x & (lanes - 1))) * 16;
-    const int rows = kMoveThreads >> p.lanes_log2;  // at a time
-    const int r0 = from + (threadIdx.x >> p.lanes_log2);
-    uint4 x[U], y[U];
-    int64_t to[U], to_next[U];  // < 0: nothing to write
-    auto load = [&](int at, uint4(&v)[U], int64_t(&dst)[U]) {
+    const int step = kMoveThreads >> p.lanes_log2;  // rows that the block takes at a time
+    const int rows = min(U * step, kMostRows);      // of a chunk
+    const int r0 = threadIdx.x >> p.lanes_log2;
+    const int tid = threadIdx.x;
+    int pos[EACH], page[EACH], to[EACH], pos_of[EACH];
+    auto positions = [&](int at) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = at + u * rows + r0 - from;
-        int page, slot, to_page;
-        dst[u] = -1;
-        if (place(i, page, slot, to_page)) {
-          v[u] = fresh(reinterpret_cast<const uint4*>(cache + page * p.cache_stride[kv][0] + slot * p.cache_stride[kv][2]));
-          dst[u] = to_page * p.cache_stride[kv][0] + (i & mask) * p.cache_stride[kv][2];
+      for (int e = 0; e < EACH; ++e)
+        pos[e] = tid + e * kMoveThreads < rows ? position(at + tid + e * kMoveThreads) : -1;
+    };
+    auto pages = [&](int at) {
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        pos_of[e] = pos[e];
+        page[e] = to[e] = -1;
+        if (pos[e] >= 0) {
+          page[e] = page_entry(p.seqs, b, pos[e]);
+          to[e] = page_to(at + tid + e * kMoveThreads);
         }
       }
     };
-    load(from, x, to);
-    for (int at = from; at < stay; at += U * rows) {
-      load(at + U * rows, y, to_next);
-      __syncthreads();  // the chunk has been read by all
+    auto publish = [&](int slot) {
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int r = tid + e * kMoveThreads;
+        if (r >= rows) continue;
+        const bool moves = pos_of[e] >= 0 && is_page(page[e]) && is_page(to[e]);
+        s_from[slot][r] = moves ? page[e] * st_page + (pos_of[e] & mask) * st_row : -1;
+        s_to[slot][r] = to[e];
+      }
+    };
+    uint4 x[U], y[U];
+    auto load = [&](int slot, uint4(&v)[U]) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (to[u] >= 0) *reinterpret_cast<uint4*>(cache + to[u]) = x[u];
-        x[u] = y[u];
-        to[u] = to_next[u];
+        const int r = r0 + u * step;
+        if (r < rows && s_from[slot][r] >= 0) v[u] = fresh(reinterpret_cast<const uint4*>(cache + s_from[slot][r]));
       }
+    };
+    positions(from);
+    pages(from);
+    publish(0);
+    positions(from + rows);
+    pages(from + rows);
+    positions(from + 2 * rows);
+    __syncthreads();
+    load(0, x);
+    int slot = 0;  // of the chunk that is written in this turn
+    auto turn = [&](int at, uint4(&now)[U], uint4(&then)[U]) {
+      const int next = slot == 2 ? 0 : slot + 1;
+      publish(next);
+      pages(at + 2 * rows);
+      positions(at + 3 * rows);
+      __syncthreads();  // the next chunk's places are there, and this one has been read by all
+      load(next, then);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = r0 + u * step;
+        if (r < rows && s_from[slot][r] >= 0)
+          *reinterpret_cast<uint4*>(cache + s_to[slot][r] * st_page + ((at + r) & mask) * st_row) = now[u];
+      }
+      slot = next;
+    };
+    for (int at = from; at < stay; at += 2 * rows) {
+      turn(at, x, y);
+      if (at + rows < stay) turn(at + rows, y, x);
     }
     return;
   }
+  // rank i's place in the weights and scales; false: stays where it is, or has no place
+  auto place = [&](int i, int& page, int& slot, int& to_page) -> bool {
+    const int pos = position(i);
+    if (pos < 0) return false;
+    page = page_entry(p.seqs, b, pos);
+    to_page = page_to(i);
+    slot = pos & mask;
+    return is_page(page) && is_page(to_page);
+  };
   for (int at = from; at < stay; at += kMoveThreads) {
     const int i = at + threadIdx.x;
     int page, slot, to_page;
@@ -378,14 +470,18 @@ int evict(const FaPagedEvictArgs* a, void* stream) {
   const int64_t items = c.seqs * c.heads_kv, capacity = c.table_cols * c.page_size;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
 
-  // A (sequence, head) gets more CTAs while they find an SM and have 2048 keys each.
+  // A (sequence, head) gets more CTAs while all of them find a place and have 2048 keys each.
   int cluster = 1;
-  while (cluster < kMostCluster && items * cluster * 2 <= sms && capacity > 2048 * cluster) cluster *= 2;
-  const int64_t share = (capacity + cluster - 1) / cluster + 4;
-  p.cached = static_cast<int>(std::min<int64_t>(share, 44 * 1024));  // 176 KB, 34 KB are the kernel's own
-  const int smem = p.cached * 4;
-  static SmemOptIn opt_in;
-  if (!opt_in(reinterpret_cast<const void*>(paged_select_kernel), 44 * 1024 * 4)) return FA_ERR_LAUNCH;
+  while (cluster < kMostCluster && items * cluster * 2 <= 2 * sms && capacity > 2048 * cluster) cluster *= 2;
+  const int64_t share = ((capacity + cluster - 1) / cluster + 3) / 4 * 4 + 4;
+  const int cols = share > 8192 ? 32 : 4;
+  constexpr int kMostBytes = 208 * 1024;
+  p.cached = static_cast<int>(std::min<int64_t>(share, (kMostBytes - 4 * kBins * cols) / 4));
+  const int smem = 4 * (p.cached + kBins * cols);
+  const auto kernel = cluster > 1 ? (cols == 32 ? paged_select_kernel<32, true> : paged_select_kernel<4, true>)
+                                  : (cols == 32 ? paged_select_kernel<32, false> : paged_select_kernel<4, false>);
+  static SmemOptIn opt_in[4];
+  if (!opt_in[2 * (cluster > 1) + (cols == 32)](reinterpret_cast<const void*>(kernel), kMostBytes)) return FA_ERR_LAUNCH;
   {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(items * cluster));
@@ -400,8 +496,8 @@ int evict(const FaPagedEvictArgs* a, void* stream) {
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    if (cudaLaunchKernelEx(&cfg, paged_select_kernel, p) != cudaSuccess) {
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
       (void)cudaGetLastError();
       return FA_ERR_LAUNCH;
     }
@@ -410,7 +506,7 @@ int evict(const FaPagedEvictArgs* a, void* stream) {
   // Slices: rows whole, or in parts of at least 32 bytes while that finds SMs without work.
   const int row_bytes = static_cast<int>(c.head_dim) * eb;
   p.slices = 1;
-  while (row_bytes / p.slices > 32 && items * 2 * p.slices < 2 * sms) p.slices *= 2;
+  while (row_bytes / p.slices > 32 && items * 2 * p.slices < sms) p.slices *= 2;
   p.lanes_log2 = log2_of(row_bytes / p.slices / 16);
   p.splits = 1;
   if (!p.in_place) {
