@@ -4,7 +4,7 @@
 // stay in their order: rank i goes to slot i.
 //
 // Two launches.  paged_select_kernel finds the ranks of a (sequence, head): the weight of the last token
-// that stays is found digit by digit from the top (four histograms of 8 bits), over keys that are read
+// that stays is found digit by digit from the top (histograms of 11, 11 and 10 bits), over keys that are read
 // from memory once and then lie in shared memory; an ordered scan then writes the positions that stay.  A
 // long sequence is shared by a cluster of up to 8 CTAs, which add their histograms up through distributed
 // shared memory.  paged_move_kernel moves the rows, bound by memory.
@@ -45,8 +45,7 @@ struct EvictParams {
 };
 
 // --------------------------------------------------------------------------------- selection
-constexpr int kSelectThreads = 512;
-constexpr int kBins = 256;
+constexpr int kBins = 2048;
 constexpr int kMostCluster = 8;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -80,18 +79,21 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
-// COLS: columns of the histogram, lane by lane: with 32 no two lanes of a warp meet in a word, with 4 there is
-// less to clear and add up.  CLUSTER: several CTAs share an item.
-template <int COLS, bool CLUSTER>
-__global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __grid_constant__ EvictParams p) {
-  extern __shared__ uint32_t s_mem[];
+// THREADS: 512, or 1024 for many keys, whose histogram has four columns then (lane by lane: fewer of a warp
+// meet in a word, where weights are alike).  CLUSTER: several CTAs share an item.
+template <int THREADS, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_constant__ EvictParams p) {
+  constexpr int COLS = THREADS == 1024 ? 4 : 1;
+  constexpr int EACH = kBins / THREADS;  // bins of a thread
+  constexpr int WARPS = THREADS / 32;
+  extern __shared__ __align__(16) uint32_t s_mem[];
   uint32_t* const s_hist = s_mem;                                // [kBins][COLS]
   uint4* const s_key4 = reinterpret_cast<uint4*>(s_mem + kBins * COLS);
   const uint32_t* const s_key = s_mem + kBins * COLS;
-  __shared__ uint32_t s_total[2][kBins];    // read by the cluster
+  __shared__ __align__(16) uint32_t s_total[2][kBins];  // read by the cluster
   __shared__ uint32_t s_count[2];           // ... keys above the threshold, keys at it
   __shared__ uint32_t s_found[3];           // digit, how many are wanted at it, and how many there are
-  __shared__ uint32_t s_warp[2][kSelectThreads / 32];
+  __shared__ uint32_t s_warp[2][WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cs = CLUSTER ? static_cast<int>(cluster_size()) : 1;
   const int rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0;
@@ -111,14 +113,14 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
     p.new_lens[b] = stay;
     if (fresh(p.seqs.kv_lens + b) != n) report(p.seqs.status, kStatusPageTable);
   }
-  for (int i = stay + rank * kSelectThreads + tid; i < p.keep; i += cs * kSelectThreads) kept[i] = -1;
+  for (int i = stay + rank * THREADS + tid; i < p.keep; i += cs * THREADS) kept[i] = -1;
   if (n <= p.keep) {  // (the whole cluster)
-    for (int i = rank * kSelectThreads + tid; i < n; i += cs * kSelectThreads) kept[i] = i;
+    for (int i = rank * THREADS + tid; i < n; i += cs * THREADS) kept[i] = i;
     return;
   }
   const int old = n - p.recent;             // positions that may go
   const uint32_t want = p.keep - p.recent;  // and how many of them stay
-  for (int i = rank * kSelectThreads + tid; i < p.recent; i += cs * kSelectThreads) kept[want + i] = old + i;
+  for (int i = rank * THREADS + tid; i < p.recent; i += cs * THREADS) kept[want + i] = old + i;
   if (want == 0) return;
 
   // this CTA's positions, four at a time: they lie in one page, 16 bytes together
@@ -135,59 +137,70 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
   const int count4 = (count + 3) / 4, cached4 = min(count4, p.cached / 4);
   auto keys = [&](int i4) -> uint4 { return i4 < cached4 ? s_key4[i4] : from_memory(i4); };
 #pragma unroll 4
-  for (int i = tid; i < cached4; i += kSelectThreads) s_key4[i] = from_memory(i);
+  for (int i = tid; i < cached4; i += THREADS) s_key4[i] = from_memory(i);
 
   // A key stays if its upper digits are above `found`, and of the keys that have them equal the first `left`.
   uint32_t found = 0, left = want;
-  int shift = 32;
-  do {
-    shift -= 8;
-    const int turn = shift >> 3 & 1;
-    for (int i = tid; i < kBins * COLS; i += kSelectThreads) s_hist[i] = 0;
+  int shift = 32, turn = 0;
+  do {  // digits of 11, 11 and 10 bits
+    const int bits = min(shift, 11);
+    const int above_bits = shift;
+    shift -= bits;
+    turn ^= 1;
+    for (int i = tid; i < kBins * COLS / 4; i += THREADS) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int i = tid; i < count4; i += kSelectThreads) {
+    for (int i = tid; i < count4; i += THREADS) {
       const uint4 k4 = keys(i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t k = (&k4.x)[j];
-        if (4 * i + j < count && (shift == 24 || (k ^ found) >> (shift + 8) == 0))
-          atomicAdd(&s_hist[(k >> shift & 255) * COLS + lane % COLS], 1u);
+        if (4 * i + j < count && (above_bits == 32 || (k ^ found) >> above_bits == 0))
+          atomicAdd(&s_hist[(k >> shift & ((1u << bits) - 1)) * COLS + lane % COLS], 1u);
       }
     }
     __syncthreads();
-    if (tid < kBins) {
-      uint32_t sum = 0;
+    // a thread's bins, the highest first: EACH of them below bin `top`
+    const int top = kBins - 1 - tid * EACH;
+    uint32_t bins[EACH], sum = 0;
 #pragma unroll
-      for (int j = 0; j < COLS; ++j) sum += s_hist[tid * COLS + (j + lane) % COLS];
-      s_total[turn][tid] = sum;
+    for (int j = 0; j < EACH; ++j) {
+      if constexpr (COLS == 4) {
+        const uint4 x = reinterpret_cast<const uint4*>(s_hist)[top - j];
+        bins[j] = x.x + x.y + x.z + x.w;
+      } else {
+        bins[j] = s_hist[top - j];
+      }
+      if (CLUSTER) s_total[turn][top - j] = bins[j];
     }
-    sync_all();
-    if (warp == 0) {  // a lane for 8 bins, the highest first
-      uint32_t bins[8], sum = 0;
+    if (CLUSTER) {
+      cluster_sync();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int bin = kBins - 1 - (lane * 8 + j);
-        bins[j] = 0;
-        for (int c = 0; c < cs; ++c) bins[j] += of_cta(s_total[turn][bin], c);
-        sum += bins[j];
-      }
-      uint32_t upto = sum;
+      for (int j = 0; j < EACH; ++j)
+        for (int c = 0; c < cs; ++c)
+          if (c != rank) bins[j] += of_cta(s_total[turn][top - j], c);
+    }
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += v;
-      }
-      uint32_t before = upto - sum;
-      if (before < left && left <= upto) {  // one lane
+    for (int j = 0; j < EACH; ++j) sum += bins[j];
+    uint32_t upto = sum;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (before < left && left <= before + bins[j]) {
-            s_found[0] = kBins - 1 - (lane * 8 + j);
-            s_found[1] = left - before;
-            s_found[2] = bins[j];
-          }
-          before += bins[j];
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += v;
+    }
+    if (lane == 31) s_warp[0][warp] = upto;
+    __syncthreads();
+    uint32_t before = upto - sum;
+#pragma unroll
+    for (int x = 0; x < WARPS; ++x) before += x < warp ? s_warp[0][x] : 0;
+    if (before < left && left <= before + sum) {  // one thread
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) {
+        if (before < left && left <= before + bins[j]) {
+          s_found[0] = top - j;
+          s_found[1] = left - before;
+          s_found[2] = bins[j];
         }
+        before += bins[j];
       }
     }
     __syncthreads();
@@ -197,7 +210,7 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
   found >>= shift;
   uint32_t above = 0, equal = 0;
   if (CLUSTER) {  // this CTA's numbers of them, for those behind it
-    for (int i = tid; i < count4; i += kSelectThreads) {
+    for (int i = tid; i < count4; i += THREADS) {
       const uint4 k4 = keys(i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -218,7 +231,7 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
     __syncthreads();
     if (tid < 2) {
       uint32_t sum = 0;
-      for (int w = 0; w < kSelectThreads / 32; ++w) sum += s_warp[tid][w];
+      for (int w = 0; w < WARPS; ++w) sum += s_warp[tid][w];
       s_count[tid] = sum;
     }
     cluster_sync();
@@ -229,7 +242,7 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
     equal += of_cta(s_count[1], c);
   }
   constexpr int kEach = 4;  // keys of a thread at a time
-  for (int at = 0; at < count; at += kSelectThreads * kEach) {
+  for (int at = 0; at < count; at += THREADS * kEach) {
     uint32_t k[kEach], mine = 0;  // above in the low half, equal in the high one
     const int i0 = at + tid * kEach;
     const uint4 k4 = i0 < count ? keys(i0 / 4) : make_uint4(0, 0, 0, 0);
@@ -249,7 +262,7 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
     __syncthreads();
     uint32_t before = upto - mine, all = 0;
 #pragma unroll
-    for (int w = 0; w < kSelectThreads / 32; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       if (w < warp) before += s_warp[0][w];
       all += s_warp[0][w];
     }
@@ -297,15 +310,14 @@ __global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __gri
   if (from >= stay) return;
   const int* const kept = p.kept + static_cast<int64_t>(item) * p.keep;
   const int mask = (1 << p.seqs.page_log2) - 1;
-  // position of rank i; -1: stays where it is
-  auto position = [&](int i) -> int {
-    if (i >= stay) return -1;
-    const int pos = fresh(kept + i);
-    if (static_cast<uint32_t>(pos) >= static_cast<uint32_t>(n)) {
-      report(p.seqs.status, kStatusPageTable);
-      return -1;
-    }
-    return p.in_place && pos == i ? -1 : pos;
+  // Position of rank i, not looked at yet (a stage may not wait for its own loads); and what it says: -1, the
+  // rank stays where it is.
+  auto position = [&](int i) -> int { return i < stay ? fresh(kept + i) : -1; };
+  auto moving = [&](int pos, int i) -> int {
+    if (i >= stay || (p.in_place && pos == i)) return -1;
+    if (static_cast<uint32_t>(pos) < static_cast<uint32_t>(n)) return pos;
+    report(p.seqs.status, kStatusPageTable);
+    return -1;
   };
   // page that rank i goes to, or -1
   auto page_to = [&](int i) -> int {
@@ -335,11 +347,12 @@ __global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __gri
     auto pages = [&](int at) {
 #pragma unroll
       for (int e = 0; e < EACH; ++e) {
-        pos_of[e] = pos[e];
+        const int i = at + tid + e * kMoveThreads;
+        pos_of[e] = tid + e * kMoveThreads < rows ? moving(pos[e], i) : -1;
         page[e] = to[e] = -1;
-        if (pos[e] >= 0) {
-          page[e] = page_entry(p.seqs, b, pos[e]);
-          to[e] = page_to(at + tid + e * kMoveThreads);
+        if (pos_of[e] >= 0) {
+          page[e] = page_entry(p.seqs, b, pos_of[e]);
+          to[e] = page_to(i);
         }
       }
     };
@@ -391,34 +404,46 @@ __global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __gri
     }
     return;
   }
-  // rank i's place in the weights and scales; false: stays where it is, or has no place
-  auto place = [&](int i, int& page, int& slot, int& to_page) -> bool {
-    const int pos = position(i);
-    if (pos < 0) return false;
-    page = page_entry(p.seqs, b, pos);
-    to_page = page_to(i);
-    slot = pos & mask;
-    return is_page(page) && is_page(to_page);
-  };
-  for (int at = from; at < stay; at += kMoveThreads) {
-    const int i = at + threadIdx.x;
-    int page, slot, to_page;
-    const bool moves = place(i, page, slot, to_page);
-    float w = 0.f, s[2] = {0.f, 0.f};
-    if (moves) {
-      w = fresh(p.weights + page * p.weights_stride[0] + head * p.weights_stride[1] + slot);
+  // The weights and scales: a float each, eight ranks to a thread at a time.
+  constexpr int M = 8;
+  for (int at = from; at < stay; at += M * kMoveThreads) {
+    int pos[M], page[M], to[M];
+    float w[M], s[2][M];
+#pragma unroll
+    for (int e = 0; e < M; ++e) pos[e] = position(at + threadIdx.x + e * kMoveThreads);
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+      pos[e] = moving(pos[e], at + threadIdx.x + e * kMoveThreads);
+      page[e] = to[e] = 0;
+      if (pos[e] >= 0) {
+        page[e] = page_entry(p.seqs, b, pos[e]);
+        to[e] = page_to(at + threadIdx.x + e * kMoveThreads);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+      if (pos[e] < 0) continue;
+      if (!is_page(page[e]) || !is_page(to[e])) {
+        pos[e] = -1;
+        continue;
+      }
+      const int slot = pos[e] & mask;
+      w[e] = fresh(p.weights + page[e] * p.weights_stride[0] + head * p.weights_stride[1] + slot);
       if (p.scale[0])
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv)
-          s[kv] = fresh(p.scale[kv] + page * p.scale_stride[kv][0] + head * p.scale_stride[kv][1] + slot);
+          s[kv][e] = fresh(p.scale[kv] + page[e] * p.scale_stride[kv][0] + head * p.scale_stride[kv][1] + slot);
     }
     __syncthreads();
-    if (moves) {
-      p.weights[to_page * p.weights_stride[0] + head * p.weights_stride[1] + (i & mask)] = w;
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+      if (pos[e] < 0) continue;
+      const int slot = (at + threadIdx.x + e * kMoveThreads) & mask;
+      p.weights[to[e] * p.weights_stride[0] + head * p.weights_stride[1] + slot] = w[e];
       if (p.scale[0])
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv)
-          p.scale[kv][to_page * p.scale_stride[kv][0] + head * p.scale_stride[kv][1] + (i & mask)] = s[kv];
+          p.scale[kv][to[e] * p.scale_stride[kv][0] + head * p.scale_stride[kv][1] + slot] = s[kv][e];
     }
   }
 }
@@ -474,18 +499,19 @@ int evict(const FaPagedEvictArgs* a, void* stream) {
   int cluster = 1;
   while (cluster < kMostCluster && items * cluster * 2 <= 2 * sms && capacity > 2048 * cluster) cluster *= 2;
   const int64_t share = ((capacity + cluster - 1) / cluster + 3) / 4 * 4 + 4;
-  const int cols = share > 8192 ? 32 : 4;
-  constexpr int kMostBytes = 208 * 1024;
+  const bool many = share > 8192;
+  const int cols = many ? 4 : 1, threads = many ? 1024 : 512;
+  constexpr int kMostBytes = 200 * 1024;  // (16 KB more are the kernel's own)
   p.cached = static_cast<int>(std::min<int64_t>(share, (kMostBytes - 4 * kBins * cols) / 4));
   const int smem = 4 * (p.cached + kBins * cols);
-  const auto kernel = cluster > 1 ? (cols == 32 ? paged_select_kernel<32, true> : paged_select_kernel<4, true>)
-                                  : (cols == 32 ? paged_select_kernel<32, false> : paged_select_kernel<4, false>);
+  const auto kernel = cluster > 1 ? (many ? paged_select_kernel<1024, true> : paged_select_kernel<512, true>)
+                                  : (many ? paged_select_kernel<1024, false> : paged_select_kernel<512, false>);
   static SmemOptIn opt_in[4];
-  if (!opt_in[2 * (cluster > 1) + (cols == 32)](reinterpret_cast<const void*>(kernel), kMostBytes)) return FA_ERR_LAUNCH;
+  if (!opt_in[2 * (cluster > 1) + many](reinterpret_cast<const void*>(kernel), kMostBytes)) return FA_ERR_LAUNCH;
   {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(items * cluster));
-    cfg.blockDim = dim3(kSelectThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -512,8 +538,10 @@ int evict(const FaPagedEvictArgs* a, void* stream) {
   if (!p.in_place) {
     p.slices = 1;
     p.lanes_log2 = log2_of(row_bytes / 16);
+    // ranges of ranks while there are SMs without a pair of blocks: a block's start costs three latencies
     const int64_t chunk = kMoveThreads * kMoveUnroll >> p.lanes_log2;
-    p.splits = static_cast<int>(std::min<int64_t>((p.keep + 2 * chunk - 1) / (2 * chunk), 1024));
+    p.splits = static_cast<int>(
+        std::max<int64_t>(1, std::min({(2 * sms + 2 * items - 1) / (2 * items), (p.keep + chunk - 1) / chunk, int64_t{1024}})));
   }
   const dim3 grid(static_cast<unsigned>(items * (2 * p.slices + 1)), static_cast<unsigned>(p.splits));
   return launch_dependent(paged_move_kernel, grid, kMoveThreads, 0, s, p);
