@@ -53,6 +53,7 @@ EXPORTED_SYMBOLS = (
     "fa_paged_weights_sm100",
     "fa_paged_weights_workspace_bytes",
     "fa_paged_evict_sm100",
+    "fa_paged_evict_workspace_bytes",
 )
 
 
@@ -198,7 +199,7 @@ def load() -> ctypes.CDLL:
             fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
             fn.restype = ctypes.c_int
         for name in ("fa_paged_workspace_bytes", "fa_paged_prefix_workspace_bytes",
-                     "fa_paged_weights_workspace_bytes"):
+                     "fa_paged_weights_workspace_bytes", "fa_paged_evict_workspace_bytes"):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.c_void_p]
             fn.restype = ctypes.c_int64

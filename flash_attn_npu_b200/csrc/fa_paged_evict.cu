@@ -9,10 +9,12 @@
 // long sequence is shared by a cluster of up to 8 CTAs, which add their histograms up through distributed
 // shared memory.  paged_move_kernel moves the rows, bound by memory.
 //
-// In place: slot i is written by rank i and read by a rank <= i, as rank(s) <= s.  So a CTA that goes
-// through the ranks in order, a chunk at a time, may write a chunk once it has read it and all before it,
-// and may read any number of chunks ahead.  CTAs that must not wait for one another take different columns
-// of the rows.
+// In place: slot i is written by rank i and read by rank(i) <= i.  A block that goes through the ranks in order,
+// a chunk at a time, may write a chunk once it has read it and all before it, and may read any number of chunks
+// ahead.  Where there are too few such blocks, a block moves one chunk of ranks: it reads
+// them into registers, says so (a flag for each chunk), and writes them once all chunks before it have been
+// read.  Blocks take their chunks in the order of a ticket and none waits before it has said so, so whatever a
+// block waits for is already being read.
 #include <algorithm>
 
 #include "fa_paged_host.h"
@@ -39,9 +41,11 @@ struct EvictParams {
   int64_t cache_stride[2][3];  // bytes
   float* scale[2];             // null: 16-bit cache
   int64_t scale_stride[2][2];
-  int slices;      // column slices of a row of K or V
-  int lanes_log2;  // 16-byte pieces of a slice
-  int splits;      // ranges of ranks (not in place)
+  int lanes_log2;   // 16-byte pieces of a row of K or V
+  int rows;         // of a chunk of K or V
+  int chunks[2];    // of K and of V; of the weights and scales
+  uint32_t* flags;  // [seqs * heads][2 * chunks[0] + chunks[1]]: the chunk has been read
+  uint32_t* ticket;
 };
 
 // --------------------------------------------------------------------------------- selection
@@ -89,7 +93,6 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
   extern __shared__ __align__(16) uint32_t s_mem[];
   uint32_t* const s_hist = s_mem;                                // [kBins][COLS]
   uint4* const s_key4 = reinterpret_cast<uint4*>(s_mem + kBins * COLS);
-  const uint32_t* const s_key = s_mem + kBins * COLS;
   __shared__ __align__(16) uint32_t s_total[2][kBins];  // read by the cluster
   __shared__ uint32_t s_count[2];           // ... keys above the threshold, keys at it
   __shared__ uint32_t s_found[3];           // digit, how many are wanted at it, and how many there are
@@ -112,6 +115,11 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
   if (rank == 0 && head == 0 && tid == 0) {
     p.new_lens[b] = stay;
     if (fresh(p.seqs.kv_lens + b) != n) report(p.seqs.status, kStatusPageTable);
+  }
+  if (p.flags && rank == 0) {
+    const int units = 2 * p.chunks[0] + p.chunks[1];
+    for (int i = tid; i < units; i += THREADS) p.flags[static_cast<int64_t>(item) * units + i] = 0;
+    if (blockIdx.x == 0 && tid == 0) *p.ticket = 0;
   }
   for (int i = stay + rank * THREADS + tid; i < p.keep; i += cs * THREADS) kept[i] = -1;
   if (n <= p.keep) {  // (the whole cluster)
@@ -142,6 +150,22 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
   // A key stays if its upper digits are above `found`, and of the keys that have them equal the first `left`.
   uint32_t found = 0, left = want;
   int shift = 32, turn = 0;
+  uint32_t above = 0, equal = 0;  // of this thread's bins: keys of the CTA above and at the digits found
+  // Sum over the warps before this one, and over all, of what lane 31 of each holds.
+  auto scan_warps = [&](uint32_t last, uint32_t& all) -> uint32_t {
+    __syncthreads();
+    if (lane == 31) s_warp[0][warp] = last;
+    __syncthreads();
+    uint32_t v = lane < WARPS ? s_warp[0][lane] : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += u;
+    }
+    all = __shfl_sync(0xffffffffu, v, 31);
+    const uint32_t before = __shfl_sync(0xffffffffu, v, (warp + 31) & 31);
+    return warp == 0 ? 0u : before;
+  };
   do {  // digits of 11, 11 and 10 bits
     const int bits = min(shift, 11);
     const int above_bits = shift;
@@ -161,7 +185,7 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
     __syncthreads();
     // a thread's bins, the highest first: EACH of them below bin `top`
     const int top = kBins - 1 - tid * EACH;
-    uint32_t bins[EACH], sum = 0;
+    uint32_t bins[EACH], own[EACH], sum = 0;
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
       if constexpr (COLS == 4) {
@@ -170,6 +194,7 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
       } else {
         bins[j] = s_hist[top - j];
       }
+      own[j] = bins[j];
       if (CLUSTER) s_total[turn][top - j] = bins[j];
     }
     if (CLUSTER) {
@@ -187,11 +212,8 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
       const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += v;
     }
-    if (lane == 31) s_warp[0][warp] = upto;
-    __syncthreads();
-    uint32_t before = upto - sum;
-#pragma unroll
-    for (int x = 0; x < WARPS; ++x) before += x < warp ? s_warp[0][x] : 0;
+    uint32_t all;
+    uint32_t before = upto - sum + scan_warps(upto, all);
     if (before < left && left <= before + sum) {  // one thread
 #pragma unroll
       for (int j = 0; j < EACH; ++j) {
@@ -206,24 +228,20 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
     __syncthreads();
     found |= s_found[0] << shift;
     left = s_found[1];
+#pragma unroll
+    for (int j = 0; CLUSTER && j < EACH; ++j) {
+      above += top - j > static_cast<int>(s_found[0]) ? own[j] : 0;
+      equal = top - j == static_cast<int>(s_found[0]) ? own[j] : j == 0 ? 0 : equal;
+    }
   } while (shift > 0 && left < s_found[2]);  // (all of a bin stay: its lower digits do not matter)
   found >>= shift;
-  uint32_t above = 0, equal = 0;
-  if (CLUSTER) {  // this CTA's numbers of them, for those behind it
-    for (int i = tid; i < count4; i += THREADS) {
-      const uint4 k4 = keys(i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t k = (&k4.x)[j] >> shift;
-        above += 4 * i + j < count && k > found;
-        equal += 4 * i + j < count && k == found;
-      }
-    }
+  if (CLUSTER) {  // this CTA's numbers, for those behind it
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
       above += __shfl_xor_sync(0xffffffffu, above, d);
       equal += __shfl_xor_sync(0xffffffffu, equal, d);
     }
+    __syncthreads();
     if (lane == 0) {
       s_warp[0][warp] = above;
       s_warp[1][warp] = equal;
@@ -241,14 +259,17 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
     above += of_cta(s_count[0], c);
     equal += of_cta(s_count[1], c);
   }
-  constexpr int kEach = 4;  // keys of a thread at a time
+  constexpr int kEach = 8;  // keys of a thread at a time
   for (int at = 0; at < count; at += THREADS * kEach) {
     uint32_t k[kEach], mine = 0;  // above in the low half, equal in the high one
     const int i0 = at + tid * kEach;
-    const uint4 k4 = i0 < count ? keys(i0 / 4) : make_uint4(0, 0, 0, 0);
+    uint4 k4[kEach / 4];
+#pragma unroll
+    for (int j = 0; j < kEach / 4; ++j)
+      k4[j] = i0 + 4 * j < count ? keys(i0 / 4 + j) : make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-      k[j] = (&k4.x)[j] >> shift;
+      k[j] = (&k4[j / 4].x)[j % 4] >> shift;
       if (i0 + j < count) mine += (k[j] > found) | (k[j] == found) << 16;
     }
     uint32_t upto = mine;
@@ -257,15 +278,8 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
       const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += v;
     }
-    __syncthreads();
-    if (lane == 31) s_warp[0][warp] = upto;
-    __syncthreads();
-    uint32_t before = upto - mine, all = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) before += s_warp[0][w];
-      all += s_warp[0][w];
-    }
+    uint32_t all;
+    const uint32_t before = upto - mine + scan_warps(upto, all);
     uint32_t a = above + (before & 0xffffu), e = equal + (before >> 16);
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
@@ -281,40 +295,178 @@ __global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_cons
 
 // ------------------------------------------------------------------------------------ moving
 constexpr int kMoveThreads = 512;
-constexpr int kMoveUnroll = 4;
-constexpr int kMostRows = kMoveThreads * kMoveUnroll / 2;  // of a chunk (rows of 16 bytes: half of what they could be)
+constexpr int kMoveUnroll = 4;                            // 16-byte pieces of a thread
+constexpr int kMoveRows = kMoveThreads * kMoveUnroll;     // of the smallest rows: the most of a chunk
+constexpr int kMetaUnroll = 4;                            // ranks of a thread, of the weights and scales
 
-// One block: (sequence, head), and a column slice of K or V, or the weights and scales.
+// One block moves one chunk of ranks of a (sequence, head): of K, of V, or of the weights and scales.
+__global__ void __launch_bounds__(kMoveThreads, 3) paged_move_kernel(const __grid_constant__ EvictParams p) {
+  constexpr int U = kMoveUnroll, M = kMetaUnroll;
+  __shared__ int64_t s_from[kMoveRows];  // bytes from the head's first; < 0: stays, or has no place
+  __shared__ int s_to[kMoveRows];        // page
+  __shared__ uint32_t s_unit;
+  __shared__ int s_gave_up;
+  const int tid = threadIdx.x;
+  const int units = 2 * p.chunks[0] + p.chunks[1];
+  let_next_launch();
+  wait_for_launch_before();
+  if (tid == 0) {
+    s_unit = p.in_place ? atomicAdd(p.ticket, 1u) : blockIdx.x;
+    s_gave_up = 0;
+  }
+  __syncthreads();
+  const int item = s_unit / units, unit = s_unit - item * units;
+  const int kind = min(unit / p.chunks[0], 2), chunk = unit - kind * p.chunks[0];
+  const int b = item / p.heads, head = item - b * p.heads;
+  const int n = seq_len(p.seqs, b);
+  const int rows = kind < 2 ? p.rows : M * kMoveThreads;
+  const int at = chunk * rows, stay = min(n, p.keep);
+  if (at >= stay || (p.in_place && n <= p.keep)) return;
+  const int* const kept = p.kept + static_cast<int64_t>(item) * p.keep;
+  const int mask = (1 << p.seqs.page_log2) - 1;
+  // page that rank i goes to, or -1
+  auto page_to = [&](int i) -> int {
+    const int col = i >> p.seqs.page_log2;
+    return col < p.to_cols ? fresh(p.to_table + b * p.to_stride + col) : -1;
+  };
+  auto is_page = [&](int page) -> bool {
+    if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.seqs.num_pages)) return true;
+    report(p.seqs.status, kStatusPageTable);
+    return false;
+  };
+  // Rank i's position, its page, and the page it goes to; false: it stays where it is, or has no place.
+  auto place = [&](int i, int& pos, int& page, int& to) -> bool {
+    if (i >= stay) return false;
+    pos = fresh(kept + i);
+    if (p.in_place && pos == i) return false;
+    if (static_cast<uint32_t>(pos) >= static_cast<uint32_t>(n)) {
+      report(p.seqs.status, kStatusPageTable);
+      return false;
+    }
+    page = page_entry(p.seqs, b, pos);
+    to = page_to(i);
+    return is_page(page) && is_page(to);
+  };
+  // Says that this chunk has been read, and waits until all before it have been: false if that took too long.
+  // `seen` depends on all that the thread has read, so the barrier is behind the reads themselves.
+  auto read_by_all = [&](bool seen) -> bool {
+    __syncthreads_or(seen);
+    if (!p.in_place) return true;
+    uint32_t* const flags = p.flags + static_cast<int64_t>(item) * units + kind * p.chunks[0];
+    if (tid == 0) {
+      __threadfence();
+      asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flags + chunk), "r"(1u) : "memory");
+    }
+    const uint64_t t0 = globaltimer_ns();
+    for (int c = tid; c < chunk; c += kMoveThreads) {
+      uint32_t read = 0;
+      while (true) {
+        asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(read) : "l"(flags + c) : "memory");
+        if (read) break;
+        if (globaltimer_ns() - t0 >= FA_WAIT_TIMEOUT_NS) {
+          report(p.seqs.status, kStatusTimeout);
+          s_gave_up = 1;
+          break;
+        }
+      }
+      if (!read) break;
+    }
+    __threadfence();  // (the flags were seen before anything is written)
+    __syncthreads();
+    return s_gave_up == 0;
+  };
+  if (kind < 2) {
+    const int lanes = 1 << p.lanes_log2;
+    const int64_t st_page = p.cache_stride[kind][0], st_row = p.cache_stride[kind][2];
+    char* const cache =
+        static_cast<char*>(p.cache[kind]) + head * p.cache_stride[kind][1] + (tid & (lanes - 1)) * 16;
+    for (int r = tid; r < rows; r += kMoveThreads) {
+      int pos, page, to = 0;
+      const bool moves = place(at + r, pos, page, to);
+      s_from[r] = moves ? page * st_page + (pos & mask) * st_row : -1;
+      s_to[r] = to;
+    }
+    __syncthreads();
+    const int step = kMoveThreads >> p.lanes_log2, r0 = tid >> p.lanes_log2;
+    uint4 x[U];
+    uint32_t any = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      x[u] = make_uint4(0, 0, 0, 0);
+      const int64_t from = s_from[r0 + u * step];
+      if (from >= 0) x[u] = fresh(reinterpret_cast<const uint4*>(cache + from));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) any |= x[u].x | x[u].y | x[u].z | x[u].w;
+    if (!read_by_all(any != 0)) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * step;
+      if (s_from[r] >= 0)
+        *reinterpret_cast<uint4*>(cache + s_to[r] * st_page + ((at + r) & mask) * st_row) = x[u];
+    }
+    return;
+  }
+  int to[M];
+  float w[M], sc[2][M];
+  uint32_t any = 0;
+#pragma unroll
+  for (int e = 0; e < M; ++e) {
+    int pos, page;
+    w[e] = sc[0][e] = sc[1][e] = 0.f;
+    if (!place(at + tid + e * kMoveThreads, pos, page, to[e])) {
+      to[e] = -1;
+      continue;
+    }
+    const int slot = pos & mask;
+    w[e] = fresh(p.weights + page * p.weights_stride[0] + head * p.weights_stride[1] + slot);
+    if (p.scale[0])
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+        sc[kv][e] = fresh(p.scale[kv] + page * p.scale_stride[kv][0] + head * p.scale_stride[kv][1] + slot);
+  }
+#pragma unroll
+  for (int e = 0; e < M; ++e) any |= __float_as_uint(w[e]) | __float_as_uint(sc[0][e]) | __float_as_uint(sc[1][e]);
+  if (!read_by_all(any != 0)) return;
+#pragma unroll
+  for (int e = 0; e < M; ++e) {
+    if (to[e] < 0) continue;
+    const int slot = (at + tid + e * kMoveThreads) & mask;
+    p.weights[to[e] * p.weights_stride[0] + head * p.weights_stride[1] + slot] = w[e];
+    if (p.scale[0])
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+        p.scale[kv][to[e] * p.scale_stride[kv][0] + head * p.scale_stride[kv][1] + slot] = sc[kv][e];
+  }
+}
+
+// In place, where there are (sequence, head) pairs enough: one block moves all of K, of V, or of the weights
+// and scales, chunk by chunk in order, so it needs no flags.
 //
 // A chunk's ranks go through four stages, one turn of the loop each, so that no turn waits for more than one
 // load: positions, pages, rows into registers, rows into their places.  Positions and pages are looked up
 // once for a row and go through shared memory to the threads that share it.
-__global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __grid_constant__ EvictParams p) {
+// EACH: rows that a thread looks up, 1 where rows have 64 bytes at least.
+template <int EACH>
+__global__ void __launch_bounds__(kMoveThreads, 2) paged_move_in_order_kernel(const __grid_constant__ EvictParams p) {
   constexpr int U = kMoveUnroll;
-  constexpr int EACH = kMostRows / kMoveThreads;  // rows that a thread looks up
-  __shared__ int64_t s_from[3][kMostRows];        // bytes from the head's first; < 0: stays, or has no place
-  __shared__ int s_to[3][kMostRows];              // page
-  const int pieces = 2 * p.slices + 1;
-  const int piece = blockIdx.x % pieces, item = blockIdx.x / pieces;
+  constexpr int ROWS = EACH * kMoveThreads;   // (rows of 16 bytes: half of what they could be)
+  __shared__ int64_t s_from[3][ROWS];         // bytes from the head's first; < 0: stays, or has no place
+  __shared__ int s_to[3][ROWS];               // page
+  const int kind = blockIdx.x % 3, item = blockIdx.x / 3;
   const int b = item / p.heads, head = item - b * p.heads;
   let_next_launch();
   wait_for_launch_before();
   const int n = seq_len(p.seqs, b);
-  if (p.in_place && n <= p.keep) return;
-  int stay = min(n, p.keep), from = 0;
-  if (p.splits > 1) {  // (not in place)
-    const int each = (stay + p.splits - 1) / p.splits;
-    from = min(static_cast<int>(blockIdx.y) * each, stay);
-    stay = min(from + each, stay);
-  }
-  if (from >= stay) return;
+  if (n <= p.keep) return;
+  const int stay = p.keep;
   const int* const kept = p.kept + static_cast<int64_t>(item) * p.keep;
   const int mask = (1 << p.seqs.page_log2) - 1;
   // Position of rank i, not looked at yet (a stage may not wait for its own loads); and what it says: -1, the
   // rank stays where it is.
   auto position = [&](int i) -> int { return i < stay ? fresh(kept + i) : -1; };
   auto moving = [&](int pos, int i) -> int {
-    if (i >= stay || (p.in_place && pos == i)) return -1;
+    if (i >= stay || pos == i) return -1;
     if (static_cast<uint32_t>(pos) < static_cast<uint32_t>(n)) return pos;
     report(p.seqs.status, kStatusPageTable);
     return -1;
@@ -329,13 +481,13 @@ __global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __gri
     report(p.seqs.status, kStatusPageTable);
     return false;
   };
-  if (piece < 2 * p.slices) {
-    const int kv = piece / p.slices, lanes = 1 << p.lanes_log2;
-    const int64_t st_page = p.cache_stride[kv][0], st_row = p.cache_stride[kv][2];
-    char* const cache = static_cast<char*>(p.cache[kv]) + head * p.cache_stride[kv][1] +
-                        ((piece % p.slices) * lanes + (threadIdx.x & (lanes - 1))) * 16;
+  if (kind < 2) {
+    const int lanes = 1 << p.lanes_log2;
+    const int64_t st_page = p.cache_stride[kind][0], st_row = p.cache_stride[kind][2];
+    char* const cache = static_cast<char*>(p.cache[kind]) + head * p.cache_stride[kind][1] +
+                        (threadIdx.x & (lanes - 1)) * 16;
     const int step = kMoveThreads >> p.lanes_log2;  // rows that the block takes at a time
-    const int rows = min(U * step, kMostRows);      // of a chunk
+    const int rows = min(U * step, ROWS);      // of a chunk
     const int r0 = threadIdx.x >> p.lanes_log2;
     const int tid = threadIdx.x;
     int pos[EACH], page[EACH], to[EACH], pos_of[EACH];
@@ -374,12 +526,12 @@ __global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __gri
         if (r < rows && s_from[slot][r] >= 0) v[u] = fresh(reinterpret_cast<const uint4*>(cache + s_from[slot][r]));
       }
     };
-    positions(from);
-    pages(from);
+    positions(0);
+    pages(0);
     publish(0);
-    positions(from + rows);
-    pages(from + rows);
-    positions(from + 2 * rows);
+    positions(rows);
+    pages(rows);
+    positions(2 * rows);
     __syncthreads();
     load(0, x);
     int slot = 0;  // of the chunk that is written in this turn
@@ -398,7 +550,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __gri
       }
       slot = next;
     };
-    for (int at = from; at < stay; at += 2 * rows) {
+    for (int at = 0; at < stay; at += 2 * rows) {
       turn(at, x, y);
       if (at + rows < stay) turn(at + rows, y, x);
     }
@@ -406,7 +558,7 @@ __global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __gri
   }
   // The weights and scales: a float each, eight ranks to a thread at a time.
   constexpr int M = 8;
-  for (int at = from; at < stay; at += M * kMoveThreads) {
+  for (int at = 0; at < stay; at += M * kMoveThreads) {
     int pos[M], page[M], to[M];
     float w[M], s[2][M];
 #pragma unroll
@@ -448,12 +600,39 @@ __global__ void __launch_bounds__(kMoveThreads, 2) paged_move_kernel(const __gri
   }
 }
 
-int evict(const FaPagedEvictArgs* a, void* stream) {
+// The division of the moving among blocks, and the workspace: a ticket, a flag for each chunk.
+struct EvictChoice {
+  int lanes_log2, rows, chunks[2];
+  int64_t blocks, bytes;
+  bool in_order;
+};
+
+EvictChoice choose(const FaPagedEvictArgs* a) {
+  EvictChoice c{};
+  const int64_t capacity = (a->in_place ? a->cache.table_cols : a->to_cols) * a->cache.page_size;
+  const int64_t most = std::max<int64_t>(1, std::min(a->keep, capacity));
+  const int row_bytes = static_cast<int>(a->cache.head_dim) * (a->cache.dtype == FA_DTYPE_FP8_E4M3 ? 1 : 2);
+  c.lanes_log2 = log2_of(row_bytes / 16);
+  c.rows = kMoveRows >> c.lanes_log2;
+  c.chunks[0] = static_cast<int>((most + c.rows - 1) / c.rows);
+  c.chunks[1] = static_cast<int>((most + kMetaUnroll * kMoveThreads - 1) / (kMetaUnroll * kMoveThreads));
+  c.blocks = a->cache.seqs * a->cache.heads_kv * (2 * c.chunks[0] + c.chunks[1]);
+  // In order where that gives every SM a block.  There are fewer latencies to a byte then: moving took 13 us and
+  // 24 with a block a chunk for 16 sequences of 8 heads cut to 512 tokens (head_dim 128, 16 bits), 45 and 65
+  // for 48 in float8 cut to 1024; one sequence of 4 heads cut to 40,000 takes 85 us with a block a chunk, and took
+  // 115 in order with the columns dealt out to 16 blocks a head.
+  const int64_t items = a->cache.seqs * a->cache.heads_kv;
+  c.in_order = a->in_place && 2 * items >= sm_count_of_current();
+  if (c.in_order) c.blocks = 3 * items;
+  c.bytes = 256 + up256(a->in_place && !c.in_order ? 4 * c.blocks : 0);
+  return c;
+}
+
+int check_evict(const FaPagedEvictArgs* a) {
   if (!a || a->struct_size != static_cast<int32_t>(sizeof(FaPagedEvictArgs))) return FA_ERR_INVALID_ARG;
   FaPagedCache c = a->cache;
-  c.offsets = c.kv_lens;  // (there are no packed rows)
   const bool f8 = c.dtype == FA_DTYPE_FP8_E4M3;
-  int rc = check_layout(c, f8 ? FA_DTYPE_BF16 : c.dtype, 0);
+  const int rc = check_layout(c, f8 ? FA_DTYPE_BF16 : c.dtype, 0);
   if (rc != FA_OK) return rc;
   constexpr int64_t kMost = int64_t{1} << 30;
   if (a->keep < 0 || a->keep > kMost || a->recent < 0 || a->recent > a->keep) return FA_ERR_INVALID_ARG;
@@ -461,13 +640,25 @@ int evict(const FaPagedEvictArgs* a, void* stream) {
     return FA_ERR_INVALID_ARG;
   for (int d = 0; d < 2; ++d)
     if (a->weights_stride[d] <= 0 || a->weights_stride[d] % 4) return FA_ERR_MISALIGNED;
-  if (c.seqs * c.heads_kv > kMost / 64) return FA_ERR_INVALID_ARG;
+  if (c.seqs * c.heads_kv > kMost / 64 || choose(a).blocks > INT32_MAX) return FA_ERR_INVALID_ARG;
+  return FA_OK;
+}
+
+int evict(const FaPagedEvictArgs* a, void* stream) {
+  int rc = check_evict(a);
+  if (rc != FA_OK) return rc;
+  FaPagedCache c = a->cache;
+  c.offsets = c.kv_lens;  // (there are no packed rows)
+  const bool f8 = c.dtype == FA_DTYPE_FP8_E4M3;
   if (c.seqs == 0) return FA_OK;
   rc = check_cache(c, f8 ? FA_DTYPE_BF16 : c.dtype, 0);
   if (rc != FA_OK) return rc;
   if (!a->weights || !a->new_lens || (a->keep > 0 && !a->kept) || (!a->in_place && a->to_cols > 0 && !a->to_table))
     return FA_ERR_INVALID_ARG;
-  if (reinterpret_cast<uintptr_t>(a->weights) % 16) return FA_ERR_MISALIGNED;
+  if (reinterpret_cast<uintptr_t>(a->weights) % 16 || reinterpret_cast<uintptr_t>(a->workspace) % 256)
+    return FA_ERR_MISALIGNED;
+  const EvictChoice choice = choose(a);
+  if (!a->workspace || a->workspace_bytes < choice.bytes) return FA_ERR_INVALID_ARG;
   rc = check_device();
   if (rc != FA_OK) return rc;
 
@@ -491,6 +682,11 @@ int evict(const FaPagedEvictArgs* a, void* stream) {
     for (int d = 0; d < 3; ++d) p.cache_stride[i][d] = (i ? c.v_stride : c.k_stride)[d] * eb;
     for (int d = 0; d < 2; ++d) p.scale_stride[i][d] = (i ? c.v_scale_stride : c.k_scale_stride)[d];
   }
+  p.lanes_log2 = choice.lanes_log2;
+  p.rows = choice.rows;
+  for (int i = 0; i < 2; ++i) p.chunks[i] = choice.chunks[i];
+  p.ticket = static_cast<uint32_t*>(a->workspace);
+  p.flags = a->in_place && !choice.in_order ? p.ticket + 64 : nullptr;
   const int sms = sm_count_of_current();
   const int64_t items = c.seqs * c.heads_kv, capacity = c.table_cols * c.page_size;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -529,28 +725,21 @@ int evict(const FaPagedEvictArgs* a, void* stream) {
     }
   }
   if (p.keep == 0) return FA_OK;
-  // Slices: rows whole, or in parts of at least 32 bytes while that finds SMs without work.
-  const int row_bytes = static_cast<int>(c.head_dim) * eb;
-  p.slices = 1;
-  while (row_bytes / p.slices > 32 && items * 2 * p.slices < sms) p.slices *= 2;
-  p.lanes_log2 = log2_of(row_bytes / p.slices / 16);
-  p.splits = 1;
-  if (!p.in_place) {
-    p.slices = 1;
-    p.lanes_log2 = log2_of(row_bytes / 16);
-    // ranges of ranks while there are SMs without a pair of blocks: a block's start costs three latencies
-    const int64_t chunk = kMoveThreads * kMoveUnroll >> p.lanes_log2;
-    p.splits = static_cast<int>(
-        std::max<int64_t>(1, std::min({(2 * sms + 2 * items - 1) / (2 * items), (p.keep + chunk - 1) / chunk, int64_t{1024}})));
-  }
-  const dim3 grid(static_cast<unsigned>(items * (2 * p.slices + 1)), static_cast<unsigned>(p.splits));
-  return launch_dependent(paged_move_kernel, grid, kMoveThreads, 0, s, p);
+  return launch_dependent(choice.in_order ? choice.lanes_log2 >= 2 ? paged_move_in_order_kernel<1>
+                                                                   : paged_move_in_order_kernel<2>
+                                          : paged_move_kernel,
+                          dim3(static_cast<unsigned>(choice.blocks)), kMoveThreads, 0, s, p);
 }
 
 }  // namespace
 }  // namespace fa
 
 extern "C" {
+
+int64_t fa_paged_evict_workspace_bytes(const FaPagedEvictArgs* a) {
+  const int rc = fa::check_evict(a);
+  return rc != FA_OK ? rc : fa::choose(a).bytes;
+}
 
 int fa_paged_evict_sm100(const FaPagedEvictArgs* args, void* stream) { return fa::evict(args, stream); }
 

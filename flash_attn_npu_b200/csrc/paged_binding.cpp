@@ -31,6 +31,7 @@ int64_t (*g_prefix_workspace)(const FaPagedPrefixArgs*) = nullptr;
 int (*g_weights)(const FaPagedWeightsArgs*, void*) = nullptr;
 int64_t (*g_weights_workspace)(const FaPagedWeightsArgs*) = nullptr;
 int (*g_evict)(const FaPagedEvictArgs*, void*) = nullptr;
+int64_t (*g_evict_workspace)(const FaPagedEvictArgs*) = nullptr;
 
 constexpr int kDevices = 64;
 // Devices that paged.py has prepared, and their status words.
@@ -461,6 +462,10 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   x.new_lens = static_cast<int32_t*>(lens.mutable_data_ptr());
   x.kept = static_cast<int32_t*>(kept.mutable_data_ptr());
   x.dev_status = g_status[index];
+  x.workspace_bytes = g_evict_workspace(&x);
+  if (x.workspace_bytes < 0) return none();
+  const c10::DataPtr workspace = c10::cuda::CUDACachingAllocator::get()->allocate(x.workspace_bytes);
+  x.workspace = workspace.get();
   const int rc = g_evict(&x, c10::cuda::getCurrentCUDAStream(index).stream());
   if (rc != FA_OK) return PyLong_FromLong(rc);
   for (int i : {0, 1, 2, 7, 8})
@@ -489,10 +494,9 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyBool_FromLong(1);
 }
 
-// setup_more(prefix attention, its workspace_bytes, weights, its workspace_bytes, evict): those of the
-// other calls
+// setup_more(prefix attention, weights, evict, each with its workspace_bytes): those of the other calls
 PyObject* setup_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  constexpr int kCalls = 5;
+  constexpr int kCalls = 6;
   void* p[kCalls];
   if (n != kCalls) return none();
   for (int i = 0; i < kCalls; ++i) {
@@ -504,6 +508,7 @@ PyObject* setup_more(PyObject*, PyObject* const* a, Py_ssize_t n) {
   g_weights = reinterpret_cast<decltype(g_weights)>(p[2]);
   g_weights_workspace = reinterpret_cast<decltype(g_weights_workspace)>(p[3]);
   g_evict = reinterpret_cast<decltype(g_evict)>(p[4]);
+  g_evict_workspace = reinterpret_cast<decltype(g_evict_workspace)>(p[5]);
   return PyBool_FromLong(1);
 }
 

@@ -257,7 +257,8 @@ def _native_binding():
             lib.fa_paged_read_sm100))
         _paged_binding.setup_more(*addresses(
             lib.fa_paged_prefix_sm100, lib.fa_paged_prefix_workspace_bytes, lib.fa_paged_weights_sm100,
-            lib.fa_paged_weights_workspace_bytes, lib.fa_paged_evict_sm100))
+            lib.fa_paged_weights_workspace_bytes, lib.fa_paged_evict_sm100,
+            lib.fa_paged_evict_workspace_bytes))
         _binding = _paged_binding
     return _binding
 

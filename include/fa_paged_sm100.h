@@ -180,6 +180,7 @@ typedef struct FaPagedEvictArgs {
   float* weights;          /* moved along with the tokens */
   int32_t* new_lens;       /* [seqs]: min(kv_lens, keep) */
   int32_t* kept;           /* [seqs, heads_kv, keep]: the positions that stay, in order, -1 behind them */
+  void* workspace;         /* fa_paged_evict_workspace_bytes() bytes, 256-byte aligned; needs no clearing */
   int32_t* dev_status;     /* optional device int, 0 on success */
   FaPagedCache cache;
   int64_t weights_stride[2]; /* element strides of (page, head); multiples of 16 bytes */
@@ -188,6 +189,7 @@ typedef struct FaPagedEvictArgs {
   int64_t to_cols;
   int64_t keep;     /* tokens that stay of a longer sequence */
   int64_t recent;   /* the last ones, which stay whatever their weight; at most keep */
+  int64_t workspace_bytes;
   int32_t in_place; /* what stays goes to the front of the sequence's own pages */
 } FaPagedEvictArgs;
 
@@ -198,6 +200,9 @@ typedef struct FaPagedEvictArgs {
  * are copied).  Pages that receive tokens must not belong to another sequence too; those of to_table must
  * not be among those of page_table. */
 FA_API int fa_paged_evict_sm100(const FaPagedEvictArgs* args, void* stream);
+
+/* Its workspace, as fa_paged_workspace_bytes. */
+FA_API int64_t fa_paged_evict_workspace_bytes(const FaPagedEvictArgs* args);
 
 #ifdef __cplusplus
 }
