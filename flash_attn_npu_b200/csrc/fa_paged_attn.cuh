@@ -163,7 +163,15 @@ __device__ __forceinline__ int ctas_for(const PagedLevelParams& p) {
   float w[2];
   level_weights(p, w);
   if (w[0] == 0.f || w[1] == 0.f || all < 2) return all;
-  const int n = min(max(__float2int_rn(all * (w[0] / (w[0] + w[1]))), 1), all - 1);
+  int n = min(max(__float2int_rn(all * (w[0] / (w[0] + w[1]))), 1), all - 1);
+  if (p.levels[0].seqs.seqs == 1) {
+    // items of one prefix are alike: as many CTAs to each, so that no CTA holds parts of two
+    int first, count;
+    seq_rows(p.levels[0].seqs, 0, first, count);
+    const int items = p.heads_kv * ((count * p.group + p.levels[0].rows - 1) / p.levels[0].rows);
+    const int m = (n + items / 2) / items * items;
+    if (m > 0 && m < all) n = m;
+  }
   return p.place == 1 ? n : all - n;
 }
 

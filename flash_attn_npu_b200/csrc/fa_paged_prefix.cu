@@ -87,22 +87,45 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     o = v.part_o + y * D;
     return fresh(v.part_lse + y);
   };
-  const float* from;
+  // Four parts at a time, so that what they say and what they hold are on their way together; O is kept
+  // relative to the largest logsumexp so far.
+  constexpr int AT_ONCE = 4;
   float top = -INFINITY, sum = 0.f;
-#pragma unroll 4
-  for (int i = split; i < count; i += PS) top = fmaxf(top, part(i, from));
-  const float base = top == -INFINITY ? 0.f : top;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = split; i < count; i += PS) {
-    const float w = exp2f(part(i, from) - base);
-    if (w == 0.f) continue;  // a part without keys for the row may have left no values
-    const float4 v = fresh(reinterpret_cast<const float4*>(from) + col);
-    sum += w;
-    acc.x += w * v.x;
-    acc.y += w * v.y;
-    acc.z += w * v.z;
-    acc.w += w * v.w;
+  for (int i = split; i < count; i += AT_ONCE * PS) {
+    float l[AT_ONCE];
+    float4 v[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const float* from = nullptr;
+      l[u] = -INFINITY;
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i + u * PS < count) {
+        l[u] = part(i + u * PS, from);
+        v[u] = fresh(reinterpret_cast<const float4*>(from) + col);
+      }
+    }
+    float to = top;
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) to = fmaxf(to, l[u]);
+    const float base = to == -INFINITY ? 0.f : to;
+    const float f = top == -INFINITY ? 0.f : exp2f(top - base);
+    sum *= f;
+    acc.x *= f;
+    acc.y *= f;
+    acc.z *= f;
+    acc.w *= f;
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const float w = exp2f(l[u] - base);
+      if (w == 0.f) continue;  // a part without keys for the row may have left no values
+      sum += w;
+      acc.x += w * v[u].x;
+      acc.y += w * v[u].y;
+      acc.z += w * v[u].z;
+      acc.w += w * v[u].w;
+    }
+    top = to;
   }
   if constexpr (PS > 1) {
     s_o[threadIdx.x] = acc;
@@ -179,6 +202,7 @@ int check_prefix(const FaPagedPrefixArgs* a) {
 // for the prefixes beside the row kernel for the own tokens.
 struct PrefixChoice {
   int launches;
+  bool lone_tile;  // the rows of a prefix fit one query tile
   PagedChoice kernel[2];
   int64_t own[2], whole_o, whole_lse, where, bytes;  // workspace: the kernels' own, and what the join reads
 };
@@ -190,6 +214,7 @@ PrefixChoice choose(const FaPagedPrefixArgs* a) {
   int64_t most[2] = {a->max_prefix_q_len, x.max_q_len};
   for (int64_t& m : most) m = (m ? std::min(m, total) : total) * group;
   c.launches = most[0] > 32 && most[1] <= 32 && tile_kernel_takes(&x) ? 2 : 1;
+  c.lone_tile = most[0] <= 128;
   if (c.launches == 1) most[0] = std::max(most[0], most[1]);
   for (int i = 0; i < c.launches; ++i) {
     c.kernel[i] = choose_for_rows(&x, most[i]);
@@ -216,14 +241,18 @@ int launch_levels(const PagedPlan& plan) {
   }
 }
 
-// What a tile takes of an SM, in 10 ns (measured at head_dim 128, both kernels at work): 128 keys of two
-// query tiles 3.0 us in the tile kernel, 64 KB 1.05 us in the row kernel with blocks of 8 rows; blocks of
-// 32 rows are bound by their chain, 1.2 us a tile.
-int unit_of(const PagedPlan& plan, const PagedInfo& info) {
-  if (plan.rows == 0) return 300;
-  if (plan.rows == 32) return 120;
+// What a tile takes of an SM, relative to 200 for one of the tile kernel; 0: the two kernels do not run side by
+// side but one behind the other on all SMs.  Found by trying (head_dim 128, 8 kv heads, prefixes of 8000 to
+// 60,000 tokens, 16 to 128 sequences): side by side took 80 us where one behind the other took 101 for 64
+// single tokens in 16 bits (8-row blocks), 99 and 127 for 4 new tokens of 48 sequences (16-row blocks), 100 and
+// 118 for 8 of 32 (32-row blocks), 117 and 132 for 64 single tokens in float8; but 176 and 169 for 4 of 40 in
+// float8, where the row kernel is bound by its chain and its blocks differ in time.
+int unit_of(const PagedPlan& plan, const PagedInfo& info, const PagedPlan& own, bool lone_tile) {
+  if (own.fp8 && own.rows > 8) return 0;
+  if (plan.rows == 0) return lone_tile ? 130 : 200;  // (both sides of a CTA work on a lone query tile)
+  if (plan.rows > 8) return plan.rows == 16 ? 150 : 120;
   const int bytes = 2 * info.keys * plan.params.head_dim * (plan.fp8 ? 1 : 2);
-  return std::max(60, bytes * 105 / 65536);
+  return std::max(40, bytes * (plan.fp8 ? 100 : 70) / 65536);
 }
 
 int prefix_attention(const FaPagedPrefixArgs* a, void* stream) {
@@ -261,12 +290,18 @@ int prefix_attention(const FaPagedPrefixArgs* a, void* stream) {
     if (c.launches == 2) {
       p.place = i + 1;
       (i == 0 ? p.own : p.seqs).seqs = 0;
-      const int rows = plan[i].rows == 0 ? info.rows / 128 * p.tile_live : info.rows;
-      const PagedLevel v{seqs[i], rows, info.keys, p.item_cost, unit_of(plan[i], info)};
-      plan[0].params.levels[i] = plan[1].params.levels[i] = v;
     }
     for (int k = c.launches == 2 ? i : 0; k < (c.launches == 2 ? i + 1 : 2); ++k)
       j.level[k] = JoinLevel{p.part_o, p.part_lse, seqs[k].offsets, seqs[k].seqs, info.rows, c.kernel[i].grid};
+  }
+  for (int i = 0; c.launches == 2 && i < 2; ++i) {
+    const PagedAttnParams& p = plan[i].params;
+    const PagedInfo& info = c.kernel[i].info;
+    const int rows = plan[i].rows == 0 ? info.rows / 128 * p.tile_live : info.rows;
+    // (short sequences cost their start more than the line counts)
+    const PagedLevel v{seqs[i], rows, info.keys, p.item_cost + 2 * (plan[i].rows > 0),
+                       unit_of(plan[i], info, plan[1], c.lone_tile)};
+    plan[0].params.levels[i] = plan[1].params.levels[i] = v;
   }
   for (int i = 0; i < c.launches; ++i) {
     rc = launch_levels(plan[i]);
