@@ -150,6 +150,62 @@ class FaPagedAttnArgs(ctypes.Structure):
     ]
 
 
+class FaPagedPrefixArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_int32),
+        ("attn", FaPagedAttnArgs),
+        ("prefix_table", ctypes.c_void_p),
+        ("prefix_offsets", ctypes.c_void_p),
+        ("prefix_lens", ctypes.c_void_p),
+        ("prefix_stride", ctypes.c_int64),
+        ("prefix_cols", ctypes.c_int64),
+        ("prefixes", ctypes.c_int64),
+        ("max_prefix_q_len", ctypes.c_int64),
+    ]
+
+
+class FaPagedWeightsArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("dev_status", ctypes.c_void_p),
+        ("cache", FaPagedCache),
+        ("q_stride", ctypes.c_int64 * 2),
+        ("weights_stride", ctypes.c_int64 * 2),
+        ("total", ctypes.c_int64),
+        ("heads_q", ctypes.c_int64),
+        ("max_q_len", ctypes.c_int64),
+        ("workspace_bytes", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("reset_new", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
+    ]
+
+
+class FaPagedEvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_int32),
+        ("weights", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("dev_status", ctypes.c_void_p),
+        ("cache", FaPagedCache),
+        ("weights_stride", ctypes.c_int64 * 2),
+        ("to_table", ctypes.c_void_p),
+        ("to_stride", ctypes.c_int64),
+        ("to_cols", ctypes.c_int64),
+        ("keep", ctypes.c_int64),
+        ("recent", ctypes.c_int64),
+        ("workspace_bytes", ctypes.c_int64),
+        ("in_place", ctypes.c_int32),
+    ]
+
+
 class NativeError(RuntimeError):
     """Raised for a non-zero status from the C ABI."""
 
