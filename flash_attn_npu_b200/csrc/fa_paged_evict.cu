@@ -86,7 +86,7 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 // THREADS: 512, or 1024 for many keys, whose histogram has four columns then (lane by lane: fewer of a warp
 // meet in a word, where weights are alike).  CLUSTER: several CTAs share an item.
 template <int THREADS, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS) paged_select_kernel(const __grid_constant__ EvictParams p) {
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select_kernel(const __grid_constant__ EvictParams p) {
   constexpr int COLS = THREADS == 1024 ? 4 : 1;
   constexpr int EACH = kBins / THREADS;  // bins of a thread
   constexpr int WARPS = THREADS / 32;
@@ -353,25 +353,28 @@ __global__ void __launch_bounds__(kMoveThreads, 3) paged_move_kernel(const __gri
     __syncthreads_or(seen);
     if (!p.in_place) return true;
     uint32_t* const flags = p.flags + static_cast<int64_t>(item) * units + kind * p.chunks[0];
-    if (tid == 0) {
-      __threadfence();
+    // One warp speaks for the block (a fence by every thread would wait for everybody's stores).
+    if (tid == 0)
       asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flags + chunk), "r"(1u) : "memory");
-    }
-    const uint64_t t0 = globaltimer_ns();
-    for (int c = tid; c < chunk; c += kMoveThreads) {
-      uint32_t read = 0;
-      while (true) {
-        asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(read) : "l"(flags + c) : "memory");
-        if (read) break;
-        if (globaltimer_ns() - t0 >= FA_WAIT_TIMEOUT_NS) {
-          report(p.seqs.status, kStatusTimeout);
-          s_gave_up = 1;
-          break;
+    if (tid < 32) {
+      uint64_t t0 = 0;
+      for (int c = tid; c < chunk; c += 32) {
+        uint32_t read = 0;
+        while (true) {
+          asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(read) : "l"(flags + c) : "memory");
+          if (read) break;
+          const uint64_t t = globaltimer_ns();
+          if (t0 == 0) t0 = t;
+          if (t - t0 >= FA_WAIT_TIMEOUT_NS) {
+            report(p.seqs.status, kStatusTimeout);
+            s_gave_up = 1;
+            break;
+          }
         }
+        if (!read) break;
       }
-      if (!read) break;
+      asm volatile("fence.acq_rel.gpu;" ::: "memory");  // (the flags were seen before anything is written)
     }
-    __threadfence();  // (the flags were seen before anything is written)
     __syncthreads();
     return s_gave_up == 0;
   };
