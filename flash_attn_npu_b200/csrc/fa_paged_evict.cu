@@ -6,7 +6,7 @@
 // Two launches.  paged_select_kernel finds the ranks of a (sequence, head): the weight of the last token
 // that stays is found digit by digit from the top (histograms of 11, 11 and 10 bits), over keys that are read
 // from memory once and then lie in shared memory; an ordered scan then writes the positions that stay.  A
-// long sequence is shared by a cluster of up to 8 CTAs, which add their histograms up through distributed
+// long sequence is shared by a cluster of up to 16 CTAs, which add their histograms up through distributed
 // shared memory.  paged_move_kernel moves the rows, bound by memory.
 //
 // In place: slot i is written by rank i and read by rank(i) <= i.  A block that goes through the ranks in order,
@@ -50,7 +50,7 @@ struct EvictParams {
 
 // --------------------------------------------------------------------------------- selection
 constexpr int kBins = 2048;
-constexpr int kMostCluster = 8;
+constexpr int kMostCluster = 16;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t x;
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
   extern __shared__ __align__(16) uint32_t s_mem[];
   uint32_t* const s_hist = s_mem;                                // [kBins][COLS]
   uint4* const s_key4 = reinterpret_cast<uint4*>(s_mem + kBins * COLS);
-  __shared__ __align__(16) uint32_t s_total[2][kBins];  // read by the cluster
+  __shared__ uint32_t s_own[CLUSTER ? kBins : 1], s_total[CLUSTER ? kBins : 1];  // read by the cluster
   __shared__ uint32_t s_count[2];           // ... keys above the threshold, keys at it
   __shared__ uint32_t s_found[3];           // digit, how many are wanted at it, and how many there are
   __shared__ uint32_t s_warp[2][WARPS];
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
 
   // A key stays if its upper digits are above `found`, and of the keys that have them equal the first `left`.
   uint32_t found = 0, left = want;
-  int shift = 32, turn = 0;
+  int shift = 32;
   uint32_t above = 0, equal = 0;  // of this thread's bins: keys of the CTA above and at the digits found
   // Sum over the warps before this one, and over all, of what lane 31 of each holds.
   auto scan_warps = [&](uint32_t last, uint32_t& all) -> uint32_t {
@@ -170,7 +170,6 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
     const int bits = min(shift, 11);
     const int above_bits = shift;
     shift -= bits;
-    turn ^= 1;
     for (int i = tid; i < kBins * COLS / 4; i += THREADS) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     for (int i = tid; i < count4; i += THREADS) {
@@ -195,14 +194,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
         bins[j] = s_hist[top - j];
       }
       own[j] = bins[j];
-      if (CLUSTER) s_total[turn][top - j] = bins[j];
+      if (CLUSTER) s_own[top - j] = bins[j];
     }
     if (CLUSTER) {
+      // a CTA adds up a slice of the bins, and all read the slices: all of every CTA's would be cs times as much
+      const int slice = kBins / cs;
+      cluster_sync();
+      for (int i = tid; i < slice; i += THREADS) {
+        uint32_t all = 0;
+        for (int c = 0; c < cs; ++c) all += of_cta(s_own[rank * slice + i], c);
+        s_total[rank * slice + i] = all;
+      }
       cluster_sync();
 #pragma unroll
-      for (int j = 0; j < EACH; ++j)
-        for (int c = 0; c < cs; ++c)
-          if (c != rank) bins[j] += of_cta(s_total[turn][top - j], c);
+      for (int j = 0; j < EACH; ++j) bins[j] = of_cta(s_total[top - j], (top - j) / slice);
     }
 #pragma unroll
     for (int j = 0; j < EACH; ++j) sum += bins[j];
@@ -647,6 +652,38 @@ int check_evict(const FaPagedEvictArgs* a) {
   return FA_OK;
 }
 
+constexpr int kMostBytes = 200 * 1024;  // of a selecting block's shared memory (16 KB more are the kernel's own)
+
+// Whether clusters of 16 selecting blocks find a place on the current device (more than 8 have to be asked for).
+bool large_clusters() {
+  static std::atomic<int> known[16] = {};  // 1: yes, 2: no
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 16) return false;
+  int is = known[dev].load(std::memory_order_acquire);
+  if (is == 0) {
+    const auto kernel = paged_select_kernel<1024, true>;
+    const void* const fn = reinterpret_cast<const void*>(kernel);
+    int n = 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(1024);
+    cfg.dynamicSmemBytes = kMostBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 16;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const bool ok = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes) == cudaSuccess &&
+                    cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                    cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0;
+    if (!ok) (void)cudaGetLastError();
+    is = ok ? 1 : 2;
+    known[dev].store(is, std::memory_order_release);
+  }
+  return is == 1;
+}
+
 int evict(const FaPagedEvictArgs* a, void* stream) {
   int rc = check_evict(a);
   if (rc != FA_OK) return rc;
@@ -697,10 +734,10 @@ int evict(const FaPagedEvictArgs* a, void* stream) {
   // A (sequence, head) gets more CTAs while all of them find a place and have 2048 keys each.
   int cluster = 1;
   while (cluster < kMostCluster && items * cluster * 2 <= 2 * sms && capacity > 2048 * cluster) cluster *= 2;
+  if (cluster > 8 && !large_clusters()) cluster = 8;
   const int64_t share = ((capacity + cluster - 1) / cluster + 3) / 4 * 4 + 4;
-  const bool many = share > 8192;
+  const bool many = share > 8192 || cluster > 8;
   const int cols = many ? 4 : 1, threads = many ? 1024 : 512;
-  constexpr int kMostBytes = 200 * 1024;  // (16 KB more are the kernel's own)
   p.cached = static_cast<int>(std::min<int64_t>(share, (kMostBytes - 4 * kBins * cols) / 4));
   const int smem = 4 * (p.cached + kBins * cols);
   const auto kernel = cluster > 1 ? (many ? paged_select_kernel<1024, true> : paged_select_kernel<512, true>)
