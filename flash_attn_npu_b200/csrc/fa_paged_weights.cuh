@@ -73,7 +73,7 @@ struct WeightsGeo {
   static constexpr int K_SLOTS = D <= 64 ? (FP8 ? 3 : 4) : D == 128 ? 2 : 1;  // of each key tile of an item
   static constexpr int Q_SLOTS = D <= 64 && !FP8 ? 4 : 2;
   static constexpr int RAW_SLOTS = !FP8 ? 0 : D == 256 ? 1 : D == 128 ? 3 : 6;
-  static constexpr int L_SLOTS = 4;  // logsumexps of query tiles
+  static constexpr int L_SLOTS = 2;  // logsumexps of query tiles, for steps of each parity
   static constexpr int I_SLOTS = 4;  // pages and scales of each key tile of an item
   static constexpr int P_SLOTS = 8;  // parts
   static constexpr int SHARED = 11 * 1024;
@@ -96,8 +96,12 @@ struct WeightsSeq {
 
   WeightsSeq() = default;
   __device__ __forceinline__ WeightsSeq(const PagedWeightsParams& p, int b) {
-    seq_rows(p.seqs, b, first, count);
-    len = seq_len(p.seqs, b);
+    const int a = fresh(p.seqs.offsets + b), z = fresh(p.seqs.offsets + b + 1), n = fresh(p.seqs.kv_lens + b);
+    first = min(max(a, 0), p.seqs.total);
+    count = max(min(z, p.seqs.total) - first, 0);
+    const int64_t cap = static_cast<int64_t>(p.seqs.table_cols) << p.seqs.page_log2;
+    len = n < 0 ? 0 : static_cast<int>(n < cap ? n : cap);
+    if (len != n || count != z - a) report(p.seqs.status, kStatusPageTable);
     blocks = count ? (len + kWeightsBlock - 1) / kWeightsBlock : 0;
     qtiles = (count + p.tile_toks - 1) / p.tile_toks * p.chunks;
     const int past = len - count;
@@ -200,7 +204,7 @@ template <typename G>
 struct WeightsShared {
   uint64_t k_full[2][G::K_SLOTS], k_empty[2][G::K_SLOTS];
   uint64_t q_full[G::Q_SLOTS], q_empty[G::Q_SLOTS];
-  uint64_t l_full[G::L_SLOTS], l_empty[G::L_SLOTS];
+  uint64_t l_full[2][G::L_SLOTS], l_empty[2][G::L_SLOTS];
   uint64_t i_full[2][G::I_SLOTS], i_empty[2][G::I_SLOTS];
   uint64_t p_full[G::P_SLOTS], p_empty[G::P_SLOTS];
   uint64_t raw_full[8], raw_empty[8];
@@ -212,7 +216,7 @@ struct WeightsShared {
   int raw_page[8][16];
   float scale[2][G::I_SLOTS][128];   // float8: of a key tile's rows
   float sum[2][128];              // of the steps of the other warpgroup
-  alignas(16) float neg_lse[G::L_SLOTS][G::QN];  // -l of a query tile's rows
+  alignas(16) float neg_lse[2][G::L_SLOTS][G::QN];  // -l of a query tile's rows
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
 };
@@ -269,14 +273,14 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     init(sh->k_empty[0], 2 * K_SLOTS, 1);
     init(sh->q_full, Q_SLOTS, 1);
     init(sh->q_empty, Q_SLOTS, 2);  // the issuers
-    init(sh->l_full, G::L_SLOTS, 1);
-    init(sh->l_empty, G::L_SLOTS, 16);  // the epilogue
+    init(sh->l_full[0], 2 * G::L_SLOTS, 1);
+    init(sh->l_empty[0], 2 * G::L_SLOTS, 8);  // the epilogue of that parity
     init(sh->i_full[0], 2 * G::I_SLOTS, FP8 ? G::AUX : 1);
     init(sh->i_empty[0], 2 * G::I_SLOTS, 8);  // the two warpgroups of the tile
     init(sh->p_full, G::P_SLOTS, 1);
     init(sh->p_empty, G::P_SLOTS, 19 + G::AUX);  // all other warps
     init(sh->raw_full, 8, 1);
-    init(sh->raw_empty, 8, 8);
+    init(sh->raw_empty, 8, G::AUX);
     init(sh->s_full[0], 4, 1);
     init(sh->s_empty[0], 4, 4);
     init(sh->sum_full[0], 8, 1);
@@ -419,7 +423,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
   if (warp == 18) {
     // ------------------------------------------------------------------ producer of K
     Keys k;
-    int ahead[2][OPS], checked = -1;
+    int ahead[2][OPS];
     bool ok = true;
     while (ok && next_part()) {
 #pragma unroll
@@ -427,11 +431,6 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
         if (i < w.tiles && ok) ok = load_keys(i, k, ahead[i]);
       if (FP8 && w.tiles == 1) k.ahead_block = -1;  // (those of the second tile have not been fetched)
       else fetched(k);
-      if (lane == 0 && checked != w.seq &&
-          (fresh(p.seqs.kv_lens + w.seq) != w.len ||
-           fresh(p.seqs.offsets + w.seq + 1) - fresh(p.seqs.offsets + w.seq) != w.count))
-        report(status, kStatusPageTable);
-      checked = w.seq;
     }
     drain_keys(0, k);
   } else if (warp == 19) {
@@ -471,8 +470,9 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
         pph ^= 1u;
       }
     };
-    int slot = 0, lslot = 0, issued = 0;
-    uint32_t ph = 0, lph = 0;
+    int slot = 0, issued = 0, step = 0;  // (step: parity of the next one)
+    int lslot[2] = {0, 0};
+    uint32_t ph = 0, lph[2] = {0, 0};
     Keys k;
     int ahead[OPS];
     WeightsPart coming;
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
         if (ok) ok = load_keys(1, k, ahead);
         fetched(k);
       }
-      for (int t = 0; t < w.steps && ok; ++t) {
+      for (int t = 0; t < w.steps && ok; ++t, step ^= 1) {
         if (same_q()) continue;
         now_q();
         const int tok0 = w.tok0(p, t), head0 = w.head0(p, t), rows = w.rows(p, t);
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
           const int tok = p.chunks > 1 ? 0 : p.group == 1 ? c : static_cast<int>(__umulhi(c, p.group_inv));
           l[u] = fresh(from + static_cast<int64_t>(tok) * (p.heads_kv * p.group) + (c - tok * p.group));
         }
-        ok = wait(sh->q_empty[slot], ph ^ 1u) && wait(sh->l_empty[lslot], lph ^ 1u);
+        ok = wait(sh->q_empty[slot], ph ^ 1u);
         if (!ok) break;
         if (lane == 0) {
           const uint32_t bar = smem_u32(&sh->q_full[slot]);
@@ -507,22 +507,29 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
             tma_load_3d(smem_u32(q_smem + slot * G::Q_TILE + c * G::Q_BLK), &tmQ, bar, c * (G::SWZ / 2),
                         w.head * p.group + head0, w.first + tok0);
         }
+        // for steps of this parity, or for both where the tile stays
 #pragma unroll
-        for (int u = 0; u < QN / 32; ++u) {
-          // (a row without keys gives nothing)
-          const bool none = u * 32 + lane >= rows || l[u] == -INFINITY;
-          sh->neg_lse[lslot][u * 32 + lane] = none ? -INFINITY : -l[u] * kLog2e;
+        for (int par = 0; par < 2; ++par) {
+          if ((w.qtiles != 1 && par != step) || !ok) continue;
+          ok = wait(sh->l_empty[par][lslot[par]], lph[par] ^ 1u);
+          if (!ok) continue;
+#pragma unroll
+          for (int u = 0; u < QN / 32; ++u) {
+            // (a row without keys gives nothing)
+            const bool none = u * 32 + lane >= rows || l[u] == -INFINITY;
+            sh->neg_lse[par][lslot[par]][u * 32 + lane] = none ? -INFINITY : -l[u] * kLog2e;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh->l_full[par][lslot[par]]));
+          if (++lslot[par] == G::L_SLOTS) {
+            lslot[par] = 0;
+            lph[par] ^= 1u;
+          }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh->l_full[lslot]));
         ++issued;
         if (++slot == Q_SLOTS) {
           slot = 0;
           ph ^= 1u;
-        }
-        if (++lslot == G::L_SLOTS) {
-          lslot = 0;
-          lph ^= 1u;
         }
       }
     }
@@ -613,7 +620,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
           const uint8_t* raw = raw_smem + rslot * G::RAW;
           uint8_t* dst = k_smem + (i * K_SLOTS + slot[i]) * G::K_TILE;
           if (tid < 128) sh->scale[i][islot[i]][tid] = reinterpret_cast<const float*>(raw + 128 * D)[tid];
-          else if (tid < 144) sh->page[i][islot[i]][tid - 128] = sh->raw_page[rslot][tid - 128];
+          if (tid < 16) sh->page[i][islot[i]][tid] = sh->raw_page[rslot][tid];
           if (row0 < AT_ONCE) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k)
@@ -697,10 +704,12 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
       for (int t = 0; t < w.steps && ok; ++t, step ^= 1) {
         if (!same_q()) {
           now_q();
-          if (lslot >= 0 && lane == 0) mbar_arrive(smem_u32(&sh->l_empty[lslot]));
-          if (++lslot == G::L_SLOTS) lslot = 0;
-          if (lslot == 0) lph ^= 1u;
-          ok = wait(sh->l_full[lslot], lph);
+          if (w.qtiles == 1 || step == buf) {
+            if (lslot >= 0 && lane == 0) mbar_arrive(smem_u32(&sh->l_empty[buf][lslot]));
+            if (++lslot == G::L_SLOTS) lslot = 0;
+            if (lslot == 0) lph ^= 1u;
+            ok = wait(sh->l_full[buf][lslot], lph);
+          }
         }
         if (i >= w.tiles || step != buf || !ok) continue;
         ok = wait(sh->s_full[i][buf], sph);
@@ -713,7 +722,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
         const int from = p.causal ? max(0, ahead) * p.group : 0;
         const int from_all = p.causal ? max(0, ahead - lane + 31) * p.group : 0;
         const int from_any = p.causal ? max(0, ahead - lane) * p.group & ~31 : 0;
-        const float* neg = sh->neg_lse[lslot];
+        const float* neg = sh->neg_lse[buf][lslot];
 #pragma unroll 1
         for (int c0 = from_any; c0 < live; c0 += 32) {
           float s[32];
