@@ -15,6 +15,11 @@
 // them into registers, says so (a flag for each chunk), and writes them once all chunks before it have been
 // read.  Blocks take their chunks in the order of a ticket and none waits before it has said so, so whatever a
 // block waits for is already being read.
+//
+// Measured: 16 sequences cut from 576 to 512 tokens (8 heads x 128, 16 bits) 20 us; 48 of 800 to 6000 cut to 1024
+// (float8) 16 us of selecting and 37 of moving; one of 131,067 cut to 40,000 (4 heads) 26 and 57.  Selecting is
+// a few dependent passes; moving in order reaches 47 % of the memory's nominal rate, by chunks 25 %, as a
+// block writes only once all chunks before its own have been read.
 #include <algorithm>
 
 #include "fa_paged_host.h"
@@ -97,6 +102,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
   __shared__ uint32_t s_count[2];           // ... keys above the threshold, keys at it
   __shared__ uint32_t s_found[3];           // digit, how many are wanted at it, and how many there are
   __shared__ uint32_t s_warp[2][WARPS];
+  __shared__ uint32_t s_len, s_differ;      // the sequence's length as this CTA has read it; others have another
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cs = CLUSTER ? static_cast<int>(cluster_size()) : 1;
   const int rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0;
@@ -109,7 +115,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
   const int b = item / p.heads, head = item - b * p.heads;
   let_next_launch();
   wait_for_launch_before();
-  const int n = seq_len(p.seqs, b);
+  // One thread reads the length, and the CTAs of a cluster compare theirs: what threads do together must not
+  // come apart where something changes the lengths meanwhile, though the call forbids it.
+  if (tid == 0) {
+    s_len = seq_len(p.seqs, b);
+    s_differ = 0;
+  }
+  __syncthreads();
+  const int n = s_len;
   const int stay = min(n, p.keep);
   int* const kept = p.kept + static_cast<int64_t>(item) * p.keep;
   if (rank == 0 && head == 0 && tid == 0) {
@@ -124,6 +137,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
   for (int i = stay + rank * THREADS + tid; i < p.keep; i += cs * THREADS) kept[i] = -1;
   if (n <= p.keep) {  // (the whole cluster)
     for (int i = rank * THREADS + tid; i < n; i += cs * THREADS) kept[i] = i;
+    if (CLUSTER && p.keep > p.recent) {  // (the barriers behind which the others compare)
+      cluster_sync();
+      cluster_sync();
+    }
     return;
   }
   const int old = n - p.recent;             // positions that may go
@@ -166,12 +183,17 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
     const uint32_t before = __shfl_sync(0xffffffffu, v, (warp + 31) & 31);
     return warp == 0 ? 0u : before;
   };
+  bool differ = false;
   do {  // digits of 11, 11 and 10 bits
     const int bits = min(shift, 11);
     const int above_bits = shift;
     shift -= bits;
     for (int i = tid; i < kBins * COLS / 4; i += THREADS) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
+    if (tid == 0) {  // where no bin is found (weights that change meanwhile): all CTAs end alike
+      s_found[0] = s_found[2] = 0;
+      s_found[1] = left;
+    }
     for (int i = tid; i < count4; i += THREADS) {
       const uint4 k4 = keys(i);
 #pragma unroll
@@ -205,7 +227,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
         for (int c = 0; c < cs; ++c) all += of_cta(s_own[rank * slice + i], c);
         s_total[rank * slice + i] = all;
       }
+      if (above_bits == 32 && tid < cs && of_cta(s_len, tid) != n) s_differ = 1;
       cluster_sync();
+      if (above_bits == 32 && s_differ) {  // (all CTAs see it)
+        differ = true;
+        break;
+      }
 #pragma unroll
       for (int j = 0; j < EACH; ++j) bins[j] = of_cta(s_total[top - j], (top - j) / slice);
     }
@@ -239,6 +266,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
       equal = top - j == static_cast<int>(s_found[0]) ? own[j] : j == 0 ? 0 : equal;
     }
   } while (shift > 0 && left < s_found[2]);  // (all of a bin stay: its lower digits do not matter)
+  if (CLUSTER && differ) {
+    if (tid == 0) report(p.seqs.status, kStatusPageTable);
+    return;
+  }
   found >>= shift;
   if (CLUSTER) {  // this CTA's numbers, for those behind it
 #pragma unroll
@@ -289,8 +320,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       if (i0 + j >= count) break;
-      if (k[j] > found) kept[a++ + min(e, left)] = lo + i0 + j;
-      else if (k[j] == found && e++ < left) kept[a + e - 1] = lo + i0 + j;
+      uint32_t to = want;  // (weights that change meanwhile may leave more than there is place for)
+      if (k[j] > found) to = a++ + min(e, left);
+      else if (k[j] == found && e++ < left) to = a + e - 1;
+      if (to < want) kept[to] = lo + i0 + j;
     }
     above += all & 0xffffu;
     equal += all >> 16;
@@ -626,8 +659,8 @@ EvictChoice choose(const FaPagedEvictArgs* a) {
   c.chunks[1] = static_cast<int>((most + kMetaUnroll * kMoveThreads - 1) / (kMetaUnroll * kMoveThreads));
   c.blocks = a->cache.seqs * a->cache.heads_kv * (2 * c.chunks[0] + c.chunks[1]);
   // In order where that gives every SM a block.  There are fewer latencies to a byte then: moving took 13 us and
-  // 24 with a block a chunk for 16 sequences of 8 heads cut to 512 tokens (head_dim 128, 16 bits), 45 and 65
-  // for 48 in float8 cut to 1024; one sequence of 4 heads cut to 40,000 takes 85 us with a block a chunk, and took
+  // 24 with a block a chunk for 16 sequences of 8 heads cut to 512 tokens (head_dim 128, 16 bits), 37 and 65
+  // for 48 in float8 cut to 1024; one sequence of 4 heads cut to 40,000 takes 60 us with a block a chunk, and took
   // 115 in order with the columns dealt out to 16 blocks a head.
   const int64_t items = a->cache.seqs * a->cache.heads_kv;
   c.in_order = a->in_place && 2 * items >= sm_count_of_current();
