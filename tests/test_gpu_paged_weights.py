@@ -174,3 +174,18 @@ def test_pages_that_are_none_are_reported(cuda_device):
         ops.check_device_status(cuda_device)
     ops.check_device_status(cuda_device)
     assert (w[free] == 0).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lse", [float("-inf"), 200.0])
+def test_rows_that_give_nothing(lse, fp8, cuda_device):
+    """Not even the smallest number: equal weights stay equal.  (exp(-200 + |s|), |s| < 64, is below 2^-150.)"""
+    b = ref.Batch([130, 1, 70], [500, 300, 70], heads_q=4, heads_kv=2, head_dim=64, page=32, fp8=fp8, dtype=BF16,
+                  device=cuda_device, seed=8)
+    b.q.div_(16)
+    w = torch.zeros(b.k_cache.shape[:3], device=cuda_device)
+    for causal in (False, True):
+        fam.paged_attention_weights(b.q, torch.full(b.q.shape[:2], lse, device=cuda_device), b.k_cache, *b.where, w,
+                                    causal, 64 ** -0.5, k_scale=b.k_scale)
+        ops.check_device_status(cuda_device)
+        assert not w.any()
