@@ -1,4 +1,5 @@
-"""Paged key/value cache: writing new tokens, reading tokens back, attention over it.
+"""Paged key/value cache: writing new tokens, reading tokens back, attention over it, also behind prefixes
+that sequences share; the attention weight that each token received, and eviction by it.
 
 For serving, where sequences of unequal lengths keep their keys and values from call to call.
 Sequences share caches of pages,

@@ -14,7 +14,7 @@ PERSISTENT_CTAS, each 0 for the library default.
 `paged_attention`, `paged_prefix_attention`, `paged_cache_write` and `paged_cache_read` are the calls of
 `paged` in the same way.  The write is registered as one that mutates the cache (and the scales of a float8 one), and
 returns nothing; its scales have no default (a mutated argument must be there), None for a 16-bit
-cache.
+cache.  `paged_attention_weights` mutates the weights, `paged_cache_evict` the cache, the weights and the scales.
 
     out, lse = torch.ops.flash_attn_b200.paged_attention(q, k_cache, v_cache, page_table, offsets,
                                                          kv_lens, causal, sm_scale)
