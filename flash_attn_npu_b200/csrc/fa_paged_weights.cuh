@@ -32,9 +32,9 @@
 //             (16 bits) of K's key tile 1
 //   20-27     float8: convert the key tiles
 // Measured: 64 single tokens over 500 to 8192 tokens (32 / 8 heads x 128, 16 bits) 148 us, 4.3 TB/s; 16 over 100 to
-// 2000 in float8 25 us, the chain of an item; 5 prompts of 700 to 3500 tokens 112 to 121 us, 46 % of the
+// 2000 in float8 23 us, the chain of an item; 5 prompts of 700 to 3500 tokens 112 to 121 us, 46 % of the
 // exponential unit and 34 % of the tensor cores; 4 chunks of 300 to 1024 over 4096 to 16384 (16 / 4 heads x 64,
-// float8) 182 us, 59 % of the exponential unit.
+// float8) 165 us, 65 % of the exponential unit.
 //
 // What a ring holds is waited for and given back by all warps that read from it, in order, though not all
 // look at each fill: a warp that passed over fills could take an older one for its own.
@@ -87,6 +87,11 @@ struct WeightsGeo {
   static constexpr int SMEM = 1024 + TILES + SHARED > 120 * 1024 ? 1024 + TILES + SHARED : 120 * 1024;
   static constexpr int AUX = FP8 ? 8 : 0;
   static constexpr int THREADS = (20 + AUX) * 32;
+  // Float8: registers move to the epilogue (setmaxnreg), which has spilled at 72 a thread: 16 single tokens took 25.5
+  // us and take 23.5, chunks 182 and 165.  (88, with 72 for warps 16 to 19 and 40 for 20 to 27: 23.1 and 169.)
+  static constexpr int REG_LAUNCH = 72, REG_EPILOGUE = 96, REG_ISSUE = 56, REG_AUX = 32;
+  static_assert(!FP8 || 512 * REG_EPILOGUE + 128 * REG_ISSUE + AUX * 32 * REG_AUX <= THREADS * REG_LAUNCH,
+                "register split");
   static constexpr uint32_t LAYOUT = SWZ == 128 ? 2u : SWZ == 64 ? 4u : 6u;
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -425,6 +430,9 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     }
   };
 
+  if constexpr (FP8) {
+    if (warp >= 16 && warp < 20) setmaxnreg_dec<G::REG_ISSUE>();
+  }
   if (warp == 18) {
     // ------------------------------------------------------------------ producer of K
     Keys k;
@@ -602,6 +610,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
   } else if (warp >= 20) {
     if constexpr (FP8) {
       // ---------------------------------------------------------------- convert the key tiles
+      setmaxnreg_dec<G::REG_AUX>();
       // (lanes and pieces as in the tile kernel)
       constexpr int PR = D / 16;
       constexpr int LP = PR < 4 ? PR : 4;
@@ -627,7 +636,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
           if (tid < 128) sh->scale[i][islot[i]][tid] = reinterpret_cast<const float*>(raw + 128 * D)[tid];
           if (tid < 16) sh->page[i][islot[i]][tid] = sh->raw_page[rslot][tid];
           if (row0 < AT_ONCE) {
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < STEPS; ++k)
 #pragma unroll
               for (int s = 0; s < NG; ++s) {
@@ -667,6 +676,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     }
   } else {
     // -------------------------------------------------------------------- epilogue
+    if constexpr (FP8) setmaxnreg_inc<G::REG_EPILOGUE>();
     const int i = warp >> 2 & 1;     // key tile
     const int buf = warp >> 3;       // steps of this parity, and their buffer
     const int part = warp & 3;       // 32 keys of the tile

@@ -19,6 +19,10 @@ int launch_weights(const WeightsPlan& plan) {
   auto kernel = paged_weights_kernel<T, FA_HEAD_DIM, FP8>;
   static SmemOptIn opt_in;
   if (!opt_in(reinterpret_cast<const void*>(kernel), G::SMEM)) return -7;
+  if constexpr (FP8) {
+    static RegsMatch regs_match;
+    if (!regs_match(reinterpret_cast<const void*>(kernel), G::REG_LAUNCH)) return -7;
+  }
   const int rc = launch_dependent(kernel, dim3(plan.grid), G::THREADS, G::SMEM, plan.stream, plan.tmQ, plan.tmK,
                                   plan.params);
   if (rc != 0 || plan.grid == 1 || plan.params.whole_items) return rc;  // no shared item
