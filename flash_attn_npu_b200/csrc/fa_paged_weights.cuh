@@ -23,15 +23,18 @@
 // Each key tile has two warpgroups, which take every other step (and TMEM buffer): the latency of a step is
 // a few times its work.  What they add up is joined at the item's end.
 //
-// Warps (16-bit 20, float8 28):
+// Warps (16-bit 20, or 24 where the sequences have one query tile; float8 28):
 //   0-3, 4-7, 8-11, 12-15  epilogue: key tile 0 and 1 of even steps, key tile 0 and 1 of odd ones
 //   16, 17    MMA issuers of key tile 0 and 1 (the first owns TMEM)
-//   18        TMA producer of K (16 bits: of key tile 0)
+//   18        TMA producer of K (16 bits: of key tile 0; of 24: idle)
 //   19        walks the line and tells the others the parts (a ring of descriptions: every warp walking
 //             by itself took 1500 cycles an item); TMA producer of Q, and the logsumexps of its rows, and
-//             (16 bits) of K's key tile 1
+//             (16 bits, of 20) of K's key tile 1
+//   20-23     of 24: TMA producers of K, two for each key tile.  With one query tile an item is over as soon as its
+//             keys are there, and walking while loading held them up: 64 single tokens took 148 us and take
+//             117.  Prompts take 111 us with 20 warps and 123 with 24.
 //   20-27     float8: convert the key tiles
-// Measured: 64 single tokens over 500 to 8192 tokens (32 / 8 heads x 128, 16 bits) 148 us, 4.3 TB/s; 16 over 100 to
+// Measured: 64 single tokens over 500 to 8192 tokens (32 / 8 heads x 128, 16 bits) 117 us, 5.4 TB/s; 16 over 100 to
 // 2000 in float8 23 us, the chain of an item; 5 prompts of 700 to 3500 tokens 112 to 121 us, 46 % of the
 // exponential unit and 34 % of the tensor cores; 4 chunks of 300 to 1024 over 4096 to 16384 (16 / 4 heads x 64,
 // float8) 165 us, 65 % of the exponential unit.
@@ -64,7 +67,8 @@ struct PagedWeightsParams : PagedAttnParams {  // (o, lse, v: not used)
 
 constexpr int kWeightsBlock = 256;  // keys of an item
 
-template <int D, bool FP8>
+// ONE: of a 16-bit cache, a call whose sequences have one query tile (see `weights` in fa_paged_weights.cu).
+template <int D, bool FP8, bool ONE = false>
 struct WeightsGeo {
   static constexpr int QN = D <= 64 ? 128 : D == 128 ? (FP8 ? 64 : 128) : (FP8 ? 32 : 64);  // rows of a query tile
   static constexpr int ROW_BYTES = 2 * D;
@@ -85,13 +89,17 @@ struct WeightsGeo {
   static constexpr int TILES = 2 * K_SLOTS * K_TILE + Q_SLOTS * Q_TILE + RAW_SLOTS * RAW;
   // more than half of an SM's shared memory in any case: one CTA per SM, which takes all its TMEM
   static constexpr int SMEM = 1024 + TILES + SHARED > 120 * 1024 ? 1024 + TILES + SHARED : 120 * 1024;
-  static constexpr int AUX = FP8 ? 8 : 0;
+  static constexpr int AUX = FP8 ? 8 : ONE ? 4 : 0;
   static constexpr int THREADS = (20 + AUX) * 32;
-  // Float8: registers move to the epilogue (setmaxnreg), which has spilled at 72 a thread: 16 single tokens took 25.5
-  // us and take 23.5, chunks 182 and 165.  (88, with 72 for warps 16 to 19 and 40 for 20 to 27: 23.1 and 169.)
-  static constexpr int REG_LAUNCH = 72, REG_EPILOGUE = 96, REG_ISSUE = 56, REG_AUX = 32;
-  static_assert(!FP8 || 512 * REG_EPILOGUE + 128 * REG_ISSUE + AUX * 32 * REG_AUX <= THREADS * REG_LAUNCH,
+  // With AUX warps registers move to the epilogue (setmaxnreg).  Float8 has spilled at 72 a thread for all: 16 single
+  // tokens took 25.5 us and take 23.5, chunks 182 and 165.  (88, with 72 for warps 16 to 19 and 40 for 20 to 27:
+  // 23.1 and 169.)  16 bits: 117 us for 64 single tokens; 125 with 96, 56 and 40.
+  static constexpr bool SPLIT = AUX > 0;
+  static constexpr int REG_LAUNCH = FP8 ? 72 : 80, REG_EPILOGUE = FP8 ? 96 : 88, REG_ISSUE = FP8 ? 56 : 72,
+                       REG_AUX = FP8 ? 32 : 56;
+  static_assert(!SPLIT || 512 * REG_EPILOGUE + 128 * REG_ISSUE + AUX * 32 * REG_AUX <= THREADS * REG_LAUNCH,
                 "register split");
+  static constexpr int SHARE = ONE ? 2 : 1;  // producers of a key tile
   static constexpr uint32_t LAYOUT = SWZ == 128 ? 2u : SWZ == 64 ? 4u : 6u;
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -212,7 +220,8 @@ struct alignas(16) WeightsPart {
 
 template <typename G>
 struct WeightsShared {
-  uint64_t k_full[2][G::K_SLOTS], k_empty[2][G::K_SLOTS];
+  uint64_t k_full[2][G::SHARE][G::K_SLOTS];  // from each producer
+  uint64_t k_empty[2][G::K_SLOTS];
   uint64_t q_full[G::Q_SLOTS], q_empty[G::Q_SLOTS];
   uint64_t l_full[2][G::L_SLOTS], l_empty[2][G::L_SLOTS];
   uint64_t i_full[2][G::I_SLOTS], i_empty[2][G::I_SLOTS];
@@ -256,11 +265,11 @@ __device__ __forceinline__ float2 add_exp2_poly(float2 x, float2 acc) {
   return ffma2(q, scale, acc);
 }
 
-template <typename T, int D, bool FP8>
-__global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
+template <typename T, int D, bool FP8, bool ONE>
+__global__ void __launch_bounds__(WeightsGeo<D, FP8, ONE>::THREADS, 1)
     paged_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ PagedWeightsParams p) {
-  using G = WeightsGeo<D, FP8>;
+  using G = WeightsGeo<D, FP8, ONE>;
   using Sh = WeightsShared<G>;
   static_assert(sizeof(Sh) <= G::SHARED, "barrier block");
   constexpr int QN = G::QN, K_SLOTS = G::K_SLOTS, Q_SLOTS = G::Q_SLOTS;
@@ -279,16 +288,16 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     auto init = [](uint64_t* bars, int n, uint32_t count) {
       for (int s = 0; s < n; ++s) mbar_init(smem_u32(bars + s), count);
     };
-    init(sh->k_full[0], 2 * K_SLOTS, FP8 ? G::AUX : 1);
+    init(sh->k_full[0][0], 2 * G::SHARE * K_SLOTS, FP8 ? G::AUX : 1);
     init(sh->k_empty[0], 2 * K_SLOTS, 1);
     init(sh->q_full, Q_SLOTS, 1);
     init(sh->q_empty, Q_SLOTS, 2);  // the issuers
     init(sh->l_full[0], 2 * G::L_SLOTS, 1);
     init(sh->l_empty[0], 2 * G::L_SLOTS, 8);  // the epilogue of that parity
-    init(sh->i_full[0], 2 * G::I_SLOTS, FP8 ? G::AUX : 1);
+    init(sh->i_full[0], 2 * G::I_SLOTS, FP8 ? G::AUX : G::SHARE);
     init(sh->i_empty[0], 2 * G::I_SLOTS, 8);  // the two warpgroups of the tile
     init(sh->p_full, G::P_SLOTS, 1);
-    init(sh->p_empty, G::P_SLOTS, 19 + G::AUX);  // all other warps
+    init(sh->p_empty, G::P_SLOTS, (ONE ? 18 : 19) + G::AUX);  // all other warps that work
     init(sh->raw_full, 8, 1);
     init(sh->raw_empty, 8, G::AUX);
     init(sh->s_full[0], 4, 1);
@@ -336,10 +345,11 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     q_head = w.head;
   };
 
-  // Producer of key tiles: both of an item, or one of them.
+  // Producer of key tiles: of both of an item, of one of them, or of every other page of one.
   // The copies of a tile, a lane each (two where the smallest pages have long rows).
   constexpr int COPIES = FP8 ? 2 : G::NBLK;  // of one page
-  constexpr int OPS = (16 * COPIES + 31) / 32;
+  constexpr int SHARE = G::SHARE;
+  constexpr int OPS = (16 / SHARE * COPIES + 31) / 32;
   struct Keys {
     int slot = 0, islot = 0;
     uint32_t ph = 0, iph = 0;
@@ -350,10 +360,10 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
   const int box = min(size, 128);
   const int boxes = 128 / box;
   // (float8: `k` of the ring of raw tiles, which both key tiles share)
-  auto load_keys = [&](int i, Keys& k, int (&ahead)[OPS]) -> bool {
+  auto load_keys = [&](int i, int half, Keys& k, int (&ahead)[OPS]) -> bool {
     const int key0 = w.key0() + i * 128;
     auto fetch = [&](int u, int first) {
-      const int my_box = (lane + 32 * u) / COPIES;
+      const int my_box = (lane + 32 * u) / COPIES * SHARE + half;
       const int pos = first + my_box * box;
       return my_box < boxes && pos < w.len ? page_entry(p.seqs, w.seq, pos) : -1;
     };
@@ -369,12 +379,12 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     bool ok = FP8 ? wait(sh->raw_empty[k.slot], k.ph ^ 1u) : wait(sh->k_empty[i][k.slot], k.ph ^ 1u);
     if (!FP8 && ok) ok = wait(sh->i_empty[i][k.islot], k.iph ^ 1u);
     if (!ok) return false;
-    const uint32_t bar = smem_u32(FP8 ? &sh->raw_full[k.slot] : &sh->k_full[i][k.slot]);
+    const uint32_t bar = smem_u32(FP8 ? &sh->raw_full[k.slot] : &sh->k_full[i][half][k.slot]);
     const uint32_t dst = smem_u32(FP8 ? raw_smem + k.slot * G::RAW : k_smem + (i * K_SLOTS + k.slot) * G::K_TILE);
     int page[OPS];
 #pragma unroll
     for (int u = 0; u < OPS; ++u) {
-      const int my_box = (lane + 32 * u) / COPIES, part = (lane + 32 * u) % COPIES;
+      const int my_box = (lane + 32 * u) / COPIES * SHARE + half, part = (lane + 32 * u) % COPIES;
       const bool in = my_box < boxes && key0 + my_box * box < w.len;
       page[u] = in ? checked_page(p.seqs, entry[u]) : -1;
       // (what is no page is copied from another one, and gets no weight)
@@ -384,12 +394,12 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     __syncwarp();
     if (lane == 0) {  // (behind the page numbers, which those read who see the barrier complete)
       const int live = min(boxes, (w.len - key0 + box - 1) / box);  // with a key
-      mbar_arrive_expect_tx(bar, live * box * (FP8 ? D + 4 : G::ROW_BYTES));
+      mbar_arrive_expect_tx(bar, (live - half + SHARE - 1) / SHARE * box * (FP8 ? D + 4 : G::ROW_BYTES));
     }
     __syncwarp();
 #pragma unroll
     for (int u = 0; u < OPS; ++u) {
-      const int my_box = (lane + 32 * u) / COPIES, part = (lane + 32 * u) % COPIES;
+      const int my_box = (lane + 32 * u) / COPIES * SHARE + half, part = (lane + 32 * u) % COPIES;
       const int row = (key0 + my_box * box) & (size - 1);
       if (page[u] < 0) continue;
       if constexpr (FP8) {
@@ -421,31 +431,33 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     k.ahead_block = w.key0() + kWeightsBlock < w.len ? w.block + 1 : 0;
   };
   // The copies issued last land before shared memory goes away.
-  auto drain_keys = [&](int i, const Keys& k) {
+  auto drain_keys = [&](int i, int half, const Keys& k) {
     constexpr int RING = FP8 ? G::RAW_SLOTS : K_SLOTS;
     for (int u = 0; u < min(k.issued, RING); ++u) {
       const int x = k.issued - 1 - u;
-      drain_bar(smem_u32(FP8 ? &sh->raw_full[x % RING] : &sh->k_full[i][x % RING]),
+      drain_bar(smem_u32(FP8 ? &sh->raw_full[x % RING] : &sh->k_full[i][half][x % RING]),
                 static_cast<uint32_t>((x / RING) & 1));
     }
   };
 
-  if constexpr (FP8) {
+  if constexpr (G::SPLIT) {
     if (warp >= 16 && warp < 20) setmaxnreg_dec<G::REG_ISSUE>();
   }
   if (warp == 18) {
     // ------------------------------------------------------------------ producer of K
-    Keys k;
-    int ahead[2][OPS];
-    bool ok = true;
-    while (ok && next_part()) {
+    if constexpr (!ONE) {
+      Keys k;
+      int ahead[2][OPS];
+      bool ok = true;
+      while (ok && next_part()) {
 #pragma unroll
-      for (int i = 0; i < (FP8 ? 2 : 1); ++i)
-        if (i < w.tiles && ok) ok = load_keys(i, k, ahead[i]);
-      if (FP8 && w.tiles == 1) k.ahead_block = -1;  // (those of the second tile have not been fetched)
-      else fetched(k);
+        for (int i = 0; i < (FP8 ? 2 : 1); ++i)
+          if (i < w.tiles && ok) ok = load_keys(i, 0, k, ahead[i]);
+        if (FP8 && w.tiles == 1) k.ahead_block = -1;  // (those of the second tile have not been fetched)
+        else fetched(k);
+      }
+      drain_keys(0, 0, k);
     }
-    drain_keys(0, k);
   } else if (warp == 19) {
     // ------------------------------------------------------------------ the line, and Q
     if (lane == 0) p.notes[blockIdx.x].first_cta = -1;
@@ -493,8 +505,8 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
     while (ok && coming.tiles > 0) {
       w = coming;
       tell(coming);
-      if (!FP8 && w.tiles == 2) {
-        if (ok) ok = load_keys(1, k, ahead);
+      if (!FP8 && !ONE && w.tiles == 2) {
+        if (ok) ok = load_keys(1, 0, k, ahead);
         fetched(k);
       }
       for (int t = 0; t < w.steps && ok; ++t, step ^= 1) {
@@ -550,7 +562,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
       const int x = issued - 1 - u;
       drain_bar(smem_u32(&sh->q_full[x % Q_SLOTS]), static_cast<uint32_t>((x / Q_SLOTS) & 1));
     }
-    if constexpr (!FP8) drain_keys(1, k);
+    if constexpr (!FP8 && !ONE) drain_keys(1, 0, k);
   } else if (warp == 16 || warp == 17) {
     // ------------------------------------------------------------------ MMA issuers
     constexpr uint32_t hi = ((8u * G::SWZ) >> 4) | (1u << 14) | (G::LAYOUT << 29);
@@ -574,7 +586,9 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
           ok = wait(sh->q_full[qslot], qph);
         }
         if (mine) {
-          if (t == 0 && ok) ok = wait(sh->k_full[i][kslot], kph);
+#pragma unroll
+          for (int half = 0; half < SHARE; ++half)
+            if (t == 0 && ok) ok = wait(sh->k_full[i][half][kslot], kph);
           if (ok) ok = wait(sh->s_empty[i][buf], sph[buf] ^ 1u);
           if (!ok) break;
           sph[buf] ^= 1u;
@@ -665,7 +679,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(smem_u32(&sh->i_full[i][islot[i]]));
-            mbar_arrive(smem_u32(&sh->k_full[i][slot[i]]));
+            mbar_arrive(smem_u32(&sh->k_full[i][0][slot[i]]));
             mbar_arrive(smem_u32(&sh->raw_empty[rslot]));
           }
           if (++islot[i] == G::I_SLOTS) { islot[i] = 0; iph[i] ^= 1u; }
@@ -674,9 +688,23 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8>::THREADS, 1)
         }
       }
     }
+    if constexpr (ONE) {
+      // ---------------------------------------------------------------- producers of K
+      setmaxnreg_dec<G::REG_AUX>();
+      const int i = warp >> 1 & 1, half = warp & 1;
+      Keys k;
+      int ahead[OPS];
+      bool ok = true;
+      while (ok && next_part()) {
+        if (i >= w.tiles) continue;
+        ok = load_keys(i, half, k, ahead);
+        fetched(k);
+      }
+      drain_keys(i, half, k);
+    }
   } else {
     // -------------------------------------------------------------------- epilogue
-    if constexpr (FP8) setmaxnreg_inc<G::REG_EPILOGUE>();
+    if constexpr (G::SPLIT) setmaxnreg_inc<G::REG_EPILOGUE>();
     const int i = warp >> 2 & 1;     // key tile
     const int buf = warp >> 3;       // steps of this parity, and their buffer
     const int part = warp & 3;       // 32 keys of the tile

@@ -13,13 +13,13 @@
 namespace fa {
 namespace {
 
-template <typename T, bool FP8>
+template <typename T, bool FP8, bool ONE>
 int launch_weights(const WeightsPlan& plan) {
-  using G = WeightsGeo<FA_HEAD_DIM, FP8>;
-  auto kernel = paged_weights_kernel<T, FA_HEAD_DIM, FP8>;
+  using G = WeightsGeo<FA_HEAD_DIM, FP8, ONE>;
+  auto kernel = paged_weights_kernel<T, FA_HEAD_DIM, FP8, ONE>;
   static SmemOptIn opt_in;
   if (!opt_in(reinterpret_cast<const void*>(kernel), G::SMEM)) return -7;
-  if constexpr (FP8) {
+  if constexpr (G::SPLIT) {
     static RegsMatch regs_match;
     if (!regs_match(reinterpret_cast<const void*>(kernel), G::REG_LAUNCH)) return -7;
   }
@@ -32,8 +32,10 @@ int launch_weights(const WeightsPlan& plan) {
 
 int launch_any(const WeightsPlan& plan) {
   if (plan.fp8)
-    return plan.half ? launch_weights<__half, true>(plan) : launch_weights<__nv_bfloat16, true>(plan);
-  return plan.half ? launch_weights<__half, false>(plan) : launch_weights<__nv_bfloat16, false>(plan);
+    return plan.half ? launch_weights<__half, true, false>(plan) : launch_weights<__nv_bfloat16, true, false>(plan);
+  if (plan.params.whole_items)
+    return plan.half ? launch_weights<__half, false, true>(plan) : launch_weights<__nv_bfloat16, false, true>(plan);
+  return plan.half ? launch_weights<__half, false, false>(plan) : launch_weights<__nv_bfloat16, false, false>(plan);
 }
 
 }  // namespace
