@@ -37,7 +37,7 @@
 // Measured: 64 single tokens over 500 to 8192 tokens (32 / 8 heads x 128, 16 bits) 117 us, 5.4 TB/s; 16 over 100 to
 // 2000 in float8 23 us, the chain of an item; 5 prompts of 700 to 3500 tokens 112 to 121 us, 46 % of the
 // exponential unit and 34 % of the tensor cores; 4 chunks of 300 to 1024 over 4096 to 16384 (16 / 4 heads x 64,
-// float8) 165 us, 65 % of the exponential unit.
+// float8) 165 us, 64 % of the exponential unit.
 //
 // What a ring holds is waited for and given back by all warps that read from it, in order, though not all
 // look at each fill: a warp that passed over fills could take an older one for its own.
