@@ -127,7 +127,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 3) paged_select
   int* const kept = p.kept + static_cast<int64_t>(item) * p.keep;
   if (rank == 0 && head == 0 && tid == 0) {
     p.new_lens[b] = stay;
-    if (fresh(p.seqs.kv_lens + b) != n) report(p.seqs.status, kStatusPageTable);
+    // (a rank behind the last column that receives is in no chunk where a chunk ends there: nothing else says so)
+    if (fresh(p.seqs.kv_lens + b) != n || stay > static_cast<int64_t>(p.to_cols) << p.seqs.page_log2)
+      report(p.seqs.status, kStatusPageTable);
   }
   if (p.flags && rank == 0) {
     const int units = 2 * p.chunks[0] + p.chunks[1];

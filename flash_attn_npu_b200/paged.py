@@ -517,7 +517,8 @@ def evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale=
     keep - recent with the largest weights (of equal ones the earlier; NaN counts as the largest).  They
     keep their order and move to positions 0 .. keep - 1, with their scales and weights: in place, or into
     the pages of `to_table` [seqs, columns], which also receive the sequences that are not longer, and must
-    not be among those of `page_table`.  What lies behind the new length is left as it was.  Pages that
+    not be among those of `page_table`; a row of it has to name min(kv_len, keep) places, or the call reports it
+    as it does an entry outside the cache.  What lies behind the new length is left as it was.  Pages that
     receive tokens must not belong to another sequence too (a shared prefix among them).
 
     new_lens [seqs] int32 is min(kv_lens, keep); kept [seqs, heads_kv, keep] int32 the positions that

@@ -198,7 +198,8 @@ typedef struct FaPagedEvictArgs {
  * order and go to positions 0 .. keep - 1, in K, V, the scales of a float8 cache and the weights.  What
  * lies behind the new length is left as it was.  Shorter sequences stay as they are (not in place: they
  * are copied).  Pages that receive tokens must not belong to another sequence too; those of to_table must
- * not be among those of page_table. */
+ * not be among those of page_table.  A to_table with fewer places than a sequence has tokens to stay is reported
+ * through the device status, and that sequence's results are undefined. */
 FA_API int fa_paged_evict_sm100(const FaPagedEvictArgs* args, void* stream);
 
 /* Its workspace, as fa_paged_workspace_bytes. */

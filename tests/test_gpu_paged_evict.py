@@ -144,3 +144,19 @@ def test_pages_that_are_none_are_reported(cuda_device):
         with pytest.raises(RuntimeError, match="page"):
             ops.check_device_status(cuda_device)
     ops.check_device_status(cuda_device)
+
+
+@pytest.mark.parametrize("cols", [0, 1, 16])
+@pytest.mark.parametrize("lens", [[5000], [70, 3000], [5000] * 40])
+def test_a_table_too_narrow_for_what_stays_is_reported(lens, cols, cuda_device):
+    """Also where it ends with a chunk of ranks (of K and V 128, of weights and scales 2048)."""
+    b = _batch(lens, cuda_device, heads_kv=2, heads_q=2, head_dim=128, page=128, spare=16 * len(lens), seed=4)
+    w = _weights(b.k_cache.shape[:3], 9, "spread").to(cuda_device)
+    free = [i for i in range(b.k_cache.shape[0]) if i not in set(b.table.flatten().tolist())]
+    to = torch.tensor(free[:cols * len(lens)], dtype=torch.int32, device=cuda_device).view(len(lens), cols)
+    fam.paged_cache_evict(b.k_cache, b.v_cache, w, b.table, b.lens, 4096, 10, to_table=to)
+    with pytest.raises(RuntimeError, match="page"):
+        ops.check_device_status(cuda_device)
+    # what fits is no matter: the same call with a budget of as many tokens as the table has places
+    fam.paged_cache_evict(b.k_cache, b.v_cache, w, b.table, b.lens, cols * 128, 0, to_table=to)
+    ops.check_device_status(cuda_device)
