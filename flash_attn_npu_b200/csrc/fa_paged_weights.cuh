@@ -748,6 +748,7 @@ __global__ void __launch_bounds__(WeightsGeo<D, FP8, ONE>::THREADS, 1)
         if (!same_q()) {
           now_q();
           if (w.qtiles == 1 || step == buf) {
+            __syncwarp();  // (lanes leave the last columns at their own pace)
             if (lslot >= 0 && lane == 0) mbar_arrive(smem_u32(&sh->l_empty[buf][lslot]));
             if (++lslot == G::L_SLOTS) lslot = 0;
             if (lslot == 0) lph ^= 1u;

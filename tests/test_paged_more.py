@@ -241,3 +241,18 @@ def test_native_checks(native_lib):
         assert fn(ctypes.byref(a), None) == _native.FA_OK
         if not torch.cuda.is_available():
             assert fn(ctypes.byref(_native_args(kind)), None) == _native.FA_ERR_DEVICE
+
+
+# ---------------------------------------------------------------------------------------------- ring slots
+@pytest.mark.parametrize("name", ["fa_paged_weights.cuh", "fa_paged_tile.cuh", "fa_paged_rows.cuh"])
+def test_a_slot_is_given_back_behind_its_last_reader(name):
+    """Where lane 0 gives a ring's slot back for its warp, the warp has met right before: else a lane that lags
+    reads what the next fill has put there.  (A race: it is looked for in the source, not by running it.)"""
+    source = (build.CSRC / name).read_text()
+    lines = [ln.split("//")[0].strip() for ln in source.splitlines()]
+    lines = [ln for ln in lines if ln]
+    gives = [i for i, ln in enumerate(lines) if "lane == 0) mbar_arrive(" in ln and "empty" in ln]
+    assert gives
+    for i in gives:
+        before = lines[i - 1] if "tc_fence_before" not in lines[i - 1] else lines[i - 2]
+        assert before == "__syncwarp();", lines[i]
