@@ -485,12 +485,13 @@ def attention_weights(q, lse, k_cache, page_table, offsets, kv_lens, weights, ca
     grows by the sum of the probabilities exp(sm_scale q k - lse) of all rows and query heads that attend to
     it: `q`, `causal`, `sm_scale` and the sequences are those of the attention call that `lse` [total,
     heads_q] float32 comes from.  With `reset_new` the places of the sequences' new tokens (the last
-    offsets[b + 1] - offsets[b]) start from 0, so pages need no clearing.  Rows with lse = -inf give nothing.
+    offsets[b + 1] - offsets[b]) start from 0, so pages need no clearing.  Rows with lse = -inf give nothing,
+    whatever q holds there: a caller can leave rows out that way.
 
     With the joint `lse` of `prefix_attention`, one call over the sequences' own tokens, and one over the
     prefixes (prefix_table, prefix_offsets, prefix_lens, causal=False, reset_new=False) give the weights of
-    both.  Pages that get weight must not belong to two sequences of a call.  What a key or row holds shows
-    in its own weight only, and in those that a row attends to.
+    both.  Pages that get weight must not belong to two sequences of a call.  What a key holds shows in its
+    own weight only, and what a row holds in those of the keys that it attends to.
     """
     res = None
     if _binding is not None:

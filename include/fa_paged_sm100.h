@@ -166,7 +166,7 @@ typedef struct FaPagedWeightsArgs {
 } FaPagedWeightsArgs;
 
 /* For each sequence, kv head and position: weights += the sum of exp(sm_scale q k - lse) over the rows
- * that attend to it and share the head.  A row with lse = -inf gives nothing.  Sequences with new tokens
+ * that attend to it and share the head.  A row with lse = -inf gives nothing, whatever q holds.  Sequences with new tokens
  * only; pages must not belong to two sequences of a call. */
 FA_API int fa_paged_weights_sm100(const FaPagedWeightsArgs* args, void* stream);
 

@@ -189,3 +189,31 @@ def test_rows_that_give_nothing(lse, fp8, cuda_device):
                                     causal, 64 ** -0.5, k_scale=b.k_scale)
         ops.check_device_status(cuda_device)
         assert not w.any()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_rows_left_out_may_hold_anything(head_dim, fp8, bad, cuda_device):
+    """A caller leaves rows out by lse = -inf: they give nothing to any key, whatever q holds there."""
+    b = ref.Batch([130, 1, 40, 6], [500, 300, 40, 700], heads_q=8, heads_kv=2, head_dim=head_dim, page=32, fp8=fp8,
+                  device=cuda_device, seed=8)
+    for causal in (False, True):
+        lse = ref_w.logsumexps(b, causal, head_dim ** -0.5)
+        out = torch.rand(lse.shape, generator=torch.Generator().manual_seed(1)) < 0.2
+        out[:33] = False   # a query tile without such rows,
+        out[64:96] = True  # and one of nothing else
+        lse[out.to(lse.device)] = float("-inf")
+        b.q[out.to(lse.device)] = bad
+        for longest in (None, 1):
+            _check(b, causal, lse=lse, max_q_len=longest)
+        b.q[out.to(lse.device)] = 1.0
+
+
+def test_decoding_rows_left_out(cuda_device):
+    """... and in a step of single tokens, a whole sequence's among them."""
+    b = ref.Batch([1] * 40, [1 + 37 * i for i in range(40)], heads_q=8, heads_kv=2, head_dim=128, device=cuda_device, seed=9)
+    lse = ref_w.logsumexps(b, True, 0.1)
+    lse[7], lse[8, 3], lse[20, ::2] = (float("-inf"),) * 3
+    b.q[torch.isneginf(lse)] = float("nan")
+    _check(b, lse=lse, scale=0.1, max_q_len=1)
