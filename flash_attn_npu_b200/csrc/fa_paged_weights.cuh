@@ -241,16 +241,17 @@ struct WeightsShared {
   volatile uint32_t abort_flag;
 };
 
-// acc + 2^x of a pair on the FMA pipe: 2^n 2^f with n = round(x), f = x - n in [-1/2, 1/2], and a polynomial
-// of degree 5 that minimises the relative error of 2^f there (the fit of exp2_poly_fit.py at degree 5: 2.3e-7,
-// as ex2.approx).  0 below -126.5 (2^-127 has no bits in `scale`), infinite from 128 on; NaN stays NaN.
+// acc + 2^x of a pair on the FMA pipe: 2^(n - 1) 2^(f + 1) with n = round(x), f = x - n in [-1/2, 1/2], and twice the
+// polynomial of degree 5 that minimises the relative error of 2^f there (the fit of exp2_poly_fit.py at degree 5:
+// 2.3e-7, as ex2.approx; 5e-8 too large on average).  As 2^(n - 1) it is finite wherever 2^x is: up to 128.
+// 0 below -125.5 (2^-127 has no bits in `scale`); NaN stays NaN.
 __device__ __forceinline__ float2 add_exp2_poly(float2 x, float2 acc) {
   constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the low bits of x + kRound are n
-  constexpr float c0 = 1.000000119e+00f, c1 = 6.931469440e-01f, c2 = 2.402212024e-01f, c3 = 5.550713092e-02f,
-                  c4 = 9.675540961e-03f, c5 = 1.327647129e-03f;
+  constexpr float c0 = 2.000000238e+00f, c1 = 1.386293888e+00f, c2 = 4.804424047e-01f, c3 = 1.110142618e-01f,
+                  c4 = 1.935108192e-02f, c5 = 2.655294258e-03f;
   auto both = [](float c) { return make_float2(c, c); };
   auto clamp = [](float v) {
-    asm("max.NaN.f32 %0, %0, 0fC2FE0000;\n\tmin.NaN.f32 %0, %0, 0f43000000;" : "+f"(v));  // -127, 128
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;\n\tmin.NaN.f32 %0, %0, 0f43000000;" : "+f"(v));  // -126, 128
     return v;
   };
   x = make_float2(clamp(x.x), clamp(x.y));
@@ -261,8 +262,8 @@ __device__ __forceinline__ float2 add_exp2_poly(float2 x, float2 acc) {
   q = ffma2(q, f, both(c2));
   q = ffma2(q, f, both(c1));
   q = ffma2(q, f, both(c0));
-  const float2 scale = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000),
-                                   __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000));
+  const float2 scale = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f000000),
+                                   __int_as_float((__float_as_int(t.y) << 23) + 0x3f000000));
   return ffma2(q, scale, acc);
 }
 

@@ -217,3 +217,22 @@ def test_decoding_rows_left_out(cuda_device):
     lse[7], lse[8, 3], lse[20, ::2] = (float("-inf"),) * 3
     b.q[torch.isneginf(lse)] = float("nan")
     _check(b, lse=lse, scale=0.1, max_q_len=1)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("l", [-88.0, -88.6, 80.0, 86.5])
+def test_the_largest_and_smallest_weights_are_alike_in_every_row(l, fp8, cuda_device):
+    """One row of 32 gives exp(-l), wherever it is: 88.6 is past 127.5 ln 2, 88.72 would be infinite.  (The others give
+    exp(-200) = 0.)"""
+    b = ref.Batch([32], [300], heads_q=1, heads_kv=1, head_dim=64, page=64, fp8=fp8, device=cuda_device, seed=8)
+    b.q.zero_()
+    args = (b.k_cache, *b.where)
+    for r in range(32):
+        w = torch.zeros(b.k_cache.shape[:3], device=cuda_device)
+        lse = torch.full((32, 1), 200.0, device=cuda_device)
+        lse[r] = l
+        fam.paged_attention_weights(b.q, lse, *args, w, False, 0.125, k_scale=b.k_scale)
+        flat = ref.gather(w, b.table, 0, 300).double()
+        want = torch.exp(torch.tensor(-l, dtype=torch.float64, device=cuda_device))
+        # (the tolerance of paged_weights_ref.py)
+        assert ((flat - want).abs() <= 2.0 ** -21 * (1 + abs(l)) * want + 2.0 ** -126).all(), r
