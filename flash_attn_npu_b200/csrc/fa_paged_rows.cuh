@@ -199,7 +199,9 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
   }
   __syncthreads();
   begin(p);
-  if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
+  if constexpr (!LV) {  // (behind shared prefixes the join goes by `where` alone)
+    if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
+  }
   const PagedRange range =
       paged_range(p, [&](int b) { return paged_seq<ROWS, KEYS>(p, b).steps; });
   PagedWalk<ROWS, KEYS, PagedParams<LV>> w(p, range);
@@ -690,7 +692,9 @@ __global__ void __launch_bounds__(RowsGeo<D, FP8, ROWS>::THREADS, 1)
     named_barrier_sync(1, NW * 32);
     const bool whole = w.whole();
     const int64_t part_row = (static_cast<int64_t>(blockIdx.x) * 2 + w.slot()) * ROWS + my_r;
-    if (!whole && w.slot() == 0 && threadIdx.x == 0) p.parts[blockIdx.x] = w.note();
+    if constexpr (!LV) {
+      if (!whole && w.slot() == 0 && threadIdx.x == 0) p.parts[blockIdx.x] = w.note();
+    }
     // the largest base of a row's warps
     auto top_of = [&](int r) -> float {
       float x = -INFINITY;

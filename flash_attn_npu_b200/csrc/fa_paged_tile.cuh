@@ -209,7 +209,9 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
   begin(p);
-  if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
+  if constexpr (!LV) {  // (behind shared prefixes the join goes by `where` alone)
+    if (threadIdx.x == 0) p.parts[blockIdx.x].first_cta = -2;
+  }
   if (warp == 0) {
     const PagedRange r =
         paged_range(p, [&](int b) { return PagedTiles<TILES, KEYS, PagedParams<LV>>(p, b).steps(p); });
@@ -713,7 +715,9 @@ __global__ void __launch_bounds__(TileGeo<D, FP8>::THREADS, 1)
         const int64_t part_row = (static_cast<int64_t>(blockIdx.x) * 2 + w.slot()) * (128 * TILES) +
                                  tile * 128 + r;
         const bool whole = w.whole();
-        if (threadIdx.x == 0 && !whole && w.slot() == 0) p.parts[blockIdx.x] = w.note(range, p.item_cost);
+        if constexpr (!LV) {
+          if (threadIdx.x == 0 && !whole && w.slot() == 0) p.parts[blockIdx.x] = w.note(range, p.item_cost);
+        }
         if (n == 0) {
           // nothing of this part concerns the tile (no token, or keys behind all of them)
           if (live && !whole) p.part_lse[part_row] = -INFINITY;
