@@ -160,3 +160,11 @@ def test_a_table_too_narrow_for_what_stays_is_reported(lens, cols, cuda_device):
     # what fits is no matter: the same call with a budget of as many tokens as the table has places
     fam.paged_cache_evict(b.k_cache, b.v_cache, w, b.table, b.lens, cols * 128, 0, to_table=to)
     ops.check_device_status(cuda_device)
+
+
+@pytest.mark.parametrize("kind", ["mixed", "equal"])
+def test_positions_beyond_the_shared_memory_of_a_cluster(kind, cuda_device):
+    """16 blocks hold 43,008 keys each: here they read 6,992 each from memory in every pass."""
+    b = _batch([800001], cuda_device, heads_kv=1, heads_q=1, head_dim=16, page=1024, seed=1)
+    w = _weights(b.k_cache.shape[:3], 3, kind).to(cuda_device)
+    _check(b, w, 30011, 11)
