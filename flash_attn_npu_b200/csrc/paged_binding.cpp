@@ -454,16 +454,16 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     x.to_table = static_cast<const int32_t*>(to->const_data_ptr());
   }
   const c10::cuda::OptionalCUDAGuard guard(cache.device());
+  strides(*weights, x.weights_stride);
+  x.workspace_bytes = g_evict_workspace(&x);
+  if (x.workspace_bytes < 0) return none();
   const auto options = cache.options().dtype(at::kInt);
   Tensor lens = at::empty({x.cache.seqs}, options);
   Tensor kept = at::empty({x.cache.seqs, x.cache.heads_kv, x.keep}, options);
-  strides(*weights, x.weights_stride);
   x.weights = static_cast<float*>(const_cast<void*>(weights->const_data_ptr()));
   x.new_lens = static_cast<int32_t*>(lens.mutable_data_ptr());
   x.kept = static_cast<int32_t*>(kept.mutable_data_ptr());
   x.dev_status = g_status[index];
-  x.workspace_bytes = g_evict_workspace(&x);
-  if (x.workspace_bytes < 0) return none();
   const c10::DataPtr workspace = c10::cuda::CUDACachingAllocator::get()->allocate(x.workspace_bytes);
   x.workspace = workspace.get();
   const int rc = g_evict(&x, c10::cuda::getCurrentCUDAStream(index).stream());

@@ -186,6 +186,8 @@ def validate_evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent,
     _validate_weights(weights, k_cache)
     if not 0 <= recent <= keep <= 1 << 30:
         raise ValueError("keep and recent must be 0 <= recent <= keep <= 2^30")
+    if page_table.shape[0] * k_cache.shape[1] > 1 << 24:
+        raise ValueError("an eviction takes at most 2^24 heads of sequences")
     if to_table is not None:
         if to_table.ndim != 2 or to_table.shape[0] != page_table.shape[0] or to_table.dtype != torch.int32:
             raise ValueError("to_table must be int32 [seqs, columns]")

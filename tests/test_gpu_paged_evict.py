@@ -168,3 +168,42 @@ def test_positions_beyond_the_shared_memory_of_a_cluster(kind, cuda_device):
     b = _batch([800001], cuda_device, heads_kv=1, heads_q=1, head_dim=16, page=1024, seed=1)
     w = _weights(b.k_cache.shape[:3], 3, kind).to(cuda_device)
     _check(b, w, 30011, 11)
+
+
+@pytest.mark.parametrize("seqs", [1, 6, 48])
+def test_tables_wider_than_their_sequences(seqs, cuda_device):
+    """The plan goes by the table's width: clusters whose last blocks have nothing, for short sequences."""
+    b = _batch([40 + 61 * i for i in range(seqs)], cuda_device, heads_kv=2, heads_q=2, head_dim=64, page=64, seed=seqs)
+    wide = torch.full((seqs, 2048), -1, dtype=torch.int32, device=cuda_device)
+    wide[:, :b.table.shape[1]] = b.table
+    before = [x.clone() for x in (b.k_cache, b.v_cache)]
+    w = _weights(b.k_cache.shape[:3], 9).to(cuda_device)
+    first = w.clone()
+    narrow = b.table
+    b.table = wide
+    lens, kept = _check(b, w, 150, 20)
+    # columns of the same table give the same
+    b.k_cache, b.v_cache, b.table = *before, wide[:, :narrow.shape[1]]
+    again = _check(b, first, 150, 20)
+    assert torch.equal(again[0], lens) and torch.equal(again[1], kept)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_captured_long_context(head_dim, cuda_device):
+    """Clusters, tickets and flags: every replay finds them as the first did."""
+    b = _batch([60000, 41000], cuda_device, heads_kv=2, heads_q=2, head_dim=head_dim, page=64, seed=3)
+    w = _weights(b.k_cache.shape[:3], 9, "spread").to(cuda_device)
+    fam.paged_cache_evict(b.k_cache.clone(), b.v_cache.clone(), w.clone(), b.table, b.lens, 9000, 10)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lens, kept = fam.paged_cache_evict(b.k_cache, b.v_cache, w, b.table, b.lens, 9000, 10, return_kept=True)
+    for turn in range(3):
+        held = [b.k_cache, b.v_cache, w]
+        want_lens, want_kept, want = ref_e.evict(held, w, b.table, b.lens, 9000, 10)
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.check_device_status(cuda_device)
+        assert torch.equal(lens.cpu(), want_lens) and torch.equal(kept.cpu(), want_kept)
+        for x, y in zip(held, want):
+            assert torch.equal(ref_e.bits(x.cpu()).view(y.shape), y)
+        b.lens -= 9000

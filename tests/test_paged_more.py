@@ -256,3 +256,12 @@ def test_a_slot_is_given_back_behind_its_last_reader(name):
     for i in gives:
         before = lines[i - 1] if "tc_fence_before" not in lines[i - 1] else lines[i - 2]
         assert before == "__syncwarp();", lines[i]
+
+
+def test_too_many_heads_of_sequences_are_named():
+    k, v = (torch.empty(1, 65536, 8, 16, dtype=BF16, device="meta") for _ in range(2))
+    w = torch.empty(1, 65536, 8, device="meta")
+    table, lens = (torch.empty(s, dtype=torch.int32, device="meta") for s in ((257, 1), 257))
+    with pytest.raises(ValueError, match="heads"):
+        paged.validate_evict(k, v, w, table, lens, 4, 2)
+    paged.validate_evict(k, v, w, table[:256], lens[:256], 4, 2)
