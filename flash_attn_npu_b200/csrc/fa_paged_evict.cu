@@ -663,7 +663,7 @@ EvictChoice choose(const FaPagedEvictArgs* a) {
   // In order where that gives every SM a block.  There are fewer latencies to a byte then: moving took 13 us and
   // 24 with a block a chunk for 16 sequences of 8 heads cut to 512 tokens (head_dim 128, 16 bits), 37 and 65
   // for 48 in float8 cut to 1024; one sequence of 4 heads cut to 40,000 takes 60 us with a block a chunk, and took
-  // 115 in order with the columns dealt out to 16 blocks a head.
+  // 115 in order with the columns dealt out to 16 blocks a head.  (Between 4 and 128 heads neither was measured.)
   const int64_t items = a->cache.seqs * a->cache.heads_kv;
   c.in_order = a->in_place && 2 * items >= sm_count_of_current();
   if (c.in_order) c.blocks = 3 * items;

@@ -14,9 +14,13 @@
 // one kernel suits both levels, one launch has the prefixes and the sequences in one line.
 //
 // Measured: 4 single tokens behind 1000 tokens (16 heads x 128) 12 us, launches and their loads; 64 behind 8191
-// with 100 to 2000 of their own (32 / 8 heads x 128) 81 us, 4.0 TB/s; 40 drafts of 1 to 5 tokens behind three
+// with 100 to 2000 of their own (32 / 8 heads x 128) 80 us, 4.1 TB/s; 40 drafts of 1 to 5 tokens behind three
 // prefixes of up to 20,000 in float8 163 us, the row kernel's chain in 32-row blocks; 6 chunks of 200 to 700
-// tokens behind 6001 (16 / 4 heads x 64) 130 us, 500 TFLOP/s, where exponentials take 56.
+// tokens behind 6001 (16 / 4 heads x 64) 127 us, 510 TFLOP/s, where exponentials take 56.
+//
+// The parts, their logsumexps and the join are fp32.  The probabilities meet the values in 16 bits, as in the
+// kernels' ordinary calls, since that is what the tensor cores multiply: bf16 outputs are 2.3e-3 off (root mean
+// square, relative) where one rounding of the exact result is 1.7e-3.
 #include <algorithm>
 
 #include "fa_paged_host.h"
@@ -251,7 +255,8 @@ int launch_levels(const PagedPlan& plan) {
 // 60,000 tokens, 16 to 128 sequences): side by side took 80 us where one behind the other took 101 for 64
 // single tokens in 16 bits (8-row blocks), 99 and 127 for 4 new tokens of 48 sequences (16-row blocks), 100 and
 // 118 for 8 of 32 (32-row blocks), 117 and 132 for 64 single tokens in float8; but 176 and 169 for 4 of 40 in
-// float8, where the row kernel is bound by its chain and its blocks differ in time.
+// float8, where the row kernel is bound by its chain and its blocks differ in time.  Other head_dims go by the same
+// numbers, unmeasured; nothing but the balance depends on them.
 int unit_of(const PagedPlan& plan, const PagedInfo& info, const PagedPlan& own, bool lone_tile) {
   if (own.fp8 && own.rows > 8) return 0;
   if (plan.rows == 0) return lone_tile ? 130 : 200;  // (both sides of a CTA work on a lone query tile)

@@ -31,13 +31,13 @@
 //             by itself took 1500 cycles an item); TMA producer of Q, and the logsumexps of its rows, and
 //             (16 bits, of 20) of K's key tile 1
 //   20-23     of 24: TMA producers of K, two for each key tile.  With one query tile an item is over as soon as its
-//             keys are there, and walking while loading held them up: 64 single tokens took 148 us and take
+//             keys are there, and walking while loading held them up: 64 single tokens took 148 us and then
 //             117.  Prompts take 111 us with 20 warps and 123 with 24.
 //   20-27     float8: convert the key tiles
-// Measured: 64 single tokens over 500 to 8192 tokens (32 / 8 heads x 128, 16 bits) 117 us, 5.4 TB/s; 16 over 100 to
-// 2000 in float8 23 us, the chain of an item; 5 prompts of 700 to 3500 tokens 112 to 121 us, 46 % of the
-// exponential unit and 34 % of the tensor cores; 4 chunks of 300 to 1024 over 4096 to 16384 (16 / 4 heads x 64,
-// float8) 165 us, 64 % of the exponential unit.
+// Measured: 64 single tokens over 500 to 8192 tokens (32 / 8 heads x 128, 16 bits) 119 us, 5.3 TB/s; 16 over 100 to
+// 2000 in float8 23 us, the chain of an item; 5 prompts of 700 to 3500 tokens 112 us, 45 % of the
+// exponential unit and 33 % of the tensor cores; 4 chunks of 300 to 1024 over 4096 to 16384 (16 / 4 heads x 64,
+// float8) 166 us, 64 % of the exponential unit.
 //
 // What a ring holds is waited for and given back by all warps that read from it, in order, though not all
 // look at each fill: a warp that passed over fills could take an older one for its own.

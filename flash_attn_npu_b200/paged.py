@@ -488,7 +488,7 @@ def attention_weights(q, lse, k_cache, page_table, offsets, kv_lens, weights, ca
     it: `q`, `causal`, `sm_scale` and the sequences are those of the attention call that `lse` [total,
     heads_q] float32 comes from.  With `reset_new` the places of the sequences' new tokens (the last
     offsets[b + 1] - offsets[b]) start from 0, so pages need no clearing.  Rows with lse = -inf give nothing,
-    whatever q holds there: a caller can leave rows out that way.
+    whatever q holds there: a caller can leave rows out that way.  `max_q_len` as in `attention`.
 
     With the joint `lse` of `prefix_attention`, one call over the sequences' own tokens, and one over the
     prefixes (prefix_table, prefix_offsets, prefix_lens, causal=False, reset_new=False) give the weights of
@@ -525,7 +525,8 @@ def evict(k_cache, v_cache, weights, page_table, kv_lens, keep, recent, k_scale=
     receive tokens must not belong to another sequence too (a shared prefix among them).
 
     new_lens [seqs] int32 is min(kv_lens, keep); kept [seqs, heads_kv, keep] int32 the positions that
-    stayed, -1 behind them.  Both stay on the device, and nothing waits for it.
+    stayed, -1 behind them.  Both stay on the device, and nothing waits for it.  So the launch is planned by the
+    width of `page_table`: columns beyond the longest sequence cost time.
     """
     res = None
     if _binding is not None:
